@@ -275,6 +275,79 @@ ILL_API int ill_gemv_info(const ill_gemv* g, int* slices, int* blocks_per_slice,
 ILL_API int ill_gemv_run_noalloc(ill_gemv* g, int copy, const float* x, const float* gamma, float* y, int32_t* argmax, void* stream);
 ILL_API int ill_gemv_destroy(ill_gemv* g);
 
+/* ---- Paged cache: several sequences at once (no counterpart in the reference) --------------
+ * Operators on device buffers for programs that serve many requests: keys and values live in
+ * pages of a cache that the caller owns, and a batch names each sequence's pages. Like
+ * ill_gemv_run_noalloc, the calls take device pointers, enqueue on the caller's `stream` (a
+ * hipStream_t; NULL: the device's default stream), allocate nothing, wait for nothing and can
+ * be captured into a graph.
+ *
+ * A handle holds a model's geometry: `heads` query heads over `kv_heads` key/value heads (query
+ * head h reads key/value head h / (heads / kv_heads)) of `head_dim` 64 or 128; a cache of type
+ * ILL_F16 or ILL_BF16 in pages of `page_size` positions (a power of two, 16 .. 1024). Element
+ * (page, slot, head, dim) of either cache is at page * page_stride + slot * slot_stride +
+ * head * head_stride + dim elements (all 0: [pages][page_size][kv_heads][head_dim]); strides are
+ * multiples of 8. The rotation turns the first `rotary_dim` dims of a head (a multiple of 16;
+ * 0: none) by position * rope_base^(-2 i / rotary_dim), pairing dim i with i + rotary_dim / 2, or
+ * with interleaved != 0 dims 2 i and 2 i + 1. norm_eps belongs to the head norms; scale
+ * multiplies the scores (0: 1 / sqrt(head_dim)). A handle belongs to the GPU that was current
+ * when it was created; one thread at a time calls on it. */
+enum { ILL_F32 = 0, ILL_F16 = 1, ILL_BF16 = 2 };
+typedef struct ill_paged ill_paged;
+typedef struct {
+  int32_t dtype, heads, kv_heads, head_dim, page_size, rotary_dim, interleaved, reserved;
+  int64_t page_stride, slot_stride, head_stride;
+  double rope_base;
+  float norm_eps, scale;
+} ill_paged_desc;
+ILL_API int ill_paged_create(const ill_paged_desc* desc, ill_paged** out);
+ILL_API int ill_paged_destroy(ill_paged* p);
+
+/* A batch. lens, table and row0 are device arrays that the kernels read when they run, so a
+ * captured call follows what they then hold. lens [seqs]: the positions of each sequence, its
+ * new rows included (below 0 counts as 0). table [seqs][table_stride], table_width entries used: the page of positions
+ * i * page_size .. in entry i; entries behind a sequence's last position are not read. row0
+ * [seqs + 1]: sequence s has the new rows row0[s] .. row0[s + 1] - 1, which stand at its last
+ * positions; NULL: row s is sequence s's only one. rows: rows of the buffers (the ones behind
+ * the last sequence's are left alone). max_rows: the most new rows that a sequence has, if
+ * known (0: unknown; a hint for the launch only). pages: pages of the cache. A page number
+ * outside 0 .. pages - 1 is not followed: its positions are neither written nor seen, and so are
+ * positions past table_width pages or below 0. Pages may be shared for reading. */
+typedef struct {
+  int32_t seqs, table_width;
+  int64_t table_stride, rows, max_rows, pages;
+  const int32_t *lens, *table, *row0;
+} ill_paged_batch;
+
+/* New rows into the cache. q, k, v: rows of heads x head_dim (kv_heads x head_dim) values of
+ * type `dtype` (ILL_F32, or the cache's), row r at r * stride elements; parts of one fused
+ * product will do. q NULL: keys and values only. To each head's x: x + bias (bias [(heads + 2
+ * kv_heads) x head_dim], q then k then v), then for q and k x / sqrt(mean(x^2) + norm_eps) *
+ * q_norm (k_norm) [head_dim], then the rotation by the row's position (positions [rows]: by
+ * these instead), computed in float32 from angles in float64 and rounded once. NULL leaves a
+ * step out. Keys and values go to their slots, queries to q_out (the cache's type; q itself
+ * will do where type and stride agree). Two rows of one batch must not share a slot. Buffers
+ * and caches are aligned to 16 bytes, strides are multiples of 8 elements (float32: 4). */
+typedef struct {
+  const void *q, *k, *v;
+  void* q_out;
+  int64_t q_stride, k_stride, v_stride, q_out_stride;
+  const float *bias, *q_norm, *k_norm;
+  const int32_t* positions;
+  int32_t dtype, reserved;
+} ill_paged_rows;
+ILL_API int ill_paged_append(ill_paged* p, const ill_paged_batch* batch, const ill_paged_rows* rows, void* k_cache, void* v_cache,
+                             void* stream);
+
+/* Attention of the new rows over the cache (what ill_paged_append has written included): the
+ * row at position p sees the positions j <= p with j > p - window (window 0: all of them) or
+ * j < sinks. out [rows][heads x head_dim], row r at r * out_stride, of type out_dtype (the
+ * cache's, or ILL_F32): the values weighted by the softmax of the scaled scores; zeros for a row
+ * that sees nothing (or whose scores are all -inf). q [rows][heads x head_dim] is of the
+ * cache's type. What a row does not see never reaches it, infinities and NaN included. */
+ILL_API int ill_paged_attend(ill_paged* p, const ill_paged_batch* batch, const void* q, int64_t q_stride, const void* k_cache,
+                             const void* v_cache, int window, int sinks, void* out, int64_t out_stride, int out_dtype, void* stream);
+
 /* The converter's quantizers (Converter.quantizeQ4Raw / quantGroup and quantizeQ8,
  * Sources/Engine/Convert.swift:252-370), host code that needs no GPU. w is a row-major
  * float32 [rows][cols] matrix; `threads` CPU threads split the rows (any count gives the

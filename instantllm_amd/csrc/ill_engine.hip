@@ -2132,3 +2132,5 @@ int ill_tok_encode_cb(void* user, const char* text, int32_t* ids, int cap) {
 }
 
 }  // extern "C"
+
+#include "ill_paged_host.h"

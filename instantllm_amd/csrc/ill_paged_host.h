@@ -1,0 +1,157 @@
+// Host side of the paged-cache operators: argument checks and launches (ill_paged_* in
+// include/ill_hip.h). Included by ill_engine.hip after its error helpers.
+#pragma once
+#include "ill_paged.h"
+#include "ill_paged_check.h"
+
+struct ill_paged {
+  ill_paged_desc d{};
+  int device = 0, page_log = 0;
+  double* freq = nullptr;   // [rotary_dim / 2] turns per position
+};
+
+namespace illp {
+
+// The current device is the handle's while this lives.
+struct OnDevice {
+  int was = -1, rc = ILL_OK;
+  explicit OnDevice(int dev) {
+    if (hipGetDevice(&was) != hipSuccess) rc = fail(ILL_E_HIP, "no HIP device");
+    else if (was != dev && hipSetDevice(dev) != hipSuccess) rc = fail(ILL_E_HIP, "device %d cannot be made current", dev);
+    if (was == dev || rc) was = -1;
+  }
+  ~OnDevice() {
+    if (was >= 0) hipSetDevice(was);
+  }
+};
+
+PgBatch batch_of(const ill_paged* p, const ill_paged_batch& b) {
+  return {b.lens, b.table, b.row0, b.table_stride, b.pages, b.seqs, (int)b.rows, b.table_width, p->page_log};
+}
+
+template <int TX, int TC>
+void launch_append(const PgAppend& a, int D, int R, int lds, hipStream_t st) {
+  const dim3 grid((a.b.rows + R - 1) / R);
+  if (D == 64) hipLaunchKernelGGL((pg_append_kernel<TX, TC, 64>), grid, dim3(256), lds, st, a, R);
+  else hipLaunchKernelGGL((pg_append_kernel<TX, TC, 128>), grid, dim3(256), lds, st, a, R);
+}
+
+}  // namespace illp
+
+extern "C" {
+
+int ill_paged_destroy(ill_paged* p) {
+  if (!p) return ILL_OK;
+  {
+    illp::OnDevice on(p->device);
+    hipFree(p->freq);
+  }
+  delete p;
+  return ILL_OK;
+}
+
+int ill_paged_create(const ill_paged_desc* desc, ill_paged** out) {
+  if (!out) return fail(ILL_E_ARG, "null output handle");
+  *out = nullptr;
+  if (!desc) return fail(ILL_E_ARG, "paged: null description");
+  ill_paged_desc d = *desc;
+  if (int rc = illp::check_desc(d)) return rc;
+  ill_paged* p = new (std::nothrow) ill_paged();
+  if (!p) return fail(ILL_E_ARG, "paged: out of host memory");
+  auto bad = [&](int rc) { ill_paged_destroy(p); return rc; };
+  p->d = d;
+  while (1 << p->page_log < d.page_size) p->page_log++;
+  if (hipGetDevice(&p->device) != hipSuccess) return bad(fail(ILL_E_HIP, "no HIP device"));
+  double freq[64] = {};
+  for (int i = 0; i < d.rotary_dim / 2; i++) freq[i] = std::pow(d.rope_base, -2.0 * i / d.rotary_dim) / (2 * M_PI);
+  if (hipMalloc(&p->freq, sizeof freq) != hipSuccess || hipMemcpy(p->freq, freq, sizeof freq, hipMemcpyHostToDevice) != hipSuccess)
+    return bad(fail(ILL_E_HIP, "paged: buffer allocation failed"));
+  *out = p;
+  return ILL_OK;
+}
+
+int ill_paged_append(ill_paged* p, const ill_paged_batch* batch, const ill_paged_rows* x, void* k_cache, void* v_cache, void* stream) {
+  if (!p) return fail(ILL_E_ARG, "paged: null handle");
+  const ill_paged_desc& d = p->d;
+  if (int rc = illp::check_append(d, batch, x, k_cache, v_cache)) return rc;
+  if (!batch->seqs || !batch->rows) return ILL_OK;
+  PgAppend a{};
+  a.b = illp::batch_of(p, *batch);
+  a.q = (const uint8_t*)x->q;
+  a.k = (const uint8_t*)x->k;
+  a.v = (const uint8_t*)x->v;
+  a.qo = (uint8_t*)x->q_out;
+  a.kc = (uint8_t*)k_cache;
+  a.vc = (uint8_t*)v_cache;
+  a.qs = x->q_stride;
+  a.ks = x->k_stride;
+  a.vs = x->v_stride;
+  a.qos = x->q_out_stride;
+  a.page_stride = d.page_stride;
+  a.slot_stride = d.slot_stride;
+  a.head_stride = d.head_stride;
+  a.bias = x->bias;
+  a.qn = x->q ? x->q_norm : nullptr;
+  a.kn = x->k_norm;
+  a.freq = p->freq;
+  a.positions = x->positions;
+  a.heads = d.heads;
+  a.kv = d.kv_heads;
+  a.rot = d.rotary_dim;
+  a.interleaved = d.interleaved != 0;
+  a.eps = d.norm_eps;
+  illp::OnDevice on(p->device);
+  if (on.rc) return on.rc;
+  const int R = 4, lds = R * 8 + (R + 1) / 2 * 8 + R * (d.rotary_dim / 2) * 8;
+  hipStream_t st = (hipStream_t)stream;
+  if (x->dtype == ILL_F32) {
+    if (d.dtype == ILL_F16) illp::launch_append<PG_F32, PG_F16>(a, d.head_dim, R, lds, st);
+    else illp::launch_append<PG_F32, PG_BF16>(a, d.head_dim, R, lds, st);
+  } else if (d.dtype == ILL_F16) {
+    illp::launch_append<PG_F16, PG_F16>(a, d.head_dim, R, lds, st);
+  } else {
+    illp::launch_append<PG_BF16, PG_BF16>(a, d.head_dim, R, lds, st);
+  }
+  HCK(hipGetLastError());
+  return ILL_OK;
+}
+
+int ill_paged_attend(ill_paged* p, const ill_paged_batch* batch, const void* q, int64_t q_stride, const void* k_cache, const void* v_cache,
+                     int window, int sinks, void* out, int64_t out_stride, int out_dtype, void* stream) {
+  if (!p) return fail(ILL_E_ARG, "paged: null handle");
+  const ill_paged_desc& d = p->d;
+  if (int rc = illp::check_attend(d, batch, q, q_stride, k_cache, v_cache, window, sinks, out, out_stride, out_dtype)) return rc;
+  if (!batch->seqs || !batch->rows) return ILL_OK;
+  PgAttend a{};
+  a.b = illp::batch_of(p, *batch);
+  a.q = (const uint16_t*)q;
+  a.kc = (const uint16_t*)k_cache;
+  a.vc = (const uint16_t*)v_cache;
+  a.out = out;
+  a.qs = q_stride;
+  a.os = out_stride;
+  a.page_stride = d.page_stride;
+  a.slot_stride = d.slot_stride;
+  a.head_stride = d.head_stride;
+  a.heads = d.heads;
+  a.kv = d.kv_heads;
+  a.window = (int)std::min<int64_t>(window, illp::kMost);
+  a.sinks = (int)std::min<int64_t>(sinks, illp::kMost);
+  a.out_f32 = out_dtype == ILL_F32;
+  a.scale = d.scale;
+  illp::OnDevice on(p->device);
+  if (on.rc) return on.rc;
+  hipStream_t st = (hipStream_t)stream;
+  const dim3 grid(a.b.rows, d.heads);
+  if (d.dtype == ILL_F16) {
+    if (d.head_dim == 64) hipLaunchKernelGGL((pg_attend_simple_kernel<PG_F16, 64>), grid, dim3(64), 0, st, a);
+    else hipLaunchKernelGGL((pg_attend_simple_kernel<PG_F16, 128>), grid, dim3(64), 0, st, a);
+  } else {
+    if (d.head_dim == 64) hipLaunchKernelGGL((pg_attend_simple_kernel<PG_BF16, 64>), grid, dim3(64), 0, st, a);
+    else hipLaunchKernelGGL((pg_attend_simple_kernel<PG_BF16, 128>), grid, dim3(64), 0, st, a);
+  }
+  HCK(hipGetLastError());
+  return ILL_OK;
+}
+
+}  // extern "C"

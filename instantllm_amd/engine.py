@@ -117,6 +117,10 @@ def load_library(path: str | os.PathLike | None = None) -> C.CDLL:
         "ill_gemv_info": (C.c_int, [P, C.POINTER(C.c_int), C.POINTER(C.c_int), C.POINTER(C.c_int64)]),
         "ill_gemv_destroy": (C.c_int, [P]),
         "ill_gemv_run_noalloc": (C.c_int, [P, C.c_int, P, P, P, P, P]),
+        "ill_paged_create": (C.c_int, [P, C.POINTER(P)]),
+        "ill_paged_destroy": (C.c_int, [P]),
+        "ill_paged_append": (C.c_int, [P, P, P, P, P, P]),
+        "ill_paged_attend": (C.c_int, [P, P, P, C.c_int64, P, P, C.c_int, C.c_int, P, C.c_int64, C.c_int, P]),
         "ill_quantize_q4": (C.c_int, [C.POINTER(F32), C.c_int64, C.c_int, C.POINTER(C.c_uint8), C.POINTER(C.c_uint16), C.c_int]),
         "ill_quantize_q8": (C.c_int, [C.POINTER(F32), C.c_int64, C.c_int, C.c_int, C.POINTER(C.c_int8), C.POINTER(C.c_uint16), C.c_int]),
         "ill_ildraft_open": (P, [C.c_char_p]),

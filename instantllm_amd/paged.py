@@ -1,0 +1,102 @@
+"""Python binding of the paged-cache operators (ill_paged_* in include/ill_hip.h): new rows into
+a paged key/value cache, and attention over it, for several sequences at once.
+
+As in `Gemv.run_noalloc`, buffers are device addresses that the caller owns, work is enqueued on
+the caller's stream (None: the default one), nothing is allocated and nothing waited for.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+from .engine import ILL_OK, IllError, load_library
+
+DTYPES = {"f32": 0, "f16": 1, "bf16": 2}
+
+
+class _Desc(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "heads", "kv_heads", "head_dim", "page_size", "rotary_dim", "interleaved", "reserved")] + \
+               [(n, C.c_int64) for n in ("page_stride", "slot_stride", "head_stride")] + \
+               [("rope_base", C.c_double), ("norm_eps", C.c_float), ("scale", C.c_float)]
+
+
+class Batch(C.Structure):
+    """The sequences of a call (ill_paged_batch); the arrays are read when the kernels run."""
+    _fields_ = [("seqs", C.c_int32), ("table_width", C.c_int32)] + \
+               [(n, C.c_int64) for n in ("table_stride", "rows", "max_rows", "pages")] + [(n, C.c_void_p) for n in ("lens", "table", "row0")]
+
+
+class _Rows(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "q_out")] + [(n, C.c_int64) for n in ("q_stride", "k_stride", "v_stride", "q_out_stride")] + \
+               [(n, C.c_void_p) for n in ("bias", "q_norm", "k_norm", "positions")] + [("dtype", C.c_int32), ("reserved", C.c_int32)]
+
+
+def _dtype(name: str) -> int:
+    if name not in DTYPES:
+        raise ValueError(f"type {name!r}: one of {', '.join(DTYPES)}")
+    return DTYPES[name]
+
+
+class PagedAttention:
+    """A model's head geometry and cache layout. `strides`: (page, slot, head) strides of the
+    caches in elements (None: [pages][page_size][kv_heads][head_dim]); `rotary_dim` None: the
+    whole head."""
+
+    def __init__(self, heads: int, kv_heads: int, head_dim: int, page_size: int = 16, dtype: str = "f16", rotary_dim: int | None = None,
+                 rope_base: float = 1e6, interleaved: bool = False, norm_eps: float = 1e-6, scale: float | None = None,
+                 strides: tuple[int, int, int] | None = None):
+        self.h = None
+        self.lib = load_library()
+        self.heads, self.kv_heads, self.head_dim, self.dtype = heads, kv_heads, head_dim, dtype
+        d = _Desc(_dtype(dtype), heads, kv_heads, head_dim, page_size, head_dim if rotary_dim is None else rotary_dim, int(interleaved), 0,
+                  *(strides or (0, 0, 0)), rope_base, norm_eps, scale or 0.0)
+        h = C.c_void_p()
+        self._check(self.lib.ill_paged_create(C.byref(d), C.byref(h)))
+        self.h = h
+
+    def _check(self, rc: int):
+        if rc != ILL_OK:
+            raise IllError(rc, self.lib.ill_last_error().decode())
+
+    def batch(self, lens: int, table: int, table_width: int, pages: int, seqs: int, rows: int | None = None, row0: int | None = None,
+              max_rows: int = 0, table_stride: int | None = None) -> Batch:
+        """lens [seqs], table [seqs][table_stride], row0 [seqs + 1] (None: one row each): device addresses of int32 arrays."""
+        return Batch(seqs, table_width, table_width if table_stride is None else table_stride, seqs if rows is None else rows, max_rows, pages,
+                     lens, table, row0)
+
+    def append(self, batch: Batch, k_cache: int, v_cache: int, k: int, v: int, q: int | None = None, q_out: int | None = None,
+               x_dtype: str | None = None, x_stride: int | None = None, q_stride: int | None = None, k_stride: int | None = None,
+               v_stride: int | None = None, q_out_stride: int | None = None, bias: int | None = None, q_norm: int | None = None,
+               k_norm: int | None = None, positions: int | None = None, stream: int | None = None):
+        """New rows into the cache; the turned queries go to q_out. x_dtype None: the cache's. x_stride: the row stride of q, k and
+        v, where one is not given; without either, rows are contiguous."""
+        qw, kw = self.heads * self.head_dim, self.kv_heads * self.head_dim
+
+        def pick(stride, width):
+            return stride if stride is not None else x_stride if x_stride is not None else width
+        x = _Rows(q, k, v, q_out, pick(q_stride, qw), pick(k_stride, kw), pick(v_stride, kw), qw if q_out_stride is None else q_out_stride,
+                  bias, q_norm, k_norm, positions, _dtype(x_dtype or self.dtype), 0)
+        self._check(self.lib.ill_paged_append(self.h, C.byref(batch), C.byref(x), k_cache, v_cache, stream))
+
+    def attend(self, batch: Batch, k_cache: int, v_cache: int, q: int, out: int, out_dtype: str | None = None, window: int = 0, sinks: int = 0,
+               q_stride: int | None = None, out_stride: int | None = None, stream: int | None = None):
+        """Attention of the new rows over the cache, all earlier positions or the last `window` and the first `sinks`."""
+        w = self.heads * self.head_dim
+        self._check(self.lib.ill_paged_attend(self.h, C.byref(batch), q, w if q_stride is None else q_stride, k_cache, v_cache, window, sinks,
+                                              out, w if out_stride is None else out_stride, _dtype(out_dtype or self.dtype), stream))
+
+    def close(self):
+        if getattr(self, "h", None):
+            self.lib.ill_paged_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()

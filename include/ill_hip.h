@@ -291,17 +291,25 @@ ILL_API int ill_gemv_destroy(ill_gemv* g);
  * 0: none) by position * rope_base^(-2 i / rotary_dim), pairing dim i with i + rotary_dim / 2, or
  * with interleaved != 0 dims 2 i and 2 i + 1. norm_eps belongs to the head norms; scale
  * multiplies the scores (0: 1 / sqrt(head_dim)). A handle belongs to the GPU that was current
- * when it was created; one thread at a time calls on it. */
+ * when it was created; one thread at a time calls on it.
+ * Attention that is split over the keys joins its parts through a workspace that the handle
+ * holds, one for each stream that calls come on and one for each capture of a stream, `streams`
+ * of them (0: 8; about 9 MB each): calls on different streams, and graphs, may run at the same
+ * time. What is enqueued on one stream, or captured on one stream in one capture, shares a
+ * workspace: such a graph is instantiated once. A call that would need one more is refused;
+ * ill_paged_release, called when nothing that the handle has enqueued or captured will run any
+ * more, makes all of them free again. */
 enum { ILL_F32 = 0, ILL_F16 = 1, ILL_BF16 = 2 };
 typedef struct ill_paged ill_paged;
 typedef struct {
-  int32_t dtype, heads, kv_heads, head_dim, page_size, rotary_dim, interleaved, reserved;
+  int32_t dtype, heads, kv_heads, head_dim, page_size, rotary_dim, interleaved, streams;
   int64_t page_stride, slot_stride, head_stride;
   double rope_base;
   float norm_eps, scale;
 } ill_paged_desc;
 ILL_API int ill_paged_create(const ill_paged_desc* desc, ill_paged** out);
 ILL_API int ill_paged_destroy(ill_paged* p);
+ILL_API int ill_paged_release(ill_paged* p);
 
 /* A batch. lens, table and row0 are device arrays that the kernels read when they run, so a
  * captured call follows what they then hold. lens [seqs]: the positions of each sequence, its

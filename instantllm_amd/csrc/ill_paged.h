@@ -42,12 +42,6 @@ template <int T>
 __device__ __forceinline__ uint4 pg_pack8(const float* x) {
   return {pg_pack2<T>(x[0], x[1]), pg_pack2<T>(x[2], x[3]), pg_pack2<T>(x[4], x[5]), pg_pack2<T>(x[6], x[7])};
 }
-template <int T>
-__device__ __forceinline__ float pg_one(const uint16_t* p) {
-  const uint16_t w = gld(p);
-  return T == PG_BF16 ? __uint_as_float((uint32_t)w << 16) : (float)__builtin_bit_cast(_Float16, w);
-}
-
 // ---- new rows into the cache -------------------------------------------------------------
 struct PgAppend {
   PgBatch b;
@@ -73,6 +67,11 @@ __device__ __forceinline__ int pg_seq_of(const PgBatch& b, int r, int lane) {
   return below - 1;
 }
 
+__device__ __forceinline__ PgSeq pg_seq_at(const PgBatch& b, int s) {
+  const int begin = b.row0 ? gld(b.row0 + s) : s, end = b.row0 ? gld(b.row0 + s + 1) : s + 1;
+  return pg_seq(begin, end, gld(b.lens + s), b.rows);
+}
+
 // A workgroup takes R rows; a thread takes 16 values of one head at a time: the eight first and the
 // eight second halves of eight rotated pairs (or eight whole pairs twice where pairs are
 // interleaved), so that a pair never leaves its thread and a head's square sum stays within D / 16
@@ -93,8 +92,8 @@ __global__ __launch_bounds__(256) void pg_append_kernel(PgAppend a, int R) {
     int at = 0;
     const int s = r >= a.b.rows ? -1 : a.b.row0 ? pg_seq_of(a.b, r, lane) : r;
     if (s >= 0 && s < a.b.seqs) {
-      const int len = pg_len(gld(a.b.lens + s));
-      const int t = a.b.row0 ? len - (gld(a.b.row0 + s + 1) - r) : len - 1;
+      const PgSeq q = pg_seq_at(a.b, s);
+      const int t = q.p0 + (r - q.first);
       at = a.positions ? gld(a.positions + r) : t;
       if (t >= 0 && t < pg_cap(a.b)) {
         const int page = gld(a.b.table + s * a.b.table_stride + (t >> a.b.page_log));
@@ -202,52 +201,465 @@ struct PgAttend {
   float scale;
 };
 
-// One wave per new row and query head: 64 positions at a time, a lane's score each, then the
-// running softmax and the values, a lane's D / 64 dims each.
-template <int TC, int D>
-__global__ __launch_bounds__(64) void pg_attend_simple_kernel(PgAttend a) {
-  const int r = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-  const int s = a.b.row0 ? pg_seq_of(a.b, r, lane) : r;
-  if (s < 0 || s >= a.b.seqs) return;
-  const int len = pg_len(gld(a.b.lens + s));
-  const int p = a.b.row0 ? len - (gld(a.b.row0 + s + 1) - r) : len - 1;
-  __shared__ float q[D];
-  for (int d = lane; d < D; d += 64) q[d] = pg_one<TC>(a.q + r * a.qs + (int64_t)h * D + d);
-  __syncthreads();
-  const int64_t hoff = (int64_t)(h / (a.heads / a.kv)) * a.head_stride;
-  const int mask = (1 << a.b.page_log) - 1;
-  float m = -INFINITY, l = 0.f, o[D / 64] = {};
-  const int end = min(p + 1, pg_cap(a.b));
-  for (int j0 = 0; j0 < end; j0 += 64) {
-    const int j = j0 + lane;
-    const int page = j < end ? gld(a.b.table + s * a.b.table_stride + (j >> a.b.page_log)) : -1;
-    const bool on = pg_sees(p, j, a.window, a.sinks) && page >= 0 && page < a.b.pages;
-    const int64_t off = on ? page * a.page_stride + (j & mask) * a.slot_stride + hoff : 0;
-    float sc = -INFINITY;
-    if (on) {
-      float x = 0.f;
-      for (int d = 0; d < D; d++) x = fmaf(q[d], pg_one<TC>(a.kc + off + d), x);
-      sc = x * a.scale;
+// What the unit of work u is: a part of the keys for a tile of rows of one key/value head.
+struct PgUnit {
+  int s, head, q, split, splits, part_at, tile_at;   // part_at, tile_at: its places in the workspace, if it is one of several parts
+  PgSeq seq;
+};
+
+// Every wave finds its unit by itself: the sequences' numbers of units, 64 at a time, a lane each.
+struct PgFinder {
+  const PgBatch& b;
+  const PgCut& c;
+  int part, units;   // tiles of keys in a part; units of work in all
+  __device__ __forceinline__ int of(int s, PgSeq& q, int& most) const {   // tiles of rows x heads of sequence s
+    q = {0, 0, 0};
+    most = 0;
+    if (s >= b.seqs) return 0;
+    q = pg_seq_at(b, s);
+    most = pg_most(q.p0 + q.n, pg_cap(b), c);
+    return pg_qtiles(q.n, c) * c.kv;
+  }
+  __device__ __forceinline__ PgFinder(const PgBatch& b_, const PgCut& c_) : b(b_), c(c_) {
+    const int lane = threadIdx.x & 63;
+    int64_t tiles = 0, work = 0;
+    PgSeq q;
+    int most;
+    for (int s0 = 0; s0 < b.seqs; s0 += 64) {
+      const int n = of(s0 + lane, q, most);
+      tiles += n;
+      work += (int64_t)n * most;
     }
-    float mn = fmaxf(m, sc);
-    for (int k = 1; k < 64; k <<= 1) mn = fmaxf(mn, __shfl_xor(mn, k));
-    if (mn == -INFINITY) continue;
-    const float up = expf(m - mn), e = on ? expf(sc - mn) : 0.f;
-    m = mn;
-    l = l * up + e;
-    for (int u = 0; u < D / 64; u++) o[u] *= up;
-    for (uint64_t left = __ballot(on); left; left &= left - 1) {
-      const int k = __ffsll((unsigned long long)left) - 1;
-      const int64_t ok = __shfl(off, k);
-      const float ek = __shfl(e, k);
-      for (int u = 0; u < D / 64; u++) o[u] = fmaf(ek, pg_one<TC>(a.vc + ok + lane + 64 * u), o[u]);
+    if (b.seqs == 1) {
+      tiles = __shfl(tiles, 0);
+      work = __shfl(work, 0);
+    } else {
+#pragma unroll
+      for (int m = 1; m < 64; m <<= 1) {
+        tiles += __shfl_xor(tiles, m);
+        work += __shfl_xor(work, m);
+      }
+    }
+    part = pg_part(tiles, work, c);
+    units = 0;
+    for (int s0 = 0; s0 < b.seqs; s0 += 64) {
+      const int n = of(s0 + lane, q, most);
+      int u = n * pg_splits(most, part);
+#pragma unroll
+      for (int m = 1; m < 64; m <<= 1) u += __shfl_xor(u, m);
+      units += u;
     }
   }
-  for (int k = 1; k < 64; k <<= 1) l += __shfl_xor(l, k);
-  for (int u = 0; u < D / 64; u++) {
-    const float y = m == -INFINITY ? 0.f : o[u] / l;
-    const int64_t at = r * a.os + (int64_t)h * D + lane + 64 * u;
-    if (a.out_f32) gst((float*)a.out + at, y);
-    else gst((uint16_t*)a.out + at, (uint16_t)pg_pack2<TC>(y, 0.f));
+  __device__ __forceinline__ PgUnit find(int u) const {
+    const int lane = threadIdx.x & 63;
+    int parts = 0, tiles = 0;
+    for (int s0 = 0;; s0 += 64) {
+      PgSeq q;
+      int most;
+      const int n = of(s0 + lane, q, most), splits = pg_splits(most, part);
+      int3 sum = {n * splits, splits > 1 ? n * splits : 0, splits > 1 ? n : 0}, own = sum;
+#pragma unroll
+      for (int m = 1; m < 64; m <<= 1) {
+        const int x = __shfl_up(sum.x, m), y = __shfl_up(sum.y, m), z = __shfl_up(sum.z, m);
+        if (lane >= m) {
+          sum.x += x;
+          sum.y += y;
+          sum.z += z;
+        }
+      }
+      const int all = __builtin_amdgcn_readlane(sum.x, 63);
+      if (u >= all) {   // (u < units, so a later 64 have it; the bound ends the search also where lengths change meanwhile)
+        if (s0 + 64 >= b.seqs) return {0, 0, 0, 0, 1, 0, 0, {0, 0, 0}};
+        u -= all;
+        parts += __builtin_amdgcn_readlane(sum.y, 63);
+        tiles += __builtin_amdgcn_readlane(sum.z, 63);
+        continue;
+      }
+      const int at = __ffsll((unsigned long long)__ballot(sum.x > u)) - 1;
+      auto lane_of = [&](int v) { return __builtin_amdgcn_readlane(v, at); };
+      PgUnit r;
+      r.s = s0 + at;
+      r.splits = lane_of(splits);
+      r.seq = {lane_of(q.first), lane_of(q.n), lane_of(q.p0)};
+      u -= lane_of(sum.x - own.x);
+      // the heads in turn, so that the workgroups of an XCD (every eighth) read few heads; of a head, the
+      // parts of its last rows first, which have the most keys
+      const int qt = lane_of(n) / c.kv;
+      r.head = u % c.kv;
+      const int v = u / c.kv;
+      r.split = v % r.splits;
+      r.q = qt - 1 - v / r.splits;
+      r.tile_at = tiles + lane_of(sum.z - own.z) + (r.head * qt + r.q);
+      r.part_at = parts + lane_of(sum.y - own.y) + (r.head * qt + r.q) * r.splits;
+      return r;
+    }
+  }
+};
+
+template <int TC>
+__device__ __forceinline__ v4f pg_mfma16(uint4 a, uint4 b, v4f c) {   // 16 x 16 x 32
+  if constexpr (TC == PG_BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+}
+
+// 16 bytes from each lane's address into LDS, lane i's at lds + 16 i. In inline assembly, because the
+// compiler cannot tell the buffers apart and would wait for every load in flight before each LDS read;
+// the kernels wait themselves (PG_WAIT), and extra loads of the compiler's own only make that wait longer.
+__device__ __forceinline__ void pg_dma16(const void* g, const void* lds) {
+  const uint32_t m = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)lds);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(m), "v"(g) : "memory");
+}
+#define PG_WAIT(n) asm volatile("s_waitcnt vmcnt(" #n ")" ::: "memory")
+#define PG_WAIT_LDS() asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory")
+
+// Where the 16-byte unit u of key `key` of a tile lies in LDS, in units: a key's units in a row, permuted so
+// that the eight keys of an operand read, and the four keys by 32 bytes of four transposed reads, are on
+// different banks.
+template <int D>
+__device__ __forceinline__ int pg_swz(int key) {
+  return D == 64 ? ((key >> 4) & 1) | (key & 2) | ((key >> 1) & 4) : ((key >> 4) & 1) | ((key & 3) << 1) | (key & 8);
+}
+template <int D>
+__device__ __forceinline__ int pg_unit_at(int key, int u) { return key * (D / 8) + (u ^ pg_swz<D>(key)); }
+
+// Four keys (key, .., key + 3) of dim 16 nb + lane % 16, from the rows of a tile of values: each 16 lanes read
+// 4 keys x 16 dims, and the transposing read hands lane i its dim.
+__device__ __forceinline__ uint2 pg_tr(const void* p) {
+  typedef short v4s __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)p));
+}
+template <int D>
+__device__ __forceinline__ uint4 pg_values(const uint4* v, int key, int nb, int i) {   // keys key .. key + 7
+  const int u = 2 * nb + ((i >> 1) & 1), k0 = key + (i >> 2), k1 = k0 + 4;
+  const uint2 a = pg_tr((const uint8_t*)(v + pg_unit_at<D>(k0, u)) + 8 * (i & 1)), b = pg_tr((const uint8_t*)(v + pg_unit_at<D>(k1, u)) + 8 * (i & 1));
+  return {a.x, a.y, b.x, b.y};
+}
+
+// Infinities and NaN of eight values: whether there are any; the values with zeros in their place; and marks
+// that a product with ones for the keys a row sees adds up (1 for inf, 64 for -inf, 4096 for NaN; 32 keys).
+template <int TC>
+__device__ __forceinline__ bool pg_wild(uint4 v) {
+  constexpr uint32_t E = TC == PG_BF16 ? 0x7F80u : 0x7C00u;
+  bool w = false;
+  for (const uint32_t x : {v.x, v.y, v.z, v.w}) w = w || (x & E) == E || (x >> 16 & E) == E;
+  return w;
+}
+template <int TC>
+__device__ __forceinline__ uint4 pg_tamed(uint4 v, uint4& marks) {
+  constexpr uint32_t E = TC == PG_BF16 ? 0x7F80u : 0x7C00u, S = TC == PG_BF16 ? 0x007Fu : 0x03FFu;
+  constexpr uint32_t ONE = TC == PG_BF16 ? 0x3F80u : 0x3C00u, STEP = TC == PG_BF16 ? 0x0300u : 0x1800u;   // 1, and a factor of 64
+  uint32_t y[4] = {v.x, v.y, v.z, v.w}, k[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    k[i] = 0;
+#pragma unroll
+    for (int h = 0; h < 32; h += 16) {
+      const uint32_t x = y[i] >> h & 0xFFFFu;
+      if ((x & E) == E) {
+        k[i] |= ((x & S) ? ONE + 2 * STEP : x >> 15 ? ONE + STEP : ONE) << h;
+        y[i] &= ~(0xFFFFu << h);
+      }
+    }
+  }
+  marks = {k[0], k[1], k[2], k[3]};
+  return {y[0], y[1], y[2], y[3]};
+}
+__device__ __forceinline__ float pg_wild_sum(float marks) {
+  const int n = (int)marks;
+  float y = n & 63 ? INFINITY : 0.f;
+  if (n >> 6 & 63) y -= INFINITY;
+  return n >> 12 ? NAN : y;
+}
+
+// The exponents' reference of a row follows its greatest score, PG_UP below it, and is moved only when a score
+// passes it by more than PG_UP + PG_SLACK: weights then stay below 2^15, in f16's range, and their rounding
+// keeps its 11 bits down to 2^-24 of the greatest one.
+#define PG_UP 10.f
+#define PG_SLACK 5.f
+
+struct PgWork {        // a call's share of the handle's workspace
+  float2* ml;          // [2 target][M] reference and sum of a part's rows
+  float* o;            // [2 target][M][D] its weighted values
+  int32_t* joined;     // [target] parts of a tile of rows that are done; 0 between calls
+};
+
+// Four dims of a row's output.
+template <int TC>
+__device__ __forceinline__ void pg_store(const PgAttend& a, int row, int head, int d, int D, v4f y) {
+  const int64_t at = row * a.os + (int64_t)head * D + d;
+  if (a.out_f32) gst((gu32x4*)((float*)a.out + at), __builtin_bit_cast(gu32x4, y));
+  else gst((gu32x2*)((uint16_t*)a.out + at), (gu32x2){pg_pack2<TC>(y[0], y[1]), pg_pack2<TC>(y[2], y[3])});
+}
+
+// The parts of a tile of rows, joined in their order by one workgroup of 256 threads. wt: LDS for their weights
+// (PG_MAXSPLIT x M floats).
+template <int TC, int D, int M, class P>
+__device__ __forceinline__ void pg_join(const P& p, const PgUnit& un, int f0, int live, float* wt) {
+  const int tid = threadIdx.x;
+  const float2* ml = p.w.ml + (size_t)un.part_at * M;
+  __syncthreads();
+  for (int r = tid; r < live; r += 256) {
+    float m = -INFINITY, l = 0.f;
+    for (int x = 0; x < un.splits; x++) m = fmaxf(m, gld(ml + (size_t)x * M + r).x);
+    for (int x = 0; x < un.splits; x++) {
+      const float2 v = gld(ml + (size_t)x * M + r);
+      const float e = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(v.x - m);
+      wt[x * M + r] = e;
+      l += v.y * e;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    for (int x = 0; x < un.splits; x++) wt[x * M + r] *= inv;
+  }
+  __syncthreads();
+  for (int i = tid; i < live * (D / 4); i += 256) {
+    const int r = i / (D / 4), d = 4 * (i % (D / 4));
+    const float* o = p.w.o + ((size_t)un.part_at * M + r) * D + d;
+    v4f y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int x = 0; x < un.splits; x++) {
+      const float e = wt[x * M + r];
+      const v4f v = __builtin_bit_cast(v4f, gld((const uint4*)(o + (size_t)x * M * D)));
+      if (e != 0.f) y += v * e;
+    }
+    pg_store<TC>(p.a, un.seq.first + (f0 + r) / p.c.G, un.head * p.c.G + (f0 + r) % p.c.G, d, D, y);
+  }
+}
+
+struct PgStep {
+  PgAttend a;
+  PgCut c;
+  PgWork w;
+};
+
+// Attention of few rows per sequence. A workgroup of four waves takes a part of the keys for 16 flat rows of a
+// key/value head, and each wave every fourth tile of keys of it: 8 KB of keys and 8 KB of values at a time go
+// straight into the wave's own LDS, so that the waves never wait for each other; the next tile's keys start
+// as soon as this one's have been read, its values after this one's. Scores are keys x rows and outputs dims
+// x rows (v_mfma 16 x 16 x 32), so a row's statistics are its lanes' own, and the keys are dealt to the score
+// products' rows such that a lane's weights are the next product's operand as they stand (block b, row 4 g
+// + r: key 32 (b / 2) + 8 g + 4 (b % 2) + r). Values are transposed by the LDS read. The waves' states are
+// joined in LDS; a tile of rows whose keys are in several parts is joined by the workgroup that ends last, in
+// the parts' order.
+template <int TC, int D, bool FINE>   // FINE: weights in two parts (float32 outputs)
+__global__ __launch_bounds__(256, 2) void pg_step_kernel(PgStep p) {
+  constexpr int KT = D == 64 ? 64 : 32, UPR = D / 8, KPI = 64 / UPR, NB = KT / 16, KS = D / 32, ND = D / 16, NS = KT / 32, NG = KT / 16;
+  constexpr int RF = D + 4;   // floats between the rows of a state in LDS
+  __shared__ __attribute__((aligned(16))) uint4 lds[4][1024];
+  __shared__ float smx[4][16], sls[4][16];
+  __shared__ int last;
+  const PgAttend& a = p.a;
+  const PgCut& c = p.c;
+  const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, n = lane & 15, kg = lane >> 4;
+  const int cap = pg_cap(a.b), pmask = (1 << a.b.page_log) - 1;
+  uint4* kl = lds[w];
+  uint4* vl = lds[w] + 512;
+  const float sc2 = a.scale * 1.4426950408889634f;
+  const PgFinder finder(a.b, c);
+  auto over_kg = [](float v, auto op) {   // over the lanes of the same row
+    const auto x = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
+    v = op(__int_as_float((int)x[0]), __int_as_float((int)x[1]));
+    const auto y = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
+    return op(__int_as_float((int)y[0]), __int_as_float((int)y[1]));
+  };
+  int64_t row_off[16 / KPI];   // this lane's key of each group of KPI within 16
+#pragma unroll
+  for (int i = 0; i < 16 / KPI; i++) row_off[i] = (KPI * i + lane / UPR) * a.slot_stride;
+  for (int u = blockIdx.x; u < finder.units; u += gridDim.x) {
+    const PgUnit un = finder.find(u);
+    if (un.seq.n == 0) continue;
+    const int flat = un.seq.n * c.G, f0 = 16 * un.q, live = min(16, flat - f0);   // (n G is at most 2^30)
+    const int f = min(f0 + n, flat - 1), row = un.seq.first + f / c.G, head = un.head * c.G + f % c.G;
+    const int pos = un.seq.p0 + f / c.G, p0 = un.seq.p0 + f0 / c.G, p1 = un.seq.p0 + (f0 + live - 1) / c.G;
+    const PgRange range = pg_range(p0, p1, cap, c);
+    const int per = pg_up(range.n, un.splits), c0 = min(un.split * per, range.n), c1 = min(c0 + per, range.n);
+    const int end = min(p1 + 1, cap);
+    uint4 qf[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) qf[ks] = gld((const uint4*)(a.q + row * a.qs + (int64_t)head * D + 32 * ks + 8 * kg));
+    const int mine = c0 + w < c1 ? (c1 - c0 - w + 3) / 4 : 0;   // this wave's tiles
+    // pages of the wave's next 64 / NG tiles, 16 positions a lane; -1: not to be followed
+    int page = -1;
+    auto pages = [&](int k) {
+      const int t = c0 + w + 4 * (k + lane / NG);
+      page = -1;
+      if (t < c1) {
+        const int key = min(pg_key_tile(range, t) * KT + 16 * (lane % NG), end - 1);
+        page = gld(a.b.table + un.s * a.b.table_stride + (key >> a.b.page_log));
+        if (page < 0 || page >= a.b.pages) page = -1;
+      }
+    };
+    auto load = [&](const uint16_t* from, uint4* to, int k) {
+      const int kt = pg_key_tile(range, c0 + w + 4 * k) * KT;
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const int g = i * KPI / 16, key = KPI * i + lane / UPR;
+        const int pg = max(__builtin_amdgcn_readlane(page, (k * NG + g) & 63), 0);   // (page 0 is there, and masked)
+        const int64_t at = pg * a.page_stride + ((kt + 16 * g) & pmask) * a.slot_stride + un.head * a.head_stride;
+        pg_dma16(from + at + row_off[i % (16 / KPI)] + 8 * ((lane % UPR) ^ pg_swz<D>(key)), to + 64 * i);
+      }
+    };
+    float Mx = -INFINITY, Ls = 0.f;   // Ls: this lane's keys only
+    v4f O[ND];
+#pragma unroll
+    for (int d = 0; d < ND; d++) O[d] = (v4f){0.f, 0.f, 0.f, 0.f};
+    if (mine > 0) {
+      pages(0);
+      load(a.kc, kl, 0);
+      load(a.vc, vl, 0);
+    }
+    for (int k = 0; k < mine; k++) {
+      const int kt = pg_key_tile(range, c0 + w + 4 * k) * KT;
+      const bool more = k + 1 < mine;
+      int good = 0;   // groups of 16 keys whose pages are there
+#pragma unroll
+      for (int g = 0; g < NG; g++) good |= (__builtin_amdgcn_readlane(page, (k * NG + g) & 63) >= 0) << g;
+      PG_WAIT(8);   // the keys; the 8 loads after them are the values
+      v4f s[NB];
+#pragma unroll
+      for (int b = 0; b < NB; b++) {
+        const int key = 32 * (b >> 1) + 8 * (n >> 2) + 4 * (b & 1) + (n & 3);
+        s[b] = (v4f){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) s[b] = pg_mfma16<TC>(kl[pg_unit_at<D>(key, 4 * ks + kg)], qf[ks], s[b]);
+      }
+      PG_WAIT_LDS();   // the keys have been read
+      if (more) {
+        if (((k + 1) & (64 / NG - 1)) == 0) pages(k + 1);
+        load(a.kc, kl, k + 1);
+      }
+      // every row sees the whole tile, or the rows' masks (wave-uniform)
+      const bool whole = good == (1 << NG) - 1 && kt + KT - 1 <= p0 && kt + KT <= end && (c.window == 0 || kt > p1 - c.window || kt + KT <= c.sinks);
+      uint32_t seen = ~0u;
+      if (!whole) {
+        seen = 0;
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            const int key = 32 * (b >> 1) + 8 * kg + 4 * (b & 1) + r, j = kt + key;
+            const bool on = j < cap && pg_sees(pos, j, c.window, c.sinks) && (good >> (key >> 4) & 1);
+            if (!on) s[b][r] = -INFINITY;
+            seen |= (uint32_t)on << (4 * b + r);
+          }
+      }
+      float mc = s[0][0];
+#pragma unroll
+      for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) mc = fmaxf(mc, s[b][r]);
+      mc *= sc2;
+      if (__any(mc > Mx + (PG_UP + PG_SLACK))) {
+        mc = over_kg(mc, OpMaxF{});
+        const float mn = mc == -INFINITY ? Mx : fmaxf(mc - PG_UP, Mx), up = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(Mx - mn);
+        Mx = mn;
+        Ls *= up;
+#pragma unroll
+        for (int d = 0; d < ND; d++) O[d] *= up;
+      }
+      const float ref = Mx == -INFINITY ? 0.f : Mx;
+      uint4 ph[NS], pl[NS];
+#pragma unroll
+      for (int b = 0; b < NB; b++) {
+        float e[4], h[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          e[r] = __builtin_amdgcn_exp2f(fmaf(s[b][r], sc2, -ref));
+          Ls += e[r];
+        }
+        const uint32_t x = pg_pack2<TC>(e[0], e[1]), y = pg_pack2<TC>(e[2], e[3]);
+        (&ph[b >> 1].x)[2 * (b & 1)] = x;
+        (&ph[b >> 1].x)[2 * (b & 1) + 1] = y;
+        if constexpr (FINE) {
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            const uint16_t z = (uint16_t)((r < 2 ? x : y) >> (16 * (r & 1)));
+            h[r] = TC == PG_BF16 ? __uint_as_float((uint32_t)z << 16) : (float)__builtin_bit_cast(_Float16, z);
+          }
+          (&pl[b >> 1].x)[2 * (b & 1)] = pg_pack2<TC>(e[0] - h[0], e[1] - h[1]);
+          (&pl[b >> 1].x)[2 * (b & 1) + 1] = pg_pack2<TC>(e[2] - h[2], e[3] - h[3]);
+        }
+      }
+      if (more) PG_WAIT(8);   // the values; the 8 loads after them are the next keys
+      else PG_WAIT(0);
+      bool wild = false;
+      if (!whole) {   // what a row does not see must not reach it as 0 x inf
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+          for (int t = 0; t < NS; t++) wild = wild || pg_wild<TC>(pg_values<D>(vl, 32 * t + 8 * kg, d, n));
+        wild = __any(wild);
+      }
+      if (!wild) {
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+          for (int t = 0; t < NS; t++) {
+            const uint4 v = pg_values<D>(vl, 32 * t + 8 * kg, d, n);
+            O[d] = pg_mfma16<TC>(v, ph[t], O[d]);
+            if constexpr (FINE) O[d] = pg_mfma16<TC>(v, pl[t], O[d]);
+          }
+      } else {
+        constexpr uint32_t ONE = TC == PG_BF16 ? 0x3F80u : 0x3C00u;
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+          for (int t = 0; t < NS; t++) {
+            uint4 marks, ones;
+            const uint4 v = pg_tamed<TC>(pg_values<D>(vl, 32 * t + 8 * kg, d, n), marks);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+              (&ones.x)[i] = (seen >> (8 * t + 2 * i) & 1 ? ONE : 0u) | (seen >> (8 * t + 2 * i + 1) & 1 ? ONE << 16 : 0u);
+            O[d] = pg_mfma16<TC>(v, ph[t], O[d]);
+            if constexpr (FINE) O[d] = pg_mfma16<TC>(v, pl[t], O[d]);
+            const v4f m = pg_mfma16<TC>(marks, ones, (v4f){0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+            for (int r = 0; r < 4; r++) O[d][r] += pg_wild_sum(m[r]);
+          }
+      }
+      PG_WAIT_LDS();   // the values have been read
+      if (more) load(a.vc, vl, k + 1);
+    }
+    // the waves' states, each in its own LDS
+    Ls = over_kg(Ls, OpAddF{});
+    float* st = (float*)lds[w];
+#pragma unroll
+    for (int d = 0; d < ND; d++) *(v4f*)(st + n * RF + 16 * d + 4 * kg) = O[d];
+    if (kg == 0) {
+      smx[w][n] = Mx;
+      sls[w][n] = Ls;
+    }
+    __syncthreads();
+    for (int i = tid; i < live * (D / 4); i += 256) {
+      const int r = i / (D / 4), d = 4 * (i % (D / 4));
+      float m = smx[0][r];
+#pragma unroll
+      for (int x = 1; x < 4; x++) m = fmaxf(m, smx[x][r]);
+      float l = 0.f;
+      v4f o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int x = 0; x < 4; x++) {
+        const float e = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(smx[x][r] - m);
+        l += sls[x][r] * e;
+        if (e != 0.f) o += *(const v4f*)((const float*)lds[x] + r * RF + d) * e;
+      }
+      if (un.splits == 1) {
+        pg_store<TC>(a, un.seq.first + (f0 + r) / c.G, un.head * c.G + (f0 + r) % c.G, d, D, l == 0.f ? (v4f){0.f, 0.f, 0.f, 0.f} : o / l);
+      } else {
+        if (d == 0) gst((gu32x2*)(p.w.ml + (size_t)(un.part_at + un.split) * 16 + r), (gu32x2){__float_as_uint(m), __float_as_uint(l)});
+        gst((gu32x4*)(p.w.o + ((size_t)(un.part_at + un.split) * 16 + r) * D + d), __builtin_bit_cast(gu32x4, o));
+      }
+    }
+    if (un.splits > 1) {
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) last = atomicAdd(p.w.joined + un.tile_at, 1) == un.splits - 1;
+      __syncthreads();
+      if (last) {
+        __threadfence();
+        pg_join<TC, D, 16>(p, un, f0, live, (float*)lds);
+        if (tid == 0) atomicExch(p.w.joined + un.tile_at, 0);
+      }
+    }
+    __syncthreads();   // LDS is the next unit's
   }
 }

@@ -44,6 +44,8 @@ inline int check_desc(ill_paged_desc& d) {
   if (!(d.norm_eps >= 0 && std::isfinite(d.norm_eps))) return fail(ILL_E_ARG, "paged: norm_eps %g", d.norm_eps);
   if (d.scale == 0) d.scale = (float)(1 / std::sqrt((double)d.head_dim));
   if (!(d.scale > 0 && std::isfinite(d.scale))) return fail(ILL_E_ARG, "paged: scale %g", d.scale);
+  if (d.streams == 0) d.streams = 8;
+  if (d.streams < 1 || d.streams > 256) return fail(ILL_E_ARG, "paged: %d streams (up to 256)", d.streams);
   if (!d.page_stride && !d.slot_stride && !d.head_stride) {
     d.head_stride = d.head_dim;
     d.slot_stride = (int64_t)d.kv_heads * d.head_dim;

@@ -8,6 +8,15 @@ struct ill_paged {
   ill_paged_desc d{};
   int device = 0, page_log = 0;
   double* freq = nullptr;   // [rotary_dim / 2] turns per position
+  // Workspaces of attention parts: one for each stream, and for each capture of a stream, that calls have come on. What
+  // runs on one stream, or in one captured graph's branch, is in order; two of them never share a workspace.
+  uint8_t* work = nullptr;
+  size_t work_bytes = 0;
+  struct Claim {
+    hipStream_t stream;
+    unsigned long long capture;   // 0: not captured
+  };
+  std::vector<Claim> claims;
 };
 
 namespace illp {
@@ -29,6 +38,52 @@ PgBatch batch_of(const ill_paged* p, const ill_paged_batch& b) {
   return {b.lens, b.table, b.row0, b.table_stride, b.pages, b.seqs, (int)b.rows, b.table_width, p->page_log};
 }
 
+// Parts of a call of few rows per sequence: two workgroups per CU, and no part below four tiles of keys, one for each wave.
+constexpr int kStepTarget = 512, kStepLeast = 4;
+
+PgCut step_cut(const ill_paged_desc& d, int window, int sinks) {
+  return {d.heads / d.kv_heads, d.kv_heads, 16, d.head_dim == 64 ? 64 : 32, window, sinks, kStepTarget, kStepLeast, INT32_MAX, 0, INT32_MAX};
+}
+
+// Bytes of a workspace of `target` parts wanted over tiles of M rows.
+size_t work_size(int target, int M, int D) { return (size_t)2 * target * M * (D + 2) * 4 + al256((size_t)target * 4); }
+
+PgWork work_of(uint8_t* at, int target, int M, int D) {
+  PgWork w;
+  w.joined = (int32_t*)at;
+  w.o = (float*)(at + al256((size_t)target * 4));
+  w.ml = (float2*)(w.o + (size_t)2 * target * M * D);
+  return w;
+}
+
+// The workspace of the stream, or of its capture.
+int workspace(ill_paged* p, hipStream_t st, uint8_t** out) {
+  if (st == hipStreamPerThread) return fail(ILL_E_ARG, "paged: the per-thread default stream is several streams; pass a stream of your own");
+  unsigned long long id = 0;
+  if (st && st != hipStreamLegacy) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    HCK(hipStreamGetCaptureInfo(st, &status, &id));
+    if (status == hipStreamCaptureStatusNone) id = 0;
+  } else {
+    st = nullptr;
+  }
+  size_t i = 0;
+  while (i < p->claims.size() && !(p->claims[i].stream == st && p->claims[i].capture == id)) i++;
+  if (i == p->claims.size()) {
+    if ((int)i == p->d.streams)
+      return fail(ILL_E_ARG, "paged: calls have come on %d streams and captures, as many as the handle has workspaces for (ill_paged_release)", (int)i);
+    p->claims.push_back({st, id});
+  }
+  *out = p->work + i * p->work_bytes;
+  return ILL_OK;
+}
+
+template <int TC, int D>
+void launch_step(const PgStep& s, int64_t grid, hipStream_t st) {
+  if (s.a.out_f32) hipLaunchKernelGGL((pg_step_kernel<TC, D, true>), dim3(grid), dim3(256), 0, st, s);
+  else hipLaunchKernelGGL((pg_step_kernel<TC, D, false>), dim3(grid), dim3(256), 0, st, s);
+}
+
 template <int TX, int TC>
 void launch_append(const PgAppend& a, int D, int R, int lds, hipStream_t st) {
   const dim3 grid((a.b.rows + R - 1) / R);
@@ -45,6 +100,7 @@ int ill_paged_destroy(ill_paged* p) {
   {
     illp::OnDevice on(p->device);
     hipFree(p->freq);
+    hipFree(p->work);
   }
   delete p;
   return ILL_OK;
@@ -66,7 +122,22 @@ int ill_paged_create(const ill_paged_desc* desc, ill_paged** out) {
   for (int i = 0; i < d.rotary_dim / 2; i++) freq[i] = std::pow(d.rope_base, -2.0 * i / d.rotary_dim) / (2 * M_PI);
   if (hipMalloc(&p->freq, sizeof freq) != hipSuccess || hipMemcpy(p->freq, freq, sizeof freq, hipMemcpyHostToDevice) != hipSuccess)
     return bad(fail(ILL_E_HIP, "paged: buffer allocation failed"));
+  p->work_bytes = al256(illp::work_size(illp::kStepTarget, 16, d.head_dim));
+  if (hipMalloc(&p->work, p->work_bytes * d.streams) != hipSuccess || hipMemset(p->work, 0, p->work_bytes * d.streams) != hipSuccess ||
+      hipDeviceSynchronize() != hipSuccess)
+    return bad(fail(ILL_E_HIP, "paged: %d workspaces of %zu bytes cannot be allocated", d.streams, p->work_bytes));
+  try {
+    p->claims.reserve(d.streams);
+  } catch (const std::exception&) {
+    return bad(fail(ILL_E_ARG, "paged: out of host memory"));
+  }
   *out = p;
+  return ILL_OK;
+}
+
+int ill_paged_release(ill_paged* p) {
+  if (!p) return fail(ILL_E_ARG, "paged: null handle");
+  p->claims.clear();
   return ILL_OK;
 }
 
@@ -142,13 +213,20 @@ int ill_paged_attend(ill_paged* p, const ill_paged_batch* batch, const void* q, 
   illp::OnDevice on(p->device);
   if (on.rc) return on.rc;
   hipStream_t st = (hipStream_t)stream;
-  const dim3 grid(a.b.rows, d.heads);
+  PgStep s{a, illp::step_cut(d, a.window, a.sinks), {}};
+  const int cap = pg_cap(a.b);
+  const int64_t grid = std::min<int64_t>(pg_grid(a.b.seqs, a.b.rows, batch->max_rows, !a.b.row0, cap, s.c), 1 << 20);
+  if (pg_splits(pg_most(cap, cap, s.c), s.c.least) > 1) {
+    uint8_t* work = nullptr;
+    if (int rc = illp::workspace(p, st, &work)) return rc;
+    s.w = illp::work_of(work, s.c.target, s.c.M, d.head_dim);
+  }
   if (d.dtype == ILL_F16) {
-    if (d.head_dim == 64) hipLaunchKernelGGL((pg_attend_simple_kernel<PG_F16, 64>), grid, dim3(64), 0, st, a);
-    else hipLaunchKernelGGL((pg_attend_simple_kernel<PG_F16, 128>), grid, dim3(64), 0, st, a);
+    if (d.head_dim == 64) illp::launch_step<PG_F16, 64>(s, grid, st);
+    else illp::launch_step<PG_F16, 128>(s, grid, st);
   } else {
-    if (d.head_dim == 64) hipLaunchKernelGGL((pg_attend_simple_kernel<PG_BF16, 64>), grid, dim3(64), 0, st, a);
-    else hipLaunchKernelGGL((pg_attend_simple_kernel<PG_BF16, 128>), grid, dim3(64), 0, st, a);
+    if (d.head_dim == 64) illp::launch_step<PG_BF16, 64>(s, grid, st);
+    else illp::launch_step<PG_BF16, 128>(s, grid, st);
   }
   HCK(hipGetLastError());
   return ILL_OK;

@@ -1,12 +1,15 @@
-// Index bounds of the paged-cache operators: plain functions of sizes, used by the host, by the
-// kernels and, compiled by themselves, by the CPU tests.
+// Work division and index bounds of the paged-cache operators: plain functions of sizes, used by
+// the host, by the kernels and, compiled by themselves, by the CPU tests.
 #pragma once
 #include <stdint.h>
-#ifndef __host__
-#define PG_FN inline
-#else
+#ifdef __HIPCC__
 #define PG_FN __host__ __device__ __forceinline__
+#else
+#define PG_FN inline
 #endif
+
+#define PG_MOST (1 << 30)    // positions, rows x heads, windows and sinks: at most this many
+#define PG_MAXSPLIT 256      // parts that the keys of a tile of rows are cut into at most
 
 // A batch as the kernels read it (ill_paged_batch with the handle's geometry).
 struct PgBatch {
@@ -17,12 +20,86 @@ struct PgBatch {
   int32_t seqs, rows, table_width, page_log;
 };
 
+PG_FN int pg_min(int a, int b) { return a < b ? a : b; }
+PG_FN int pg_max(int a, int b) { return a > b ? a : b; }
+PG_FN int pg_up(int a, int b) { return a / b + (a % b != 0); }   // a / b rounded up, a >= 0
+
 // Lengths as the kernels use them: none below 0, and none whose positions pass 2^30.
-PG_FN int pg_len(int len) { return len < 0 ? 0 : len < 1 << 30 ? len : 1 << 30; }
+PG_FN int pg_len(int len) { return pg_min(pg_max(len, 0), PG_MOST); }
 
 // Positions that a sequence's table has pages for (at most 2^30: the entry points check it); the
 // ones past them are neither written nor seen.
 PG_FN int pg_cap(const PgBatch& b) { return b.table_width << b.page_log; }
 
+// A sequence's new rows: rows first .. first + n - 1 of the buffers, at positions p0 ..; `begin` and
+// `end` are its entries of row0. Rows that the buffers do not have are left out.
+struct PgSeq {
+  int first, n, p0;
+};
+PG_FN PgSeq pg_seq(int begin, int end, int len, int rows) {
+  const int a = pg_min(pg_max(begin, 0), rows), e = pg_min(pg_max(end, a), rows);
+  const int64_t p0 = (int64_t)pg_len(len) - ((int64_t)end - a);
+  return {a, e - a, p0 < -PG_MOST ? -PG_MOST : (int)p0};
+}
+
 // Whether the row at position p sees position j.
 PG_FN bool pg_sees(int p, int j, int window, int sinks) { return j >= 0 && j <= p && (window == 0 || j > p - window || j < sinks); }
+
+// ---- the work of an attention call -------------------------------------------------------
+// A sequence's n new rows and the G query heads of a key/value head make n G flat rows (row f / G,
+// head f % G), which read the same keys; M of them are a tile of rows. Keys come in tiles of KT.
+struct PgCut {
+  int32_t G, kv, M, KT, window, sinks;
+  int32_t target;    // parts wanted in all, where there are that many
+  int32_t least;     // tiles of keys in a part at least
+  int32_t whole;     // from this many tiles of rows on, none is cut
+  int32_t lo, hi;    // sequences with lo < n G <= hi are this kernel's
+};
+
+PG_FN int pg_qtiles(int n, const PgCut& c) {
+  const int64_t f = (int64_t)n * c.G;
+  return f > c.lo && f <= c.hi ? (int)((f + c.M - 1) / c.M) : 0;
+}
+
+// Tiles of keys that rows at positions p0 .. p1 see some of: 0 .. sink - 1, and the ones from lo on, n
+// in all. Positions from `cap` on are not there.
+struct PgRange {
+  int sink, lo, n;
+};
+PG_FN PgRange pg_range(int p0, int p1, int cap, const PgCut& c) {
+  const int end = pg_min(p1 + 1, cap);
+  if (end <= 0) return {0, 0, 0};
+  const int hi = pg_up(end, c.KT);
+  const int lo = c.window ? pg_min(pg_max(p0 - c.window + 1, 0) / c.KT, hi) : 0;
+  const int sink = pg_min(pg_up(c.sinks, c.KT), lo);
+  return {sink, lo, sink + hi - lo};
+}
+PG_FN int pg_key_tile(const PgRange& r, int t) { return t < r.sink ? t : t - r.sink + r.lo; }
+
+// A bound of pg_range(..).n over the tiles of rows of a sequence with `end` positions.
+PG_FN int pg_most(int end, int cap, const PgCut& c) {
+  const int all = pg_up(pg_max(pg_min(end, cap), 0), c.KT);
+  if (!c.window) return all;
+  const int span = (c.M - 2) / c.G + 2;   // rows that M flat rows reach into
+  const int64_t some = (int64_t)pg_up(c.sinks, c.KT) + ((int64_t)c.window + span - 1 + c.KT - 2) / c.KT + 1;
+  return some < all ? (int)some : all;
+}
+
+// Tiles of keys in a part, from the sums over the sequences of qtiles x kv (`tiles`) and of qtiles x kv x
+// most (`work`). A sequence is cut into parts if its `most` is over that; the parts of all cut ones are
+// then at most 2 target (most / part + 1 <= 2 most / part each), their tiles of rows at most target.
+PG_FN int pg_part(int64_t tiles, int64_t work, const PgCut& c) {
+  if (tiles >= c.whole) return PG_MOST;
+  const int64_t p = (work + c.target - 1) / c.target;
+  return p < c.least ? c.least : p < PG_MOST ? (int)p : PG_MOST;
+}
+PG_FN int pg_splits(int most, int part) { return pg_min(pg_max(pg_up(most, part), 1), PG_MAXSPLIT); }
+
+// Workgroups that have something to do, at most, as far as the host can tell.
+PG_FN int64_t pg_grid(int seqs, int rows, int64_t max_rows, bool one_row, int cap, const PgCut& c) {
+  int64_t q = (int64_t)rows * c.G / c.M + seqs;
+  const int64_t each = one_row ? 1 : max_rows;
+  if (each > 0 && each <= PG_MOST && (each * c.G + c.M - 1) / c.M * seqs < q) q = (each * c.G + c.M - 1) / c.M * seqs;
+  const int64_t tiles = q * c.kv, cut = tiles * pg_splits(pg_most(cap, cap, c), c.least);
+  return cut < tiles + c.target ? cut : tiles + c.target;
+}

@@ -14,7 +14,7 @@ DTYPES = {"f32": 0, "f16": 1, "bf16": 2}
 
 
 class _Desc(C.Structure):
-    _fields_ = [(n, C.c_int32) for n in ("dtype", "heads", "kv_heads", "head_dim", "page_size", "rotary_dim", "interleaved", "reserved")] + \
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "heads", "kv_heads", "head_dim", "page_size", "rotary_dim", "interleaved", "streams")] + \
                [(n, C.c_int64) for n in ("page_stride", "slot_stride", "head_stride")] + \
                [("rope_base", C.c_double), ("norm_eps", C.c_float), ("scale", C.c_float)]
 
@@ -39,15 +39,15 @@ def _dtype(name: str) -> int:
 class PagedAttention:
     """A model's head geometry and cache layout. `strides`: (page, slot, head) strides of the
     caches in elements (None: [pages][page_size][kv_heads][head_dim]); `rotary_dim` None: the
-    whole head."""
+    whole head; `streams`: how many streams, and captures of streams, attention calls may come on."""
 
     def __init__(self, heads: int, kv_heads: int, head_dim: int, page_size: int = 16, dtype: str = "f16", rotary_dim: int | None = None,
                  rope_base: float = 1e6, interleaved: bool = False, norm_eps: float = 1e-6, scale: float | None = None,
-                 strides: tuple[int, int, int] | None = None):
+                 strides: tuple[int, int, int] | None = None, streams: int = 8):
         self.h = None
         self.lib = load_library()
         self.heads, self.kv_heads, self.head_dim, self.dtype = heads, kv_heads, head_dim, dtype
-        d = _Desc(_dtype(dtype), heads, kv_heads, head_dim, page_size, head_dim if rotary_dim is None else rotary_dim, int(interleaved), 0,
+        d = _Desc(_dtype(dtype), heads, kv_heads, head_dim, page_size, head_dim if rotary_dim is None else rotary_dim, int(interleaved), streams,
                   *(strides or (0, 0, 0)), rope_base, norm_eps, scale or 0.0)
         h = C.c_void_p()
         self._check(self.lib.ill_paged_create(C.byref(d), C.byref(h)))
@@ -83,6 +83,10 @@ class PagedAttention:
         w = self.heads * self.head_dim
         self._check(self.lib.ill_paged_attend(self.h, C.byref(batch), q, w if q_stride is None else q_stride, k_cache, v_cache, window, sinks,
                                               out, w if out_stride is None else out_stride, _dtype(out_dtype or self.dtype), stream))
+
+    def release(self):
+        """Frees the workspaces of all streams and captures (when nothing enqueued or captured will run any more)."""
+        self._check(self.lib.ill_paged_release(self.h))
 
     def close(self):
         if getattr(self, "h", None):

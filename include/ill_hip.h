@@ -287,7 +287,7 @@ ILL_API int ill_gemv_destroy(ill_gemv* g);
  * ILL_F16 or ILL_BF16 in pages of `page_size` positions (a power of two, 16 .. 1024). Element
  * (page, slot, head, dim) of either cache is at page * page_stride + slot * slot_stride +
  * head * head_stride + dim elements (all 0: [pages][page_size][kv_heads][head_dim]); strides are
- * multiples of 8. The rotation turns the first `rotary_dim` dims of a head (a multiple of 16;
+ * multiples of 8, slot_stride at most 2^24. The rotation turns the first `rotary_dim` dims of a head (a multiple of 16;
  * 0: none) by position * rope_base^(-2 i / rotary_dim), pairing dim i with i + rotary_dim / 2, or
  * with interleaved != 0 dims 2 i and 2 i + 1. norm_eps belongs to the head norms; scale
  * multiplies the scores (0: 1 / sqrt(head_dim)). A handle belongs to the GPU that was current

@@ -207,12 +207,20 @@ struct PgUnit {
   PgSeq seq;
 };
 
-// Every wave finds its unit by itself: the sequences' numbers of units, 64 at a time, a lane each.
+// The division of a call's work, found by every workgroup of 256 threads from the lengths: sequence s is thread s % 256's.
 struct PgFinder {
   const PgBatch& b;
   const PgCut& c;
   int part, units;   // tiles of keys in a part; units of work in all
-  __device__ __forceinline__ int of(int s, PgSeq& q, int& most) const {   // tiles of rows x heads of sequence s
+  struct Lds {
+    int64_t tiles[4], work[4];
+    int units[4], parts[4], cut[4];
+    PgUnit found;
+  };
+  Lds& lds;
+
+  // Tiles of rows x heads of sequence s, its rows, and a bound of their tiles of keys.
+  __device__ __forceinline__ int of(int s, PgSeq& q, int& most) const {
     q = {0, 0, 0};
     most = 0;
     if (s >= b.seqs) return 0;
@@ -220,43 +228,66 @@ struct PgFinder {
     most = pg_most(q.p0 + q.n, pg_cap(b), c);
     return pg_qtiles(q.n, c) * c.kv;
   }
-  __device__ __forceinline__ PgFinder(const PgBatch& b_, const PgCut& c_) : b(b_), c(c_) {
-    const int lane = threadIdx.x & 63;
-    int64_t tiles = 0, work = 0;
+  template <class T>
+  static __device__ __forceinline__ T over_wave(T v) {
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
+    return v;
+  }
+  __device__ __forceinline__ PgFinder(const PgBatch& b_, const PgCut& c_, Lds& lds_) : b(b_), c(c_), lds(lds_) {
     PgSeq q;
     int most;
-    for (int s0 = 0; s0 < b.seqs; s0 += 64) {
-      const int n = of(s0 + lane, q, most);
+    if (b.seqs == 1) {
+      const int n = of(0, q, most);
+      part = pg_part(n, (int64_t)n * most, c);
+      units = n * pg_splits(most, part);
+      return;
+    }
+    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    int64_t tiles = 0, work = 0;
+    for (int s = threadIdx.x; s < b.seqs; s += 256) {
+      const int n = of(s, q, most);
       tiles += n;
       work += (int64_t)n * most;
     }
-    if (b.seqs == 1) {
-      tiles = __shfl(tiles, 0);
-      work = __shfl(work, 0);
-    } else {
-#pragma unroll
-      for (int m = 1; m < 64; m <<= 1) {
-        tiles += __shfl_xor(tiles, m);
-        work += __shfl_xor(work, m);
-      }
+    tiles = over_wave(tiles);
+    work = over_wave(work);
+    if (lane == 0) {
+      lds.tiles[w] = tiles;
+      lds.work[w] = work;
     }
-    part = pg_part(tiles, work, c);
-    units = 0;
-    for (int s0 = 0; s0 < b.seqs; s0 += 64) {
-      const int n = of(s0 + lane, q, most);
-      int u = n * pg_splits(most, part);
-#pragma unroll
-      for (int m = 1; m < 64; m <<= 1) u += __shfl_xor(u, m);
-      units += u;
+    __syncthreads();
+    part = pg_part(lds.tiles[0] + lds.tiles[1] + lds.tiles[2] + lds.tiles[3], lds.work[0] + lds.work[1] + lds.work[2] + lds.work[3], c);
+    int u = 0;
+    for (int s = threadIdx.x; s < b.seqs; s += 256) {
+      const int n = of(s, q, most);
+      u += n * pg_splits(most, part);
     }
+    u = over_wave(u);
+    if (lane == 0) lds.units[w] = u;
+    __syncthreads();
+    units = lds.units[0] + lds.units[1] + lds.units[2] + lds.units[3];
+  }
+
+  // Unit u of sequence s: u is counted from the sequence's first, parts and tiles are what the sequences before it have.
+  __device__ __forceinline__ PgUnit unit(int u, int s, const PgSeq& q, int n, int splits, int parts, int tiles) const {
+    // the heads in turn, so that the workgroups of an XCD (every eighth) read few heads; of a head, the
+    // parts of its last rows first, which have the most keys
+    const int qt = n / c.kv, head = u % c.kv, v = u / c.kv, at = qt - 1 - v / splits;
+    return {s, head, at, v % splits, splits, parts + (head * qt + at) * splits, tiles + head * qt + at, q};
   }
   __device__ __forceinline__ PgUnit find(int u) const {
-    const int lane = threadIdx.x & 63;
-    int parts = 0, tiles = 0;
-    for (int s0 = 0;; s0 += 64) {
-      PgSeq q;
-      int most;
-      const int n = of(s0 + lane, q, most), splits = pg_splits(most, part);
+    PgSeq q;
+    int most;
+    if (b.seqs == 1) {
+      const int n = of(0, q, most);
+      return unit(u, 0, q, n, pg_splits(most, part), 0, 0);
+    }
+    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    int before = 0, parts = 0, tiles = 0;
+    if (threadIdx.x == 0) lds.found.seq.n = 0;   // (stays so only where lengths change meanwhile)
+    for (int s0 = 0; s0 < b.seqs; s0 += 256) {
+      const int n = of(s0 + threadIdx.x, q, most), splits = pg_splits(most, part);
       int3 sum = {n * splits, splits > 1 ? n * splits : 0, splits > 1 ? n : 0}, own = sum;
 #pragma unroll
       for (int m = 1; m < 64; m <<= 1) {
@@ -267,32 +298,30 @@ struct PgFinder {
           sum.z += z;
         }
       }
-      const int all = __builtin_amdgcn_readlane(sum.x, 63);
-      if (u >= all) {   // (u < units, so a later 64 have it; the bound ends the search also where lengths change meanwhile)
-        if (s0 + 64 >= b.seqs) return {0, 0, 0, 0, 1, 0, 0, {0, 0, 0}};
-        u -= all;
-        parts += __builtin_amdgcn_readlane(sum.y, 63);
-        tiles += __builtin_amdgcn_readlane(sum.z, 63);
-        continue;
+      __syncthreads();
+      if (lane == 63) {
+        lds.units[w] = sum.x;
+        lds.parts[w] = sum.y;
+        lds.cut[w] = sum.z;
       }
-      const int at = __ffsll((unsigned long long)__ballot(sum.x > u)) - 1;
-      auto lane_of = [&](int v) { return __builtin_amdgcn_readlane(v, at); };
-      PgUnit r;
-      r.s = s0 + at;
-      r.splits = lane_of(splits);
-      r.seq = {lane_of(q.first), lane_of(q.n), lane_of(q.p0)};
-      u -= lane_of(sum.x - own.x);
-      // the heads in turn, so that the workgroups of an XCD (every eighth) read few heads; of a head, the
-      // parts of its last rows first, which have the most keys
-      const int qt = lane_of(n) / c.kv;
-      r.head = u % c.kv;
-      const int v = u / c.kv;
-      r.split = v % r.splits;
-      r.q = qt - 1 - v / r.splits;
-      r.tile_at = tiles + lane_of(sum.z - own.z) + (r.head * qt + r.q);
-      r.part_at = parts + lane_of(sum.y - own.y) + (r.head * qt + r.q) * r.splits;
-      return r;
+      __syncthreads();
+      int x = before, y = parts, z = tiles;
+      for (int i = 0; i < 4; i++) {
+        if (i == w) {
+          const int first = x + sum.x - own.x;
+          if (u >= first && u < first + own.x) lds.found = unit(u - first, s0 + threadIdx.x, q, n, splits, y + sum.y - own.y, z + sum.z - own.z);
+        }
+        x += lds.units[i];
+        y += lds.parts[i];
+        z += lds.cut[i];
+      }
+      before = x;
+      parts = y;
+      tiles = z;
+      if (u < before) break;
     }
+    __syncthreads();
+    return lds.found;
   }
 };
 
@@ -302,12 +331,12 @@ __device__ __forceinline__ v4f pg_mfma16(uint4 a, uint4 b, v4f c) {   // 16 x 16
   else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
-// 16 bytes from each lane's address into LDS, lane i's at lds + 16 i. In inline assembly, because the
+// 16 bytes from base + each lane's offset into LDS, lane i's at lds + 16 i. In inline assembly, because the
 // compiler cannot tell the buffers apart and would wait for every load in flight before each LDS read;
 // the kernels wait themselves (PG_WAIT), and extra loads of the compiler's own only make that wait longer.
-__device__ __forceinline__ void pg_dma16(const void* g, const void* lds) {
+__device__ __forceinline__ void pg_dma16(const void* base, uint32_t off, const void* lds) {   // base: the same for every lane
   const uint32_t m = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)lds);
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(m), "v"(g) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m), "v"(off), "s"(base) : "memory");
 }
 #define PG_WAIT(n) asm volatile("s_waitcnt vmcnt(" #n ")" ::: "memory")
 #define PG_WAIT_LDS() asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory")
@@ -391,37 +420,82 @@ __device__ __forceinline__ void pg_store(const PgAttend& a, int row, int head, i
   else gst((gu32x2*)((uint16_t*)a.out + at), (gu32x2){pg_pack2<TC>(y[0], y[1]), pg_pack2<TC>(y[2], y[3])});
 }
 
-// The parts of a tile of rows, joined in their order by one workgroup of 256 threads. wt: LDS for their weights
-// (PG_MAXSPLIT x M floats).
+// A workgroup's parts are written and read with agent-scope accesses, which are coherent across the XCDs without a
+// fence; a part counts as done (pg_part_done) when its workgroup's stores have been acknowledged.
+__device__ __forceinline__ void pg_share(float* p, v4f v) {
+  const gu32x4 x = __builtin_bit_cast(gu32x4, v);
+  astore64((uint64_t*)p, (uint64_t)x[0] | (uint64_t)x[1] << 32);
+  astore64((uint64_t*)p + 1, (uint64_t)x[2] | (uint64_t)x[3] << 32);
+}
+__device__ __forceinline__ v4f pg_shared(const float* p) {
+  const uint64_t x = aload64((const uint64_t*)p), y = aload64((const uint64_t*)p + 1);
+  return (v4f){__uint_as_float((uint32_t)x), __uint_as_float((uint32_t)(x >> 32)), __uint_as_float((uint32_t)y), __uint_as_float((uint32_t)(y >> 32))};
+}
+// Whether all parts of the tile of rows are done with this one (the same for every thread).
+__device__ __forceinline__ bool pg_part_done(int32_t* joined, int splits, int* lds) {
+  PG_WAIT(0);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const bool all = __hip_atomic_fetch_add((GAS int32_t*)joined, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == splits - 1;
+    if (all) astore32(joined, 0);   // for the next call
+    *lds = all;
+  }
+  __syncthreads();
+  return *lds != 0;
+}
+
+// The parts of a tile of rows, joined in their order by one workgroup of 256 threads, `SUM` groups of threads with every
+// SUM-th part each. wt: LDS for the parts' weights, [splits][M], and SUM - 1 groups' sums behind them.
 template <int TC, int D, int M, class P>
 __device__ __forceinline__ void pg_join(const P& p, const PgUnit& un, int f0, int live, float* wt) {
   const int tid = threadIdx.x;
   const float2* ml = p.w.ml + (size_t)un.part_at * M;
-  __syncthreads();
-  for (int r = tid; r < live; r += 256) {
-    float m = -INFINITY, l = 0.f;
-    for (int x = 0; x < un.splits; x++) m = fmaxf(m, gld(ml + (size_t)x * M + r).x);
-    for (int x = 0; x < un.splits; x++) {
-      const float2 v = gld(ml + (size_t)x * M + r);
-      const float e = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(v.x - m);
-      wt[x * M + r] = e;
-      l += v.y * e;
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    for (int x = 0; x < un.splits; x++) wt[x * M + r] *= inv;
+  float* ls = wt + un.splits * M;
+  for (int i = tid; i < un.splits * M; i += 256) {
+    const uint64_t v = i % M < live ? aload64((const uint64_t*)(ml + i)) : 0;
+    wt[i] = __uint_as_float((uint32_t)v);
+    ls[i] = __uint_as_float((uint32_t)(v >> 32));
   }
   __syncthreads();
-  for (int i = tid; i < live * (D / 4); i += 256) {
-    const int r = i / (D / 4), d = 4 * (i % (D / 4));
-    const float* o = p.w.o + ((size_t)un.part_at * M + r) * D + d;
-    v4f y = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int x = 0; x < un.splits; x++) {
-      const float e = wt[x * M + r];
-      const v4f v = __builtin_bit_cast(v4f, gld((const uint4*)(o + (size_t)x * M * D)));
-      if (e != 0.f) y += v * e;
+  constexpr int T = 256 / M;   // threads of a row, neighbours in a wave
+  {
+    const int r = tid / T, j = tid % T;
+    float m = -INFINITY, l = 0.f;
+    for (int x = j; x < un.splits; x += T) m = fmaxf(m, wt[x * M + r]);
+#pragma unroll
+    for (int k = 1; k < T; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
+    for (int x = j; x < un.splits; x += T) {
+      const float e = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(wt[x * M + r] - m);
+      wt[x * M + r] = e;
+      l += ls[x * M + r] * e;
     }
-    pg_store<TC>(p.a, un.seq.first + (f0 + r) / p.c.G, un.head * p.c.G + (f0 + r) % p.c.G, d, D, y);
+#pragma unroll
+    for (int k = 1; k < T; k <<= 1) l += __shfl_xor(l, k);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    for (int x = j; x < un.splits; x += T) wt[x * M + r] *= inv;
+  }
+  __syncthreads();
+  const int items = live * (D / 4), groups = items <= 64 ? 4 : items <= 128 ? 2 : 1, width = 256 / groups;
+  for (int i0 = 0; i0 < items; i0 += width) {
+    const int i = i0 + tid % width, g = tid / width, r = i / (D / 4), d = 4 * (i % (D / 4));
+    v4f y = {0.f, 0.f, 0.f, 0.f};
+    if (i < items) {
+      const float* o = p.w.o + ((size_t)un.part_at * M + r) * D + d;
+#pragma unroll 8
+      for (int x = g; x < un.splits; x += groups) {
+        const float e = wt[x * M + r];
+        const v4f v = pg_shared(o + (size_t)x * M * D);
+        if (e != 0.f) y += v * e;
+      }
+    }
+    if (groups > 1) {   // (items <= width: once)
+      v4f* sums = (v4f*)(ls + un.splits * M);
+      if (g && i < items) sums[(g - 1) * width + i] = y;
+      __syncthreads();
+      if (g == 0 && i < items)
+        for (int x = 1; x < groups; x++) y += sums[(x - 1) * width + i];
+    }
+    if (g == 0 && i < items) pg_store<TC>(p.a, un.seq.first + (f0 + r) / p.c.G, un.head * p.c.G + (f0 + r) % p.c.G, d, D, y);
   }
 }
 
@@ -447,6 +521,7 @@ __global__ __launch_bounds__(256, 2) void pg_step_kernel(PgStep p) {
   __shared__ __attribute__((aligned(16))) uint4 lds[4][1024];
   __shared__ float smx[4][16], sls[4][16];
   __shared__ int last;
+  __shared__ PgFinder::Lds found;
   const PgAttend& a = p.a;
   const PgCut& c = p.c;
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, n = lane & 15, kg = lane >> 4;
@@ -454,16 +529,19 @@ __global__ __launch_bounds__(256, 2) void pg_step_kernel(PgStep p) {
   uint4* kl = lds[w];
   uint4* vl = lds[w] + 512;
   const float sc2 = a.scale * 1.4426950408889634f;
-  const PgFinder finder(a.b, c);
+  const PgFinder finder(a.b, c, found);
   auto over_kg = [](float v, auto op) {   // over the lanes of the same row
     const auto x = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
     v = op(__int_as_float((int)x[0]), __int_as_float((int)x[1]));
     const auto y = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
     return op(__int_as_float((int)y[0]), __int_as_float((int)y[1]));
   };
-  int64_t row_off[16 / KPI];   // this lane's key of each group of KPI within 16
+  uint32_t lane_off[8];   // bytes from a group of 16 keys to what this lane loads of it, per load
 #pragma unroll
-  for (int i = 0; i < 16 / KPI; i++) row_off[i] = (KPI * i + lane / UPR) * a.slot_stride;
+  for (int i = 0; i < 8; i++) {
+    const int key = KPI * i + lane / UPR;
+    lane_off[i] = 2 * ((uint32_t)(key & 15) * (uint32_t)a.slot_stride + 8 * ((lane % UPR) ^ pg_swz<D>(key)));
+  }
   for (int u = blockIdx.x; u < finder.units; u += gridDim.x) {
     const PgUnit un = finder.find(u);
     if (un.seq.n == 0) continue;
@@ -477,25 +555,29 @@ __global__ __launch_bounds__(256, 2) void pg_step_kernel(PgStep p) {
 #pragma unroll
     for (int ks = 0; ks < KS; ks++) qf[ks] = gld((const uint4*)(a.q + row * a.qs + (int64_t)head * D + 32 * ks + 8 * kg));
     const int mine = c0 + w < c1 ? (c1 - c0 - w + 3) / 4 : 0;   // this wave's tiles
-    // pages of the wave's next 64 / NG tiles, 16 positions a lane; -1: not to be followed
-    int page = -1;
-    auto pages = [&](int k) {
+    // where the keys of the wave's next 64 / NG tiles are, 16 of them a lane: elements from the cache's begin; -1: not there
+    int64_t group = -1;
+    auto groups = [&](int k) {
       const int t = c0 + w + 4 * (k + lane / NG);
-      page = -1;
+      group = -1;
       if (t < c1) {
-        const int key = min(pg_key_tile(range, t) * KT + 16 * (lane % NG), end - 1);
-        page = gld(a.b.table + un.s * a.b.table_stride + (key >> a.b.page_log));
-        if (page < 0 || page >= a.b.pages) page = -1;
+        const int g = pg_key_tile(range, t) * KT + 16 * (lane % NG), key = min(g, end - 1);
+        const int page = gld(a.b.table + un.s * a.b.table_stride + (key >> a.b.page_log));
+        if (page >= 0 && page < a.b.pages) group = page * a.page_stride + (g & pmask) * a.slot_stride + un.head * a.head_stride;
       }
     };
+    auto group_at = [&](int k, int g) {   // (the same for every lane)
+      const int at = (k * NG + g) & 63;
+      return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)group, at) |
+                       (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(group >> 32), at) << 32);
+    };
     auto load = [&](const uint16_t* from, uint4* to, int k) {
-      const int kt = pg_key_tile(range, c0 + w + 4 * k) * KT;
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const int g = i * KPI / 16, key = KPI * i + lane / UPR;
-        const int pg = max(__builtin_amdgcn_readlane(page, (k * NG + g) & 63), 0);   // (page 0 is there, and masked)
-        const int64_t at = pg * a.page_stride + ((kt + 16 * g) & pmask) * a.slot_stride + un.head * a.head_stride;
-        pg_dma16(from + at + row_off[i % (16 / KPI)] + 8 * ((lane % UPR) ^ pg_swz<D>(key)), to + 64 * i);
+      for (int g = 0; g < NG; g++) {
+        const int64_t at = group_at(k, g);
+        const uint16_t* base = from + (at < 0 ? 0 : at);   // (the first page is there, and masked)
+#pragma unroll
+        for (int i = g * 8 / NG; i < (g + 1) * 8 / NG; i++) pg_dma16(base, lane_off[i], to + 64 * i);
       }
     };
     float Mx = -INFINITY, Ls = 0.f;   // Ls: this lane's keys only
@@ -503,7 +585,7 @@ __global__ __launch_bounds__(256, 2) void pg_step_kernel(PgStep p) {
 #pragma unroll
     for (int d = 0; d < ND; d++) O[d] = (v4f){0.f, 0.f, 0.f, 0.f};
     if (mine > 0) {
-      pages(0);
+      groups(0);
       load(a.kc, kl, 0);
       load(a.vc, vl, 0);
     }
@@ -512,7 +594,7 @@ __global__ __launch_bounds__(256, 2) void pg_step_kernel(PgStep p) {
       const bool more = k + 1 < mine;
       int good = 0;   // groups of 16 keys whose pages are there
 #pragma unroll
-      for (int g = 0; g < NG; g++) good |= (__builtin_amdgcn_readlane(page, (k * NG + g) & 63) >= 0) << g;
+      for (int g = 0; g < NG; g++) good |= (__builtin_amdgcn_readlane((int)(group >> 32), (k * NG + g) & 63) >= 0) << g;
       PG_WAIT(8);   // the keys; the 8 loads after them are the values
       v4f s[NB];
 #pragma unroll
@@ -524,7 +606,7 @@ __global__ __launch_bounds__(256, 2) void pg_step_kernel(PgStep p) {
       }
       PG_WAIT_LDS();   // the keys have been read
       if (more) {
-        if (((k + 1) & (64 / NG - 1)) == 0) pages(k + 1);
+        if (((k + 1) & (64 / NG - 1)) == 0) groups(k + 1);
         load(a.kc, kl, k + 1);
       }
       // every row sees the whole tile, or the rows' masks (wave-uniform)
@@ -645,21 +727,12 @@ __global__ __launch_bounds__(256, 2) void pg_step_kernel(PgStep p) {
       if (un.splits == 1) {
         pg_store<TC>(a, un.seq.first + (f0 + r) / c.G, un.head * c.G + (f0 + r) % c.G, d, D, l == 0.f ? (v4f){0.f, 0.f, 0.f, 0.f} : o / l);
       } else {
-        if (d == 0) gst((gu32x2*)(p.w.ml + (size_t)(un.part_at + un.split) * 16 + r), (gu32x2){__float_as_uint(m), __float_as_uint(l)});
-        gst((gu32x4*)(p.w.o + ((size_t)(un.part_at + un.split) * 16 + r) * D + d), __builtin_bit_cast(gu32x4, o));
+        const size_t at = (size_t)(un.part_at + un.split) * 16 + r;
+        if (d == 0) astore64((uint64_t*)(p.w.ml + at), (uint64_t)__float_as_uint(m) | (uint64_t)__float_as_uint(l) << 32);
+        pg_share(p.w.o + at * D + d, o);
       }
     }
-    if (un.splits > 1) {
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) last = atomicAdd(p.w.joined + un.tile_at, 1) == un.splits - 1;
-      __syncthreads();
-      if (last) {
-        __threadfence();
-        pg_join<TC, D, 16>(p, un, f0, live, (float*)lds);
-        if (tid == 0) atomicExch(p.w.joined + un.tile_at, 0);
-      }
-    }
+    if (un.splits > 1 && pg_part_done(p.w.joined + un.tile_at, un.splits, &last)) pg_join<TC, D, 16>(p, un, f0, live, (float*)lds);
     __syncthreads();   // LDS is the next unit's
   }
 }

@@ -53,6 +53,7 @@ inline int check_desc(ill_paged_desc& d) {
   }
   for (const int64_t s : {d.page_stride, d.slot_stride, d.head_stride})
     if (s < d.head_dim || s % 8) return fail(ILL_E_ARG, "paged: cache stride %lld (at least the head size, a multiple of 8)", (long long)s);
+  if (d.slot_stride > kMost / 64) return fail(ILL_E_ARG, "paged: slot stride %lld (at most 2^24)", (long long)d.slot_stride);
   if (!nested(d.head_dim, d.page_stride, 1, d.slot_stride, d.page_size, d.head_stride, d.kv_heads))
     return fail(ILL_E_ARG, "paged: cache strides %lld, %lld, %lld overlap", (long long)d.page_stride, (long long)d.slot_stride,
                 (long long)d.head_stride);

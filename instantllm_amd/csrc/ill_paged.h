@@ -10,6 +10,7 @@
 enum PgType { PG_F32 = 0, PG_F16 = 1, PG_BF16 = 2 };   // ILL_F32, ILL_F16, ILL_BF16
 
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+#define LAS __attribute__((address_space(3)))   // LDS: named, as GAS is, or an access counts as one to memory too
 
 // Eight values of type T as floats, and back with one rounding to nearest, ties to even.
 template <int T>
@@ -207,26 +208,30 @@ struct PgUnit {
   PgSeq seq;
 };
 
-// The division of a call's work, found by every workgroup of 256 threads from the lengths: sequence s is thread s % 256's.
+// The division of a call's work, found by every workgroup of NW waves from the lengths: sequence s is thread s % NT's.
+template <int NW>
 struct PgFinder {
+  static constexpr int NT = 64 * NW;
   const PgBatch& b;
   const PgCut& c;
   int part, units;   // tiles of keys in a part; units of work in all
   struct Lds {
-    int64_t tiles[4], work[4];
-    int units[4], parts[4], cut[4];
+    int64_t tiles[NW], work[NW];
+    int units[NW], parts[NW], cut[NW];
     PgUnit found;
   };
   Lds& lds;
 
-  // Tiles of rows x heads of sequence s, its rows, and a bound of their tiles of keys.
-  __device__ __forceinline__ int of(int s, PgSeq& q, int& most) const {
+  PgSeq q;
+  int most, n;   // the rows of sequence `threadIdx.x` (of one sequence: every thread's), a bound of their tiles of keys, their tiles x heads
+
+  __device__ __forceinline__ void look(int s) {
     q = {0, 0, 0};
-    most = 0;
-    if (s >= b.seqs) return 0;
+    most = n = 0;
+    if (s >= b.seqs) return;
     q = pg_seq_at(b, s);
     most = pg_most(q.p0 + q.n, pg_cap(b), c);
-    return pg_qtiles(q.n, c) * c.kv;
+    n = pg_qtiles(q.n, c) * (int)c.kv;
   }
   template <class T>
   static __device__ __forceinline__ T over_wave(T v) {
@@ -235,21 +240,21 @@ struct PgFinder {
     return v;
   }
   __device__ __forceinline__ PgFinder(const PgBatch& b_, const PgCut& c_, Lds& lds_) : b(b_), c(c_), lds(lds_) {
-    PgSeq q;
-    int most;
     if (b.seqs == 1) {
-      const int n = of(0, q, most);
+      look(0);
       part = pg_part(n, (int64_t)n * most, c);
       units = n * pg_splits(most, part);
       return;
     }
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
     int64_t tiles = 0, work = 0;
-    for (int s = threadIdx.x; s < b.seqs; s += 256) {
-      const int n = of(s, q, most);
+    int s = threadIdx.x;
+    do {
+      look(s);
       tiles += n;
       work += (int64_t)n * most;
-    }
+      s += NT;
+    } while (s - (int)threadIdx.x < b.seqs);
     tiles = over_wave(tiles);
     work = over_wave(work);
     if (lane == 0) {
@@ -257,37 +262,43 @@ struct PgFinder {
       lds.work[w] = work;
     }
     __syncthreads();
-    part = pg_part(lds.tiles[0] + lds.tiles[1] + lds.tiles[2] + lds.tiles[3], lds.work[0] + lds.work[1] + lds.work[2] + lds.work[3], c);
+    tiles = work = 0;
+#pragma unroll
+    for (int i = 0; i < NW; i++) {
+      tiles += lds.tiles[i];
+      work += lds.work[i];
+    }
+    part = pg_part(tiles, work, c);
+    units = (int)tiles;   // of uncut sequences: a unit for each
+    if (part >= PG_MOST) return;
     int u = 0;
-    for (int s = threadIdx.x; s < b.seqs; s += 256) {
-      const int n = of(s, q, most);
-      u += n * pg_splits(most, part);
+    for (s = threadIdx.x; s - (int)threadIdx.x < b.seqs; s += NT) {
+      if (b.seqs > NT) look(s);
+      u += n * (pg_splits(most, part) - 1);
     }
     u = over_wave(u);
     if (lane == 0) lds.units[w] = u;
     __syncthreads();
-    units = lds.units[0] + lds.units[1] + lds.units[2] + lds.units[3];
+#pragma unroll
+    for (int i = 0; i < NW; i++) units += lds.units[i];
   }
 
   // Unit u of sequence s: u is counted from the sequence's first, parts and tiles are what the sequences before it have.
-  __device__ __forceinline__ PgUnit unit(int u, int s, const PgSeq& q, int n, int splits, int parts, int tiles) const {
+  __device__ __forceinline__ PgUnit unit(uint32_t u, int s, uint32_t splits, int parts, int tiles) const {
     // the heads in turn, so that the workgroups of an XCD (every eighth) read few heads; of a head, the
     // parts of its last rows first, which have the most keys
-    const int qt = n / c.kv, head = u % c.kv, v = u / c.kv, at = qt - 1 - v / splits;
-    return {s, head, at, v % splits, splits, parts + (head * qt + at) * splits, tiles + head * qt + at, q};
+    const uint32_t qt = (uint32_t)n / c.kv, v = u / c.kv, head = u - v * c.kv, back = splits == 1 ? v : v / splits, at = qt - 1 - back;
+    const int tile = (int)(head * qt + at);
+    return {s, (int)head, (int)at, (int)(v - back * splits), (int)splits, parts + tile * (int)splits, tiles + tile, q};
   }
-  __device__ __forceinline__ PgUnit find(int u) const {
-    PgSeq q;
-    int most;
-    if (b.seqs == 1) {
-      const int n = of(0, q, most);
-      return unit(u, 0, q, n, pg_splits(most, part), 0, 0);
-    }
+  __device__ __forceinline__ PgUnit find(int u) {
+    if (b.seqs == 1) return unit(u, 0, pg_splits(most, part), 0, 0);
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
     int before = 0, parts = 0, tiles = 0;
     if (threadIdx.x == 0) lds.found.seq.n = 0;   // (stays so only where lengths change meanwhile)
-    for (int s0 = 0; s0 < b.seqs; s0 += 256) {
-      const int n = of(s0 + threadIdx.x, q, most), splits = pg_splits(most, part);
+    for (int s0 = 0; s0 < b.seqs; s0 += NT) {
+      if (b.seqs > NT) look(s0 + threadIdx.x);
+      const int splits = pg_splits(most, part);
       int3 sum = {n * splits, splits > 1 ? n * splits : 0, splits > 1 ? n : 0}, own = sum;
 #pragma unroll
       for (int m = 1; m < 64; m <<= 1) {
@@ -305,19 +316,20 @@ struct PgFinder {
         lds.cut[w] = sum.z;
       }
       __syncthreads();
-      int x = before, y = parts, z = tiles;
-      for (int i = 0; i < 4; i++) {
-        if (i == w) {
-          const int first = x + sum.x - own.x;
-          if (u >= first && u < first + own.x) lds.found = unit(u - first, s0 + threadIdx.x, q, n, splits, y + sum.y - own.y, z + sum.z - own.z);
+      int first = before + sum.x - own.x, y = parts + sum.y - own.y, z = tiles + sum.z - own.z;
+#pragma unroll
+      for (int i = 0; i < NW; i++) {
+        const int x = lds.units[i], p = lds.parts[i], t = lds.cut[i];
+        if (i < w) {
+          first += x;
+          y += p;
+          z += t;
         }
-        x += lds.units[i];
-        y += lds.parts[i];
-        z += lds.cut[i];
+        before += x;
+        parts += p;
+        tiles += t;
       }
-      before = x;
-      parts = y;
-      tiles = z;
+      if (u >= first && u < first + own.x) lds.found = unit(u - first, s0 + threadIdx.x, splits, y, z);
       if (u < before) break;
     }
     __syncthreads();
@@ -334,8 +346,8 @@ __device__ __forceinline__ v4f pg_mfma16(uint4 a, uint4 b, v4f c) {   // 16 x 16
 // 16 bytes from base + each lane's offset into LDS, lane i's at lds + 16 i. In inline assembly, because the
 // compiler cannot tell the buffers apart and would wait for every load in flight before each LDS read;
 // the kernels wait themselves (PG_WAIT), and extra loads of the compiler's own only make that wait longer.
-__device__ __forceinline__ void pg_dma16(const void* base, uint32_t off, const void* lds) {   // base: the same for every lane
-  const uint32_t m = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)lds);
+__device__ __forceinline__ void pg_dma16(const void* base, uint32_t off, const LAS gu32x4* lds) {   // base: the same for every lane
+  const uint32_t m = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m), "v"(off), "s"(base) : "memory");
 }
 #define PG_WAIT(n) asm volatile("s_waitcnt vmcnt(" #n ")" ::: "memory")
@@ -353,42 +365,44 @@ __device__ __forceinline__ int pg_unit_at(int key, int u) { return key * (D / 8)
 
 // Four keys (key, .., key + 3) of dim 16 nb + lane % 16, from the rows of a tile of values: each 16 lanes read
 // 4 keys x 16 dims, and the transposing read hands lane i its dim.
-__device__ __forceinline__ uint2 pg_tr(const void* p) {
+__device__ __forceinline__ uint2 pg_tr(const LAS gu32x4* p, int bytes) {
   typedef short v4s __attribute__((ext_vector_type(4)));
-  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)p));
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LAS v4s*)((const LAS uint8_t*)p + bytes)));
+}
+typedef LAS gu32x4 pg_lds4;   // 16 bytes of a tile
+__device__ __forceinline__ uint4 pg_get(const pg_lds4* p) {
+  const gu32x4 x = *p;
+  return {x[0], x[1], x[2], x[3]};
 }
 template <int D>
-__device__ __forceinline__ uint4 pg_values(const uint4* v, int key, int nb, int i) {   // keys key .. key + 7
+__device__ __forceinline__ uint4 pg_values(const pg_lds4* v, int key, int nb, int i) {   // keys key .. key + 7
   const int u = 2 * nb + ((i >> 1) & 1), k0 = key + (i >> 2), k1 = k0 + 4;
-  const uint2 a = pg_tr((const uint8_t*)(v + pg_unit_at<D>(k0, u)) + 8 * (i & 1)), b = pg_tr((const uint8_t*)(v + pg_unit_at<D>(k1, u)) + 8 * (i & 1));
+  const uint2 a = pg_tr(v + pg_unit_at<D>(k0, u), 8 * (i & 1)), b = pg_tr(v + pg_unit_at<D>(k1, u), 8 * (i & 1));
   return {a.x, a.y, b.x, b.y};
 }
 
 // Infinities and NaN of eight values: whether there are any; the values with zeros in their place; and marks
 // that a product with ones for the keys a row sees adds up (1 for inf, 64 for -inf, 4096 for NaN; 32 keys).
 template <int TC>
-__device__ __forceinline__ bool pg_wild(uint4 v) {
-  constexpr uint32_t E = TC == PG_BF16 ? 0x7F80u : 0x7C00u;
-  bool w = false;
-  for (const uint32_t x : {v.x, v.y, v.z, v.w}) w = w || (x & E) == E || (x >> 16 & E) == E;
-  return w;
+__device__ __forceinline__ uint32_t pg_wild2(uint32_t x) {   // the top bit of each half: its exponent is all ones
+  constexpr uint32_t E = TC == PG_BF16 ? 0x7F807F80u : 0x7C007C00u, STEP = TC == PG_BF16 ? 0x00800080u : 0x04000400u;
+  return ((x & E) + STEP) & 0x80008000u;
+}
+template <int TC>
+__device__ __forceinline__ uint32_t pg_wild(uint4 v) {
+  return pg_wild2<TC>(v.x) | pg_wild2<TC>(v.y) | pg_wild2<TC>(v.z) | pg_wild2<TC>(v.w);
 }
 template <int TC>
 __device__ __forceinline__ uint4 pg_tamed(uint4 v, uint4& marks) {
-  constexpr uint32_t E = TC == PG_BF16 ? 0x7F80u : 0x7C00u, S = TC == PG_BF16 ? 0x007Fu : 0x03FFu;
-  constexpr uint32_t ONE = TC == PG_BF16 ? 0x3F80u : 0x3C00u, STEP = TC == PG_BF16 ? 0x0300u : 0x1800u;   // 1, and a factor of 64
+  constexpr uint32_t ONE = TC == PG_BF16 ? 0x3F803F80u : 0x3C003C00u, STEP = TC == PG_BF16 ? 0x03000300u : 0x18001800u;   // 1, and a factor of 64
+  constexpr uint32_t S = TC == PG_BF16 ? 0x007F007Fu : 0x03FF03FFu;
+  auto all = [](uint32_t top) { return top | (top - (top >> 15)); };   // all bits of the halves whose top bit is set
   uint32_t y[4] = {v.x, v.y, v.z, v.w}, k[4];
 #pragma unroll
   for (int i = 0; i < 4; i++) {
-    k[i] = 0;
-#pragma unroll
-    for (int h = 0; h < 32; h += 16) {
-      const uint32_t x = y[i] >> h & 0xFFFFu;
-      if ((x & E) == E) {
-        k[i] |= ((x & S) ? ONE + 2 * STEP : x >> 15 ? ONE + STEP : ONE) << h;
-        y[i] &= ~(0xFFFFu << h);
-      }
-    }
+    const uint32_t wild = all(pg_wild2<TC>(y[i])), nan = all(((y[i] & S) + (0x80008000u - 0x00010001u)) & 0x80008000u);
+    k[i] = wild & (ONE + (nan & 2 * STEP) + (~nan & all(y[i] & 0x80008000u) & STEP));
+    y[i] &= ~wild;
   }
   marks = {k[0], k[1], k[2], k[3]};
   return {y[0], y[1], y[2], y[3]};
@@ -409,7 +423,7 @@ __device__ __forceinline__ float pg_wild_sum(float marks) {
 struct PgWork {        // a call's share of the handle's workspace
   float2* ml;          // [2 target][M] reference and sum of a part's rows
   float* o;            // [2 target][M][D] its weighted values
-  int32_t* joined;     // [target] parts of a tile of rows that are done; 0 between calls
+  int32_t* joined;     // [target][1 + PG_MAXSPLIT / PG_FAN] parts of a tile of rows that are done, in all and of each PG_FAN; 0 between calls
 };
 
 // Four dims of a row's output.
@@ -420,83 +434,111 @@ __device__ __forceinline__ void pg_store(const PgAttend& a, int row, int head, i
   else gst((gu32x2*)((uint16_t*)a.out + at), (gu32x2){pg_pack2<TC>(y[0], y[1]), pg_pack2<TC>(y[2], y[3])});
 }
 
-// A workgroup's parts are written and read with agent-scope accesses, which are coherent across the XCDs without a
-// fence; a part counts as done (pg_part_done) when its workgroup's stores have been acknowledged.
+// Parts are written with agent-scope stores, which go through to where all XCDs see them, so that a workgroup only has to
+// wait until its own are acknowledged. (An agent-scope release instead writes the XCD's whole L2 back: 333 rows of 14
+// heads took 41 us with it, 18 us without.)
 __device__ __forceinline__ void pg_share(float* p, v4f v) {
   const gu32x4 x = __builtin_bit_cast(gu32x4, v);
   astore64((uint64_t*)p, (uint64_t)x[0] | (uint64_t)x[1] << 32);
   astore64((uint64_t*)p + 1, (uint64_t)x[2] | (uint64_t)x[3] << 32);
 }
-__device__ __forceinline__ v4f pg_shared(const float* p) {
-  const uint64_t x = aload64((const uint64_t*)p), y = aload64((const uint64_t*)p + 1);
-  return (v4f){__uint_as_float((uint32_t)x), __uint_as_float((uint32_t)(x >> 32)), __uint_as_float((uint32_t)y), __uint_as_float((uint32_t)(y >> 32))};
-}
-// Whether all parts of the tile of rows are done with this one (the same for every thread).
-__device__ __forceinline__ bool pg_part_done(int32_t* joined, int splits, int* lds) {
+
+// Whether this is the last of `count` workgroups to come here, whose parts it then sees (the same for every thread). The
+// counter is left at 0 for the next call.
+__device__ __forceinline__ bool pg_last(int32_t* counter, int count, int* lds) {
   PG_WAIT(0);
   __syncthreads();
   if (threadIdx.x == 0) {
-    const bool all = __hip_atomic_fetch_add((GAS int32_t*)joined, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == splits - 1;
-    if (all) astore32(joined, 0);   // for the next call
+    const bool all = __hip_atomic_fetch_add((GAS int32_t*)counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == count - 1;
+    if (all) astore32(counter, 0);
     *lds = all;
   }
   __syncthreads();
-  return *lds != 0;
+  const bool all = *lds != 0;
+  if (all) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+  return all;
 }
 
-// The parts of a tile of rows, joined in their order by one workgroup of 256 threads, `SUM` groups of threads with every
-// SUM-th part each. wt: LDS for the parts' weights, [splits][M], and SUM - 1 groups' sums behind them.
-template <int TC, int D, int M, class P>
-__device__ __forceinline__ void pg_join(const P& p, const PgUnit& un, int f0, int live, float* wt) {
+// Writes a part's state of row r, four dims from d on.
+template <int D, int M>
+__device__ __forceinline__ void pg_put_part(const PgWork& w, int part, int r, int d, float m, float l, v4f o) {
+  const size_t at = (size_t)part * M + r;
+  if (d == 0) astore64((uint64_t*)(w.ml + at), (uint64_t)__float_as_uint(m) | (uint64_t)__float_as_uint(l) << 32);
+  pg_share(w.o + at * D + d, o);
+}
+
+// Joins `count` <= PG_FAN parts (from part `first` on, every step-th) of a tile of rows in their order, by one workgroup
+// of NW waves: into the output, or into the first of them. lds: PG_FAN x M x 2 + 2 M floats and, behind them, NW x 64 states.
+template <int TC, int D, int M, int NW>
+__device__ __forceinline__ void pg_join(const PgAttend& a, const PgCut& c, const PgWork& pw, const PgUnit& un, int first, int step, int count, bool out,
+                                        int f0, int live, LAS float* lds) {
+  constexpr int NT = 64 * NW, T = NT / M >= 64 ? 64 : NT / M < 1 ? 1 : NT / M;   // T threads of a row, neighbours in a wave
   const int tid = threadIdx.x;
-  const float2* ml = p.w.ml + (size_t)un.part_at * M;
-  float* ls = wt + un.splits * M;
-  for (int i = tid; i < un.splits * M; i += 256) {
-    const uint64_t v = i % M < live ? aload64((const uint64_t*)(ml + i)) : 0;
-    wt[i] = __uint_as_float((uint32_t)v);
-    ls[i] = __uint_as_float((uint32_t)(v >> 32));
+  LAS float *wt = lds, *ls = lds + PG_FAN * M, *rows = ls + PG_FAN * M;
+  for (int i = tid; i < count * M; i += NT) {
+    const int x = i / M, r = i % M;
+    const uint2 v = r < live ? gld((const uint2*)(pw.ml + (size_t)(first + x * step) * M + r)) : make_uint2(0, 0);
+    wt[i] = __uint_as_float(v.x);
+    ls[i] = __uint_as_float(v.y);
   }
   __syncthreads();
-  constexpr int T = 256 / M;   // threads of a row, neighbours in a wave
-  {
+  if (tid < M * T) {
     const int r = tid / T, j = tid % T;
     float m = -INFINITY, l = 0.f;
-    for (int x = j; x < un.splits; x += T) m = fmaxf(m, wt[x * M + r]);
+    for (int x = j; x < count; x += T) m = fmaxf(m, wt[x * M + r]);
 #pragma unroll
     for (int k = 1; k < T; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
-    for (int x = j; x < un.splits; x += T) {
+    for (int x = j; x < count; x += T) {
       const float e = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(wt[x * M + r] - m);
       wt[x * M + r] = e;
       l += ls[x * M + r] * e;
     }
 #pragma unroll
     for (int k = 1; k < T; k <<= 1) l += __shfl_xor(l, k);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    for (int x = j; x < un.splits; x += T) wt[x * M + r] *= inv;
+    if (j == 0) {
+      rows[r] = m;
+      rows[M + r] = l;
+    }
   }
   __syncthreads();
-  const int items = live * (D / 4), groups = items <= 64 ? 4 : items <= 128 ? 2 : 1, width = 256 / groups;
+  // few items: `groups` threads each, every groups-th part to one of them
+  const int items = live * (D / 4), groups = items <= NT / 4 ? 4 : items <= NT / 2 ? 2 : 1, width = NT / groups;
   for (int i0 = 0; i0 < items; i0 += width) {
     const int i = i0 + tid % width, g = tid / width, r = i / (D / 4), d = 4 * (i % (D / 4));
     v4f y = {0.f, 0.f, 0.f, 0.f};
     if (i < items) {
-      const float* o = p.w.o + ((size_t)un.part_at * M + r) * D + d;
+      const float* o = pw.o + ((size_t)first * M + r) * D + d;
 #pragma unroll 8
-      for (int x = g; x < un.splits; x += groups) {
+      for (int x = g; x < count; x += groups) {
         const float e = wt[x * M + r];
-        const v4f v = pg_shared(o + (size_t)x * M * D);
+        const v4f v = __builtin_bit_cast(v4f, gld((const uint4*)(o + (size_t)x * step * M * D)));
         if (e != 0.f) y += v * e;
       }
     }
     if (groups > 1) {   // (items <= width: once)
-      v4f* sums = (v4f*)(ls + un.splits * M);
+      LAS v4f* sums = (LAS v4f*)(rows + 2 * M);
       if (g && i < items) sums[(g - 1) * width + i] = y;
       __syncthreads();
       if (g == 0 && i < items)
         for (int x = 1; x < groups; x++) y += sums[(x - 1) * width + i];
     }
-    if (g == 0 && i < items) pg_store<TC>(p.a, un.seq.first + (f0 + r) / p.c.G, un.head * p.c.G + (f0 + r) % p.c.G, d, D, y);
+    if (g == 0 && i < items) {
+      const float m = rows[r], l = rows[M + r];
+      if (out) pg_store<TC>(a, un.seq.first + (uint32_t)(f0 + r) / c.G, un.head * c.G + (uint32_t)(f0 + r) % c.G, d, D, l == 0.f ? (v4f){0.f, 0.f, 0.f, 0.f} : y / l);
+      else pg_put_part<D, M>(pw, first, r, d, m, l, y);
+    }
   }
+}
+
+// What follows a part of several: the last workgroup of PG_FAN parts joins them, and the last of those joins theirs.
+template <int TC, int D, int M, int NW>
+__device__ __forceinline__ void pg_finish(const PgAttend& a, const PgCut& c, const PgWork& w, const PgUnit& un, int f0, int live, LAS float* lds, int* last) {
+  const int g = un.split / PG_FAN, groups = pg_up(un.splits, PG_FAN), count = min(PG_FAN, un.splits - g * PG_FAN);
+  int32_t* joined = w.joined + un.tile_at * (PG_MAXSPLIT / PG_FAN + 1);
+  if (!pg_last(joined + 1 + g, count, last)) return;
+  pg_join<TC, D, M, NW>(a, c, w, un, un.part_at + g * PG_FAN, 1, count, groups == 1, f0, live, lds);
+  if (groups == 1 || !pg_last(joined, groups, last)) return;
+  pg_join<TC, D, M, NW>(a, c, w, un, un.part_at, PG_FAN, groups, true, f0, live, lds);
 }
 
 struct PgStep {
@@ -514,22 +556,24 @@ struct PgStep {
 // + r: key 32 (b / 2) + 8 g + 4 (b % 2) + r). Values are transposed by the LDS read. The waves' states are
 // joined in LDS; a tile of rows whose keys are in several parts is joined by the workgroup that ends last, in
 // the parts' order.
-template <int TC, int D, bool FINE>   // FINE: weights in two parts (float32 outputs)
-__global__ __launch_bounds__(256, 2) void pg_step_kernel(PgStep p) {
+template <int TC, int D, bool FINE, int NW>   // FINE: weights in two parts (float32 outputs)
+__global__ __launch_bounds__(64 * NW, 2) void pg_step_kernel(PgStep p) {
   constexpr int KT = D == 64 ? 64 : 32, UPR = D / 8, KPI = 64 / UPR, NB = KT / 16, KS = D / 32, ND = D / 16, NS = KT / 32, NG = KT / 16;
   constexpr int RF = D + 4;   // floats between the rows of a state in LDS
-  __shared__ __attribute__((aligned(16))) uint4 lds[4][1024];
-  __shared__ float smx[4][16], sls[4][16];
+  __shared__ __attribute__((aligned(16))) uint4 lds[NW][1024];
+  __shared__ float smx[NW][16], sls[NW][16];
   __shared__ int last;
-  __shared__ PgFinder::Lds found;
+  __shared__ typename PgFinder<NW>::Lds found;
   const PgAttend& a = p.a;
-  const PgCut& c = p.c;
-  const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, n = lane & 15, kg = lane >> 4;
+  PgCut c = p.c;
+  c.M = 16;   // (as the host has them, for the compiler)
+  c.KT = KT;
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, kg = lane >> 4;
   const int cap = pg_cap(a.b), pmask = (1 << a.b.page_log) - 1;
-  uint4* kl = lds[w];
-  uint4* vl = lds[w] + 512;
+  pg_lds4* kl = (pg_lds4*)lds[w];
+  pg_lds4* vl = kl + 512;
   const float sc2 = a.scale * 1.4426950408889634f;
-  const PgFinder finder(a.b, c, found);
+  PgFinder<NW> finder(a.b, c, found);
   auto over_kg = [](float v, auto op) {   // over the lanes of the same row
     const auto x = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
     v = op(__int_as_float((int)x[0]), __int_as_float((int)x[1]));
@@ -545,20 +589,21 @@ __global__ __launch_bounds__(256, 2) void pg_step_kernel(PgStep p) {
   for (int u = blockIdx.x; u < finder.units; u += gridDim.x) {
     const PgUnit un = finder.find(u);
     if (un.seq.n == 0) continue;
-    const int flat = un.seq.n * c.G, f0 = 16 * un.q, live = min(16, flat - f0);   // (n G is at most 2^30)
-    const int f = min(f0 + n, flat - 1), row = un.seq.first + f / c.G, head = un.head * c.G + f % c.G;
-    const int pos = un.seq.p0 + f / c.G, p0 = un.seq.p0 + f0 / c.G, p1 = un.seq.p0 + (f0 + live - 1) / c.G;
+    const int G = c.G, flat = un.seq.n * G, f0 = 16 * un.q, live = min(16, flat - f0);   // (n G is at most 2^30)
+    const uint32_t f = min(f0 + n, flat - 1), at_row = f / c.G;
+    const int row = un.seq.first + at_row, head = un.head * G + (f - at_row * c.G);
+    const int pos = un.seq.p0 + at_row, p0 = __builtin_amdgcn_readlane(pos, 0), p1 = __builtin_amdgcn_readlane(pos, 15);
     const PgRange range = pg_range(p0, p1, cap, c);
     const int per = pg_up(range.n, un.splits), c0 = min(un.split * per, range.n), c1 = min(c0 + per, range.n);
     const int end = min(p1 + 1, cap);
     uint4 qf[KS];
 #pragma unroll
     for (int ks = 0; ks < KS; ks++) qf[ks] = gld((const uint4*)(a.q + row * a.qs + (int64_t)head * D + 32 * ks + 8 * kg));
-    const int mine = c0 + w < c1 ? (c1 - c0 - w + 3) / 4 : 0;   // this wave's tiles
+    const int mine = c0 + w < c1 ? (c1 - c0 - w + NW - 1) / NW : 0;   // this wave's tiles
     // where the keys of the wave's next 64 / NG tiles are, 16 of them a lane: elements from the cache's begin; -1: not there
     int64_t group = -1;
     auto groups = [&](int k) {
-      const int t = c0 + w + 4 * (k + lane / NG);
+      const int t = c0 + w + NW * (k + lane / NG);
       group = -1;
       if (t < c1) {
         const int g = pg_key_tile(range, t) * KT + 16 * (lane % NG), key = min(g, end - 1);
@@ -571,7 +616,7 @@ __global__ __launch_bounds__(256, 2) void pg_step_kernel(PgStep p) {
       return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)group, at) |
                        (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(group >> 32), at) << 32);
     };
-    auto load = [&](const uint16_t* from, uint4* to, int k) {
+    auto load = [&](const uint16_t* from, pg_lds4* to, int k) {
 #pragma unroll
       for (int g = 0; g < NG; g++) {
         const int64_t at = group_at(k, g);
@@ -590,7 +635,7 @@ __global__ __launch_bounds__(256, 2) void pg_step_kernel(PgStep p) {
       load(a.vc, vl, 0);
     }
     for (int k = 0; k < mine; k++) {
-      const int kt = pg_key_tile(range, c0 + w + 4 * k) * KT;
+      const int kt = pg_key_tile(range, c0 + w + NW * k) * KT;
       const bool more = k + 1 < mine;
       int good = 0;   // groups of 16 keys whose pages are there
 #pragma unroll
@@ -602,7 +647,7 @@ __global__ __launch_bounds__(256, 2) void pg_step_kernel(PgStep p) {
         const int key = 32 * (b >> 1) + 8 * (n >> 2) + 4 * (b & 1) + (n & 3);
         s[b] = (v4f){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++) s[b] = pg_mfma16<TC>(kl[pg_unit_at<D>(key, 4 * ks + kg)], qf[ks], s[b]);
+        for (int ks = 0; ks < KS; ks++) s[b] = pg_mfma16<TC>(pg_get(kl + pg_unit_at<D>(key, 4 * ks + kg)), qf[ks], s[b]);
       }
       PG_WAIT_LDS();   // the keys have been read
       if (more) {
@@ -663,12 +708,12 @@ __global__ __launch_bounds__(256, 2) void pg_step_kernel(PgStep p) {
       }
       if (more) PG_WAIT(8);   // the values; the 8 loads after them are the next keys
       else PG_WAIT(0);
-      bool wild = false;
+      uint32_t wild = 0;
       if (!whole) {   // what a row does not see must not reach it as 0 x inf
 #pragma unroll
         for (int d = 0; d < ND; d++)
 #pragma unroll
-          for (int t = 0; t < NS; t++) wild = wild || pg_wild<TC>(pg_values<D>(vl, 32 * t + 8 * kg, d, n));
+          for (int t = 0; t < NS; t++) wild |= pg_wild<TC>(pg_values<D>(vl, 32 * t + 8 * kg, d, n));
         wild = __any(wild);
       }
       if (!wild) {
@@ -703,36 +748,34 @@ __global__ __launch_bounds__(256, 2) void pg_step_kernel(PgStep p) {
     }
     // the waves' states, each in its own LDS
     Ls = over_kg(Ls, OpAddF{});
-    float* st = (float*)lds[w];
+    LAS float* st = (LAS float*)lds[w];
 #pragma unroll
-    for (int d = 0; d < ND; d++) *(v4f*)(st + n * RF + 16 * d + 4 * kg) = O[d];
+    for (int d = 0; d < ND; d++) *(LAS v4f*)(st + n * RF + 16 * d + 4 * kg) = O[d];
     if (kg == 0) {
       smx[w][n] = Mx;
       sls[w][n] = Ls;
     }
     __syncthreads();
-    for (int i = tid; i < live * (D / 4); i += 256) {
+    for (int i = tid; i < live * (D / 4); i += 64 * NW) {
       const int r = i / (D / 4), d = 4 * (i % (D / 4));
       float m = smx[0][r];
 #pragma unroll
-      for (int x = 1; x < 4; x++) m = fmaxf(m, smx[x][r]);
+      for (int x = 1; x < NW; x++) m = fmaxf(m, smx[x][r]);
       float l = 0.f;
       v4f o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int x = 0; x < 4; x++) {
+      for (int x = 0; x < NW; x++) {
         const float e = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(smx[x][r] - m);
         l += sls[x][r] * e;
-        if (e != 0.f) o += *(const v4f*)((const float*)lds[x] + r * RF + d) * e;
+        if (e != 0.f) o += *(const LAS v4f*)((const LAS float*)lds[x] + r * RF + d) * e;
       }
       if (un.splits == 1) {
-        pg_store<TC>(a, un.seq.first + (f0 + r) / c.G, un.head * c.G + (f0 + r) % c.G, d, D, l == 0.f ? (v4f){0.f, 0.f, 0.f, 0.f} : o / l);
+        pg_store<TC>(a, un.seq.first + (uint32_t)(f0 + r) / c.G, un.head * c.G + (uint32_t)(f0 + r) % c.G, d, D, l == 0.f ? (v4f){0.f, 0.f, 0.f, 0.f} : o / l);
       } else {
-        const size_t at = (size_t)(un.part_at + un.split) * 16 + r;
-        if (d == 0) astore64((uint64_t*)(p.w.ml + at), (uint64_t)__float_as_uint(m) | (uint64_t)__float_as_uint(l) << 32);
-        pg_share(p.w.o + at * D + d, o);
+        pg_put_part<D, 16>(p.w, un.part_at + un.split, r, d, m, l, o);
       }
     }
-    if (un.splits > 1 && pg_part_done(p.w.joined + un.tile_at, un.splits, &last)) pg_join<TC, D, 16>(p, un, f0, live, (float*)lds);
+    if (un.splits > 1) pg_finish<TC, D, 16, NW>(a, c, p.w, un, f0, live, (LAS float*)lds, &last);
     __syncthreads();   // LDS is the next unit's
   }
 }

@@ -39,20 +39,30 @@ PgBatch batch_of(const ill_paged* p, const ill_paged_batch& b) {
 }
 
 // Parts of a call of few rows per sequence: two workgroups per CU, and no part below four tiles of keys, one for each wave.
-constexpr int kStepTarget = 512, kStepLeast = 4;
+#ifndef STEP_NW
+#define STEP_NW 4
+#endif
+#ifndef STEP_LOG
+#define STEP_LOG 8
+#endif
+#ifndef STEP_LEAST
+#define STEP_LEAST 8
+#endif
+constexpr int kStepLog = STEP_LOG, kStepLeast = STEP_LEAST;
 
 PgCut step_cut(const ill_paged_desc& d, int window, int sinks) {
-  return {d.heads / d.kv_heads, d.kv_heads, 16, d.head_dim == 64 ? 64 : 32, window, sinks, kStepTarget, kStepLeast, INT32_MAX, 0, INT32_MAX};
+  return {(uint32_t)(d.heads / d.kv_heads), (uint32_t)d.kv_heads, 16, d.head_dim == 64 ? 64 : 32, window, sinks, kStepLog, kStepLeast, INT32_MAX, 0, INT32_MAX};
 }
 
-// Bytes of a workspace of `target` parts wanted over tiles of M rows.
-size_t work_size(int target, int M, int D) { return (size_t)2 * target * M * (D + 2) * 4 + al256((size_t)target * 4); }
+// Bytes of a workspace where 2^log parts are wanted, over tiles of M rows.
+size_t counters(int log) { return al256(((size_t)(PG_MAXSPLIT / PG_FAN + 1) << log) * 4); }
+size_t work_size(int log, int M, int D) { return ((size_t)M * (D + 2) * 4 << (log + 1)) + counters(log); }
 
-PgWork work_of(uint8_t* at, int target, int M, int D) {
+PgWork work_of(uint8_t* at, int log, int M, int D) {
   PgWork w;
   w.joined = (int32_t*)at;
-  w.o = (float*)(at + al256((size_t)target * 4));
-  w.ml = (float2*)(w.o + (size_t)2 * target * M * D);
+  w.o = (float*)(at + counters(log));
+  w.ml = (float2*)(w.o + ((size_t)M * D << (log + 1)));
   return w;
 }
 
@@ -80,8 +90,8 @@ int workspace(ill_paged* p, hipStream_t st, uint8_t** out) {
 
 template <int TC, int D>
 void launch_step(const PgStep& s, int64_t grid, hipStream_t st) {
-  if (s.a.out_f32) hipLaunchKernelGGL((pg_step_kernel<TC, D, true>), dim3(grid), dim3(256), 0, st, s);
-  else hipLaunchKernelGGL((pg_step_kernel<TC, D, false>), dim3(grid), dim3(256), 0, st, s);
+  if (s.a.out_f32) hipLaunchKernelGGL((pg_step_kernel<TC, D, true, STEP_NW>), dim3(grid), dim3(64 * STEP_NW), 0, st, s);
+  else hipLaunchKernelGGL((pg_step_kernel<TC, D, false, STEP_NW>), dim3(grid), dim3(64 * STEP_NW), 0, st, s);
 }
 
 template <int TX, int TC>
@@ -122,7 +132,7 @@ int ill_paged_create(const ill_paged_desc* desc, ill_paged** out) {
   for (int i = 0; i < d.rotary_dim / 2; i++) freq[i] = std::pow(d.rope_base, -2.0 * i / d.rotary_dim) / (2 * M_PI);
   if (hipMalloc(&p->freq, sizeof freq) != hipSuccess || hipMemcpy(p->freq, freq, sizeof freq, hipMemcpyHostToDevice) != hipSuccess)
     return bad(fail(ILL_E_HIP, "paged: buffer allocation failed"));
-  p->work_bytes = al256(illp::work_size(illp::kStepTarget, 16, d.head_dim));
+  p->work_bytes = al256(illp::work_size(illp::kStepLog, 16, d.head_dim));
   if (hipMalloc(&p->work, p->work_bytes * d.streams) != hipSuccess || hipMemset(p->work, 0, p->work_bytes * d.streams) != hipSuccess ||
       hipDeviceSynchronize() != hipSuccess)
     return bad(fail(ILL_E_HIP, "paged: %d workspaces of %zu bytes cannot be allocated", d.streams, p->work_bytes));
@@ -219,7 +229,7 @@ int ill_paged_attend(ill_paged* p, const ill_paged_batch* batch, const void* q, 
   if (pg_splits(pg_most(cap, cap, s.c), s.c.least) > 1) {
     uint8_t* work = nullptr;
     if (int rc = illp::workspace(p, st, &work)) return rc;
-    s.w = illp::work_of(work, s.c.target, s.c.M, d.head_dim);
+    s.w = illp::work_of(work, s.c.log, s.c.M, d.head_dim);
   }
   if (d.dtype == ILL_F16) {
     if (d.head_dim == 64) illp::launch_step<PG_F16, 64>(s, grid, st);

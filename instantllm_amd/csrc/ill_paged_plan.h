@@ -10,6 +10,7 @@
 
 #define PG_MOST (1 << 30)    // positions, rows x heads, windows and sinks: at most this many
 #define PG_MAXSPLIT 256      // parts that the keys of a tile of rows are cut into at most
+#define PG_FAN 16            // of which so many are joined at a time
 
 // A batch as the kernels read it (ill_paged_batch with the handle's geometry).
 struct PgBatch {
@@ -22,7 +23,7 @@ struct PgBatch {
 
 PG_FN int pg_min(int a, int b) { return a < b ? a : b; }
 PG_FN int pg_max(int a, int b) { return a > b ? a : b; }
-PG_FN int pg_up(int a, int b) { return a / b + (a % b != 0); }   // a / b rounded up, a >= 0
+PG_FN int pg_up(uint32_t a, uint32_t b) { return (int)((a + b - 1) / b); }   // a / b rounded up, a <= 2^30
 
 // Lengths as the kernels use them: none below 0, and none whose positions pass 2^30.
 PG_FN int pg_len(int len) { return pg_min(pg_max(len, 0), PG_MOST); }
@@ -49,16 +50,17 @@ PG_FN bool pg_sees(int p, int j, int window, int sinks) { return j >= 0 && j <= 
 // A sequence's n new rows and the G query heads of a key/value head make n G flat rows (row f / G,
 // head f % G), which read the same keys; M of them are a tile of rows. Keys come in tiles of KT.
 struct PgCut {
-  int32_t G, kv, M, KT, window, sinks;
-  int32_t target;    // parts wanted in all, where there are that many
+  uint32_t G, kv;
+  int32_t M, KT, window, sinks;
+  int32_t log;       // 2^log parts are wanted in all, where there are that many
   int32_t least;     // tiles of keys in a part at least
   int32_t whole;     // from this many tiles of rows on, none is cut
   int32_t lo, hi;    // sequences with lo < n G <= hi are this kernel's
 };
 
 PG_FN int pg_qtiles(int n, const PgCut& c) {
-  const int64_t f = (int64_t)n * c.G;
-  return f > c.lo && f <= c.hi ? (int)((f + c.M - 1) / c.M) : 0;
+  const uint32_t f = (uint32_t)n * c.G;   // (rows x heads: at most 2^30)
+  return f > (uint32_t)c.lo && f <= (uint32_t)c.hi ? (int)((f + c.M - 1) / (uint32_t)c.M) : 0;
 }
 
 // Tiles of keys that rows at positions p0 .. p1 see some of: 0 .. sink - 1, and the ones from lo on, n
@@ -70,7 +72,7 @@ PG_FN PgRange pg_range(int p0, int p1, int cap, const PgCut& c) {
   const int end = pg_min(p1 + 1, cap);
   if (end <= 0) return {0, 0, 0};
   const int hi = pg_up(end, c.KT);
-  const int lo = c.window ? pg_min(pg_max(p0 - c.window + 1, 0) / c.KT, hi) : 0;
+  const int lo = c.window ? pg_min((int)((uint32_t)pg_max(p0 - c.window + 1, 0) / (uint32_t)c.KT), hi) : 0;
   const int sink = pg_min(pg_up(c.sinks, c.KT), lo);
   return {sink, lo, sink + hi - lo};
 }
@@ -80,26 +82,27 @@ PG_FN int pg_key_tile(const PgRange& r, int t) { return t < r.sink ? t : t - r.s
 PG_FN int pg_most(int end, int cap, const PgCut& c) {
   const int all = pg_up(pg_max(pg_min(end, cap), 0), c.KT);
   if (!c.window) return all;
-  const int span = (c.M - 2) / c.G + 2;   // rows that M flat rows reach into
-  const int64_t some = (int64_t)pg_up(c.sinks, c.KT) + ((int64_t)c.window + span - 1 + c.KT - 2) / c.KT + 1;
-  return some < all ? (int)some : all;
+  // M flat rows reach into at most (M - 2) / G + 2 rows
+  const int some = pg_up(c.sinks, c.KT) + pg_up(c.window + (int)((uint32_t)(c.M - 2) / c.G) + c.KT, c.KT) + 1;
+  return pg_min(some, all);
 }
 
 // Tiles of keys in a part, from the sums over the sequences of qtiles x kv (`tiles`) and of qtiles x kv x
 // most (`work`). A sequence is cut into parts if its `most` is over that; the parts of all cut ones are
-// then at most 2 target (most / part + 1 <= 2 most / part each), their tiles of rows at most target.
+// then at most 2 x 2^log (most / part + 1 <= 2 most / part each), their tiles of rows at most 2^log.
 PG_FN int pg_part(int64_t tiles, int64_t work, const PgCut& c) {
   if (tiles >= c.whole) return PG_MOST;
-  const int64_t p = (work + c.target - 1) / c.target;
+  const int64_t p = (work + (1ll << c.log) - 1) >> c.log;
   return p < c.least ? c.least : p < PG_MOST ? (int)p : PG_MOST;
 }
-PG_FN int pg_splits(int most, int part) { return pg_min(pg_max(pg_up(most, part), 1), PG_MAXSPLIT); }
+PG_FN int pg_splits(int most, int part) { return most <= part ? 1 : pg_min(pg_up(most, part), PG_MAXSPLIT); }
 
 // Workgroups that have something to do, at most, as far as the host can tell.
 PG_FN int64_t pg_grid(int seqs, int rows, int64_t max_rows, bool one_row, int cap, const PgCut& c) {
-  int64_t q = (int64_t)rows * c.G / c.M + seqs;
+  const int64_t G = c.G;
+  int64_t q = rows * G / c.M + seqs;
   const int64_t each = one_row ? 1 : max_rows;
-  if (each > 0 && each <= PG_MOST && (each * c.G + c.M - 1) / c.M * seqs < q) q = (each * c.G + c.M - 1) / c.M * seqs;
+  if (each > 0 && each <= PG_MOST && (each * G + c.M - 1) / c.M * seqs < q) q = (each * G + c.M - 1) / c.M * seqs;
   const int64_t tiles = q * c.kv, cut = tiles * pg_splits(pg_most(cap, cap, c), c.least);
-  return cut < tiles + c.target ? cut : tiles + c.target;
+  return cut < tiles + (1 << c.log) ? cut : tiles + (1 << c.log);
 }

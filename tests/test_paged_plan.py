@@ -40,7 +40,7 @@ int main() {
     c.G = draw(1, 20); c.kv = draw(1, 4); c.M = draw(0, 1) ? 16 : 128; c.KT = draw(0, 1) ? 64 : 32;
     c.window = draw(0, 2) ? 0 : draw(1, 300); c.sinks = draw(0, 1) ? 0 : draw(0, 200);
     if (draw(0, 50) == 0) c.window = PG_MOST, c.sinks = PG_MOST;
-    c.target = draw(1, 64); c.least = draw(1, 5); c.whole = draw(0, 1) ? 2147483647 : draw(1, 60); c.lo = draw(0, 1) ? 0 : draw(0, 64); c.hi = draw(0, 3) ? 2147483647 : draw(1, 64);
+    c.log = draw(0, 6); c.least = draw(1, 5); c.whole = draw(0, 1) ? 2147483647 : draw(1, 60); c.lo = draw(0, 1) ? 0 : draw(0, 64); c.hi = draw(0, 3) ? 2147483647 : draw(1, 64);
     const int seqs = draw(1, 6), width = draw(1, 40), log = 4;
     std::vector<PgSeq> seq(seqs);
     int rows = 0, most_rows = 0;
@@ -66,7 +66,7 @@ int main() {
       if (splits > 1) { parts += (long long)t * c.kv * splits; cut += t * c.kv; }
       for (int k = 0; k < t; k++) {
         const int f0 = k * c.M, live = pg_min(c.M, (int)flat - f0);
-        const int p0 = q.p0 + f0 / c.G, p1 = q.p0 + (f0 + live - 1) / c.G;
+        const int G = c.G, p0 = q.p0 + f0 / G, p1 = q.p0 + (f0 + live - 1) / G;
         const PgRange r = pg_range(p0, p1, cap, c);
         CHECK(r.n >= 0 && r.n <= most && r.sink <= r.n);
         // the tiles are distinct, ascending, and inside the cache
@@ -93,7 +93,7 @@ int main() {
         CHECK(next == r.n);
       }
     }
-    CHECK(parts <= 2ll * c.target && cut <= c.target);
+    CHECK(parts <= 2ll << c.log && cut <= 1ll << c.log);
     // the launch has a workgroup for every unit, where the sizes that the host knows hold
     CHECK(units <= pg_grid(seqs, rows, 0, false, cap, c));
     CHECK(units <= pg_grid(seqs, rows, most_rows, false, cap, c));

@@ -9,27 +9,30 @@
 
 enum PgType { PG_F32 = 0, PG_F16 = 1, PG_BF16 = 2 };   // ILL_F32, ILL_F16, ILL_BF16
 
+typedef float v16f __attribute__((ext_vector_type(16)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 #define LAS __attribute__((address_space(3)))   // LDS: named, as GAS is, or an access counts as one to memory too
 
-// Eight values of type T as floats, and back with one rounding to nearest, ties to even.
+// 16-bit values as floats, and back with one rounding to nearest, ties to even.
 template <int T>
-__device__ __forceinline__ void pg_unpack(const uint4* p, float* x) {
+__device__ __forceinline__ void pg_unpack2(uint32_t w, float* x) {
+  if constexpr (T == PG_BF16) {
+    x[0] = __uint_as_float(w << 16);
+    x[1] = __uint_as_float(w & 0xFFFF0000u);
+  } else {
+    x[0] = (float)__builtin_bit_cast(_Float16, (uint16_t)w);
+    x[1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w >> 16));
+  }
+}
+template <int T>
+__device__ __forceinline__ void pg_unpack(const uint4* p, float* x) {   // eight values of type T
   if constexpr (T == PG_F32) {
     *(uint4*)x = p[0];
     *(uint4*)(x + 4) = p[1];
   } else {
     const uint32_t w[4] = {p->x, p->y, p->z, p->w};
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      if constexpr (T == PG_BF16) {
-        x[2 * i] = __uint_as_float(w[i] << 16);
-        x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-      } else {
-        x[2 * i] = (float)__builtin_bit_cast(_Float16, (uint16_t)w[i]);
-        x[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[i] >> 16));
-      }
-    }
+    for (int i = 0; i < 4; i++) pg_unpack2<T>(w[i], x + 2 * i);
   }
 }
 template <int T>
@@ -382,7 +385,7 @@ __device__ __forceinline__ uint4 pg_values(const pg_lds4* v, int key, int nb, in
 }
 
 // Infinities and NaN of eight values: whether there are any; the values with zeros in their place; and marks
-// that a product with ones for the keys a row sees adds up (1 for inf, 64 for -inf, 4096 for NaN; 32 keys).
+// that a product with ones for the keys a row sees adds up (1 for inf, 2^7 for -inf, 2^14 for NaN; at most 64 keys).
 template <int TC>
 __device__ __forceinline__ uint32_t pg_wild2(uint32_t x) {   // the top bit of each half: its exponent is all ones
   constexpr uint32_t E = TC == PG_BF16 ? 0x7F807F80u : 0x7C007C00u, STEP = TC == PG_BF16 ? 0x00800080u : 0x04000400u;
@@ -394,7 +397,7 @@ __device__ __forceinline__ uint32_t pg_wild(uint4 v) {
 }
 template <int TC>
 __device__ __forceinline__ uint4 pg_tamed(uint4 v, uint4& marks) {
-  constexpr uint32_t ONE = TC == PG_BF16 ? 0x3F803F80u : 0x3C003C00u, STEP = TC == PG_BF16 ? 0x03000300u : 0x18001800u;   // 1, and a factor of 64
+  constexpr uint32_t ONE = TC == PG_BF16 ? 0x3F803F80u : 0x3C003C00u, STEP = TC == PG_BF16 ? 0x03800380u : 0x1C001C00u;   // 1, and a factor of 2^7
   constexpr uint32_t S = TC == PG_BF16 ? 0x007F007Fu : 0x03FF03FFu;
   auto all = [](uint32_t top) { return top | (top - (top >> 15)); };   // all bits of the halves whose top bit is set
   uint32_t y[4] = {v.x, v.y, v.z, v.w}, k[4];
@@ -407,11 +410,28 @@ __device__ __forceinline__ uint4 pg_tamed(uint4 v, uint4& marks) {
   marks = {k[0], k[1], k[2], k[3]};
   return {y[0], y[1], y[2], y[3]};
 }
+// Whether a tile of N units has any, for the whole wave.
+template <int TC, int N>
+__device__ __forceinline__ bool pg_wild_tile(const pg_lds4* v, int lane) {
+  uint32_t w = 0;
+#pragma unroll 2
+  for (int i = lane; i < N; i += 64) w |= pg_wild<TC>(pg_get(v + i));
+  return __any(w != 0);
+}
+// Ones for the keys of eight bits.
+template <int TC>
+__device__ __forceinline__ uint4 pg_ones(uint32_t seen) {
+  constexpr uint32_t ONE = TC == PG_BF16 ? 0x3F80u : 0x3C00u;
+  uint32_t y[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) y[i] = (seen >> (2 * i) & 1 ? ONE : 0u) | (seen >> (2 * i + 1) & 1 ? ONE << 16 : 0u);
+  return {y[0], y[1], y[2], y[3]};
+}
 __device__ __forceinline__ float pg_wild_sum(float marks) {
   const int n = (int)marks;
-  float y = n & 63 ? INFINITY : 0.f;
-  if (n >> 6 & 63) y -= INFINITY;
-  return n >> 12 ? NAN : y;
+  float y = n & 127 ? INFINITY : 0.f;
+  if (n >> 7 & 127) y -= INFINITY;
+  return n >> 14 ? NAN : y;
 }
 
 // The exponents' reference of a row follows its greatest score, PG_UP below it, and is moved only when a score
@@ -687,62 +707,50 @@ __global__ __launch_bounds__(64 * NW, 2) void pg_step_kernel(PgStep p) {
       uint4 ph[NS], pl[NS];
 #pragma unroll
       for (int b = 0; b < NB; b++) {
-        float e[4], h[4];
+        float e[4];
 #pragma unroll
         for (int r = 0; r < 4; r++) {
           e[r] = __builtin_amdgcn_exp2f(fmaf(s[b][r], sc2, -ref));
           Ls += e[r];
         }
-        const uint32_t x = pg_pack2<TC>(e[0], e[1]), y = pg_pack2<TC>(e[2], e[3]);
-        (&ph[b >> 1].x)[2 * (b & 1)] = x;
-        (&ph[b >> 1].x)[2 * (b & 1) + 1] = y;
-        if constexpr (FINE) {
 #pragma unroll
-          for (int r = 0; r < 4; r++) {
-            const uint16_t z = (uint16_t)((r < 2 ? x : y) >> (16 * (r & 1)));
-            h[r] = TC == PG_BF16 ? __uint_as_float((uint32_t)z << 16) : (float)__builtin_bit_cast(_Float16, z);
+        for (int r = 0; r < 4; r += 2) {
+          const uint32_t x = pg_pack2<TC>(e[r], e[r + 1]);
+          (&ph[b >> 1].x)[2 * (b & 1) + r / 2] = x;
+          if constexpr (FINE) {
+            float y[2];
+            pg_unpack2<TC>(x, y);
+            (&pl[b >> 1].x)[2 * (b & 1) + r / 2] = pg_pack2<TC>(e[r] - y[0], e[r + 1] - y[1]);
           }
-          (&pl[b >> 1].x)[2 * (b & 1)] = pg_pack2<TC>(e[0] - h[0], e[1] - h[1]);
-          (&pl[b >> 1].x)[2 * (b & 1) + 1] = pg_pack2<TC>(e[2] - h[2], e[3] - h[3]);
         }
       }
       if (more) PG_WAIT(8);   // the values; the 8 loads after them are the next keys
       else PG_WAIT(0);
-      uint32_t wild = 0;
-      if (!whole) {   // what a row does not see must not reach it as 0 x inf
+      bool wild = false;
+      if (!whole) wild = pg_wild_tile<TC, KT * UPR>(vl, lane);   // what a row does not see must not reach it as 0 x inf
+      if (wild) {
 #pragma unroll
-        for (int d = 0; d < ND; d++)
-#pragma unroll
-          for (int t = 0; t < NS; t++) wild |= pg_wild<TC>(pg_values<D>(vl, 32 * t + 8 * kg, d, n));
-        wild = __any(wild);
-      }
-      if (!wild) {
-#pragma unroll
-        for (int d = 0; d < ND; d++)
+        for (int d = 0; d < ND; d++) {
+          v4f m = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int t = 0; t < NS; t++) {
-            const uint4 v = pg_values<D>(vl, 32 * t + 8 * kg, d, n);
-            O[d] = pg_mfma16<TC>(v, ph[t], O[d]);
-            if constexpr (FINE) O[d] = pg_mfma16<TC>(v, pl[t], O[d]);
+            uint4 marks;
+            pg_tamed<TC>(pg_values<D>(vl, 32 * t + 8 * kg, d, n), marks);
+            m = pg_mfma16<TC>(marks, pg_ones<TC>(seen >> (8 * t)), m);
           }
-      } else {
-        constexpr uint32_t ONE = TC == PG_BF16 ? 0x3F80u : 0x3C00u;
 #pragma unroll
-        for (int d = 0; d < ND; d++)
-#pragma unroll
-          for (int t = 0; t < NS; t++) {
-            uint4 marks, ones;
-            const uint4 v = pg_tamed<TC>(pg_values<D>(vl, 32 * t + 8 * kg, d, n), marks);
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-              (&ones.x)[i] = (seen >> (8 * t + 2 * i) & 1 ? ONE : 0u) | (seen >> (8 * t + 2 * i + 1) & 1 ? ONE << 16 : 0u);
-            O[d] = pg_mfma16<TC>(v, ph[t], O[d]);
-            if constexpr (FINE) O[d] = pg_mfma16<TC>(v, pl[t], O[d]);
-            const v4f m = pg_mfma16<TC>(marks, ones, (v4f){0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-            for (int r = 0; r < 4; r++) O[d][r] += pg_wild_sum(m[r]);
-          }
+          for (int r = 0; r < 4; r++) O[d][r] += pg_wild_sum(m[r]);
+        }
       }
+#pragma unroll
+      for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int t = 0; t < NS; t++) {
+          uint4 v = pg_values<D>(vl, 32 * t + 8 * kg, d, n), marks;
+          if (wild) v = pg_tamed<TC>(v, marks);
+          O[d] = pg_mfma16<TC>(v, ph[t], O[d]);
+          if constexpr (FINE) O[d] = pg_mfma16<TC>(v, pl[t], O[d]);
+        }
       PG_WAIT_LDS();   // the values have been read
       if (more) load(a.vc, vl, k + 1);
     }
@@ -776,6 +784,197 @@ __global__ __launch_bounds__(64 * NW, 2) void pg_step_kernel(PgStep p) {
       }
     }
     if (un.splits > 1) pg_finish<TC, D, 16, NW>(a, c, p.w, un, f0, live, (LAS float*)lds, &last);
+    __syncthreads();   // LDS is the next unit's
+  }
+}
+
+template <int TC>
+__device__ __forceinline__ v16f pg_mfma32(uint4 a, uint4 b, v16f c) {   // 32 x 32 x 16
+  if constexpr (TC == PG_BF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+}
+
+// Attention of many rows per sequence. A workgroup of four waves takes 128 flat rows of a key/value head, 32 to a wave;
+// tiles of 64 keys and their values go straight into LDS, one while the one before is evaluated. As in the step kernel,
+// scores are keys x rows and outputs dims x rows (v_mfma 32 x 32 x 16), so a row's statistics are two lanes' own, and
+// the keys are dealt to the score products' rows such that a lane's weights are the next product's operand as they
+// stand (row m of block b: key 32 b + m with bits 2 and 3 of m swapped).
+template <int TC, int D, bool FINE>   // FINE: weights in two parts (float32 outputs)
+__global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
+  constexpr int M = 128, KT = 64, UPR = D / 8, KS = D / 16, ND = D / 32, T = KT * UPR, LOADS = T / 256;   // LOADS: of keys, and of values, per wave and tile
+  __shared__ __attribute__((aligned(16))) uint4 lds[2][2][T];   // [buffer][keys, values]
+  __shared__ int last;
+  __shared__ PgFinder<4>::Lds found;
+  const PgAttend& a = p.a;
+  PgCut c = p.c;
+  c.M = M;   // (as the host has them, for the compiler)
+  c.KT = KT;
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 31, h = lane >> 5;
+  const int cap = pg_cap(a.b), pmask = (1 << a.b.page_log) - 1;
+  const float sc2 = a.scale * 1.4426950408889634f;
+  PgFinder<4> finder(a.b, c, found);
+  auto over_h = [](float v, auto op) {   // over the two lanes of a row
+    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
+    return op(__int_as_float((int)x[0]), __int_as_float((int)x[1]));
+  };
+  // a wave loads 16 keys of a tile, and their values: bytes from the group to what this lane loads of it, per load
+  uint32_t lane_off[LOADS];
+#pragma unroll
+  for (int i = 0; i < LOADS; i++) {
+    const int key = 16 * w + (64 / UPR) * i + lane / UPR;
+    lane_off[i] = 2 * ((uint32_t)(key & 15) * (uint32_t)a.slot_stride + 8 * ((lane % UPR) ^ pg_swz<D>(key)));
+  }
+  for (int u = blockIdx.x; u < finder.units; u += gridDim.x) {
+    const PgUnit un = finder.find(u);
+    if (un.seq.n == 0) continue;
+    const int G = c.G, flat = un.seq.n * G, f0 = M * un.q, live = min(M, flat - f0);   // (n G is at most 2^30)
+    const uint32_t f = min(f0 + 32 * w + n, flat - 1), at_row = f / c.G;
+    const int row = un.seq.first + at_row, head = un.head * G + (f - at_row * c.G);
+    const int pos = un.seq.p0 + at_row, w0 = __builtin_amdgcn_readlane(pos, 0), w1 = __builtin_amdgcn_readlane(pos, 31);   // of the wave's rows
+    const int p0 = un.seq.p0 + (uint32_t)f0 / c.G, p1 = un.seq.p0 + (uint32_t)(f0 + live - 1) / c.G;
+    const PgRange range = pg_range(p0, p1, cap, c);
+    const int per = pg_up(range.n, un.splits), c0 = min(un.split * per, range.n), c1 = min(c0 + per, range.n);
+    const int end = min(p1 + 1, cap), wend = 32 * w < live ? min(w1 + 1, cap) : 0;
+    uint4 qf[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) qf[ks] = gld((const uint4*)(a.q + row * a.qs + (int64_t)head * D + 16 * ks + 8 * h));
+    // where the keys of the next 16 tiles are, 16 of them a lane: elements from the cache's begin; -1: not there
+    int64_t group = -1;
+    auto groups = [&](int k) {
+      const int t = c0 + k + lane / 4;
+      group = -1;
+      if (t < c1) {
+        const int g = pg_key_tile(range, t) * KT + 16 * (lane % 4), key = min(g, end - 1);
+        const int page = gld(a.b.table + un.s * a.b.table_stride + (key >> a.b.page_log));
+        if (page >= 0 && page < a.b.pages) group = page * a.page_stride + (g & pmask) * a.slot_stride + un.head * a.head_stride;
+      }
+    };
+    auto load = [&](int k) {
+      const int at = (4 * k + w) & 63;
+      const int64_t e = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)group, at) |
+                                  (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(group >> 32), at) << 32);
+      const int64_t off = e < 0 ? 0 : e;   // (the first page is there, and masked)
+      pg_lds4* to = (pg_lds4*)lds[k & 1][0] + 64 * LOADS * w;
+#pragma unroll
+      for (int i = 0; i < LOADS; i++) pg_dma16(a.kc + off, lane_off[i], to + 64 * i);
+#pragma unroll
+      for (int i = 0; i < LOADS; i++) pg_dma16(a.vc + off, lane_off[i], to + T + 64 * i);
+    };
+    float Mx = -INFINITY, Ls = 0.f;   // Ls: this lane's keys only
+    v16f O[ND];
+#pragma unroll
+    for (int d = 0; d < ND; d++) O[d] = (v16f){};
+    if (c0 < c1) {
+      groups(0);
+      load(0);
+    }
+    for (int k = 0; c0 + k < c1; k++) {
+      const int kt = pg_key_tile(range, c0 + k) * KT;
+      int good = 0;   // groups of 16 keys whose pages are there
+#pragma unroll
+      for (int g = 0; g < 4; g++) good |= (__builtin_amdgcn_readlane((int)(group >> 32), (4 * k + g) & 63) >= 0) << g;
+      if (c0 + k + 1 < c1 && ((k + 1) & 15) == 0) groups(k + 1);
+      PG_WAIT(0);
+      __syncthreads();   // the tile is there, and every wave is done with the buffer filled next
+      if (c0 + k + 1 < c1) load(k + 1);
+      if (kt >= wend) continue;   // behind all of the wave's rows
+      const pg_lds4* kl = (const pg_lds4*)lds[k & 1][0];
+      const pg_lds4* vl = kl + T;
+      v16f s[2];
+#pragma unroll
+      for (int b = 0; b < 2; b++) {
+        const int key = 32 * b + (n & 19) + ((n & 4) << 1) + ((n & 8) >> 1);
+        s[b] = (v16f){};
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) s[b] = pg_mfma32<TC>(pg_get(kl + pg_unit_at<D>(key, 2 * ks + h)), qf[ks], s[b]);
+      }
+      // every row sees the whole tile, or the rows' masks (wave-uniform)
+      const bool whole = good == 15 && kt + KT - 1 <= w0 && kt + KT <= wend && (c.window == 0 || kt > w1 - c.window || kt + KT <= c.sinks);
+      uint32_t seen = ~0u;
+      if (!whole) {
+        seen = 0;
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) {
+            const int key = 32 * b + 16 * (r >> 3) + 8 * h + (r & 7), j = kt + key;
+            const bool on = j < cap && pg_sees(pos, j, c.window, c.sinks) && (good >> (2 * b + (r >> 3)) & 1);
+            if (!on) s[b][r] = -INFINITY;
+            seen |= (uint32_t)on << (16 * b + r);
+          }
+      }
+      float mc = s[0][0];
+#pragma unroll
+      for (int b = 0; b < 2; b++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) mc = fmaxf(mc, s[b][r]);
+      mc *= sc2;
+      if (__any(mc > Mx + (PG_UP + PG_SLACK))) {
+        mc = over_h(mc, OpMaxF{});
+        const float mn = mc == -INFINITY ? Mx : fmaxf(mc - PG_UP, Mx), up = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(Mx - mn);
+        Mx = mn;
+        Ls *= up;
+#pragma unroll
+        for (int d = 0; d < ND; d++) O[d] *= up;
+      }
+      const float ref = Mx == -INFINITY ? 0.f : Mx;
+      uint4 ph[4], pl[4];   // weights of 16 keys each
+#pragma unroll
+      for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          const float e0 = __builtin_amdgcn_exp2f(fmaf(s[t >> 1][8 * (t & 1) + i], sc2, -ref)), e1 = __builtin_amdgcn_exp2f(fmaf(s[t >> 1][8 * (t & 1) + i + 1], sc2, -ref));
+          Ls += e0 + e1;
+          const uint32_t x = pg_pack2<TC>(e0, e1);
+          (&ph[t].x)[i >> 1] = x;
+          if constexpr (FINE) {
+            float y[2];
+            pg_unpack2<TC>(x, y);
+            (&pl[t].x)[i >> 1] = pg_pack2<TC>(e0 - y[0], e1 - y[1]);
+          }
+        }
+      bool wild = false;
+      if (!whole) wild = pg_wild_tile<TC, T>(vl, lane);   // what a row does not see must not reach it as 0 x inf
+      const int vn = (lane >> 4) & 1, vi = lane & 15;
+      if (wild) {
+#pragma unroll
+        for (int d = 0; d < ND; d++) {
+          v16f m = {};
+#pragma unroll
+          for (int t = 0; t < 4; t++) {
+            uint4 marks;
+            pg_tamed<TC>(pg_values<D>(vl, 16 * t + 8 * h, 2 * d + vn, vi), marks);
+            m = pg_mfma32<TC>(marks, pg_ones<TC>(seen >> (8 * t)), m);
+          }
+#pragma unroll
+          for (int r = 0; r < 16; r++) O[d][r] += pg_wild_sum(m[r]);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int d = 0; d < ND; d++) {
+          uint4 v = pg_values<D>(vl, 16 * t + 8 * h, 2 * d + vn, vi), marks;
+          if (wild) v = pg_tamed<TC>(v, marks);
+          O[d] = pg_mfma32<TC>(v, ph[t], O[d]);
+          if constexpr (FINE) O[d] = pg_mfma32<TC>(v, pl[t], O[d]);
+        }
+    }
+    Ls = over_h(Ls, OpAddF{});
+    const int r = 32 * w + n;
+    if (r < live) {
+      const float inv = Ls == 0.f ? 0.f : 1.f / Ls;
+#pragma unroll
+      for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const v4f o = {O[d][4 * i], O[d][4 * i + 1], O[d][4 * i + 2], O[d][4 * i + 3]};
+          const int dim = 32 * d + 8 * i + 4 * h;
+          if (un.splits == 1) pg_store<TC>(a, row, head, dim, D, Ls == 0.f ? (v4f){0.f, 0.f, 0.f, 0.f} : o * inv);
+          else pg_put_part<D, M>(p.w, un.part_at + un.split, r, dim, Mx, Ls, o);
+        }
+    }
+    if (un.splits > 1) pg_finish<TC, D, M, 4>(a, c, p.w, un, f0, live, (LAS float*)lds, &last);
     __syncthreads();   // LDS is the next unit's
   }
 }

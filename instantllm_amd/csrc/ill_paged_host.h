@@ -38,20 +38,23 @@ PgBatch batch_of(const ill_paged* p, const ill_paged_batch& b) {
   return {b.lens, b.table, b.row0, b.table_stride, b.pages, b.seqs, (int)b.rows, b.table_width, p->page_log};
 }
 
-// Parts of a call of few rows per sequence: two workgroups per CU, and no part below four tiles of keys, one for each wave.
 #ifndef STEP_NW
 #define STEP_NW 4
 #endif
-#ifndef STEP_LOG
-#define STEP_LOG 8
+#ifndef PROMPT_FROM
+#define PROMPT_FROM 32
 #endif
-#ifndef STEP_LEAST
-#define STEP_LEAST 8
+#ifndef PROMPT_WHOLE
+#define PROMPT_WHOLE 256
 #endif
-constexpr int kStepLog = STEP_LOG, kStepLeast = STEP_LEAST;
+constexpr int kLog = 8;            // parts wanted: 2^8, one workgroup per CU
+constexpr int kFew = PROMPT_FROM;  // flat rows of a sequence up to which the step kernel takes it
 
 PgCut step_cut(const ill_paged_desc& d, int window, int sinks) {
-  return {(uint32_t)(d.heads / d.kv_heads), (uint32_t)d.kv_heads, 16, d.head_dim == 64 ? 64 : 32, window, sinks, kStepLog, kStepLeast, INT32_MAX, 0, INT32_MAX};
+  return {(uint32_t)(d.heads / d.kv_heads), (uint32_t)d.kv_heads, 16, d.head_dim == 64 ? 64 : 32, window, sinks, kLog, 8, INT32_MAX, 0, INT32_MAX};
+}
+PgCut prompt_cut(const ill_paged_desc& d, int window, int sinks) {
+  return {(uint32_t)(d.heads / d.kv_heads), (uint32_t)d.kv_heads, 128, 64, window, sinks, kLog, 4, PROMPT_WHOLE, 0, INT32_MAX};
 }
 
 // Bytes of a workspace where 2^log parts are wanted, over tiles of M rows.
@@ -89,9 +92,14 @@ int workspace(ill_paged* p, hipStream_t st, uint8_t** out) {
 }
 
 template <int TC, int D>
-void launch_step(const PgStep& s, int64_t grid, hipStream_t st) {
-  if (s.a.out_f32) hipLaunchKernelGGL((pg_step_kernel<TC, D, true, STEP_NW>), dim3(grid), dim3(64 * STEP_NW), 0, st, s);
-  else hipLaunchKernelGGL((pg_step_kernel<TC, D, false, STEP_NW>), dim3(grid), dim3(64 * STEP_NW), 0, st, s);
+void launch_attend(const PgStep& s, int64_t grid, hipStream_t st) {
+  if (s.c.M == 16) {
+    if (s.a.out_f32) hipLaunchKernelGGL((pg_step_kernel<TC, D, true, STEP_NW>), dim3(grid), dim3(64 * STEP_NW), 0, st, s);
+    else hipLaunchKernelGGL((pg_step_kernel<TC, D, false, STEP_NW>), dim3(grid), dim3(64 * STEP_NW), 0, st, s);
+  } else {
+    if (s.a.out_f32) hipLaunchKernelGGL((pg_prompt_kernel<TC, D, true>), dim3(grid), dim3(256), 0, st, s);
+    else hipLaunchKernelGGL((pg_prompt_kernel<TC, D, false>), dim3(grid), dim3(256), 0, st, s);
+  }
 }
 
 template <int TX, int TC>
@@ -132,7 +140,7 @@ int ill_paged_create(const ill_paged_desc* desc, ill_paged** out) {
   for (int i = 0; i < d.rotary_dim / 2; i++) freq[i] = std::pow(d.rope_base, -2.0 * i / d.rotary_dim) / (2 * M_PI);
   if (hipMalloc(&p->freq, sizeof freq) != hipSuccess || hipMemcpy(p->freq, freq, sizeof freq, hipMemcpyHostToDevice) != hipSuccess)
     return bad(fail(ILL_E_HIP, "paged: buffer allocation failed"));
-  p->work_bytes = al256(illp::work_size(illp::kStepLog, 16, d.head_dim));
+  p->work_bytes = al256(illp::work_size(illp::kLog, 128, d.head_dim));
   if (hipMalloc(&p->work, p->work_bytes * d.streams) != hipSuccess || hipMemset(p->work, 0, p->work_bytes * d.streams) != hipSuccess ||
       hipDeviceSynchronize() != hipSuccess)
     return bad(fail(ILL_E_HIP, "paged: %d workspaces of %zu bytes cannot be allocated", d.streams, p->work_bytes));
@@ -223,20 +231,29 @@ int ill_paged_attend(ill_paged* p, const ill_paged_batch* batch, const void* q, 
   illp::OnDevice on(p->device);
   if (on.rc) return on.rc;
   hipStream_t st = (hipStream_t)stream;
-  PgStep s{a, illp::step_cut(d, a.window, a.sinks), {}};
+  // One of the kernels where it is known that no sequence has many new rows, or that the only one may; else both, each
+  // with the sequences that are its own.
+  const int64_t most = !a.b.row0 ? 1 : std::min<int64_t>(a.b.rows, batch->max_rows ? batch->max_rows : a.b.rows), G = d.heads / d.kv_heads;
+  const bool few = most * G <= illp::kFew, both = !few && a.b.seqs > 1;
+  PgStep parts[2] = {{a, illp::step_cut(d, a.window, a.sinks), {}}, {a, illp::prompt_cut(d, a.window, a.sinks), {}}};
+  if (both) parts[0].c.hi = parts[1].c.lo = illp::kFew;
   const int cap = pg_cap(a.b);
-  const int64_t grid = std::min<int64_t>(pg_grid(a.b.seqs, a.b.rows, batch->max_rows, !a.b.row0, cap, s.c), 1 << 20);
-  if (pg_splits(pg_most(cap, cap, s.c), s.c.least) > 1) {
-    uint8_t* work = nullptr;
-    if (int rc = illp::workspace(p, st, &work)) return rc;
-    s.w = illp::work_of(work, s.c.log, s.c.M, d.head_dim);
-  }
-  if (d.dtype == ILL_F16) {
-    if (d.head_dim == 64) illp::launch_step<PG_F16, 64>(s, grid, st);
-    else illp::launch_step<PG_F16, 128>(s, grid, st);
-  } else {
-    if (d.head_dim == 64) illp::launch_step<PG_BF16, 64>(s, grid, st);
-    else illp::launch_step<PG_BF16, 128>(s, grid, st);
+  uint8_t* work = nullptr;
+  for (int i = few ? 0 : both ? 0 : 1; i < (few ? 1 : 2); i++)
+    if (pg_splits(pg_most(cap, cap, parts[i].c), parts[i].c.least) > 1 && !work)
+      if (int rc = illp::workspace(p, st, &work)) return rc;
+  for (int i = few ? 0 : both ? 0 : 1; i < (few ? 1 : 2); i++) {
+    PgStep& s = parts[i];
+    const int64_t grid = std::min<int64_t>(pg_grid(a.b.seqs, a.b.rows, i == 0 && both ? illp::kFew / G : batch->max_rows, !a.b.row0, cap, s.c), 1 << 20);
+    if (!grid) continue;
+    if (work) s.w = illp::work_of(work, s.c.log, s.c.M, d.head_dim);
+    if (d.dtype == ILL_F16) {
+      if (d.head_dim == 64) illp::launch_attend<PG_F16, 64>(s, grid, st);
+      else illp::launch_attend<PG_F16, 128>(s, grid, st);
+    } else {
+      if (d.head_dim == 64) illp::launch_attend<PG_BF16, 64>(s, grid, st);
+      else illp::launch_attend<PG_BF16, 128>(s, grid, st);
+    }
   }
   HCK(hipGetLastError());
   return ILL_OK;

@@ -36,11 +36,12 @@ __device__ __forceinline__ void pg_unpack(const uint4* p, float* x) {   // eight
   }
 }
 template <int T>
-__device__ __forceinline__ uint32_t pg_pack2(float a, float b) {
-  if constexpr (T == PG_BF16)
-    return (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)a) | (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)b) << 16;
-  else
-    return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)a) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)b) << 16;
+__device__ __forceinline__ uint32_t pg_pack2(float a, float b) {   // (as a pair: one instruction)
+  typedef float v2f __attribute__((ext_vector_type(2)));
+  typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+  typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+  if constexpr (T == PG_BF16) return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){a, b}, v2bf));
+  else return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){a, b}, v2h));
 }
 template <int T>
 __device__ __forceinline__ uint4 pg_pack8(const float* x) {
@@ -211,6 +212,12 @@ struct PgUnit {
   PgSeq seq;
 };
 
+// The same unit, held as values that the compiler knows to be every lane's.
+__device__ __forceinline__ PgUnit pg_uniform(const PgUnit& u) {
+  auto one = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+  return {one(u.s), one(u.head), one(u.q), one(u.split), one(u.splits), one(u.part_at), one(u.tile_at), {one(u.seq.first), one(u.seq.n), one(u.seq.p0)}};
+}
+
 // The division of a call's work, found by every workgroup of NW waves from the lengths: sequence s is thread s % NT's.
 template <int NW>
 struct PgFinder {
@@ -349,7 +356,7 @@ __device__ __forceinline__ v4f pg_mfma16(uint4 a, uint4 b, v4f c) {   // 16 x 16
 // 16 bytes from base + each lane's offset into LDS, lane i's at lds + 16 i. In inline assembly, because the
 // compiler cannot tell the buffers apart and would wait for every load in flight before each LDS read;
 // the kernels wait themselves (PG_WAIT), and extra loads of the compiler's own only make that wait longer.
-__device__ __forceinline__ void pg_dma16(const void* base, uint32_t off, const LAS gu32x4* lds) {   // base: the same for every lane
+__device__ __forceinline__ void pg_dma16(const void* base, uint32_t off, const LAS uint8_t* lds) {   // base: the same for every lane
   const uint32_t m = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m), "v"(off), "s"(base) : "memory");
 }
@@ -366,22 +373,25 @@ __device__ __forceinline__ int pg_swz(int key) {
 template <int D>
 __device__ __forceinline__ int pg_unit_at(int key, int u) { return key * (D / 8) + (u ^ pg_swz<D>(key)); }
 
-// Four keys (key, .., key + 3) of dim 16 nb + lane % 16, from the rows of a tile of values: each 16 lanes read
-// 4 keys x 16 dims, and the transposing read hands lane i its dim.
-__device__ __forceinline__ uint2 pg_tr(const LAS gu32x4* p, int bytes) {
-  typedef short v4s __attribute__((ext_vector_type(4)));
-  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LAS v4s*)((const LAS uint8_t*)p + bytes)));
-}
 typedef LAS gu32x4 pg_lds4;   // 16 bytes of a tile
-__device__ __forceinline__ uint4 pg_get(const pg_lds4* p) {
-  const gu32x4 x = *p;
+__device__ __forceinline__ uint4 pg_get(const LAS uint8_t* p) {
+  const gu32x4 x = *(const pg_lds4*)p;
   return {x[0], x[1], x[2], x[3]};
 }
+// Keys key .. key + 7 of dim d0 + i, d0 a multiple of 16, from the rows of a tile of values; `p` is where pg_values_at says.
+// Each 16 lanes read 4 keys x 16 dims twice, and the transposing read hands lane i its dim.
+__device__ __forceinline__ uint2 pg_tr(const LAS uint8_t* p) {
+  typedef short v4s __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LAS v4s*)p));
+}
 template <int D>
-__device__ __forceinline__ uint4 pg_values(const pg_lds4* v, int key, int nb, int i) {   // keys key .. key + 7
-  const int u = 2 * nb + ((i >> 1) & 1), k0 = key + (i >> 2), k1 = k0 + 4;
-  const uint2 a = pg_tr(v + pg_unit_at<D>(k0, u), 8 * (i & 1)), b = pg_tr(v + pg_unit_at<D>(k1, u), 8 * (i & 1));
+__device__ __forceinline__ uint4 pg_values(const LAS uint8_t* p) {
+  const uint2 a = pg_tr(p), b = pg_tr(p + 4 * 2 * D);   // (the permutation ignores bit 2 of the key)
   return {a.x, a.y, b.x, b.y};
+}
+template <int D>
+__device__ __forceinline__ int pg_values_at(int key, int d0, int i) {
+  return 16 * pg_unit_at<D>(key + (i >> 2), d0 / 8 + ((i >> 1) & 1)) + 8 * (i & 1);
 }
 
 // Infinities and NaN of eight values: whether there are any; the values with zeros in their place; and marks
@@ -412,10 +422,10 @@ __device__ __forceinline__ uint4 pg_tamed(uint4 v, uint4& marks) {
 }
 // Whether a tile of N units has any, for the whole wave.
 template <int TC, int N>
-__device__ __forceinline__ bool pg_wild_tile(const pg_lds4* v, int lane) {
+__device__ __forceinline__ bool pg_wild_tile(const LAS uint8_t* v, int lane) {
   uint32_t w = 0;
 #pragma unroll 2
-  for (int i = lane; i < N; i += 64) w |= pg_wild<TC>(pg_get(v + i));
+  for (int i = lane; i < N; i += 64) w |= pg_wild<TC>(pg_get(v + 16 * i));
   return __any(w != 0);
 }
 // Ones for the keys of eight bits.
@@ -439,6 +449,9 @@ __device__ __forceinline__ float pg_wild_sum(float marks) {
 // keeps its 11 bits down to 2^-24 of the greatest one.
 #define PG_UP 10.f
 #define PG_SLACK 5.f
+#ifndef PG_AHEAD
+#define PG_AHEAD 3
+#endif
 
 struct PgWork {        // a call's share of the handle's workspace
   float2* ml;          // [2 target][M] reference and sum of a part's rows
@@ -590,8 +603,15 @@ __global__ __launch_bounds__(64 * NW, 2) void pg_step_kernel(PgStep p) {
   c.KT = KT;
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, kg = lane >> 4;
   const int cap = pg_cap(a.b), pmask = (1 << a.b.page_log) - 1;
-  pg_lds4* kl = (pg_lds4*)lds[w];
-  pg_lds4* vl = kl + 512;
+  LAS uint8_t* kl = (LAS uint8_t*)lds[w];
+  LAS uint8_t* vl = kl + 8192;
+  // this lane's operands in a tile: of the keys for each 32 dims, of the values for each 16. Other keys of the lane's are
+  // whole multiples of 4 or 32 rows further: the permutation does not see them.
+  int ka[KS], va[ND];
+#pragma unroll
+  for (int ks = 0; ks < KS; ks++) ka[ks] = 16 * pg_unit_at<D>(8 * (n >> 2) + (n & 3), 4 * ks + kg);
+#pragma unroll
+  for (int d = 0; d < ND; d++) va[d] = pg_values_at<D>(8 * kg, 16 * d, n);
   const float sc2 = a.scale * 1.4426950408889634f;
   PgFinder<NW> finder(a.b, c, found);
   auto over_kg = [](float v, auto op) {   // over the lanes of the same row
@@ -606,8 +626,8 @@ __global__ __launch_bounds__(64 * NW, 2) void pg_step_kernel(PgStep p) {
     const int key = KPI * i + lane / UPR;
     lane_off[i] = 2 * ((uint32_t)(key & 15) * (uint32_t)a.slot_stride + 8 * ((lane % UPR) ^ pg_swz<D>(key)));
   }
-  for (int u = blockIdx.x; u < finder.units; u += gridDim.x) {
-    const PgUnit un = finder.find(u);
+  for (int u = blockIdx.x, units = __builtin_amdgcn_readfirstlane(finder.units); u < units; u += gridDim.x) {
+    const PgUnit un = pg_uniform(finder.find(u));
     if (un.seq.n == 0) continue;
     const int G = c.G, flat = un.seq.n * G, f0 = 16 * un.q, live = min(16, flat - f0);   // (n G is at most 2^30)
     const uint32_t f = min(f0 + n, flat - 1), at_row = f / c.G;
@@ -636,13 +656,13 @@ __global__ __launch_bounds__(64 * NW, 2) void pg_step_kernel(PgStep p) {
       return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)group, at) |
                        (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(group >> 32), at) << 32);
     };
-    auto load = [&](const uint16_t* from, pg_lds4* to, int k) {
+    auto load = [&](const uint16_t* from, LAS uint8_t* to, int k) {
 #pragma unroll
       for (int g = 0; g < NG; g++) {
         const int64_t at = group_at(k, g);
         const uint16_t* base = from + (at < 0 ? 0 : at);   // (the first page is there, and masked)
 #pragma unroll
-        for (int i = g * 8 / NG; i < (g + 1) * 8 / NG; i++) pg_dma16(base, lane_off[i], to + 64 * i);
+        for (int i = g * 8 / NG; i < (g + 1) * 8 / NG; i++) pg_dma16(base, lane_off[i], to + 1024 * i);
       }
     };
     float Mx = -INFINITY, Ls = 0.f;   // Ls: this lane's keys only
@@ -664,10 +684,9 @@ __global__ __launch_bounds__(64 * NW, 2) void pg_step_kernel(PgStep p) {
       v4f s[NB];
 #pragma unroll
       for (int b = 0; b < NB; b++) {
-        const int key = 32 * (b >> 1) + 8 * (n >> 2) + 4 * (b & 1) + (n & 3);
         s[b] = (v4f){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++) s[b] = pg_mfma16<TC>(pg_get(kl + pg_unit_at<D>(key, 4 * ks + kg)), qf[ks], s[b]);
+        for (int ks = 0; ks < KS; ks++) s[b] = pg_mfma16<TC>(pg_get(kl + ka[ks] + (32 * (b >> 1) + 4 * (b & 1)) * 2 * D), qf[ks], s[b]);
       }
       PG_WAIT_LDS();   // the keys have been read
       if (more) {
@@ -735,22 +754,24 @@ __global__ __launch_bounds__(64 * NW, 2) void pg_step_kernel(PgStep p) {
 #pragma unroll
           for (int t = 0; t < NS; t++) {
             uint4 marks;
-            pg_tamed<TC>(pg_values<D>(vl, 32 * t + 8 * kg, d, n), marks);
+            const uint4 v = pg_tamed<TC>(pg_values<D>(vl + va[d] + 32 * t * 2 * D), marks);
+            O[d] = pg_mfma16<TC>(v, ph[t], O[d]);
+            if constexpr (FINE) O[d] = pg_mfma16<TC>(v, pl[t], O[d]);
             m = pg_mfma16<TC>(marks, pg_ones<TC>(seen >> (8 * t)), m);
           }
 #pragma unroll
           for (int r = 0; r < 4; r++) O[d][r] += pg_wild_sum(m[r]);
         }
-      }
+      } else {
 #pragma unroll
       for (int d = 0; d < ND; d++)
 #pragma unroll
         for (int t = 0; t < NS; t++) {
-          uint4 v = pg_values<D>(vl, 32 * t + 8 * kg, d, n), marks;
-          if (wild) v = pg_tamed<TC>(v, marks);
+          const uint4 v = pg_values<D>(vl + va[d] + 32 * t * 2 * D);
           O[d] = pg_mfma16<TC>(v, ph[t], O[d]);
           if constexpr (FINE) O[d] = pg_mfma16<TC>(v, pl[t], O[d]);
         }
+      }
       PG_WAIT_LDS();   // the values have been read
       if (more) load(a.vc, vl, k + 1);
     }
@@ -794,6 +815,20 @@ __device__ __forceinline__ v16f pg_mfma32(uint4 a, uint4 b, v16f c) {   // 32 x 
   else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
+// Asks for N products of R LDS reads each in this order: the reads of the first three, then a product and a later one's
+// reads in turn, so that a product's operand has been on its way for three products.
+template <int R, int N>
+__device__ __forceinline__ void pg_ahead() {
+  constexpr int READ = 0x100, MFMA = 0x8, A = N < PG_AHEAD ? N : PG_AHEAD;
+  __builtin_amdgcn_sched_group_barrier(READ, R * A, 0);
+#pragma unroll
+  for (int i = 0; i < N - A; i++) {
+    __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(READ, R, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(MFMA, A, 0);
+}
+
 // Attention of many rows per sequence. A workgroup of four waves takes 128 flat rows of a key/value head, 32 to a wave;
 // tiles of 64 keys and their values go straight into LDS, one while the one before is evaluated. As in the step kernel,
 // scores are keys x rows and outputs dims x rows (v_mfma 32 x 32 x 16), so a row's statistics are two lanes' own, and
@@ -817,20 +852,32 @@ __global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
     const auto x = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
     return op(__int_as_float((int)x[0]), __int_as_float((int)x[1]));
   };
-  // a wave loads 16 keys of a tile, and their values: bytes from the group to what this lane loads of it, per load
-  uint32_t lane_off[LOADS];
+  // a wave loads 16 keys of a tile, and their values: bytes from the group to what this lane loads of its first and last
+  // 8 keys; with LOADS 4, every second load is 4 keys further
+  uint32_t lane_off[2];
 #pragma unroll
-  for (int i = 0; i < LOADS; i++) {
-    const int key = 16 * w + (64 / UPR) * i + lane / UPR;
+  for (int i = 0; i < 2; i++) {
+    const int key = 16 * w + 8 * i + lane / UPR;
     lane_off[i] = 2 * ((uint32_t)(key & 15) * (uint32_t)a.slot_stride + 8 * ((lane % UPR) ^ pg_swz<D>(key)));
   }
-  for (int u = blockIdx.x; u < finder.units; u += gridDim.x) {
-    const PgUnit un = finder.find(u);
+  static_assert(LOADS == 2 || LOADS == 4, "two or four keys x 16 bytes x lanes");
+  // this lane's operands in a tile: of the keys for each 16 dims, of the values for each 32 and for even and odd 16 keys;
+  // others are whole multiples of 32 rows further
+  const int vn = (lane >> 4) & 1, vi = lane & 15;
+  int ka[KS], va[ND][2];
+#pragma unroll
+  for (int ks = 0; ks < KS; ks++) ka[ks] = 16 * pg_unit_at<D>((n & 19) + ((n & 4) << 1) + ((n & 8) >> 1), 2 * ks + h);
+#pragma unroll
+  for (int d = 0; d < ND; d++)
+#pragma unroll
+    for (int t = 0; t < 2; t++) va[d][t] = pg_values_at<D>(16 * t + 8 * h, 32 * d + 16 * vn, vi);
+  for (int u = blockIdx.x, units = __builtin_amdgcn_readfirstlane(finder.units); u < units; u += gridDim.x) {
+    const PgUnit un = pg_uniform(finder.find(u));
     if (un.seq.n == 0) continue;
     const int G = c.G, flat = un.seq.n * G, f0 = M * un.q, live = min(M, flat - f0);   // (n G is at most 2^30)
     const uint32_t f = min(f0 + 32 * w + n, flat - 1), at_row = f / c.G;
     const int row = un.seq.first + at_row, head = un.head * G + (f - at_row * c.G);
-    const int pos = un.seq.p0 + at_row, w0 = __builtin_amdgcn_readlane(pos, 0), w1 = __builtin_amdgcn_readlane(pos, 31);   // of the wave's rows
+    const int row_pos = un.seq.p0 + at_row, w0 = __builtin_amdgcn_readlane(row_pos, 0), w1 = __builtin_amdgcn_readlane(row_pos, 31);   // of the wave's rows
     const int p0 = un.seq.p0 + (uint32_t)f0 / c.G, p1 = un.seq.p0 + (uint32_t)(f0 + live - 1) / c.G;
     const PgRange range = pg_range(p0, p1, cap, c);
     const int per = pg_up(range.n, un.splits), c0 = min(un.split * per, range.n), c1 = min(c0 + per, range.n);
@@ -854,11 +901,11 @@ __global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
       const int64_t e = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)group, at) |
                                   (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(group >> 32), at) << 32);
       const int64_t off = e < 0 ? 0 : e;   // (the first page is there, and masked)
-      pg_lds4* to = (pg_lds4*)lds[k & 1][0] + 64 * LOADS * w;
+      LAS uint8_t* to = (LAS uint8_t*)lds[k & 1][0] + 1024 * LOADS * w;
 #pragma unroll
-      for (int i = 0; i < LOADS; i++) pg_dma16(a.kc + off, lane_off[i], to + 64 * i);
+      for (int i = 0; i < LOADS; i++) pg_dma16(a.kc + off + (LOADS == 4 && (i & 1) ? 4 * a.slot_stride : 0), lane_off[i * 2 / LOADS], to + 1024 * i);
 #pragma unroll
-      for (int i = 0; i < LOADS; i++) pg_dma16(a.vc + off, lane_off[i], to + T + 64 * i);
+      for (int i = 0; i < LOADS; i++) pg_dma16(a.vc + off + (LOADS == 4 && (i & 1) ? 4 * a.slot_stride : 0), lane_off[i * 2 / LOADS], to + 16 * T + 1024 * i);
     };
     float Mx = -INFINITY, Ls = 0.f;   // Ls: this lane's keys only
     v16f O[ND];
@@ -868,38 +915,43 @@ __global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
       groups(0);
       load(0);
     }
-    for (int k = 0; c0 + k < c1; k++) {
-      const int kt = pg_key_tile(range, c0 + k) * KT;
-      int good = 0;   // groups of 16 keys whose pages are there
+    const int count = c1 - c0;
+    int kt, good;   // first key of tile k, and which of its groups of 16 keys have pages
+    auto look = [&](int k) {   // whether every row of the wave sees the whole tile (the same for every lane)
+      kt = pg_key_tile(range, c0 + k) * KT;
+      good = 0;
 #pragma unroll
       for (int g = 0; g < 4; g++) good |= (__builtin_amdgcn_readlane((int)(group >> 32), (4 * k + g) & 63) >= 0) << g;
-      if (c0 + k + 1 < c1 && ((k + 1) & 15) == 0) groups(k + 1);
+      return good == 15 && kt + KT - 1 <= w0 && kt + KT <= wend && (c.window == 0 || kt > w1 - c.window || kt + KT <= c.sinks);
+    };
+    auto advance = [&](int k) {   // tile k is there, every wave is done with the buffer filled next, and that one's loads begin
+      if (k + 1 < count && ((k + 1) & 15) == 0) groups(k + 1);
       PG_WAIT(0);
-      __syncthreads();   // the tile is there, and every wave is done with the buffer filled next
-      if (c0 + k + 1 < c1) load(k + 1);
-      if (kt >= wend) continue;   // behind all of the wave's rows
-      const pg_lds4* kl = (const pg_lds4*)lds[k & 1][0];
-      const pg_lds4* vl = kl + T;
-      v16f s[2];
+      __syncthreads();
+      if (k + 1 < count) load(k + 1);
+    };
+    auto eval = [&](int k, auto masked) {
+      const LAS uint8_t* kl = (const LAS uint8_t*)lds[k & 1][0];
+      const LAS uint8_t* vl = kl + 16 * T;
+      v16f s[2] = {};
 #pragma unroll
-      for (int b = 0; b < 2; b++) {
-        const int key = 32 * b + (n & 19) + ((n & 4) << 1) + ((n & 8) >> 1);
-        s[b] = (v16f){};
+      for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++) s[b] = pg_mfma32<TC>(pg_get(kl + pg_unit_at<D>(key, 2 * ks + h)), qf[ks], s[b]);
-      }
-      // every row sees the whole tile, or the rows' masks (wave-uniform)
-      const bool whole = good == 15 && kt + KT - 1 <= w0 && kt + KT <= wend && (c.window == 0 || kt > w1 - c.window || kt + KT <= c.sinks);
+        for (int b = 0; b < 2; b++) s[b] = pg_mfma32<TC>(pg_get(kl + ka[ks] + 32 * b * 2 * D), qf[ks], s[b]);
+      if constexpr (!masked.value) pg_ahead<1, 2 * KS>();
       uint32_t seen = ~0u;
-      if (!whole) {
+      if constexpr (masked.value) {
         seen = 0;
+        // (opaque here, so that what masks need is not held in registers throughout)
+        int pos = row_pos, h = lane >> 5;
+        asm("" : "+v"(pos), "+v"(h));
 #pragma unroll
         for (int b = 0; b < 2; b++)
 #pragma unroll
           for (int r = 0; r < 16; r++) {
             const int key = 32 * b + 16 * (r >> 3) + 8 * h + (r & 7), j = kt + key;
-            const bool on = j < cap && pg_sees(pos, j, c.window, c.sinks) && (good >> (2 * b + (r >> 3)) & 1);
-            if (!on) s[b][r] = -INFINITY;
+            const bool on = j < cap & j <= pos & (c.window == 0 | j > pos - c.window | j < c.sinks) & (good >> (2 * b + (r >> 3)) & 1);   // pg_sees
+            s[b][r] = on ? s[b][r] : -INFINITY;
             seen |= (uint32_t)on << (16 * b + r);
           }
       }
@@ -920,11 +972,12 @@ __global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
       const float ref = Mx == -INFINITY ? 0.f : Mx;
       uint4 ph[4], pl[4];   // weights of 16 keys each
 #pragma unroll
-      for (int t = 0; t < 4; t++)
+      for (int t = 0; t < 4; t++) {
+        float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
           const float e0 = __builtin_amdgcn_exp2f(fmaf(s[t >> 1][8 * (t & 1) + i], sc2, -ref)), e1 = __builtin_amdgcn_exp2f(fmaf(s[t >> 1][8 * (t & 1) + i + 1], sc2, -ref));
-          Ls += e0 + e1;
+          sum += e0 + e1;
           const uint32_t x = pg_pack2<TC>(e0, e1);
           (&ph[t].x)[i >> 1] = x;
           if constexpr (FINE) {
@@ -933,32 +986,51 @@ __global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
             (&pl[t].x)[i >> 1] = pg_pack2<TC>(e0 - y[0], e1 - y[1]);
           }
         }
-      bool wild = false;
-      if (!whole) wild = pg_wild_tile<TC, T>(vl, lane);   // what a row does not see must not reach it as 0 x inf
-      const int vn = (lane >> 4) & 1, vi = lane & 15;
-      if (wild) {
+        Ls += sum;
+      }
+      if constexpr (masked.value) {
+        int from = lane;
+        asm("" : "+v"(from));
+        if (pg_wild_tile<TC, T>(vl, from)) {   // what a row does not see must not reach it as 0 x inf
 #pragma unroll
-        for (int d = 0; d < ND; d++) {
-          v16f m = {};
+          for (int d = 0; d < ND; d++) {
+            v16f m = {};
 #pragma unroll
-          for (int t = 0; t < 4; t++) {
-            uint4 marks;
-            pg_tamed<TC>(pg_values<D>(vl, 16 * t + 8 * h, 2 * d + vn, vi), marks);
-            m = pg_mfma32<TC>(marks, pg_ones<TC>(seen >> (8 * t)), m);
+            for (int t = 0; t < 4; t++) {
+              uint4 marks;
+              const uint4 v = pg_tamed<TC>(pg_values<D>(vl + va[d][t & 1] + 32 * (t >> 1) * 2 * D), marks);
+              O[d] = pg_mfma32<TC>(v, ph[t], O[d]);
+              if constexpr (FINE) O[d] = pg_mfma32<TC>(v, pl[t], O[d]);
+              m = pg_mfma32<TC>(marks, pg_ones<TC>(seen >> (8 * t)), m);
+              __builtin_amdgcn_sched_barrier(0);   // (rare: few registers rather than few waits)
+            }
+#pragma unroll
+            for (int r = 0; r < 16; r++) O[d][r] += pg_wild_sum(m[r]);
           }
-#pragma unroll
-          for (int r = 0; r < 16; r++) O[d][r] += pg_wild_sum(m[r]);
+          return;
         }
       }
 #pragma unroll
       for (int t = 0; t < 4; t++)
 #pragma unroll
         for (int d = 0; d < ND; d++) {
-          uint4 v = pg_values<D>(vl, 16 * t + 8 * h, 2 * d + vn, vi), marks;
-          if (wild) v = pg_tamed<TC>(v, marks);
+          const uint4 v = pg_values<D>(vl + va[d][t & 1] + 32 * (t >> 1) * 2 * D);
           O[d] = pg_mfma32<TC>(v, ph[t], O[d]);
           if constexpr (FINE) O[d] = pg_mfma32<TC>(v, pl[t], O[d]);
         }
+      if constexpr (!masked.value && !FINE) pg_ahead<2, 4 * ND>();
+    };
+    // runs of tiles that every row sees whole, and others (at a window's begin, at the end), each in a loop of its own
+    for (int k = 0; k < count;) {
+      bool whole = look(k);
+      for (; k < count && !whole; whole = ++k < count && look(k)) {
+        advance(k);
+        if (kt < wend) eval(k, std::true_type{});   // (else behind all of the wave's rows)
+      }
+      for (; k < count && whole; whole = ++k < count && look(k)) {
+        advance(k);
+        eval(k, std::false_type{});
+      }
     }
     Ls = over_h(Ls, OpAddF{});
     const int r = 32 * w + n;

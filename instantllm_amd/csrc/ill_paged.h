@@ -361,6 +361,12 @@ __device__ __forceinline__ void pg_dma16(const void* base, uint32_t off, const L
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m), "v"(off), "s"(base) : "memory");
 }
 #define PG_WAIT(n) asm volatile("s_waitcnt vmcnt(" #n ")" ::: "memory")
+#define PG_TURN()                                                        \
+  do { /* a barrier that waits for no loads, and that no work moves over */ \
+    __builtin_amdgcn_sched_barrier(0);                                   \
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");      \
+    __builtin_amdgcn_sched_barrier(0);                                   \
+  } while (0)
 #define PG_WAIT_LDS() asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory")
 
 // Where the 16-byte unit u of key `key` of a tile lies in LDS, in units: a key's units in a row, permuted so
@@ -449,9 +455,6 @@ __device__ __forceinline__ float pg_wild_sum(float marks) {
 // keeps its 11 bits down to 2^-24 of the greatest one.
 #define PG_UP 10.f
 #define PG_SLACK 5.f
-#ifndef PG_AHEAD
-#define PG_AHEAD 3
-#endif
 
 struct PgWork {        // a call's share of the handle's workspace
   float2* ml;          // [2 target][M] reference and sum of a part's rows
@@ -815,30 +818,18 @@ __device__ __forceinline__ v16f pg_mfma32(uint4 a, uint4 b, v16f c) {   // 32 x 
   else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
-// Asks for N products of R LDS reads each in this order: the reads of the first three, then a product and a later one's
-// reads in turn, so that a product's operand has been on its way for three products.
-template <int R, int N>
-__device__ __forceinline__ void pg_ahead() {
-  constexpr int READ = 0x100, MFMA = 0x8, A = N < PG_AHEAD ? N : PG_AHEAD;
-  __builtin_amdgcn_sched_group_barrier(READ, R * A, 0);
-#pragma unroll
-  for (int i = 0; i < N - A; i++) {
-    __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
-    __builtin_amdgcn_sched_group_barrier(READ, R, 0);
-  }
-  __builtin_amdgcn_sched_group_barrier(MFMA, A, 0);
-}
-
 // Attention of many rows per sequence. A workgroup of four waves takes 128 flat rows of a key/value head, 32 to a wave;
 // tiles of 64 keys and their values go straight into LDS, one while the one before is evaluated. As in the step kernel,
 // scores are keys x rows and outputs dims x rows (v_mfma 32 x 32 x 16), so a row's statistics are two lanes' own, and
 // the keys are dealt to the score products' rows such that a lane's weights are the next product's operand as they
 // stand (row m of block b: key 32 b + m with bits 2 and 3 of m swapped).
+// What a row does not see must not reach it as 0 x inf either: in a tile that some row does not see whole, infinities and
+// NaN among the values are replaced by 0 in LDS, and added afterwards to the rows that see them.
 template <int TC, int D, bool FINE>   // FINE: weights in two parts (float32 outputs)
 __global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
   constexpr int M = 128, KT = 64, UPR = D / 8, KS = D / 16, ND = D / 32, T = KT * UPR, LOADS = T / 256;   // LOADS: of keys, and of values, per wave and tile
   __shared__ __attribute__((aligned(16))) uint4 lds[2][2][T];   // [buffer][keys, values]
-  __shared__ int last;
+  __shared__ int last, tamed;   // tamed: 1 + the last tile whose values were changed
   __shared__ PgFinder<4>::Lds found;
   const PgAttend& a = p.a;
   PgCut c = p.c;
@@ -863,38 +854,37 @@ __global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
   static_assert(LOADS == 2 || LOADS == 4, "two or four keys x 16 bytes x lanes");
   // this lane's operands in a tile: of the keys for each 16 dims, of the values for each 32 and for even and odd 16 keys;
   // others are whole multiples of 32 rows further
-  const int vn = (lane >> 4) & 1, vi = lane & 15;
   int ka[KS], va[ND][2];
 #pragma unroll
   for (int ks = 0; ks < KS; ks++) ka[ks] = 16 * pg_unit_at<D>((n & 19) + ((n & 4) << 1) + ((n & 8) >> 1), 2 * ks + h);
 #pragma unroll
   for (int d = 0; d < ND; d++)
 #pragma unroll
-    for (int t = 0; t < 2; t++) va[d][t] = pg_values_at<D>(16 * t + 8 * h, 32 * d + 16 * vn, vi);
+    for (int t = 0; t < 2; t++) va[d][t] = pg_values_at<D>(16 * t + 8 * h, 32 * d + 16 * ((lane >> 4) & 1), lane & 15);
   for (int u = blockIdx.x, units = __builtin_amdgcn_readfirstlane(finder.units); u < units; u += gridDim.x) {
     const PgUnit un = pg_uniform(finder.find(u));
     if (un.seq.n == 0) continue;
     const int G = c.G, flat = un.seq.n * G, f0 = M * un.q, live = min(M, flat - f0);   // (n G is at most 2^30)
     const uint32_t f = min(f0 + 32 * w + n, flat - 1), at_row = f / c.G;
     const int row = un.seq.first + at_row, head = un.head * G + (f - at_row * c.G);
-    const int row_pos = un.seq.p0 + at_row, w0 = __builtin_amdgcn_readlane(row_pos, 0), w1 = __builtin_amdgcn_readlane(row_pos, 31);   // of the wave's rows
+    const int pos = un.seq.p0 + at_row, w0 = __builtin_amdgcn_readlane(pos, 0), w1 = __builtin_amdgcn_readlane(pos, 31);   // of the wave's rows
     const int p0 = un.seq.p0 + (uint32_t)f0 / c.G, p1 = un.seq.p0 + (uint32_t)(f0 + live - 1) / c.G;
     const PgRange range = pg_range(p0, p1, cap, c);
-    const int per = pg_up(range.n, un.splits), c0 = min(un.split * per, range.n), c1 = min(c0 + per, range.n);
+    const int per = pg_up(range.n, un.splits), c0 = min(un.split * per, range.n), count = min(per, range.n - c0);
     const int end = min(p1 + 1, cap), wend = 32 * w < live ? min(w1 + 1, cap) : 0;
     uint4 qf[KS];
 #pragma unroll
     for (int ks = 0; ks < KS; ks++) qf[ks] = gld((const uint4*)(a.q + row * a.qs + (int64_t)head * D + 16 * ks + 8 * h));
-    // where the keys of the next 16 tiles are, 16 of them a lane: elements from the cache's begin; -1: not there
-    int64_t group = -1;
+    // where the 16 keys from `key` on are: elements from the cache's begin; -1: not there
+    auto place = [&](int key) -> int64_t {
+      const int page = gld(a.b.table + un.s * a.b.table_stride + (min(key, end - 1) >> a.b.page_log));
+      return page >= 0 && page < a.b.pages ? page * a.page_stride + (key & pmask) * a.slot_stride + un.head * a.head_stride : -1;
+    };
+    int64_t group = -1;   // of the next 16 tiles, 16 keys a lane
     auto groups = [&](int k) {
-      const int t = c0 + k + lane / 4;
+      const int t = k + lane / 4;
       group = -1;
-      if (t < c1) {
-        const int g = pg_key_tile(range, t) * KT + 16 * (lane % 4), key = min(g, end - 1);
-        const int page = gld(a.b.table + un.s * a.b.table_stride + (key >> a.b.page_log));
-        if (page >= 0 && page < a.b.pages) group = page * a.page_stride + (g & pmask) * a.slot_stride + un.head * a.head_stride;
-      }
+      if (t < count) group = place(pg_key_tile(range, c0 + t) * KT + 16 * (lane % 4));
     };
     auto load = [&](int k) {
       const int at = (4 * k + w) & 63;
@@ -911,40 +901,71 @@ __global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
     v16f O[ND];
 #pragma unroll
     for (int d = 0; d < ND; d++) O[d] = (v16f){};
-    if (c0 < c1) {
+    if (tid == 0) tamed = 0;
+    if (count > 0) {
       groups(0);
       load(0);
     }
-    const int count = c1 - c0;
-    int kt, good;   // first key of tile k, and which of its groups of 16 keys have pages
-    auto look = [&](int k) {   // whether every row of the wave sees the whole tile (the same for every lane)
-      kt = pg_key_tile(range, c0 + k) * KT;
-      good = 0;
+    for (int k = 0; k < count; k++) {
+      const int kt = pg_key_tile(range, c0 + k) * KT;
+      int good = 0;   // groups of 16 keys that are there
 #pragma unroll
       for (int g = 0; g < 4; g++) good |= (__builtin_amdgcn_readlane((int)(group >> 32), (4 * k + g) & 63) >= 0) << g;
-      return good == 15 && kt + KT - 1 <= w0 && kt + KT <= wend && (c.window == 0 || kt > w1 - c.window || kt + KT <= c.sinks);
-    };
-    auto advance = [&](int k) {   // tile k is there, every wave is done with the buffer filled next, and that one's loads begin
+      // whether all rows from position x to y see the whole tile (the same for every lane)
+      auto whole = [&](int x, int y, int e) {
+        return good == 15 && kt + KT - 1 <= x && kt + KT <= e && (c.window == 0 || kt > y - c.window || kt + KT <= c.sinks);
+      };
       if (k + 1 < count && ((k + 1) & 15) == 0) groups(k + 1);
       PG_WAIT(0);
-      __syncthreads();
+      __syncthreads();   // the tile is there, and every wave is done with the buffer filled next
       if (k + 1 < count) load(k + 1);
-    };
-    auto eval = [&](int k, auto masked) {
       const LAS uint8_t* kl = (const LAS uint8_t*)lds[k & 1][0];
-      const LAS uint8_t* vl = kl + 16 * T;
+      LAS uint8_t* vl = (LAS uint8_t*)lds[k & 1][1];
+      const bool all = whole(p0, p1, end), mine = whole(w0, w1, wend);
+      if (!all) {
+#pragma unroll 1
+        for (int i = tid; i < T; i += 256) {
+          uint4 marks;
+          const uint4 v = pg_get(vl + 16 * i);
+          if (pg_wild<TC>(v)) {
+            const uint4 y = pg_tamed<TC>(v, marks);
+            *(pg_lds4*)(vl + 16 * i) = (gu32x4){y.x, y.y, y.z, y.w};
+            tamed = k + 1;
+          }
+        }
+        PG_TURN();
+      }
+      if (kt >= wend) continue;   // behind all of the wave's rows
+      // operands are read a group of products ahead; the fences keep the compiler from moving the reads back to their products
       v16f s[2] = {};
+      uint4 kf[2][2][2];   // [group's turn][16 dims][32 keys]
+      auto keys = [&](int g) {
 #pragma unroll
-      for (int ks = 0; ks < KS; ks++)
+        for (int i = 0; i < 2; i++)
 #pragma unroll
-        for (int b = 0; b < 2; b++) s[b] = pg_mfma32<TC>(pg_get(kl + ka[ks] + 32 * b * 2 * D), qf[ks], s[b]);
-      if constexpr (!masked.value) pg_ahead<1, 2 * KS>();
+          for (int b = 0; b < 2; b++) kf[g & 1][i][b] = pg_get(kl + ka[2 * g + i] + 32 * b * 2 * D);
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      keys(0);
+#pragma unroll
+      for (int g = 0; g < KS / 2; g++) {
+        if (g + 1 < KS / 2) keys(g + 1);
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+          for (int b = 0; b < 2; b++) s[b] = pg_mfma32<TC>(kf[g & 1][i][b], qf[2 * g + i], s[b]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      uint4 vf[2][ND];   // [group's turn][32 dims]: the values of 16 keys
+      auto values = [&](int t) {
+#pragma unroll
+        for (int d = 0; d < ND; d++) vf[t & 1][d] = pg_values<D>(vl + va[d][t & 1] + 32 * (t >> 1) * 2 * D);
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      values(0);
       uint32_t seen = ~0u;
-      if constexpr (masked.value) {
+      if (!mine) {
         seen = 0;
-        // (opaque here, so that what masks need is not held in registers throughout)
-        int pos = row_pos, h = lane >> 5;
-        asm("" : "+v"(pos), "+v"(h));
 #pragma unroll
         for (int b = 0; b < 2; b++)
 #pragma unroll
@@ -988,48 +1009,34 @@ __global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
         }
         Ls += sum;
       }
-      if constexpr (masked.value) {
-        int from = lane;
-        asm("" : "+v"(from));
-        if (pg_wild_tile<TC, T>(vl, from)) {   // what a row does not see must not reach it as 0 x inf
 #pragma unroll
-          for (int d = 0; d < ND; d++) {
-            v16f m = {};
-#pragma unroll
-            for (int t = 0; t < 4; t++) {
-              uint4 marks;
-              const uint4 v = pg_tamed<TC>(pg_values<D>(vl + va[d][t & 1] + 32 * (t >> 1) * 2 * D), marks);
-              O[d] = pg_mfma32<TC>(v, ph[t], O[d]);
-              if constexpr (FINE) O[d] = pg_mfma32<TC>(v, pl[t], O[d]);
-              m = pg_mfma32<TC>(marks, pg_ones<TC>(seen >> (8 * t)), m);
-              __builtin_amdgcn_sched_barrier(0);   // (rare: few registers rather than few waits)
-            }
-#pragma unroll
-            for (int r = 0; r < 16; r++) O[d][r] += pg_wild_sum(m[r]);
-          }
-          return;
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < 4; t++)
+      for (int t = 0; t < 4; t++) {
+        if (t < 3) values(t + 1);
 #pragma unroll
         for (int d = 0; d < ND; d++) {
-          const uint4 v = pg_values<D>(vl + va[d][t & 1] + 32 * (t >> 1) * 2 * D);
-          O[d] = pg_mfma32<TC>(v, ph[t], O[d]);
-          if constexpr (FINE) O[d] = pg_mfma32<TC>(v, pl[t], O[d]);
+          O[d] = pg_mfma32<TC>(vf[t & 1][d], ph[t], O[d]);
+          if constexpr (FINE) O[d] = pg_mfma32<TC>(vf[t & 1][d], pl[t], O[d]);
         }
-      if constexpr (!masked.value && !FINE) pg_ahead<2, 4 * ND>();
-    };
-    // runs of tiles that every row sees whole, and others (at a window's begin, at the end), each in a loop of its own
-    for (int k = 0; k < count;) {
-      bool whole = look(k);
-      for (; k < count && !whole; whole = ++k < count && look(k)) {
-        advance(k);
-        if (kt < wend) eval(k, std::true_type{});   // (else behind all of the wave's rows)
+        __builtin_amdgcn_sched_barrier(0);
       }
-      for (; k < count && whole; whole = ++k < count && look(k)) {
-        advance(k);
-        eval(k, std::false_type{});
+      if (!all && __builtin_amdgcn_readfirstlane(tamed) == k + 1) {   // the values as they were, from memory
+#pragma unroll
+        for (int d = 0; d < ND; d++) {
+          v16f m = {};
+#pragma unroll 1
+          for (int t = 0; t < 4; t++) {
+            const int64_t at = place(kt + 16 * t);
+            const uint16_t* v = a.vc + (at < 0 ? 0 : at) + 8 * h * a.slot_stride + 32 * d + n;
+            uint32_t x[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] = gld(v + 2 * i * a.slot_stride) | (uint32_t)gld(v + (2 * i + 1) * a.slot_stride) << 16;
+            uint4 marks;
+            pg_tamed<TC>(make_uint4(x[0], x[1], x[2], x[3]), marks);
+            m = pg_mfma32<TC>(marks, pg_ones<TC>(seen >> (8 * t)), m);
+          }
+#pragma unroll
+          for (int r = 0; r < 16; r++) O[d][r] += pg_wild_sum(m[r]);
+        }
       }
     }
     Ls = over_h(Ls, OpAddF{});

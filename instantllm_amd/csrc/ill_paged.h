@@ -360,6 +360,9 @@ __device__ __forceinline__ void pg_dma16(const void* base, uint32_t off, const L
   const uint32_t m = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m), "v"(off), "s"(base) : "memory");
 }
+// The compiler's own loads so far have arrived, and it knows it (else it would wait for them, and with them for every later
+// load of pg_dma16, where it first uses them inside a loop).
+#define PG_WAIT_OWN() __builtin_amdgcn_s_waitcnt(0x0F70)   // vmcnt(0)
 #define PG_WAIT(n) asm volatile("s_waitcnt vmcnt(" #n ")" ::: "memory")
 #define PG_TURN()                                                        \
   do { /* a barrier that waits for no loads, and that no work moves over */ \
@@ -369,12 +372,11 @@ __device__ __forceinline__ void pg_dma16(const void* base, uint32_t off, const L
   } while (0)
 #define PG_WAIT_LDS() asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory")
 
-// Where the 16-byte unit u of key `key` of a tile lies in LDS, in units: a key's units in a row, permuted so
-// that the eight keys of an operand read, and the four keys by 32 bytes of four transposed reads, are on
-// different banks.
+// Where the 16-byte unit u of key `key` of a tile lies in LDS, in units: a key's units in a row, permuted so that the
+// eight keys of an eighth of an operand read, and the 4 keys x 64 bytes of half a transposed read, are on different banks.
 template <int D>
 __device__ __forceinline__ int pg_swz(int key) {
-  return D == 64 ? ((key >> 4) & 1) | (key & 2) | ((key >> 1) & 4) : ((key >> 4) & 1) | ((key & 3) << 1) | (key & 8);
+  return D == 64 ? ((key & 2) << 1) | ((key >> 2) & 2) | ((key >> 4) & 1) : ((key & 3) << 2) | ((key >> 2) & 2) | ((key >> 4) & 1);
 }
 template <int D>
 __device__ __forceinline__ int pg_unit_at(int key, int u) { return key * (D / 8) + (u ^ pg_swz<D>(key)); }
@@ -455,6 +457,11 @@ __device__ __forceinline__ float pg_wild_sum(float marks) {
 // keeps its 11 bits down to 2^-24 of the greatest one.
 #define PG_UP 10.f
 #define PG_SLACK 5.f
+#ifdef PRIO
+#define PG_PRIO(n) __builtin_amdgcn_s_setprio(n)
+#else
+#define PG_PRIO(n)
+#endif
 
 struct PgWork {        // a call's share of the handle's workspace
   float2* ml;          // [2 target][M] reference and sum of a part's rows
@@ -672,8 +679,9 @@ __global__ __launch_bounds__(64 * NW, 2) void pg_step_kernel(PgStep p) {
     v4f O[ND];
 #pragma unroll
     for (int d = 0; d < ND; d++) O[d] = (v4f){0.f, 0.f, 0.f, 0.f};
+    groups(0);
+    PG_WAIT_OWN();
     if (mine > 0) {
-      groups(0);
       load(a.kc, kl, 0);
       load(a.vc, vl, 0);
     }
@@ -886,12 +894,12 @@ __global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
       group = -1;
       if (t < count) group = place(pg_key_tile(range, c0 + t) * KT + 16 * (lane % 4));
     };
-    auto load = [&](int k) {
+    auto load = [&](int k, int buffer) {
       const int at = (4 * k + w) & 63;
       const int64_t e = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)group, at) |
                                   (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(group >> 32), at) << 32);
       const int64_t off = e < 0 ? 0 : e;   // (the first page is there, and masked)
-      LAS uint8_t* to = (LAS uint8_t*)lds[k & 1][0] + 1024 * LOADS * w;
+      LAS uint8_t* to = (LAS uint8_t*)lds[buffer][0] + 1024 * LOADS * w;
 #pragma unroll
       for (int i = 0; i < LOADS; i++) pg_dma16(a.kc + off + (LOADS == 4 && (i & 1) ? 4 * a.slot_stride : 0), lane_off[i * 2 / LOADS], to + 1024 * i);
 #pragma unroll
@@ -902,11 +910,11 @@ __global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
 #pragma unroll
     for (int d = 0; d < ND; d++) O[d] = (v16f){};
     if (tid == 0) tamed = 0;
-    if (count > 0) {
-      groups(0);
-      load(0);
-    }
-    for (int k = 0; k < count; k++) {
+    groups(0);
+    PG_WAIT_OWN();
+    if (count > 0) load(0, 0);
+    auto tile = [&](int k, auto buffer) {   // buffer: k % 2
+      constexpr int BUF = decltype(buffer)::value;
       const int kt = pg_key_tile(range, c0 + k) * KT;
       int good = 0;   // groups of 16 keys that are there
 #pragma unroll
@@ -918,9 +926,9 @@ __global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
       if (k + 1 < count && ((k + 1) & 15) == 0) groups(k + 1);
       PG_WAIT(0);
       __syncthreads();   // the tile is there, and every wave is done with the buffer filled next
-      if (k + 1 < count) load(k + 1);
-      const LAS uint8_t* kl = (const LAS uint8_t*)lds[k & 1][0];
-      LAS uint8_t* vl = (LAS uint8_t*)lds[k & 1][1];
+      if (k + 1 < count) load(k + 1, 1 - BUF);
+      const LAS uint8_t* kl = (const LAS uint8_t*)lds[BUF][0];
+      LAS uint8_t* vl = (LAS uint8_t*)lds[BUF][1];
       const bool all = whole(p0, p1, end), mine = whole(w0, w1, wend);
       if (!all) {
 #pragma unroll 1
@@ -935,7 +943,7 @@ __global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
         }
         PG_TURN();
       }
-      if (kt >= wend) continue;   // behind all of the wave's rows
+      if (kt >= wend) return;   // behind all of the wave's rows
       // operands are read a group of products ahead; the fences keep the compiler from moving the reads back to their products
       v16f s[2] = {};
       uint4 kf[2][2][2];   // [group's turn][16 dims][32 keys]
@@ -947,6 +955,7 @@ __global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
         __builtin_amdgcn_sched_barrier(0);
       };
       keys(0);
+      PG_PRIO(1);
 #pragma unroll
       for (int g = 0; g < KS / 2; g++) {
         if (g + 1 < KS / 2) keys(g + 1);
@@ -956,6 +965,7 @@ __global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
           for (int b = 0; b < 2; b++) s[b] = pg_mfma32<TC>(kf[g & 1][i][b], qf[2 * g + i], s[b]);
         __builtin_amdgcn_sched_barrier(0);
       }
+      PG_PRIO(0);
       uint4 vf[2][ND];   // [group's turn][32 dims]: the values of 16 keys
       auto values = [&](int t) {
 #pragma unroll
@@ -1009,6 +1019,7 @@ __global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
         }
         Ls += sum;
       }
+      PG_PRIO(1);
 #pragma unroll
       for (int t = 0; t < 4; t++) {
         if (t < 3) values(t + 1);
@@ -1019,6 +1030,7 @@ __global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
         }
         __builtin_amdgcn_sched_barrier(0);
       }
+      PG_PRIO(0);
       if (!all && __builtin_amdgcn_readfirstlane(tamed) == k + 1) {   // the values as they were, from memory
 #pragma unroll
         for (int d = 0; d < ND; d++) {
@@ -1038,6 +1050,10 @@ __global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
           for (int r = 0; r < 16; r++) O[d][r] += pg_wild_sum(m[r]);
         }
       }
+    };
+    for (int k = 0; k < count; k += 2) {
+      tile(k, std::integral_constant<int, 0>{});
+      if (k + 1 < count) tile(k + 1, std::integral_constant<int, 1>{});
     }
     Ls = over_h(Ls, OpAddF{});
     const int r = 32 * w + n;

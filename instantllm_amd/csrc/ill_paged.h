@@ -4,6 +4,8 @@
 // s is slot t % page_size of page table[s][t / page_size]. A batch's new rows are the last ones
 // of their sequences. Page numbers outside 0 .. pages - 1 are never followed.
 #pragma once
+#include <type_traits>
+#include <utility>
 #include "ill_device.h"
 #include "ill_paged_plan.h"
 
@@ -356,9 +358,17 @@ __device__ __forceinline__ v4f pg_mfma16(uint4 a, uint4 b, v4f c) {   // 16 x 16
 // 16 bytes from base + each lane's offset into LDS, lane i's at lds + 16 i. In inline assembly, because the
 // compiler cannot tell the buffers apart and would wait for every load in flight before each LDS read;
 // the kernels wait themselves (PG_WAIT), and extra loads of the compiler's own only make that wait longer.
-__device__ __forceinline__ void pg_dma16(const void* base, uint32_t off, const LAS uint8_t* lds) {   // base: the same for every lane
-  const uint32_t m = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m), "v"(off), "s"(base) : "memory");
+template <int AT>
+__device__ __forceinline__ void pg_dma16(const void* base, uint32_t off, uint32_t lds) {   // to lds + AT + 16 i; base and lds: the same for every lane
+  asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base), "n"(AT) : "memory", "scc");
+}
+__device__ __forceinline__ uint32_t pg_lds_at(const void* p) {   // an LDS address, as every lane's
+  return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const LAS uint8_t*)p);
+}
+// Calls f with the constants 0 .. N - 1.
+template <int N, class F>
+__device__ __forceinline__ void pg_each(F&& f) {
+  [&]<int... I>(std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }(std::make_integer_sequence<int, N>{});
 }
 // The compiler's own loads so far have arrived, and it knows it (else it would wait for them, and with them for every later
 // load of pg_dma16, where it first uses them inside a loop).
@@ -457,11 +467,6 @@ __device__ __forceinline__ float pg_wild_sum(float marks) {
 // keeps its 11 bits down to 2^-24 of the greatest one.
 #define PG_UP 10.f
 #define PG_SLACK 5.f
-#ifdef PRIO
-#define PG_PRIO(n) __builtin_amdgcn_s_setprio(n)
-#else
-#define PG_PRIO(n)
-#endif
 
 struct PgWork {        // a call's share of the handle's workspace
   float2* ml;          // [2 target][M] reference and sum of a part's rows
@@ -615,6 +620,9 @@ __global__ __launch_bounds__(64 * NW, 2) void pg_step_kernel(PgStep p) {
   const int cap = pg_cap(a.b), pmask = (1 << a.b.page_log) - 1;
   LAS uint8_t* kl = (LAS uint8_t*)lds[w];
   LAS uint8_t* vl = kl + 8192;
+  const uint32_t mine_lds = pg_lds_at(lds[w]);
+  constexpr std::integral_constant<int, 0> KEYS{};
+  constexpr std::integral_constant<int, 8192> VALUES{};
   // this lane's operands in a tile: of the keys for each 32 dims, of the values for each 16. Other keys of the lane's are
   // whole multiples of 4 or 32 rows further: the permutation does not see them.
   int ka[KS], va[ND];
@@ -666,14 +674,15 @@ __global__ __launch_bounds__(64 * NW, 2) void pg_step_kernel(PgStep p) {
       return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)group, at) |
                        (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(group >> 32), at) << 32);
     };
-    auto load = [&](const uint16_t* from, LAS uint8_t* to, int k) {
-#pragma unroll
-      for (int g = 0; g < NG; g++) {
+    auto load = [&](const uint16_t* from, auto to, int k) {
+      pg_each<NG>([&](auto g) {
         const int64_t at = group_at(k, g);
         const uint16_t* base = from + (at < 0 ? 0 : at);   // (the first page is there, and masked)
-#pragma unroll
-        for (int i = g * 8 / NG; i < (g + 1) * 8 / NG; i++) pg_dma16(base, lane_off[i], to + 1024 * i);
-      }
+        pg_each<8 / NG>([&](auto i) {
+          constexpr int I = g * 8 / NG + i;
+          pg_dma16<to + 1024 * I>(base, lane_off[I], mine_lds);
+        });
+      });
     };
     float Mx = -INFINITY, Ls = 0.f;   // Ls: this lane's keys only
     v4f O[ND];
@@ -682,8 +691,8 @@ __global__ __launch_bounds__(64 * NW, 2) void pg_step_kernel(PgStep p) {
     groups(0);
     PG_WAIT_OWN();
     if (mine > 0) {
-      load(a.kc, kl, 0);
-      load(a.vc, vl, 0);
+      load(a.kc, KEYS, 0);
+      load(a.vc, VALUES, 0);
     }
     for (int k = 0; k < mine; k++) {
       const int kt = pg_key_tile(range, c0 + w + NW * k) * KT;
@@ -702,7 +711,7 @@ __global__ __launch_bounds__(64 * NW, 2) void pg_step_kernel(PgStep p) {
       PG_WAIT_LDS();   // the keys have been read
       if (more) {
         if (((k + 1) & (64 / NG - 1)) == 0) groups(k + 1);
-        load(a.kc, kl, k + 1);
+        load(a.kc, KEYS, k + 1);
       }
       // every row sees the whole tile, or the rows' masks (wave-uniform)
       const bool whole = good == (1 << NG) - 1 && kt + KT - 1 <= p0 && kt + KT <= end && (c.window == 0 || kt > p1 - c.window || kt + KT <= c.sinks);
@@ -784,7 +793,7 @@ __global__ __launch_bounds__(64 * NW, 2) void pg_step_kernel(PgStep p) {
         }
       }
       PG_WAIT_LDS();   // the values have been read
-      if (more) load(a.vc, vl, k + 1);
+      if (more) load(a.vc, VALUES, k + 1);
     }
     // the waves' states, each in its own LDS
     Ls = over_kg(Ls, OpAddF{});
@@ -860,6 +869,7 @@ __global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
     lane_off[i] = 2 * ((uint32_t)(key & 15) * (uint32_t)a.slot_stride + 8 * ((lane % UPR) ^ pg_swz<D>(key)));
   }
   static_assert(LOADS == 2 || LOADS == 4, "two or four keys x 16 bytes x lanes");
+  const uint32_t mine_lds = pg_lds_at(&lds[0][0][64 * LOADS * w]);
   // this lane's operands in a tile: of the keys for each 16 dims, of the values for each 32 and for even and odd 16 keys;
   // others are whole multiples of 32 rows further
   int ka[KS], va[ND][2];
@@ -888,23 +898,32 @@ __global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
       const int page = gld(a.b.table + un.s * a.b.table_stride + (min(key, end - 1) >> a.b.page_log));
       return page >= 0 && page < a.b.pages ? page * a.page_stride + (key & pmask) * a.slot_stride + un.head * a.head_stride : -1;
     };
+    const int all_hi = min(p0 + 1, end) - KT, all_lo = c.window ? p1 - c.window : -1, mine_hi = min(w0 + 1, wend) - KT, mine_lo = c.window ? w1 - c.window : -1;
     int64_t group = -1;   // of the next 16 tiles, 16 keys a lane
+    uint64_t there = 0;   // which of them have a place
     auto groups = [&](int k) {
       const int t = k + lane / 4;
       group = -1;
       if (t < count) group = place(pg_key_tile(range, c0 + t) * KT + 16 * (lane % 4));
+      there = __ballot(group >= 0);
     };
-    auto load = [&](int k, int buffer) {
+    // Loads of a tile, 2 x LOADS of them, one at a time between the products of the tile before: together, right behind the
+    // barrier, they held every wave up for 900 cycles (D 128), a quarter of a tile. A tile behind the last is the first page.
+    const uint16_t *next_k, *next_v;
+    auto next = [&](int k) {
       const int at = (4 * k + w) & 63;
       const int64_t e = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)group, at) |
                                   (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(group >> 32), at) << 32);
-      const int64_t off = e < 0 ? 0 : e;   // (the first page is there, and masked)
-      LAS uint8_t* to = (LAS uint8_t*)lds[buffer][0] + 1024 * LOADS * w;
-#pragma unroll
-      for (int i = 0; i < LOADS; i++) pg_dma16(a.kc + off + (LOADS == 4 && (i & 1) ? 4 * a.slot_stride : 0), lane_off[i * 2 / LOADS], to + 1024 * i);
-#pragma unroll
-      for (int i = 0; i < LOADS; i++) pg_dma16(a.vc + off + (LOADS == 4 && (i & 1) ? 4 * a.slot_stride : 0), lane_off[i * 2 / LOADS], to + 16 * T + 1024 * i);
+      const int64_t off = k < count && e > 0 ? e : 0;   // (where there is none, the first page is loaded, and masked)
+      next_k = a.kc + off;
+      next_v = a.vc + off;
     };
+    auto load = [&](auto i, auto buffer) {
+      constexpr int I = i % LOADS;
+      pg_dma16<32 * T * buffer + (i < LOADS ? 0 : 16 * T) + 1024 * I>((i < LOADS ? next_k : next_v) + (LOADS == 4 && (I & 1) ? 4 * a.slot_stride : 0), lane_off[I * 2 / LOADS],
+                                                                  mine_lds);
+    };
+    const auto B0 = std::integral_constant<int, 0>{};
     float Mx = -INFINITY, Ls = 0.f;   // Ls: this lane's keys only
     v16f O[ND];
 #pragma unroll
@@ -912,24 +931,23 @@ __global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
     if (tid == 0) tamed = 0;
     groups(0);
     PG_WAIT_OWN();
-    if (count > 0) load(0, 0);
+    if (count > 0) {
+      next(0);
+      pg_each<2 * LOADS>([&](auto i) { load(i, B0); });
+    }
     auto tile = [&](int k, auto buffer) {   // buffer: k % 2
       constexpr int BUF = decltype(buffer)::value;
+      constexpr std::integral_constant<int, 1 - BUF> OTHER{};
       const int kt = pg_key_tile(range, c0 + k) * KT;
-      int good = 0;   // groups of 16 keys that are there
-#pragma unroll
-      for (int g = 0; g < 4; g++) good |= (__builtin_amdgcn_readlane((int)(group >> 32), (4 * k + g) & 63) >= 0) << g;
-      // whether all rows from position x to y see the whole tile (the same for every lane)
-      auto whole = [&](int x, int y, int e) {
-        return good == 15 && kt + KT - 1 <= x && kt + KT <= e && (c.window == 0 || kt > y - c.window || kt + KT <= c.sinks);
-      };
-      if (k + 1 < count && ((k + 1) & 15) == 0) groups(k + 1);
+      const int good = (int)(there >> (4 * k & 63)) & 15;   // groups of 16 keys that are there
+      // whether all rows of the workgroup, and of the wave, see the whole tile (the same for every lane)
+      const bool all = good == 15 && kt <= all_hi && (kt > all_lo || kt + KT <= c.sinks), mine = good == 15 && kt <= mine_hi && (kt > mine_lo || kt + KT <= c.sinks);
+      if (((k + 1) & 15) == 0) groups(k + 1);
+      next(k + 1);
       PG_WAIT(0);
       __syncthreads();   // the tile is there, and every wave is done with the buffer filled next
-      if (k + 1 < count) load(k + 1, 1 - BUF);
       const LAS uint8_t* kl = (const LAS uint8_t*)lds[BUF][0];
       LAS uint8_t* vl = (LAS uint8_t*)lds[BUF][1];
-      const bool all = whole(p0, p1, end), mine = whole(w0, w1, wend);
       if (!all) {
 #pragma unroll 1
         for (int i = tid; i < T; i += 256) {
@@ -943,7 +961,10 @@ __global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
         }
         PG_TURN();
       }
-      if (kt >= wend) return;   // behind all of the wave's rows
+      if (kt >= wend) {   // behind all of the wave's rows
+        pg_each<2 * LOADS>([&](auto i) { load(i, OTHER); });
+        return;
+      }
       // operands are read a group of products ahead; the fences keep the compiler from moving the reads back to their products
       v16f s[2] = {};
       uint4 kf[2][2][2];   // [group's turn][16 dims][32 keys]
@@ -955,17 +976,15 @@ __global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
         __builtin_amdgcn_sched_barrier(0);
       };
       keys(0);
-      PG_PRIO(1);
-#pragma unroll
-      for (int g = 0; g < KS / 2; g++) {
-        if (g + 1 < KS / 2) keys(g + 1);
+      pg_each<KS / 2>([&](auto g) {
+        if constexpr (g + 1 < KS / 2) keys(g + 1);
 #pragma unroll
         for (int i = 0; i < 2; i++)
 #pragma unroll
           for (int b = 0; b < 2; b++) s[b] = pg_mfma32<TC>(kf[g & 1][i][b], qf[2 * g + i], s[b]);
+        pg_each<4 * LOADS / KS>([&](auto i) { load(std::integral_constant<int, 4 * LOADS / KS * g + i>{}, OTHER); });
         __builtin_amdgcn_sched_barrier(0);
-      }
-      PG_PRIO(0);
+      });
       uint4 vf[2][ND];   // [group's turn][32 dims]: the values of 16 keys
       auto values = [&](int t) {
 #pragma unroll
@@ -1019,7 +1038,6 @@ __global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
         }
         Ls += sum;
       }
-      PG_PRIO(1);
 #pragma unroll
       for (int t = 0; t < 4; t++) {
         if (t < 3) values(t + 1);
@@ -1030,7 +1048,6 @@ __global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
         }
         __builtin_amdgcn_sched_barrier(0);
       }
-      PG_PRIO(0);
       if (!all && __builtin_amdgcn_readfirstlane(tamed) == k + 1) {   // the values as they were, from memory
 #pragma unroll
         for (int d = 0; d < ND; d++) {
@@ -1055,6 +1072,7 @@ __global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
       tile(k, std::integral_constant<int, 0>{});
       if (k + 1 < count) tile(k + 1, std::integral_constant<int, 1>{});
     }
+    PG_WAIT(0);   // (a load behind the last tile)
     Ls = over_h(Ls, OpAddF{});
     const int r = 32 * w + n;
     if (r < live) {

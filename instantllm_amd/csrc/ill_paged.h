@@ -225,7 +225,7 @@ template <int NW>
 struct PgFinder {
   static constexpr int NT = 64 * NW;
   const PgBatch& b;
-  const PgCut& c;
+  PgCut c;
   int part, units;   // tiles of keys in a part; units of work in all
   struct Lds {
     int64_t tiles[NW], work[NW];
@@ -252,15 +252,28 @@ struct PgFinder {
     return v;
   }
   __device__ __forceinline__ PgFinder(const PgBatch& b_, const PgCut& c_, Lds& lds_) : b(b_), c(c_), lds(lds_) {
-    if (b.seqs == 1) {
+    if (b.seqs == 1) {   // (one sequence is one kernel's: shared is 0)
       look(0);
-      part = pg_part(n, (int64_t)n * most, c);
+      part = pg_part((int64_t)n * most, c);
       units = n * pg_splits(most, part);
       return;
     }
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
     int64_t tiles = 0, work = 0;
-    int s = threadIdx.x;
+    int s;
+    if (c.shared) {
+      for (s = threadIdx.x; s < b.seqs; s += NT) tiles += pg_prompt_tiles(pg_seq_at(b, s).n, c.G, c.kv);
+      tiles = over_wave(tiles);
+      if (lane == 0) lds.tiles[w] = tiles;
+      __syncthreads();
+      tiles = 0;
+#pragma unroll
+      for (int i = 0; i < NW; i++) tiles += lds.tiles[i];
+      pg_share(c, tiles);
+      tiles = 0;
+      __syncthreads();
+    }
+    s = threadIdx.x;
     do {
       look(s);
       tiles += n;
@@ -280,9 +293,8 @@ struct PgFinder {
       tiles += lds.tiles[i];
       work += lds.work[i];
     }
-    part = pg_part(tiles, work, c);
+    part = pg_part(work, c);
     units = (int)tiles;   // of uncut sequences: a unit for each
-    if (part >= PG_MOST) return;
     int u = 0;
     for (s = threadIdx.x; s - (int)threadIdx.x < b.seqs; s += NT) {
       if (b.seqs > NT) look(s);
@@ -469,9 +481,9 @@ __device__ __forceinline__ float pg_wild_sum(float marks) {
 #define PG_SLACK 5.f
 
 struct PgWork {        // a call's share of the handle's workspace
-  float2* ml;          // [2 target][M] reference and sum of a part's rows
-  float* o;            // [2 target][M][D] its weighted values
-  int32_t* joined;     // [target][1 + PG_MAXSPLIT / PG_FAN] parts of a tile of rows that are done, in all and of each PG_FAN; 0 between calls
+  float2* ml;          // [2 x 2^log][M] reference and sum of a part's rows
+  float* o;            // [2 x 2^log][M][D] its weighted values
+  int32_t* joined;     // [2^log][1 + PG_MAXSPLIT / PG_FAN] parts of a tile of rows that are done, in all and of each PG_FAN; 0 between calls
 };
 
 // Four dims of a row's output.

@@ -38,23 +38,15 @@ PgBatch batch_of(const ill_paged* p, const ill_paged_batch& b) {
   return {b.lens, b.table, b.row0, b.table_stride, b.pages, b.seqs, (int)b.rows, b.table_width, p->page_log};
 }
 
-#ifndef STEP_NW
-#define STEP_NW 4
-#endif
-#ifndef PROMPT_FROM
-#define PROMPT_FROM 32
-#endif
-#ifndef PROMPT_WHOLE
-#define PROMPT_WHOLE 256
-#endif
-constexpr int kLog = 8;            // parts wanted: 2^8, one workgroup per CU
-constexpr int kFew = PROMPT_FROM;  // flat rows of a sequence up to which the step kernel takes it
-
+// A call's parts. The step kernel cuts the keys into about a part for each CU (2^8), of 8 tiles of keys at least, two for each
+// wave: with 2^9 parts or 4 tiles the joining cost more than it gave (us, 2^8 / 2^9: one sequence of 131071 24.7 / 27.3, 200
+// through a window of 1024 27 / 43; 8 / 4 tiles: one of 500 8.8 / 10.1). The prompt kernel cuts only what is over twice the
+// average share of a CU (2^7): its parts are 128 rows, and an even batch is faster whole.
 PgCut step_cut(const ill_paged_desc& d, int window, int sinks) {
-  return {(uint32_t)(d.heads / d.kv_heads), (uint32_t)d.kv_heads, 16, d.head_dim == 64 ? 64 : 32, window, sinks, kLog, 8, INT32_MAX, 0, INT32_MAX};
+  return {(uint32_t)(d.heads / d.kv_heads), (uint32_t)d.kv_heads, 16, d.head_dim == 64 ? 64 : 32, window, sinks, 8, 8, 0, PG_MOST, 0};
 }
 PgCut prompt_cut(const ill_paged_desc& d, int window, int sinks) {
-  return {(uint32_t)(d.heads / d.kv_heads), (uint32_t)d.kv_heads, 128, 64, window, sinks, kLog, 4, PROMPT_WHOLE, 0, INT32_MAX};
+  return {(uint32_t)(d.heads / d.kv_heads), (uint32_t)d.kv_heads, 128, 64, window, sinks, 7, 4, 0, PG_MOST, 0};
 }
 
 // Bytes of a workspace where 2^log parts are wanted, over tiles of M rows.
@@ -94,8 +86,8 @@ int workspace(ill_paged* p, hipStream_t st, uint8_t** out) {
 template <int TC, int D>
 void launch_attend(const PgStep& s, int64_t grid, hipStream_t st) {
   if (s.c.M == 16) {
-    if (s.a.out_f32) hipLaunchKernelGGL((pg_step_kernel<TC, D, true, STEP_NW>), dim3(grid), dim3(64 * STEP_NW), 0, st, s);
-    else hipLaunchKernelGGL((pg_step_kernel<TC, D, false, STEP_NW>), dim3(grid), dim3(64 * STEP_NW), 0, st, s);
+    if (s.a.out_f32) hipLaunchKernelGGL((pg_step_kernel<TC, D, true, 4>), dim3(grid), dim3(256), 0, st, s);
+    else hipLaunchKernelGGL((pg_step_kernel<TC, D, false, 4>), dim3(grid), dim3(256), 0, st, s);
   } else {
     if (s.a.out_f32) hipLaunchKernelGGL((pg_prompt_kernel<TC, D, true>), dim3(grid), dim3(256), 0, st, s);
     else hipLaunchKernelGGL((pg_prompt_kernel<TC, D, false>), dim3(grid), dim3(256), 0, st, s);
@@ -140,7 +132,8 @@ int ill_paged_create(const ill_paged_desc* desc, ill_paged** out) {
   for (int i = 0; i < d.rotary_dim / 2; i++) freq[i] = std::pow(d.rope_base, -2.0 * i / d.rotary_dim) / (2 * M_PI);
   if (hipMalloc(&p->freq, sizeof freq) != hipSuccess || hipMemcpy(p->freq, freq, sizeof freq, hipMemcpyHostToDevice) != hipSuccess)
     return bad(fail(ILL_E_HIP, "paged: buffer allocation failed"));
-  p->work_bytes = al256(illp::work_size(illp::kLog, 128, d.head_dim));
+  p->work_bytes = al256(illp::work_size(illp::prompt_cut(d, 0, 0).log, 128, d.head_dim));   // (the step kernel's is smaller)
+  static_assert((16 << 8) <= (128 << 7), "rows of the step kernel's parts");
   if (hipMalloc(&p->work, p->work_bytes * d.streams) != hipSuccess || hipMemset(p->work, 0, p->work_bytes * d.streams) != hipSuccess ||
       hipDeviceSynchronize() != hipSuccess)
     return bad(fail(ILL_E_HIP, "paged: %d workspaces of %zu bytes cannot be allocated", d.streams, p->work_bytes));
@@ -231,20 +224,21 @@ int ill_paged_attend(ill_paged* p, const ill_paged_batch* batch, const void* q, 
   illp::OnDevice on(p->device);
   if (on.rc) return on.rc;
   hipStream_t st = (hipStream_t)stream;
-  // One of the kernels where it is known that no sequence has many new rows, or that the only one may; else both, each
-  // with the sequences that are its own.
-  const int64_t most = !a.b.row0 ? 1 : std::min<int64_t>(a.b.rows, batch->max_rows ? batch->max_rows : a.b.rows), G = d.heads / d.kv_heads;
-  const bool few = most * G <= illp::kFew, both = !few && a.b.seqs > 1;
+  // One of the kernels where the sizes that the host knows say which, else both: the sequences are divided by pg_share.
+  const int64_t G = d.heads / d.kv_heads, most = !a.b.row0 ? 1 : std::min<int64_t>(a.b.rows, batch->max_rows ? batch->max_rows : a.b.rows);
   PgStep parts[2] = {{a, illp::step_cut(d, a.window, a.sinks), {}}, {a, illp::prompt_cut(d, a.window, a.sinks), {}}};
-  if (both) parts[0].c.hi = parts[1].c.lo = illp::kFew;
   const int cap = pg_cap(a.b);
+  const bool prompts = most * G > PG_FEW && std::min((a.b.rows * G / 128 + a.b.seqs), (most * G + 127) / 128 * a.b.seqs) * d.kv_heads >= PG_MANY;
+  const bool both = prompts && a.b.seqs > 1;
+  parts[0].c.shared = parts[1].c.shared = both;
   uint8_t* work = nullptr;
-  for (int i = few ? 0 : both ? 0 : 1; i < (few ? 1 : 2); i++)
-    if (pg_splits(pg_most(cap, cap, parts[i].c), parts[i].c.least) > 1 && !work)
+  for (int i = 0; i < 2; i++)
+    if ((i ? prompts : both || !prompts) && !work && pg_splits(pg_most(cap, cap, parts[i].c), parts[i].c.least) > 1)
       if (int rc = illp::workspace(p, st, &work)) return rc;
-  for (int i = few ? 0 : both ? 0 : 1; i < (few ? 1 : 2); i++) {
+  for (int i = 0; i < 2; i++) {
+    if (!(i ? prompts : both || !prompts)) continue;
     PgStep& s = parts[i];
-    const int64_t grid = std::min<int64_t>(pg_grid(a.b.seqs, a.b.rows, i == 0 && both ? illp::kFew / G : batch->max_rows, !a.b.row0, cap, s.c), 1 << 20);
+    const int64_t grid = std::min<int64_t>(pg_grid(a.b.seqs, a.b.rows, most, !a.b.row0, cap, s.c), i == 0 && both ? 1024 : 1 << 20);
     if (!grid) continue;
     if (work) s.w = illp::work_of(work, s.c.log, s.c.M, d.head_dim);
     if (d.dtype == ILL_F16) {

@@ -54,9 +54,28 @@ struct PgCut {
   int32_t M, KT, window, sinks;
   int32_t log;       // 2^log parts are wanted in all, where there are that many
   int32_t least;     // tiles of keys in a part at least
-  int32_t whole;     // from this many tiles of rows on, none is cut
   int32_t lo, hi;    // sequences with lo < n G <= hi are this kernel's
+  int32_t shared;    // the other kernel runs too: lo or hi hold as pg_share says
 };
+
+// Two kernels evaluate a batch. Sequences of up to PG_FEW flat rows are always the step kernel's (16 flat rows to a tile);
+// the others are the prompt kernel's (128) if they have PG_MANY tiles of 128 in all, times key/value heads, about one for
+// each CU, and the step kernel's otherwise. (Step against prompt kernel, us, 14 / 2 heads of 64: 512 rows, 56 tiles, 8.7 against
+// 24; 1024 rows behind 4000, 112 tiles, 56.3 against 56.7; 2048 rows, 224 tiles, 39.7 against 36.2; 8 x 512 rows, 448 tiles, 63
+// against 33. 32 / 8 heads of 128: 512 rows behind 4000, 128 tiles, 84 against 81; 4 x 256, 256 tiles, 38.5 against 26.7; but 32 x
+// 8 rows, 256 tiles of 32 flat rows, 28 against 36.)
+#define PG_FEW 32
+#define PG_MANY 224
+PG_FN int pg_prompt_tiles(int n, uint32_t G, uint32_t kv) {
+  const uint32_t f = (uint32_t)n * G;
+  return f > PG_FEW ? (int)((f + 127) / 128 * kv) : 0;
+}
+// The limits of the step kernel (M 16) or of the prompt kernel, from the sum of pg_prompt_tiles over the sequences.
+PG_FN void pg_share(PgCut& c, int64_t tiles) {
+  const bool many = tiles >= PG_MANY;
+  if (c.M == 16) c.hi = many ? PG_FEW : PG_MOST;
+  else c.lo = many ? PG_FEW : PG_MOST;
+}
 
 PG_FN int pg_qtiles(int n, const PgCut& c) {
   const uint32_t f = (uint32_t)n * c.G;   // (rows x heads: at most 2^30)
@@ -87,11 +106,9 @@ PG_FN int pg_most(int end, int cap, const PgCut& c) {
   return pg_min(some, all);
 }
 
-// Tiles of keys in a part, from the sums over the sequences of qtiles x kv (`tiles`) and of qtiles x kv x
-// most (`work`). A sequence is cut into parts if its `most` is over that; the parts of all cut ones are
+// Tiles of keys in a part, from the sum over the sequences of qtiles x kv x most. A sequence is cut into parts if its `most` is over that; the parts of all cut ones are
 // then at most 2 x 2^log (most / part + 1 <= 2 most / part each), their tiles of rows at most 2^log.
-PG_FN int pg_part(int64_t tiles, int64_t work, const PgCut& c) {
-  if (tiles >= c.whole) return PG_MOST;
+PG_FN int pg_part(int64_t work, const PgCut& c) {
   const int64_t p = (work + (1ll << c.log) - 1) >> c.log;
   return p < c.least ? c.least : p < PG_MOST ? (int)p : PG_MOST;
 }

@@ -287,6 +287,17 @@ ATTEND = [
     (dict(seqs=[(9001, 1), (7000, 1)], one_row=True, page=64), dict(window=5000, sinks=9)),
     (dict(seqs=[(5000, 40)], heads=4, kv=1), dict()),
     (dict(seqs=[(5000, 40), (3000, 90)], heads=4, kv=2, dim=128, dtype="bf16"), dict(out_dtype="f32", window=2500, sinks=300)),
+    # enough tiles of 128 rows x heads for the prompt kernel: whole prompts, behind cached positions, windows, both head sizes and outputs
+    (dict(seqs=[(333, 333)], heads=84, kv=84), dict()),
+    (dict(seqs=[(200, 129), (64, 64), (31, 40), (1, 1)], heads=128, kv=64, dim=128, dtype="bf16", page=64, pad=2), dict(q_extra=8, out_extra=16)),
+    (dict(seqs=[(400, 300)], heads=96, kv=32, layout="phs"), dict(window=50, sinks=5, out_dtype="f32")),
+    (dict(seqs=[(700, 130)], heads=120, kv=120, dim=128, page=32), dict(window=1, sinks=1)),
+    (dict(seqs=[(520, 200), (90, 90)], heads=72, kv=72, dtype="bf16", page=128, layout="p1h2s3"), dict(window=64, sinks=100)),
+    (dict(seqs=[(300, 128), (129, 128)], heads=112, kv=112, dim=128, page=1024), dict(out_dtype="f32")),
+    # both kernels, the prompt kernel's longest sequence in parts
+    (dict(seqs=[(6000, 40)] + [(100 + i, 40) for i in range(7)] + [(900, 1), (64, 1), (0, 1), (5, 9), (70, 0)], heads=64, kv=32, pad=1), dict()),
+    (dict(seqs=[(6000, 40)] + [(100 + i, 40) for i in range(7)] + [(900, 1), (64, 1), (0, 1), (5, 9), (70, 0)], heads=64, kv=32, dim=128, dtype="bf16", max_rows=40),
+     dict(window=4500, sinks=70, out_dtype="f32")),
     # many sequences
     (dict(seqs=[(3 * i % 190, i % 3) for i in range(150)], heads=2, kv=1), dict(window=30, sinks=2)),
     (dict(seqs=[(7 * i % 300, 1) for i in range(130)], one_row=True, heads=4, kv=2, dim=128, scale=0.3), dict()),
@@ -300,10 +311,10 @@ def test_attend_matches_oracle(hip, setup, call):
 
 
 @pytest.mark.parametrize("dim,dtype", [(64, "f16"), (128, "bf16")])
-@pytest.mark.parametrize("rows", [1, 3, 40, 150])
-def test_what_is_not_seen_never_reaches_a_row(hip, dim, dtype, rows):
+@pytest.mark.parametrize("rows,heads,kv", [(1, 6, 2), (3, 6, 2), (40, 6, 2), (150, 6, 2), (150, 112, 112)], ids=["1", "3", "40", "150", "150-prompt-kernel"])
+def test_what_is_not_seen_never_reaches_a_row(hip, dim, dtype, rows, heads, kv):
     """NaN and infinities in every slot that no sequence has, and in positions that only later rows, or rows before them (a window's), see."""
-    s = Setup(hip, [(150, min(rows, 150)), (67, min(rows, 67)), (16, 1)], heads=6, kv=2, dim=dim, dtype=dtype)
+    s = Setup(hip, [(150, min(rows, 150)), (67, min(rows, 67)), (16, 1)], heads=heads, kv=kv, dim=dim, dtype=dtype)
     used = s.places()
     k, v = s.view(s.k_bits), s.view(s.v_bits)
     wild = O.to_bits(np.array([np.nan, np.inf, -np.inf], np.float32), dtype)
@@ -323,19 +334,21 @@ def test_what_is_not_seen_never_reaches_a_row(hip, dim, dtype, rows):
     s.attend(window=20, sinks=3, out_dtype="f32")
 
 
-def test_attend_bad_pages(hip):
+@pytest.mark.parametrize("heads,kv", [(4, 2), (228, 228)], ids=["step", "both"])
+def test_attend_bad_pages(hip, heads, kv):
     """Positions on pages out of range are not seen."""
-    s = Setup(hip, [(300, 1), (300, 60), (40, 2)], heads=4, kv=2)
+    s = Setup(hip, [(300, 1), (300, 60), (40, 2)], heads=heads, kv=kv)
     s.table[0, 3], s.table[0, 18], s.table[1, 0], s.table[1, 17], s.table[2, :3] = -1, s.pages, 0x7FFFFFFF, -0x80000000, -5
     hip.write(s.d_table, s.table)
     s.attend()
     s.attend(window=70, sinks=20, out_dtype="f32")
 
 
-def test_attend_lengths_past_the_table(hip):
+@pytest.mark.parametrize("heads,kv", [(4, 2), (232, 116)], ids=["step", "both"])
+def test_attend_lengths_past_the_table(hip, heads, kv):
     """Positions behind the table's last page are not seen; the rows stand where the length says."""
-    s = Setup(hip, [(48, 1), (48, 30)], heads=4, kv=2)
-    s.lens[:] = [60, 70]
+    s = Setup(hip, [(48, 1), (48, 30), (40, 20)], heads=heads, kv=kv)
+    s.lens[:] = [60, 70, 200]
     hip.write(s.d_lens, s.lens)
     s.attend()
     s.attend(window=25, sinks=2)
@@ -382,9 +395,9 @@ def test_offsets_past_32_bits(hip):
 
 def test_attend_is_deterministic_and_independent_of_earlier_calls(hip):
     """The same call's bits, also after calls of other sizes on the same handle."""
-    s = Setup(hip, [(9000, 1), (300, 1), (1, 1)], one_row=True)
-    q = s.random_bits(3, s.heads * s.dim)
-    first = s.attend(q=q)
+    s = Setup(hip, [(9000, 1), (300, 40), (1, 1)], heads=112, kv=112)
+    q = s.random_bits(42, s.heads * s.dim)
+    first = s.attend(q=q, check=False)
     for _ in range(3):
         s.attend(window=4000, sinks=3, check=False)
         assert np.array_equal(s.attend(q=q, check=False), first)

@@ -40,7 +40,7 @@ int main() {
     c.G = draw(1, 20); c.kv = draw(1, 4); c.M = draw(0, 1) ? 16 : 128; c.KT = draw(0, 1) ? 64 : 32;
     c.window = draw(0, 2) ? 0 : draw(1, 300); c.sinks = draw(0, 1) ? 0 : draw(0, 200);
     if (draw(0, 50) == 0) c.window = PG_MOST, c.sinks = PG_MOST;
-    c.log = draw(0, 6); c.least = draw(1, 5); c.whole = draw(0, 1) ? 2147483647 : draw(1, 60); c.lo = draw(0, 1) ? 0 : draw(0, 64); c.hi = draw(0, 3) ? 2147483647 : draw(1, 64);
+    c.log = draw(0, 6); c.least = draw(1, 5); c.lo = draw(0, 1) ? 0 : draw(0, 64); c.hi = draw(0, 3) ? PG_MOST : draw(1, 64);
     const int seqs = draw(1, 6), width = draw(1, 40), log = 4;
     std::vector<PgSeq> seq(seqs);
     int rows = 0, most_rows = 0;
@@ -52,9 +52,9 @@ int main() {
       most_rows = pg_max(most_rows, n);
     }
     const int cap = width << log;
-    long long tiles = 0, work = 0;
-    for (auto& q : seq) { const int t = pg_qtiles(q.n, c) * c.kv; tiles += t; work += (long long)t * pg_most(q.p0 + q.n, cap, c); }
-    const int part = pg_part(tiles, work, c);
+    long long work = 0;
+    for (auto& q : seq) { const int t = pg_qtiles(q.n, c) * c.kv; work += (long long)t * pg_most(q.p0 + q.n, cap, c); }
+    const int part = pg_part(work, c);
     CHECK(part >= 1);
     long long units = 0, parts = 0, cut = 0;
     for (auto& q : seq) {
@@ -97,6 +97,23 @@ int main() {
     // the launch has a workgroup for every unit, where the sizes that the host knows hold
     CHECK(units <= pg_grid(seqs, rows, 0, false, cap, c));
     CHECK(units <= pg_grid(seqs, rows, most_rows, false, cap, c));
+  }
+  // two kernels: every sequence with rows is exactly one's
+  for (int i = 0; i < 20000; i++) {
+    PgCut step{}, prompt{};
+    step.G = prompt.G = draw(1, 20); step.kv = prompt.kv = draw(1, 8); step.M = 16; prompt.M = 128;
+    step.hi = prompt.hi = PG_MOST;
+    int n[5];
+    long long tiles = 0;
+    for (int& x : n) { x = draw(0, 2) ? draw(0, 10) : draw(0, 900); tiles += pg_prompt_tiles(x, step.G, step.kv); }
+    pg_share(step, tiles);
+    pg_share(prompt, tiles);
+    long long taken = 0;
+    for (int x : n) {
+      CHECK((pg_qtiles(x, step) > 0) + (pg_qtiles(x, prompt) > 0) == (x > 0));
+      taken += pg_qtiles(x, prompt) * (int)prompt.kv;
+    }
+    CHECK(taken == (tiles >= PG_MANY ? tiles : 0));
   }
   printf("ok\n");
   return 0;

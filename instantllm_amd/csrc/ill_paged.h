@@ -79,20 +79,64 @@ __device__ __forceinline__ PgSeq pg_seq_at(const PgBatch& b, int s) {
   return pg_seq(begin, end, gld(b.lens + s), b.rows);
 }
 
+// Eight floats from an address aligned to 4 bytes.
+__device__ __forceinline__ void pg_floats8(const float* p, float* y) {
+  typedef float v4u __attribute__((ext_vector_type(4), aligned(4)));
+  const v4u a = *(const GAS v4u*)p, b = *(const GAS v4u*)(p + 4);
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    y[i] = a[i];
+    y[4 + i] = b[i];
+  }
+}
+
 // A workgroup takes R rows; a thread takes 16 values of one head at a time: the eight first and the
 // eight second halves of eight rotated pairs (or eight whole pairs twice where pairs are
 // interleaved), so that a pair never leaves its thread and a head's square sum stays within D / 16
 // neighbouring lanes. The angles' sines and cosines are computed once per row and pair, from turns
-// in float64 (a position of 2^20 has to keep 2^-20 of a turn and more), and shared through LDS.
+// in float64 (a position of 2^20 has to keep 2^-20 of a turn and more), and shared through LDS. A thread's
+// first values are on their way while the rows' places and angles are found, the next ones while it
+// computes: one row waits for three loads one after the other, many rows for memory.
 template <int TX, int TC, int D>
 __global__ __launch_bounds__(256) void pg_append_kernel(PgAppend a, int R) {
   extern __shared__ __attribute__((aligned(16))) uint8_t pg_lds[];
-  constexpr int C = D / 16;   // threads of a head
+  constexpr int C = D / 16, EB = TX == PG_F32 ? 4 : 2;   // threads of a head; bytes of a value
   const int half = a.rot >> 1;
-  int64_t* place = (int64_t*)pg_lds;             // [R] element offset of the row's slot, -1: nothing to write
+  int64_t* place = (int64_t*)pg_lds;             // [R] element offset of the row's slot; -1: no sequence's row; -2: it has no place
   int* angle_of = (int*)(place + R);             // [R] position that turns the row
   float2* cs = (float2*)(angle_of + (R + 1) / 2 * 2);   // [R][half]
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, first = blockIdx.x * R;
+  const int h0 = a.q ? 0 : a.heads, nh = a.heads + 2 * a.kv - h0, items = R * nh * C;
+  struct Item {
+    int i, r, head, kind, hk, d[2];   // row of the workgroup's and of the buffers; head of all, of its kind (q, k, v); first dims of the two runs
+    bool turn;
+  };
+  auto item = [&](int it) {
+    Item x;
+    const uint32_t c = (uint32_t)it % C, v = (uint32_t)it / C;
+    x.i = v / (uint32_t)nh;
+    x.head = h0 + v - x.i * nh;
+    x.r = first + x.i;
+    x.kind = x.head < a.heads ? 0 : x.head < a.heads + a.kv ? 1 : 2;
+    x.hk = x.head - (x.kind == 0 ? 0 : x.kind == 1 ? a.heads : a.heads + a.kv);
+    x.turn = x.kind < 2 && (int)c < a.rot / 16;
+    // values keep their order, and so do the dims behind the rotated ones
+    const bool split = x.turn && !a.interleaved;
+    x.d[0] = split ? 8 * c : 16 * c;
+    x.d[1] = x.d[0] + (split ? half : 8);
+    return x;
+  };
+  uint4 raw[2][EB / 2];
+  auto fetch = [&](const Item& x) {
+    if (x.r >= a.b.rows) return;
+    const uint8_t* src = (x.kind == 0 ? a.q : x.kind == 1 ? a.k : a.v) + EB * (x.r * (x.kind == 0 ? a.qs : x.kind == 1 ? a.ks : a.vs) + (int64_t)x.hk * D);
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+#pragma unroll
+      for (int n = 0; n < EB / 2; n++) raw[u][n] = gld((const uint4*)(src + EB * x.d[u]) + n);
+  };
+  Item x = item(tid);
+  if (tid < items) fetch(x);
   for (int i = w; i < R; i += 4) {
     const int r = first + i;
     int64_t off = -1;
@@ -102,12 +146,10 @@ __global__ __launch_bounds__(256) void pg_append_kernel(PgAppend a, int R) {
       const PgSeq q = pg_seq_at(a.b, s);
       const int t = q.p0 + (r - q.first);
       at = a.positions ? gld(a.positions + r) : t;
+      off = -2;   // (a row without a place in the cache: its query is turned all the same)
       if (t >= 0 && t < pg_cap(a.b)) {
         const int page = gld(a.b.table + s * a.b.table_stride + (t >> a.b.page_log));
         if (page >= 0 && page < a.b.pages) off = page * a.page_stride + (t & ((1 << a.b.page_log) - 1)) * a.slot_stride;
-        else off = -2;
-      } else {
-        off = -2;   // a row without a place in the cache: its query is turned all the same
       }
     }
     if (lane == 0) {
@@ -123,76 +165,76 @@ __global__ __launch_bounds__(256) void pg_append_kernel(PgAppend a, int R) {
     cs[i] = {c, s};
   }
   __syncthreads();
-  const int nh = a.heads + 2 * a.kv, h0 = a.q ? 0 : a.heads;
-  for (int it = tid; it < R * (nh - h0) * C; it += 256) {
-    const int c = it % C, head = h0 + it / C % (nh - h0), i = it / C / (nh - h0), r = first + i;
-    const bool live = place[i] != -1;   // (the same for all lanes of a head)
-    const int kind = head < a.heads ? 0 : head < a.heads + a.kv ? 1 : 2, hk = kind == 0 ? head : kind == 1 ? head - a.heads : head - a.heads - a.kv;
-    const bool turn = kind < 2 && c < a.rot / 16;
-    const int da = a.rot == 0 || c >= a.rot / 16 || a.interleaved ? 16 * c : 8 * c;
-    const int db = turn && !a.interleaved ? da + half : da + 8;
-    // values keep their order (kind 2), and so do the dims behind the rotated ones
-    const int d[2] = {kind == 2 ? 16 * c : da, kind == 2 ? 16 * c + 8 : db};
-    float x[2][8] = {};
-    constexpr int EB = TX == PG_F32 ? 4 : 2;
-    if (live) {
-      const uint8_t* src = (kind == 0 ? a.q : kind == 1 ? a.k : a.v) + EB * (r * (kind == 0 ? a.qs : kind == 1 ? a.ks : a.vs) + (int64_t)hk * D);
+  for (int it = tid; it < items; it += 256) {
+    const Item y = x;
+    float v[2][8];
+#pragma unroll
+    for (int u = 0; u < 2; u++) pg_unpack<TX>(raw[u], v[u]);
+    if (it + 256 < items) {
+      x = item(it + 256);
+      fetch(x);
+    }
+    const int64_t at = place[y.i];   // (the same for all lanes of a head)
+    if (at == -1) {
+#pragma unroll
+      for (int n = 0; n < 8; n++) v[0][n] = v[1][n] = 0.f;   // (rows past the last were not fetched)
+    }
+    if (a.bias) {
 #pragma unroll
       for (int u = 0; u < 2; u++) {
-        uint4 raw[EB / 2];
+        float b[8];
+        pg_floats8(a.bias + y.head * D + y.d[u], b);
 #pragma unroll
-        for (int n = 0; n < EB / 2; n++) raw[n] = gld((const uint4*)(src + EB * d[u]) + n);
-        pg_unpack<TX>(raw, x[u]);
-        if (a.bias)
-#pragma unroll
-          for (int n = 0; n < 8; n++) x[u][n] += gld(a.bias + head * D + d[u] + n);
+        for (int n = 0; n < 8; n++) v[u][n] += b[n];
       }
     }
-    const float* gamma = kind == 0 ? a.qn : kind == 1 ? a.kn : nullptr;
+    const float* gamma = y.kind == 0 ? a.qn : y.kind == 1 ? a.kn : nullptr;
     if (a.qn || a.kn) {   // (the lanes of a head agree; other heads' lanes take part in the exchange)
       float sum = 0.f;
 #pragma unroll
-      for (int n = 0; n < 8; n++) sum = fmaf(x[0][n], x[0][n], fmaf(x[1][n], x[1][n], sum));
+      for (int n = 0; n < 8; n++) sum = fmaf(v[0][n], v[0][n], fmaf(v[1][n], v[1][n], sum));
 #pragma unroll
       for (int m = 1; m < C; m <<= 1) sum += __shfl_xor(sum, m);
       if (gamma) {
         const float inv = 1.f / sqrtf(sum * (1.f / D) + a.eps);
 #pragma unroll
-        for (int u = 0; u < 2; u++)
+        for (int u = 0; u < 2; u++) {
+          float g[8];
+          pg_floats8(gamma + y.d[u], g);
 #pragma unroll
-          for (int n = 0; n < 8; n++) x[u][n] *= inv * gld(gamma + d[u] + n);
+          for (int n = 0; n < 8; n++) v[u][n] *= inv * g[n];
+        }
       }
     }
-    if (!live) continue;
-    if (turn) {
-      const float2* row = cs + i * half;
+    if (at == -1 || (y.kind > 0 && at < 0)) continue;
+    if (y.turn) {
+      const float2* row = cs + y.i * half;
       if (a.interleaved) {
 #pragma unroll
         for (int u = 0; u < 2; u++)
 #pragma unroll
           for (int n = 0; n < 8; n += 2) {
-            const float2 t = row[(d[u] + n) >> 1];
-            const float p = x[u][n], q = x[u][n + 1];
-            x[u][n] = fmaf(p, t.x, -(q * t.y));
-            x[u][n + 1] = fmaf(q, t.x, p * t.y);
+            const float2 t = row[(y.d[u] + n) >> 1];
+            const float p = v[u][n], q = v[u][n + 1];
+            v[u][n] = fmaf(p, t.x, -(q * t.y));
+            v[u][n + 1] = fmaf(q, t.x, p * t.y);
           }
       } else {
 #pragma unroll
         for (int n = 0; n < 8; n++) {
-          const float2 t = row[d[0] + n];
-          const float p = x[0][n], q = x[1][n];
-          x[0][n] = fmaf(p, t.x, -(q * t.y));
-          x[1][n] = fmaf(q, t.x, p * t.y);
+          const float2 t = row[y.d[0] + n];
+          const float p = v[0][n], q = v[1][n];
+          v[0][n] = fmaf(p, t.x, -(q * t.y));
+          v[1][n] = fmaf(q, t.x, p * t.y);
         }
       }
     }
-    if (kind > 0 && place[i] < 0) continue;
-    uint16_t* dst = kind == 0 ? (uint16_t*)a.qo + r * a.qos + (int64_t)hk * D
-                              : (uint16_t*)(kind == 1 ? a.kc : a.vc) + place[i] + hk * a.head_stride;
+    uint16_t* dst = y.kind == 0 ? (uint16_t*)a.qo + y.r * a.qos + (int64_t)y.hk * D
+                                : (uint16_t*)(y.kind == 1 ? a.kc : a.vc) + at + y.hk * a.head_stride;
 #pragma unroll
     for (int u = 0; u < 2; u++) {
-      const uint4 y = pg_pack8<TC>(x[u]);
-      gst((gu32x4*)(dst + d[u]), (gu32x4){y.x, y.y, y.z, y.w});
+      const uint4 z = pg_pack8<TC>(v[u]);
+      gst((gu32x4*)(dst + y.d[u]), (gu32x4){z.x, z.y, z.z, z.w});
     }
   }
 }
@@ -256,6 +298,7 @@ struct PgFinder {
       look(0);
       part = pg_part((int64_t)n * most, c);
       units = n * pg_splits(most, part);
+      whole_if_more();
       return;
     }
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -305,6 +348,11 @@ struct PgFinder {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < NW; i++) units += lds.units[i];
+    whole_if_more();
+  }
+  // The launch has a workgroup for each unit if row0 ascends. If not, nothing is cut: no part waits in vain for another.
+  __device__ __forceinline__ void whole_if_more() {
+    if (units > (int)gridDim.x) part = PG_MOST;
   }
 
   // Unit u of sequence s: u is counted from the sequence's first, parts and tiles are what the sequences before it have.
@@ -370,9 +418,11 @@ __device__ __forceinline__ v4f pg_mfma16(uint4 a, uint4 b, v4f c) {   // 16 x 16
 // 16 bytes from base + each lane's offset into LDS, lane i's at lds + 16 i. In inline assembly, because the
 // compiler cannot tell the buffers apart and would wait for every load in flight before each LDS read;
 // the kernels wait themselves (PG_WAIT), and extra loads of the compiler's own only make that wait longer.
+// `base` may have been written by a vector instruction just before (v_readlane, also from a spill): a load may read it five
+// wait states later, which the compiler, not seeing the load, does not ensure.
 template <int AT>
 __device__ __forceinline__ void pg_dma16(const void* base, uint32_t off, uint32_t lds) {   // to lds + AT + 16 i; base and lds: the same for every lane
-  asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base), "n"(AT) : "memory", "scc");
+  asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base), "n"(AT) : "memory", "scc", "m0");
 }
 __device__ __forceinline__ uint32_t pg_lds_at(const void* p) {   // an LDS address, as every lane's
   return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const LAS uint8_t*)p);
@@ -494,13 +544,24 @@ __device__ __forceinline__ void pg_store(const PgAttend& a, int row, int head, i
   else gst((gu32x2*)((uint16_t*)a.out + at), (gu32x2){pg_pack2<TC>(y[0], y[1]), pg_pack2<TC>(y[2], y[3])});
 }
 
-// Parts are written with agent-scope stores, which go through to where all XCDs see them, so that a workgroup only has to
-// wait until its own are acknowledged. (An agent-scope release instead writes the XCD's whole L2 back: 333 rows of 14
-// heads took 41 us with it, 18 us without.)
+// Parts are written and read with agent-scope accesses, which go through to where all XCDs see them: a workgroup only has
+// to wait until its own stores are acknowledged. (An agent-scope release instead writes the XCD's whole L2 back: 333 rows of
+// 14 heads took 41 us with it, 18 us without.)
 __device__ __forceinline__ void pg_share(float* p, v4f v) {
   const gu32x4 x = __builtin_bit_cast(gu32x4, v);
   astore64((uint64_t*)p, (uint64_t)x[0] | (uint64_t)x[1] << 32);
   astore64((uint64_t*)p + 1, (uint64_t)x[2] | (uint64_t)x[3] << 32);
+}
+__device__ __forceinline__ v4f pg_shared(const float* p) {
+  const uint64_t x = aload64((const uint64_t*)p), y = aload64((const uint64_t*)p + 1);
+  return (v4f){__uint_as_float((uint32_t)x), __uint_as_float((uint32_t)(x >> 32)), __uint_as_float((uint32_t)y), __uint_as_float((uint32_t)(y >> 32))};
+}
+
+// The same number, which the compiler does not know to be: what is computed from it is computed here, and not ahead of
+// the loops, where every workgroup would wait for what only the last ones need (8.8 against 8.0 us for a sequence of 500).
+__device__ __forceinline__ int pg_late(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
 }
 
 // Whether this is the last of `count` workgroups to come here, whose parts it then sees (the same for every thread). The
@@ -514,9 +575,7 @@ __device__ __forceinline__ bool pg_last(int32_t* counter, int count, int* lds) {
     *lds = all;
   }
   __syncthreads();
-  const bool all = *lds != 0;
-  if (all) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-  return all;
+  return __builtin_amdgcn_readfirstlane(*lds) != 0;
 }
 
 // Writes a part's state of row r, four dims from d on.
@@ -533,13 +592,23 @@ template <int TC, int D, int M, int NW>
 __device__ __forceinline__ void pg_join(const PgAttend& a, const PgCut& c, const PgWork& pw, const PgUnit& un, int first, int step, int count, bool out,
                                         int f0, int live, LAS float* lds) {
   constexpr int NT = 64 * NW, T = NT / M >= 64 ? 64 : NT / M < 1 ? 1 : NT / M;   // T threads of a row, neighbours in a wave
-  const int tid = threadIdx.x;
+  const int tid = pg_late(threadIdx.x);
   LAS float *wt = lds, *ls = lds + PG_FAN * M, *rows = ls + PG_FAN * M;
+  // few items (four dims of a row): `groups` threads each, every groups-th part to one of them, its values fetched along
+  // with the statistics
+  const int items = live * (D / 4), groups = items <= NT / 4 ? 4 : items <= NT / 2 ? 2 : 1, width = NT / groups;
+  const int g = tid / width, i_first = tid % width;
+  auto part_of = [&](int i, int x) { return pw.o + ((size_t)(first + x * step) * M + i / (D / 4)) * D + 4 * (i % (D / 4)); };
+  v4f ahead[PG_FAN / 2];
+  if (groups > 1)
+#pragma unroll
+    for (int u = 0; u < PG_FAN / 2; u++)
+      if (g + u * groups < count && i_first < items) ahead[u] = pg_shared(part_of(i_first, g + u * groups));
   for (int i = tid; i < count * M; i += NT) {
     const int x = i / M, r = i % M;
-    const uint2 v = r < live ? gld((const uint2*)(pw.ml + (size_t)(first + x * step) * M + r)) : make_uint2(0, 0);
-    wt[i] = __uint_as_float(v.x);
-    ls[i] = __uint_as_float(v.y);
+    const uint64_t v = r < live ? aload64((const uint64_t*)(pw.ml + (size_t)(first + x * step) * M + r)) : 0;
+    wt[i] = __uint_as_float((uint32_t)v);
+    ls[i] = __uint_as_float((uint32_t)(v >> 32));
   }
   __syncthreads();
   if (tid < M * T) {
@@ -561,18 +630,24 @@ __device__ __forceinline__ void pg_join(const PgAttend& a, const PgCut& c, const
     }
   }
   __syncthreads();
-  // few items: `groups` threads each, every groups-th part to one of them
-  const int items = live * (D / 4), groups = items <= NT / 4 ? 4 : items <= NT / 2 ? 2 : 1, width = NT / groups;
-  for (int i0 = 0; i0 < items; i0 += width) {
-    const int i = i0 + tid % width, g = tid / width, r = i / (D / 4), d = 4 * (i % (D / 4));
+  for (int i = i_first; i - i_first < items; i += width) {
+    const int r = i / (D / 4), d = 4 * (i % (D / 4));
     v4f y = {0.f, 0.f, 0.f, 0.f};
     if (i < items) {
-      const float* o = pw.o + ((size_t)first * M + r) * D + d;
+      if (groups > 1) {
+#pragma unroll
+        for (int u = 0; u < PG_FAN / 2; u++)
+          if (g + u * groups < count) {
+            const float e = wt[(g + u * groups) * M + r];
+            if (e != 0.f) y += ahead[u] * e;
+          }
+      } else {
 #pragma unroll 8
-      for (int x = g; x < count; x += groups) {
-        const float e = wt[x * M + r];
-        const v4f v = __builtin_bit_cast(v4f, gld((const uint4*)(o + (size_t)x * step * M * D)));
-        if (e != 0.f) y += v * e;
+        for (int x = 0; x < count; x++) {
+          const float e = wt[x * M + r];
+          const v4f v = pg_shared(part_of(i, x));
+          if (e != 0.f) y += v * e;
+        }
       }
     }
     if (groups > 1) {   // (items <= width: once)
@@ -593,12 +668,19 @@ __device__ __forceinline__ void pg_join(const PgAttend& a, const PgCut& c, const
 // What follows a part of several: the last workgroup of PG_FAN parts joins them, and the last of those joins theirs.
 template <int TC, int D, int M, int NW>
 __device__ __forceinline__ void pg_finish(const PgAttend& a, const PgCut& c, const PgWork& w, const PgUnit& un, int f0, int live, LAS float* lds, int* last) {
-  const int g = un.split / PG_FAN, groups = pg_up(un.splits, PG_FAN), count = min(PG_FAN, un.splits - g * PG_FAN);
+  const int g = un.split / PG_FAN, groups = pg_up(un.splits, PG_FAN);
   int32_t* joined = w.joined + un.tile_at * (PG_MAXSPLIT / PG_FAN + 1);
-  if (!pg_last(joined + 1 + g, count, last)) return;
-  pg_join<TC, D, M, NW>(a, c, w, un, un.part_at + g * PG_FAN, 1, count, groups == 1, f0, live, lds);
-  if (groups == 1 || !pg_last(joined, groups, last)) return;
-  pg_join<TC, D, M, NW>(a, c, w, un, un.part_at, PG_FAN, groups, true, f0, live, lds);
+  int first = un.part_at + g * PG_FAN, step = 1, count = min(PG_FAN, un.splits - g * PG_FAN);
+  int32_t* counter = joined + 1 + g;
+  for (bool out = groups == 1;; out = true) {   // (once or twice)
+    if (!pg_last(counter, count, last)) return;
+    pg_join<TC, D, M, NW>(a, c, w, un, first, step, count, out, f0, live, lds);
+    if (out) return;
+    first = un.part_at;
+    step = PG_FAN;
+    count = groups;
+    counter = joined;
+  }
 }
 
 struct PgStep {
@@ -656,189 +738,188 @@ __global__ __launch_bounds__(64 * NW, 2) void pg_step_kernel(PgStep p) {
     const int key = KPI * i + lane / UPR;
     lane_off[i] = 2 * ((uint32_t)(key & 15) * (uint32_t)a.slot_stride + 8 * ((lane % UPR) ^ pg_swz<D>(key)));
   }
-  for (int u = blockIdx.x, units = __builtin_amdgcn_readfirstlane(finder.units); u < units; u += gridDim.x) {
-    const PgUnit un = pg_uniform(finder.find(u));
-    if (un.seq.n == 0) continue;
-    const int G = c.G, flat = un.seq.n * G, f0 = 16 * un.q, live = min(16, flat - f0);   // (n G is at most 2^30)
-    const uint32_t f = min(f0 + n, flat - 1), at_row = f / c.G;
-    const int row = un.seq.first + at_row, head = un.head * G + (f - at_row * c.G);
-    const int pos = un.seq.p0 + at_row, p0 = __builtin_amdgcn_readlane(pos, 0), p1 = __builtin_amdgcn_readlane(pos, 15);
-    const PgRange range = pg_range(p0, p1, cap, c);
-    const int per = pg_up(range.n, un.splits), c0 = min(un.split * per, range.n), c1 = min(c0 + per, range.n);
-    const int end = min(p1 + 1, cap);
-    uint4 qf[KS];
+  if ((int)blockIdx.x >= __builtin_amdgcn_readfirstlane(finder.units)) return;
+  const PgUnit un = pg_uniform(finder.find(blockIdx.x));
+  if (un.seq.n == 0) return;
+  const int G = c.G, flat = un.seq.n * G, f0 = 16 * un.q, live = min(16, flat - f0);   // (n G is at most 2^30)
+  const uint32_t f = min(f0 + n, flat - 1), at_row = f / c.G;
+  const int row = un.seq.first + at_row, head = un.head * G + (f - at_row * c.G);
+  const int pos = un.seq.p0 + at_row, p0 = __builtin_amdgcn_readlane(pos, 0), p1 = __builtin_amdgcn_readlane(pos, 15);
+  const PgRange range = pg_range(p0, p1, cap, c);
+  const int per = pg_up(range.n, un.splits), c0 = min(un.split * per, range.n), c1 = min(c0 + per, range.n);
+  const int end = min(p1 + 1, cap);
+  uint4 qf[KS];
 #pragma unroll
-    for (int ks = 0; ks < KS; ks++) qf[ks] = gld((const uint4*)(a.q + row * a.qs + (int64_t)head * D + 32 * ks + 8 * kg));
-    const int mine = c0 + w < c1 ? (c1 - c0 - w + NW - 1) / NW : 0;   // this wave's tiles
-    // where the keys of the wave's next 64 / NG tiles are, 16 of them a lane: elements from the cache's begin; -1: not there
-    int64_t group = -1;
-    auto groups = [&](int k) {
-      const int t = c0 + w + NW * (k + lane / NG);
-      group = -1;
-      if (t < c1) {
-        const int g = pg_key_tile(range, t) * KT + 16 * (lane % NG), key = min(g, end - 1);
-        const int page = gld(a.b.table + un.s * a.b.table_stride + (key >> a.b.page_log));
-        if (page >= 0 && page < a.b.pages) group = page * a.page_stride + (g & pmask) * a.slot_stride + un.head * a.head_stride;
-      }
-    };
-    auto group_at = [&](int k, int g) {   // (the same for every lane)
-      const int at = (k * NG + g) & 63;
-      return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)group, at) |
-                       (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(group >> 32), at) << 32);
-    };
-    auto load = [&](const uint16_t* from, auto to, int k) {
-      pg_each<NG>([&](auto g) {
-        const int64_t at = group_at(k, g);
-        const uint16_t* base = from + (at < 0 ? 0 : at);   // (the first page is there, and masked)
-        pg_each<8 / NG>([&](auto i) {
-          constexpr int I = g * 8 / NG + i;
-          pg_dma16<to + 1024 * I>(base, lane_off[I], mine_lds);
-        });
-      });
-    };
-    float Mx = -INFINITY, Ls = 0.f;   // Ls: this lane's keys only
-    v4f O[ND];
-#pragma unroll
-    for (int d = 0; d < ND; d++) O[d] = (v4f){0.f, 0.f, 0.f, 0.f};
-    groups(0);
-    PG_WAIT_OWN();
-    if (mine > 0) {
-      load(a.kc, KEYS, 0);
-      load(a.vc, VALUES, 0);
+  for (int ks = 0; ks < KS; ks++) qf[ks] = gld((const uint4*)(a.q + row * a.qs + (int64_t)head * D + 32 * ks + 8 * kg));
+  const int mine = c0 + w < c1 ? (c1 - c0 - w + NW - 1) / NW : 0;   // this wave's tiles
+  // where the keys of the wave's next 64 / NG tiles are, 16 of them a lane: elements from the cache's begin; -1: not there
+  int64_t group = -1;
+  auto groups = [&](int k) {
+    const int t = c0 + w + NW * (k + lane / NG);
+    group = -1;
+    if (t < c1) {
+      const int g = pg_key_tile(range, t) * KT + 16 * (lane % NG), key = min(g, end - 1);
+      const int page = gld(a.b.table + un.s * a.b.table_stride + (key >> a.b.page_log));
+      if (page >= 0 && page < a.b.pages) group = page * a.page_stride + (g & pmask) * a.slot_stride + un.head * a.head_stride;
     }
-    for (int k = 0; k < mine; k++) {
-      const int kt = pg_key_tile(range, c0 + w + NW * k) * KT;
-      const bool more = k + 1 < mine;
-      int good = 0;   // groups of 16 keys whose pages are there
+  };
+  auto group_at = [&](int k, int g) {   // (the same for every lane)
+    const int at = (k * NG + g) & 63;
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)group, at) |
+                     (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(group >> 32), at) << 32);
+  };
+  auto load = [&](const uint16_t* from, auto to, int k) {
+    pg_each<NG>([&](auto g) {
+      const int64_t at = group_at(k, g);
+      const uint16_t* base = from + (at < 0 ? 0 : at);   // (the first page is there, and masked)
+      pg_each<8 / NG>([&](auto i) {
+        constexpr int I = g * 8 / NG + i;
+        pg_dma16<to + 1024 * I>(base, lane_off[I], mine_lds);
+      });
+    });
+  };
+  float Mx = -INFINITY, Ls = 0.f;   // Ls: this lane's keys only
+  v4f O[ND];
 #pragma unroll
-      for (int g = 0; g < NG; g++) good |= (__builtin_amdgcn_readlane((int)(group >> 32), (k * NG + g) & 63) >= 0) << g;
-      PG_WAIT(8);   // the keys; the 8 loads after them are the values
-      v4f s[NB];
+  for (int d = 0; d < ND; d++) O[d] = (v4f){0.f, 0.f, 0.f, 0.f};
+  groups(0);
+  PG_WAIT_OWN();
+  if (mine > 0) {
+    load(a.kc, KEYS, 0);
+    load(a.vc, VALUES, 0);
+  }
+  for (int k = 0; k < mine; k++) {
+    const int kt = pg_key_tile(range, c0 + w + NW * k) * KT;
+    const bool more = k + 1 < mine;
+    int good = 0;   // groups of 16 keys whose pages are there
 #pragma unroll
-      for (int b = 0; b < NB; b++) {
-        s[b] = (v4f){0.f, 0.f, 0.f, 0.f};
+    for (int g = 0; g < NG; g++) good |= (__builtin_amdgcn_readlane((int)(group >> 32), (k * NG + g) & 63) >= 0) << g;
+    PG_WAIT(8);   // the keys; the 8 loads after them are the values
+    v4f s[NB];
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++) s[b] = pg_mfma16<TC>(pg_get(kl + ka[ks] + (32 * (b >> 1) + 4 * (b & 1)) * 2 * D), qf[ks], s[b]);
-      }
-      PG_WAIT_LDS();   // the keys have been read
-      if (more) {
-        if (((k + 1) & (64 / NG - 1)) == 0) groups(k + 1);
-        load(a.kc, KEYS, k + 1);
-      }
-      // every row sees the whole tile, or the rows' masks (wave-uniform)
-      const bool whole = good == (1 << NG) - 1 && kt + KT - 1 <= p0 && kt + KT <= end && (c.window == 0 || kt > p1 - c.window || kt + KT <= c.sinks);
-      uint32_t seen = ~0u;
-      if (!whole) {
-        seen = 0;
+    for (int b = 0; b < NB; b++) {
+      s[b] = (v4f){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int b = 0; b < NB; b++)
-#pragma unroll
-          for (int r = 0; r < 4; r++) {
-            const int key = 32 * (b >> 1) + 8 * kg + 4 * (b & 1) + r, j = kt + key;
-            const bool on = j < cap && pg_sees(pos, j, c.window, c.sinks) && (good >> (key >> 4) & 1);
-            if (!on) s[b][r] = -INFINITY;
-            seen |= (uint32_t)on << (4 * b + r);
-          }
-      }
-      float mc = s[0][0];
+      for (int ks = 0; ks < KS; ks++) s[b] = pg_mfma16<TC>(pg_get(kl + ka[ks] + (32 * (b >> 1) + 4 * (b & 1)) * 2 * D), qf[ks], s[b]);
+    }
+    PG_WAIT_LDS();   // the keys have been read
+    if (more) {
+      if (((k + 1) & (64 / NG - 1)) == 0) groups(k + 1);
+      load(a.kc, KEYS, k + 1);
+    }
+    // every row sees the whole tile, or the rows' masks (wave-uniform)
+    const bool whole = good == (1 << NG) - 1 && kt + KT - 1 <= p0 && kt + KT <= end && (c.window == 0 || kt > p1 - c.window || kt + KT <= c.sinks);
+    uint32_t seen = ~0u;
+    if (!whole) {
+      seen = 0;
 #pragma unroll
       for (int b = 0; b < NB; b++)
 #pragma unroll
-        for (int r = 0; r < 4; r++) mc = fmaxf(mc, s[b][r]);
-      mc *= sc2;
-      if (__any(mc > Mx + (PG_UP + PG_SLACK))) {
-        mc = over_kg(mc, OpMaxF{});
-        const float mn = mc == -INFINITY ? Mx : fmaxf(mc - PG_UP, Mx), up = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(Mx - mn);
-        Mx = mn;
-        Ls *= up;
-#pragma unroll
-        for (int d = 0; d < ND; d++) O[d] *= up;
-      }
-      const float ref = Mx == -INFINITY ? 0.f : Mx;
-      uint4 ph[NS], pl[NS];
-#pragma unroll
-      for (int b = 0; b < NB; b++) {
-        float e[4];
-#pragma unroll
         for (int r = 0; r < 4; r++) {
-          e[r] = __builtin_amdgcn_exp2f(fmaf(s[b][r], sc2, -ref));
-          Ls += e[r];
+          const int key = 32 * (b >> 1) + 8 * kg + 4 * (b & 1) + r, j = kt + key;
+          // pg_sees. (Without branches: the compiler has lost the stores of `if (!on) s[b][r] = ..` behind && and ||.)
+          const bool on = j < cap & j <= pos & (c.window == 0 | j > pos - c.window | j < c.sinks) & (good >> (key >> 4) & 1);
+          s[b][r] = on ? s[b][r] : -INFINITY;
+          seen |= (uint32_t)on << (4 * b + r);
         }
+    }
+    float mc = s[0][0];
 #pragma unroll
-        for (int r = 0; r < 4; r += 2) {
-          const uint32_t x = pg_pack2<TC>(e[r], e[r + 1]);
-          (&ph[b >> 1].x)[2 * (b & 1) + r / 2] = x;
-          if constexpr (FINE) {
-            float y[2];
-            pg_unpack2<TC>(x, y);
-            (&pl[b >> 1].x)[2 * (b & 1) + r / 2] = pg_pack2<TC>(e[r] - y[0], e[r + 1] - y[1]);
-          }
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) mc = fmaxf(mc, s[b][r]);
+    mc *= sc2;
+    if (__any(mc > Mx + (PG_UP + PG_SLACK))) {
+      mc = over_kg(mc, OpMaxF{});
+      const float mn = mc == -INFINITY ? Mx : fmaxf(mc - PG_UP, Mx), up = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(Mx - mn);
+      Mx = mn;
+      Ls *= up;
+#pragma unroll
+      for (int d = 0; d < ND; d++) O[d] *= up;
+    }
+    const float ref = Mx == -INFINITY ? 0.f : Mx;
+    gu32x4 ph[NS], pl[NS];
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+      float e[4];
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        e[r] = __builtin_amdgcn_exp2f(fmaf(s[b][r], sc2, -ref));
+        Ls += e[r];
+      }
+#pragma unroll
+      for (int r = 0; r < 4; r += 2) {
+        const uint32_t x = pg_pack2<TC>(e[r], e[r + 1]);
+        ph[b >> 1][2 * (b & 1) + r / 2] = x;
+        if constexpr (FINE) {
+          float y[2];
+          pg_unpack2<TC>(x, y);
+          pl[b >> 1][2 * (b & 1) + r / 2] = pg_pack2<TC>(e[r] - y[0], e[r + 1] - y[1]);
         }
       }
-      if (more) PG_WAIT(8);   // the values; the 8 loads after them are the next keys
-      else PG_WAIT(0);
-      bool wild = false;
-      if (!whole) wild = pg_wild_tile<TC, KT * UPR>(vl, lane);   // what a row does not see must not reach it as 0 x inf
-      if (wild) {
+    }
+    if (more) PG_WAIT(8);   // the values; the 8 loads after them are the next keys
+    else PG_WAIT(0);
+    bool wild = false;
+    if (!whole) wild = pg_wild_tile<TC, KT * UPR>(vl, lane);   // what a row does not see must not reach it as 0 x inf
+    if (wild) {
 #pragma unroll
-        for (int d = 0; d < ND; d++) {
-          v4f m = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int t = 0; t < NS; t++) {
-            uint4 marks;
-            const uint4 v = pg_tamed<TC>(pg_values<D>(vl + va[d] + 32 * t * 2 * D), marks);
-            O[d] = pg_mfma16<TC>(v, ph[t], O[d]);
-            if constexpr (FINE) O[d] = pg_mfma16<TC>(v, pl[t], O[d]);
-            m = pg_mfma16<TC>(marks, pg_ones<TC>(seen >> (8 * t)), m);
-          }
-#pragma unroll
-          for (int r = 0; r < 4; r++) O[d][r] += pg_wild_sum(m[r]);
-        }
-      } else {
-#pragma unroll
-      for (int d = 0; d < ND; d++)
+      for (int d = 0; d < ND; d++) {
+        v4f m = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int t = 0; t < NS; t++) {
-          const uint4 v = pg_values<D>(vl + va[d] + 32 * t * 2 * D);
-          O[d] = pg_mfma16<TC>(v, ph[t], O[d]);
-          if constexpr (FINE) O[d] = pg_mfma16<TC>(v, pl[t], O[d]);
+          uint4 marks;
+          const uint4 v = pg_tamed<TC>(pg_values<D>(vl + va[d] + 32 * t * 2 * D), marks);
+          O[d] = pg_mfma16<TC>(v, __builtin_bit_cast(uint4, ph[t]), O[d]);
+          if constexpr (FINE) O[d] = pg_mfma16<TC>(v, __builtin_bit_cast(uint4, pl[t]), O[d]);
+          m = pg_mfma16<TC>(marks, pg_ones<TC>(seen >> (8 * t)), m);
         }
+#pragma unroll
+        for (int r = 0; r < 4; r++) O[d][r] += pg_wild_sum(m[r]);
       }
-      PG_WAIT_LDS();   // the values have been read
-      if (more) load(a.vc, VALUES, k + 1);
-    }
-    // the waves' states, each in its own LDS
-    Ls = over_kg(Ls, OpAddF{});
-    LAS float* st = (LAS float*)lds[w];
+    } else {
 #pragma unroll
-    for (int d = 0; d < ND; d++) *(LAS v4f*)(st + n * RF + 16 * d + 4 * kg) = O[d];
-    if (kg == 0) {
-      smx[w][n] = Mx;
-      sls[w][n] = Ls;
-    }
-    __syncthreads();
-    for (int i = tid; i < live * (D / 4); i += 64 * NW) {
-      const int r = i / (D / 4), d = 4 * (i % (D / 4));
-      float m = smx[0][r];
+    for (int d = 0; d < ND; d++)
 #pragma unroll
-      for (int x = 1; x < NW; x++) m = fmaxf(m, smx[x][r]);
-      float l = 0.f;
-      v4f o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int x = 0; x < NW; x++) {
-        const float e = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(smx[x][r] - m);
-        l += sls[x][r] * e;
-        if (e != 0.f) o += *(const LAS v4f*)((const LAS float*)lds[x] + r * RF + d) * e;
-      }
-      if (un.splits == 1) {
-        pg_store<TC>(a, un.seq.first + (uint32_t)(f0 + r) / c.G, un.head * c.G + (uint32_t)(f0 + r) % c.G, d, D, l == 0.f ? (v4f){0.f, 0.f, 0.f, 0.f} : o / l);
-      } else {
-        pg_put_part<D, 16>(p.w, un.part_at + un.split, r, d, m, l, o);
+      for (int t = 0; t < NS; t++) {
+        const uint4 v = pg_values<D>(vl + va[d] + 32 * t * 2 * D);
+        O[d] = pg_mfma16<TC>(v, __builtin_bit_cast(uint4, ph[t]), O[d]);
+        if constexpr (FINE) O[d] = pg_mfma16<TC>(v, __builtin_bit_cast(uint4, pl[t]), O[d]);
       }
     }
-    if (un.splits > 1) pg_finish<TC, D, 16, NW>(a, c, p.w, un, f0, live, (LAS float*)lds, &last);
-    __syncthreads();   // LDS is the next unit's
+    PG_WAIT_LDS();   // the values have been read
+    if (more) load(a.vc, VALUES, k + 1);
   }
+  // the waves' states, each in its own LDS
+  Ls = over_kg(Ls, OpAddF{});
+  LAS float* st = (LAS float*)lds[w];
+#pragma unroll
+  for (int d = 0; d < ND; d++) *(LAS v4f*)(st + n * RF + 16 * d + 4 * kg) = O[d];
+  if (kg == 0) {
+    smx[w][n] = Mx;
+    sls[w][n] = Ls;
+  }
+  __syncthreads();
+  for (int i = pg_late(tid); i < live * (D / 4); i += 64 * NW) {
+    const int r = i / (D / 4), d = 4 * (i % (D / 4));
+    float m = smx[0][r];
+#pragma unroll
+    for (int x = 1; x < NW; x++) m = fmaxf(m, smx[x][r]);
+    float l = 0.f;
+    v4f o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < NW; x++) {
+      const float e = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(smx[x][r] - m);
+      l += sls[x][r] * e;
+      if (e != 0.f) o += *(const LAS v4f*)((const LAS float*)lds[x] + r * RF + d) * e;
+    }
+    if (un.splits == 1) {
+      pg_store<TC>(a, un.seq.first + (uint32_t)(f0 + r) / c.G, un.head * c.G + (uint32_t)(f0 + r) % c.G, d, D, l == 0.f ? (v4f){0.f, 0.f, 0.f, 0.f} : o / l);
+    } else {
+      pg_put_part<D, 16>(p.w, un.part_at + un.split, r, d, m, l, o);
+    }
+  }
+  if (un.splits > 1) pg_finish<TC, D, 16, NW>(a, c, p.w, un, f0, live, (LAS float*)lds, &last);
 }
 
 template <int TC>
@@ -891,215 +972,213 @@ __global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
   for (int d = 0; d < ND; d++)
 #pragma unroll
     for (int t = 0; t < 2; t++) va[d][t] = pg_values_at<D>(16 * t + 8 * h, 32 * d + 16 * ((lane >> 4) & 1), lane & 15);
-  for (int u = blockIdx.x, units = __builtin_amdgcn_readfirstlane(finder.units); u < units; u += gridDim.x) {
-    const PgUnit un = pg_uniform(finder.find(u));
-    if (un.seq.n == 0) continue;
-    const int G = c.G, flat = un.seq.n * G, f0 = M * un.q, live = min(M, flat - f0);   // (n G is at most 2^30)
-    const uint32_t f = min(f0 + 32 * w + n, flat - 1), at_row = f / c.G;
-    const int row = un.seq.first + at_row, head = un.head * G + (f - at_row * c.G);
-    const int pos = un.seq.p0 + at_row, w0 = __builtin_amdgcn_readlane(pos, 0), w1 = __builtin_amdgcn_readlane(pos, 31);   // of the wave's rows
-    const int p0 = un.seq.p0 + (uint32_t)f0 / c.G, p1 = un.seq.p0 + (uint32_t)(f0 + live - 1) / c.G;
-    const PgRange range = pg_range(p0, p1, cap, c);
-    const int per = pg_up(range.n, un.splits), c0 = min(un.split * per, range.n), count = min(per, range.n - c0);
-    const int end = min(p1 + 1, cap), wend = 32 * w < live ? min(w1 + 1, cap) : 0;
-    uint4 qf[KS];
+  if ((int)blockIdx.x >= __builtin_amdgcn_readfirstlane(finder.units)) return;
+  const PgUnit un = pg_uniform(finder.find(blockIdx.x));
+  if (un.seq.n == 0) return;
+  const int G = c.G, flat = un.seq.n * G, f0 = M * un.q, live = min(M, flat - f0);   // (n G is at most 2^30)
+  const uint32_t f = min(f0 + 32 * w + n, flat - 1), at_row = f / c.G;
+  const int row = un.seq.first + at_row, head = un.head * G + (f - at_row * c.G);
+  const int pos = un.seq.p0 + at_row, w0 = __builtin_amdgcn_readlane(pos, 0), w1 = __builtin_amdgcn_readlane(pos, 31);   // of the wave's rows
+  const int p0 = un.seq.p0 + (uint32_t)f0 / c.G, p1 = un.seq.p0 + (uint32_t)(f0 + live - 1) / c.G;
+  const PgRange range = pg_range(p0, p1, cap, c);
+  const int per = pg_up(range.n, un.splits), c0 = min(un.split * per, range.n), count = min(per, range.n - c0);
+  const int end = min(p1 + 1, cap), wend = 32 * w < live ? min(w1 + 1, cap) : 0;
+  uint4 qf[KS];
 #pragma unroll
-    for (int ks = 0; ks < KS; ks++) qf[ks] = gld((const uint4*)(a.q + row * a.qs + (int64_t)head * D + 16 * ks + 8 * h));
-    // where the 16 keys from `key` on are: elements from the cache's begin; -1: not there
-    auto place = [&](int key) -> int64_t {
-      const int page = gld(a.b.table + un.s * a.b.table_stride + (min(key, end - 1) >> a.b.page_log));
-      return page >= 0 && page < a.b.pages ? page * a.page_stride + (key & pmask) * a.slot_stride + un.head * a.head_stride : -1;
-    };
-    const int all_hi = min(p0 + 1, end) - KT, all_lo = c.window ? p1 - c.window : -1, mine_hi = min(w0 + 1, wend) - KT, mine_lo = c.window ? w1 - c.window : -1;
-    int64_t group = -1;   // of the next 16 tiles, 16 keys a lane
-    uint64_t there = 0;   // which of them have a place
-    auto groups = [&](int k) {
-      const int t = k + lane / 4;
-      group = -1;
-      if (t < count) group = place(pg_key_tile(range, c0 + t) * KT + 16 * (lane % 4));
-      there = __ballot(group >= 0);
-    };
-    // Loads of a tile, 2 x LOADS of them, one at a time between the products of the tile before: together, right behind the
-    // barrier, they held every wave up for 900 cycles (D 128), a quarter of a tile. A tile behind the last is the first page.
-    const uint16_t *next_k, *next_v;
-    auto next = [&](int k) {
-      const int at = (4 * k + w) & 63;
-      const int64_t e = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)group, at) |
-                                  (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(group >> 32), at) << 32);
-      const int64_t off = k < count && e > 0 ? e : 0;   // (where there is none, the first page is loaded, and masked)
-      next_k = a.kc + off;
-      next_v = a.vc + off;
-    };
-    auto load = [&](auto i, auto buffer) {
-      constexpr int I = i % LOADS;
-      pg_dma16<32 * T * buffer + (i < LOADS ? 0 : 16 * T) + 1024 * I>((i < LOADS ? next_k : next_v) + (LOADS == 4 && (I & 1) ? 4 * a.slot_stride : 0), lane_off[I * 2 / LOADS],
-                                                                  mine_lds);
-    };
-    const auto B0 = std::integral_constant<int, 0>{};
-    float Mx = -INFINITY, Ls = 0.f;   // Ls: this lane's keys only
-    v16f O[ND];
+  for (int ks = 0; ks < KS; ks++) qf[ks] = gld((const uint4*)(a.q + row * a.qs + (int64_t)head * D + 16 * ks + 8 * h));
+  // where the 16 keys from `key` on are: elements from the cache's begin; -1: not there
+  auto place = [&](int key) -> int64_t {
+    const int page = gld(a.b.table + un.s * a.b.table_stride + (min(key, end - 1) >> a.b.page_log));
+    return page >= 0 && page < a.b.pages ? page * a.page_stride + (key & pmask) * a.slot_stride + un.head * a.head_stride : -1;
+  };
+  const int all_hi = min(p0 + 1, end) - KT, all_lo = c.window ? p1 - c.window : -1, mine_hi = min(w0 + 1, wend) - KT, mine_lo = c.window ? w1 - c.window : -1;
+  int64_t group = -1;   // of the next 16 tiles, 16 keys a lane
+  uint64_t there = 0;   // which of them have a place
+  auto groups = [&](int k) {
+    const int t = k + lane / 4;
+    group = -1;
+    if (t < count) group = place(pg_key_tile(range, c0 + t) * KT + 16 * (lane % 4));
+    there = __ballot(group >= 0);
+  };
+  // Loads of a tile, 2 x LOADS of them, one at a time between the products of the tile before: together, right behind the
+  // barrier, they held every wave up for 900 cycles (D 128), a quarter of a tile. A tile behind the last is the first page.
+  const uint16_t *next_k, *next_v;
+  auto next = [&](int k) {
+    const int at = (4 * k + w) & 63;
+    const int64_t e = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)group, at) |
+                                (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(group >> 32), at) << 32);
+    const int64_t off = k < count && e > 0 ? e : 0;   // (where there is none, the first page is loaded, and masked)
+    next_k = a.kc + off;
+    next_v = a.vc + off;
+  };
+  auto load = [&](auto i, auto buffer) {
+    constexpr int I = i % LOADS;
+    pg_dma16<32 * T * buffer + (i < LOADS ? 0 : 16 * T) + 1024 * I>((i < LOADS ? next_k : next_v) + (LOADS == 4 && (I & 1) ? 4 * a.slot_stride : 0), lane_off[I * 2 / LOADS],
+                                                                mine_lds);
+  };
+  const auto B0 = std::integral_constant<int, 0>{};
+  float Mx = -INFINITY, Ls = 0.f;   // Ls: this lane's keys only
+  v16f O[ND];
 #pragma unroll
-    for (int d = 0; d < ND; d++) O[d] = (v16f){};
-    if (tid == 0) tamed = 0;
-    groups(0);
-    PG_WAIT_OWN();
-    if (count > 0) {
-      next(0);
-      pg_each<2 * LOADS>([&](auto i) { load(i, B0); });
-    }
-    auto tile = [&](int k, auto buffer) {   // buffer: k % 2
-      constexpr int BUF = decltype(buffer)::value;
-      constexpr std::integral_constant<int, 1 - BUF> OTHER{};
-      const int kt = pg_key_tile(range, c0 + k) * KT;
-      const int good = (int)(there >> (4 * k & 63)) & 15;   // groups of 16 keys that are there
-      // whether all rows of the workgroup, and of the wave, see the whole tile (the same for every lane)
-      const bool all = good == 15 && kt <= all_hi && (kt > all_lo || kt + KT <= c.sinks), mine = good == 15 && kt <= mine_hi && (kt > mine_lo || kt + KT <= c.sinks);
-      if (((k + 1) & 15) == 0) groups(k + 1);
-      next(k + 1);
-      PG_WAIT(0);
-      __syncthreads();   // the tile is there, and every wave is done with the buffer filled next
-      const LAS uint8_t* kl = (const LAS uint8_t*)lds[BUF][0];
-      LAS uint8_t* vl = (LAS uint8_t*)lds[BUF][1];
-      if (!all) {
+  for (int d = 0; d < ND; d++) O[d] = (v16f){};
+  if (tid == 0) tamed = 0;
+  groups(0);
+  PG_WAIT_OWN();
+  if (count > 0) {
+    next(0);
+    pg_each<2 * LOADS>([&](auto i) { load(i, B0); });
+  }
+  auto tile = [&](int k, auto buffer) {   // buffer: k % 2
+    constexpr int BUF = decltype(buffer)::value;
+    constexpr std::integral_constant<int, 1 - BUF> OTHER{};
+    const int kt = pg_key_tile(range, c0 + k) * KT;
+    const int good = (int)(there >> (4 * k & 63)) & 15;   // groups of 16 keys that are there
+    // whether all rows of the workgroup, and of the wave, see the whole tile (the same for every lane)
+    const bool all = good == 15 && kt <= all_hi && (kt > all_lo || kt + KT <= c.sinks), mine = good == 15 && kt <= mine_hi && (kt > mine_lo || kt + KT <= c.sinks);
+    if (((k + 1) & 15) == 0) groups(k + 1);
+    next(k + 1);
+    PG_WAIT(0);
+    __syncthreads();   // the tile is there, and every wave is done with the buffer filled next
+    const LAS uint8_t* kl = (const LAS uint8_t*)lds[BUF][0];
+    LAS uint8_t* vl = (LAS uint8_t*)lds[BUF][1];
+    if (!all) {
 #pragma unroll 1
-        for (int i = tid; i < T; i += 256) {
-          uint4 marks;
-          const uint4 v = pg_get(vl + 16 * i);
-          if (pg_wild<TC>(v)) {
-            const uint4 y = pg_tamed<TC>(v, marks);
-            *(pg_lds4*)(vl + 16 * i) = (gu32x4){y.x, y.y, y.z, y.w};
-            tamed = k + 1;
-          }
+      for (int i = tid; i < T; i += 256) {
+        uint4 marks;
+        const uint4 v = pg_get(vl + 16 * i);
+        if (pg_wild<TC>(v)) {
+          const uint4 y = pg_tamed<TC>(v, marks);
+          *(pg_lds4*)(vl + 16 * i) = (gu32x4){y.x, y.y, y.z, y.w};
+          tamed = k + 1;
         }
-        PG_TURN();
       }
-      if (kt >= wend) {   // behind all of the wave's rows
-        pg_each<2 * LOADS>([&](auto i) { load(i, OTHER); });
-        return;
-      }
-      // operands are read a group of products ahead; the fences keep the compiler from moving the reads back to their products
-      v16f s[2] = {};
-      uint4 kf[2][2][2];   // [group's turn][16 dims][32 keys]
-      auto keys = [&](int g) {
+      PG_TURN();
+    }
+    if (kt >= wend) {   // behind all of the wave's rows
+      pg_each<2 * LOADS>([&](auto i) { load(i, OTHER); });
+      return;
+    }
+    // operands are read a group of products ahead; the fences keep the compiler from moving the reads back to their products
+    v16f s[2] = {};
+    uint4 kf[2][2][2];   // [group's turn][16 dims][32 keys]
+    auto keys = [&](int g) {
 #pragma unroll
-        for (int i = 0; i < 2; i++)
+      for (int i = 0; i < 2; i++)
 #pragma unroll
-          for (int b = 0; b < 2; b++) kf[g & 1][i][b] = pg_get(kl + ka[2 * g + i] + 32 * b * 2 * D);
-        __builtin_amdgcn_sched_barrier(0);
-      };
-      keys(0);
-      pg_each<KS / 2>([&](auto g) {
-        if constexpr (g + 1 < KS / 2) keys(g + 1);
+        for (int b = 0; b < 2; b++) kf[g & 1][i][b] = pg_get(kl + ka[2 * g + i] + 32 * b * 2 * D);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    keys(0);
+    pg_each<KS / 2>([&](auto g) {
+      if constexpr (g + 1 < KS / 2) keys(g + 1);
 #pragma unroll
-        for (int i = 0; i < 2; i++)
+      for (int i = 0; i < 2; i++)
 #pragma unroll
-          for (int b = 0; b < 2; b++) s[b] = pg_mfma32<TC>(kf[g & 1][i][b], qf[2 * g + i], s[b]);
-        pg_each<4 * LOADS / KS>([&](auto i) { load(std::integral_constant<int, 4 * LOADS / KS * g + i>{}, OTHER); });
-        __builtin_amdgcn_sched_barrier(0);
-      });
-      uint4 vf[2][ND];   // [group's turn][32 dims]: the values of 16 keys
-      auto values = [&](int t) {
+        for (int b = 0; b < 2; b++) s[b] = pg_mfma32<TC>(kf[g & 1][i][b], qf[2 * g + i], s[b]);
+      pg_each<4 * LOADS / KS>([&](auto i) { load(std::integral_constant<int, 4 * LOADS / KS * g + i>{}, OTHER); });
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    uint4 vf[2][ND];   // [group's turn][32 dims]: the values of 16 keys
+    auto values = [&](int t) {
 #pragma unroll
-        for (int d = 0; d < ND; d++) vf[t & 1][d] = pg_values<D>(vl + va[d][t & 1] + 32 * (t >> 1) * 2 * D);
-        __builtin_amdgcn_sched_barrier(0);
-      };
-      values(0);
-      uint32_t seen = ~0u;
-      if (!mine) {
-        seen = 0;
-#pragma unroll
-        for (int b = 0; b < 2; b++)
-#pragma unroll
-          for (int r = 0; r < 16; r++) {
-            const int key = 32 * b + 16 * (r >> 3) + 8 * h + (r & 7), j = kt + key;
-            const bool on = j < cap & j <= pos & (c.window == 0 | j > pos - c.window | j < c.sinks) & (good >> (2 * b + (r >> 3)) & 1);   // pg_sees
-            s[b][r] = on ? s[b][r] : -INFINITY;
-            seen |= (uint32_t)on << (16 * b + r);
-          }
-      }
-      float mc = s[0][0];
+      for (int d = 0; d < ND; d++) vf[t & 1][d] = pg_values<D>(vl + va[d][t & 1] + 32 * (t >> 1) * 2 * D);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    values(0);
+    uint32_t seen = ~0u;
+    if (!mine) {
+      seen = 0;
 #pragma unroll
       for (int b = 0; b < 2; b++)
 #pragma unroll
-        for (int r = 0; r < 16; r++) mc = fmaxf(mc, s[b][r]);
-      mc *= sc2;
-      if (__any(mc > Mx + (PG_UP + PG_SLACK))) {
-        mc = over_h(mc, OpMaxF{});
-        const float mn = mc == -INFINITY ? Mx : fmaxf(mc - PG_UP, Mx), up = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(Mx - mn);
-        Mx = mn;
-        Ls *= up;
-#pragma unroll
-        for (int d = 0; d < ND; d++) O[d] *= up;
-      }
-      const float ref = Mx == -INFINITY ? 0.f : Mx;
-      uint4 ph[4], pl[4];   // weights of 16 keys each
-#pragma unroll
-      for (int t = 0; t < 4; t++) {
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-          const float e0 = __builtin_amdgcn_exp2f(fmaf(s[t >> 1][8 * (t & 1) + i], sc2, -ref)), e1 = __builtin_amdgcn_exp2f(fmaf(s[t >> 1][8 * (t & 1) + i + 1], sc2, -ref));
-          sum += e0 + e1;
-          const uint32_t x = pg_pack2<TC>(e0, e1);
-          (&ph[t].x)[i >> 1] = x;
-          if constexpr (FINE) {
-            float y[2];
-            pg_unpack2<TC>(x, y);
-            (&pl[t].x)[i >> 1] = pg_pack2<TC>(e0 - y[0], e1 - y[1]);
-          }
+        for (int r = 0; r < 16; r++) {
+          const int key = 32 * b + 16 * (r >> 3) + 8 * h + (r & 7), j = kt + key;
+          const bool on = j < cap & j <= pos & (c.window == 0 | j > pos - c.window | j < c.sinks) & (good >> (2 * b + (r >> 3)) & 1);   // pg_sees
+          s[b][r] = on ? s[b][r] : -INFINITY;
+          seen |= (uint32_t)on << (16 * b + r);
         }
-        Ls += sum;
-      }
+    }
+    float mc = s[0][0];
 #pragma unroll
-      for (int t = 0; t < 4; t++) {
-        if (t < 3) values(t + 1);
+    for (int b = 0; b < 2; b++)
 #pragma unroll
-        for (int d = 0; d < ND; d++) {
-          O[d] = pg_mfma32<TC>(vf[t & 1][d], ph[t], O[d]);
-          if constexpr (FINE) O[d] = pg_mfma32<TC>(vf[t & 1][d], pl[t], O[d]);
+      for (int r = 0; r < 16; r++) mc = fmaxf(mc, s[b][r]);
+    mc *= sc2;
+    if (__any(mc > Mx + (PG_UP + PG_SLACK))) {
+      mc = over_h(mc, OpMaxF{});
+      const float mn = mc == -INFINITY ? Mx : fmaxf(mc - PG_UP, Mx), up = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(Mx - mn);
+      Mx = mn;
+      Ls *= up;
+#pragma unroll
+      for (int d = 0; d < ND; d++) O[d] *= up;
+    }
+    const float ref = Mx == -INFINITY ? 0.f : Mx;
+    gu32x4 ph[4], pl[4];   // weights of 16 keys each
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        const float e0 = __builtin_amdgcn_exp2f(fmaf(s[t >> 1][8 * (t & 1) + i], sc2, -ref)), e1 = __builtin_amdgcn_exp2f(fmaf(s[t >> 1][8 * (t & 1) + i + 1], sc2, -ref));
+        sum += e0 + e1;
+        const uint32_t x = pg_pack2<TC>(e0, e1);
+        ph[t][i >> 1] = x;
+        if constexpr (FINE) {
+          float y[2];
+          pg_unpack2<TC>(x, y);
+          pl[t][i >> 1] = pg_pack2<TC>(e0 - y[0], e1 - y[1]);
         }
-        __builtin_amdgcn_sched_barrier(0);
       }
-      if (!all && __builtin_amdgcn_readfirstlane(tamed) == k + 1) {   // the values as they were, from memory
+      Ls += sum;
+    }
 #pragma unroll
-        for (int d = 0; d < ND; d++) {
-          v16f m = {};
+    for (int t = 0; t < 4; t++) {
+      if (t < 3) values(t + 1);
+#pragma unroll
+      for (int d = 0; d < ND; d++) {
+        O[d] = pg_mfma32<TC>(vf[t & 1][d], __builtin_bit_cast(uint4, ph[t]), O[d]);
+        if constexpr (FINE) O[d] = pg_mfma32<TC>(vf[t & 1][d], __builtin_bit_cast(uint4, pl[t]), O[d]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (!all && __builtin_amdgcn_readfirstlane(tamed) == k + 1) {   // the values as they were, from memory
+#pragma unroll
+      for (int d = 0; d < ND; d++) {
+        v16f m = {};
 #pragma unroll 1
-          for (int t = 0; t < 4; t++) {
-            const int64_t at = place(kt + 16 * t);
-            const uint16_t* v = a.vc + (at < 0 ? 0 : at) + 8 * h * a.slot_stride + 32 * d + n;
-            uint32_t x[4];
+        for (int t = 0; t < 4; t++) {
+          const int64_t at = place(kt + 16 * t);
+          const uint16_t* v = a.vc + (at < 0 ? 0 : at) + 8 * h * a.slot_stride + 32 * d + n;
+          uint32_t x[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) x[i] = gld(v + 2 * i * a.slot_stride) | (uint32_t)gld(v + (2 * i + 1) * a.slot_stride) << 16;
-            uint4 marks;
-            pg_tamed<TC>(make_uint4(x[0], x[1], x[2], x[3]), marks);
-            m = pg_mfma32<TC>(marks, pg_ones<TC>(seen >> (8 * t)), m);
-          }
-#pragma unroll
-          for (int r = 0; r < 16; r++) O[d][r] += pg_wild_sum(m[r]);
+          for (int i = 0; i < 4; i++) x[i] = gld(v + 2 * i * a.slot_stride) | (uint32_t)gld(v + (2 * i + 1) * a.slot_stride) << 16;
+          uint4 marks;
+          pg_tamed<TC>(make_uint4(x[0], x[1], x[2], x[3]), marks);
+          m = pg_mfma32<TC>(marks, pg_ones<TC>(seen >> (8 * t)), m);
         }
+#pragma unroll
+        for (int r = 0; r < 16; r++) O[d][r] += pg_wild_sum(m[r]);
       }
-    };
-    for (int k = 0; k < count; k += 2) {
-      tile(k, std::integral_constant<int, 0>{});
-      if (k + 1 < count) tile(k + 1, std::integral_constant<int, 1>{});
     }
-    PG_WAIT(0);   // (a load behind the last tile)
-    Ls = over_h(Ls, OpAddF{});
-    const int r = 32 * w + n;
-    if (r < live) {
-      const float inv = Ls == 0.f ? 0.f : 1.f / Ls;
-#pragma unroll
-      for (int d = 0; d < ND; d++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const v4f o = {O[d][4 * i], O[d][4 * i + 1], O[d][4 * i + 2], O[d][4 * i + 3]};
-          const int dim = 32 * d + 8 * i + 4 * h;
-          if (un.splits == 1) pg_store<TC>(a, row, head, dim, D, Ls == 0.f ? (v4f){0.f, 0.f, 0.f, 0.f} : o * inv);
-          else pg_put_part<D, M>(p.w, un.part_at + un.split, r, dim, Mx, Ls, o);
-        }
-    }
-    if (un.splits > 1) pg_finish<TC, D, M, 4>(a, c, p.w, un, f0, live, (LAS float*)lds, &last);
-    __syncthreads();   // LDS is the next unit's
+  };
+  for (int k = 0; k < count; k += 2) {
+    tile(k, std::integral_constant<int, 0>{});
+    if (k + 1 < count) tile(k + 1, std::integral_constant<int, 1>{});
   }
+  PG_WAIT(0);   // (a load behind the last tile)
+  Ls = over_h(Ls, OpAddF{});
+  const int r = 32 * w + n;
+  if (r < live) {
+    const float inv = Ls == 0.f ? 0.f : 1.f / Ls;
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const v4f o = {O[d][4 * i], O[d][4 * i + 1], O[d][4 * i + 2], O[d][4 * i + 3]};
+        const int dim = 32 * d + 8 * i + 4 * h;
+        if (un.splits == 1) pg_store<TC>(a, row, head, dim, D, Ls == 0.f ? (v4f){0.f, 0.f, 0.f, 0.f} : o * inv);
+        else pg_put_part<D, M>(p.w, un.part_at + un.split, r, dim, Mx, Ls, o);
+      }
+  }
+  if (un.splits > 1) pg_finish<TC, D, M, 4>(a, c, p.w, un, f0, live, (LAS float*)lds, &last);
 }

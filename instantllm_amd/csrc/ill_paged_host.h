@@ -184,7 +184,7 @@ int ill_paged_append(ill_paged* p, const ill_paged_batch* batch, const ill_paged
   a.eps = d.norm_eps;
   illp::OnDevice on(p->device);
   if (on.rc) return on.rc;
-  const int R = 4, lds = R * 8 + (R + 1) / 2 * 8 + R * (d.rotary_dim / 2) * 8;
+  const int R = pg_append_rows(a.b.rows, ((a.q ? d.heads : 0) + 2 * d.kv_heads) * d.head_dim / 16), lds = R * 8 + (R + 1) / 2 * 8 + R * (d.rotary_dim / 2) * 8;
   hipStream_t st = (hipStream_t)stream;
   if (x->dtype == ILL_F32) {
     if (d.dtype == ILL_F16) illp::launch_append<PG_F32, PG_F16>(a, d.head_dim, R, lds, st);
@@ -238,7 +238,7 @@ int ill_paged_attend(ill_paged* p, const ill_paged_batch* batch, const void* q, 
   for (int i = 0; i < 2; i++) {
     if (!(i ? prompts : both || !prompts)) continue;
     PgStep& s = parts[i];
-    const int64_t grid = std::min<int64_t>(pg_grid(a.b.seqs, a.b.rows, most, !a.b.row0, cap, s.c), i == 0 && both ? 1024 : 1 << 20);
+    const int64_t grid = pg_grid(a.b.seqs, a.b.rows, !a.b.row0, cap, s.c);   // (below 2^31: rows x heads are at most 2^30)
     if (!grid) continue;
     if (work) s.w = illp::work_of(work, s.c.log, s.c.M, d.head_dim);
     if (d.dtype == ILL_F16) {

@@ -10,7 +10,7 @@
 
 #define PG_MOST (1 << 30)    // positions, rows x heads, windows and sinks: at most this many
 #define PG_MAXSPLIT 256      // parts that the keys of a tile of rows are cut into at most
-#define PG_FAN 16            // of which so many are joined at a time
+#define PG_FAN 16            // of which so many are joined at a time, in two steps (131071 keys in 256 parts: 24.4 us; 32: 26.2, 64: 31.4, 128: 39.6)
 
 // A batch as the kernels read it (ill_paged_batch with the handle's geometry).
 struct PgBatch {
@@ -45,6 +45,22 @@ PG_FN PgSeq pg_seq(int begin, int end, int len, int rows) {
 
 // Whether the row at position p sees position j.
 PG_FN bool pg_sees(int p, int j, int window, int sinks) { return j >= 0 && j <= p && (window == 0 || j > p - window || j < sinks); }
+
+// Rows of a workgroup of the append kernel, whose 256 threads take `items` pieces of each row: as few as fill the threads'
+// turns to four fifths, up to 8, and fewer where there would be less than two workgroups for each CU. (64 rows of 384 pieces
+// at 4 rows to a workgroup, 16 workgroups of six turns: 10.2 us.)
+PG_FN int pg_append_rows(int rows, int items) {
+  int best = 1;
+  for (int r = 1; r <= 8; r++) {
+    const int used = r * items, room = pg_up(used, 256) * 256;
+    if (5 * used >= 4 * room) {
+      best = r;
+      break;
+    }
+    if (r == 1 || used * (pg_up(best * items, 256) * 256) > best * items * room) best = r;
+  }
+  return pg_max(1, pg_min(best, rows / 512));
+}
 
 // ---- the work of an attention call -------------------------------------------------------
 // A sequence's n new rows and the G query heads of a key/value head make n G flat rows (row f / G,
@@ -114,12 +130,15 @@ PG_FN int pg_part(int64_t work, const PgCut& c) {
 }
 PG_FN int pg_splits(int most, int part) { return most <= part ? 1 : pg_min(pg_up(most, part), PG_MAXSPLIT); }
 
-// Workgroups that have something to do, at most, as far as the host can tell.
-PG_FN int64_t pg_grid(int seqs, int rows, int64_t max_rows, bool one_row, int cap, const PgCut& c) {
+// Units of work, at most, as far as the host can tell: a workgroup for each. `shared`: as pg_share divides the sequences, the step
+// kernel has the ones of PG_FEW flat rows and, where there are fewer than PG_MANY tiles of 128, also those.
+PG_FN int64_t pg_grid(int seqs, int rows, bool one_row, int cap, const PgCut& c) {
   const int64_t G = c.G;
-  int64_t q = rows * G / c.M + seqs;
-  const int64_t each = one_row ? 1 : max_rows;
-  if (each > 0 && each <= PG_MOST && (each * G + c.M - 1) / c.M * seqs < q) q = (each * G + c.M - 1) / c.M * seqs;
-  const int64_t tiles = q * c.kv, cut = tiles * pg_splits(pg_most(cap, cap, c), c.least);
+  int64_t tiles = (one_row ? (G + c.M - 1) / c.M * seqs : rows * G / c.M + seqs) * c.kv;
+  if (c.shared && c.M == 16) {
+    const int64_t some = (int64_t)seqs * c.kv * (PG_FEW / 16) + PG_MANY * (128 / 16);
+    tiles = some < tiles ? some : tiles;
+  }
+  const int64_t cut = tiles * pg_splits(pg_most(cap, cap, c), c.least);
   return cut < tiles + (1 << c.log) ? cut : tiles + (1 << c.log);
 }

@@ -95,8 +95,8 @@ int main() {
     }
     CHECK(parts <= 2ll << c.log && cut <= 1ll << c.log);
     // the launch has a workgroup for every unit, where the sizes that the host knows hold
-    CHECK(units <= pg_grid(seqs, rows, 0, false, cap, c));
-    CHECK(units <= pg_grid(seqs, rows, most_rows, false, cap, c));
+    CHECK(units <= pg_grid(seqs, rows, false, cap, c));
+    if (most_rows <= 1 && rows == seqs) CHECK(units <= pg_grid(seqs, rows, true, cap, c));
   }
   // two kernels: every sequence with rows is exactly one's
   for (int i = 0; i < 20000; i++) {
@@ -108,7 +108,11 @@ int main() {
     for (int& x : n) { x = draw(0, 2) ? draw(0, 10) : draw(0, 900); tiles += pg_prompt_tiles(x, step.G, step.kv); }
     pg_share(step, tiles);
     pg_share(prompt, tiles);
-    long long taken = 0;
+    long long taken = 0, units = 0;
+    int rows = 0;
+    for (int x : n) { units += pg_qtiles(x, step) * (int)step.kv; rows += x; }
+    step.shared = 1; step.KT = 64; step.least = 8; step.log = 8;
+    CHECK(units <= pg_grid(5, rows, false, 64, step));   // (one tile of keys: no parts)
     for (int x : n) {
       CHECK((pg_qtiles(x, step) > 0) + (pg_qtiles(x, prompt) > 0) == (x > 0));
       taken += pg_qtiles(x, prompt) * (int)prompt.kv;

@@ -287,15 +287,15 @@ ILL_API int ill_gemv_destroy(ill_gemv* g);
  * ILL_F16 or ILL_BF16 in pages of `page_size` positions (a power of two, 16 .. 1024). Element
  * (page, slot, head, dim) of either cache is at page * page_stride + slot * slot_stride +
  * head * head_stride + dim elements (all 0: [pages][page_size][kv_heads][head_dim]); strides are
- * multiples of 8, slot_stride at most 2^24. The rotation turns the first `rotary_dim` dims of a head (a multiple of 16;
- * 0: none) by position * rope_base^(-2 i / rotary_dim), pairing dim i with i + rotary_dim / 2, or
+ * multiples of 8, slot_stride at most 2^24. The rotation turns the first `rotary_dim` dims of a
+ * head (a multiple of 16; 0: none) by position * rope_base^(-2 i / rotary_dim), pairing dim i with i + rotary_dim / 2, or
  * with interleaved != 0 dims 2 i and 2 i + 1. norm_eps belongs to the head norms; scale
  * multiplies the scores (0: 1 / sqrt(head_dim)). A handle belongs to the GPU that was current
  * when it was created; one thread at a time calls on it.
  * Attention that is split over the keys joins its parts through a workspace that the handle
  * holds, one for each stream that calls come on and one for each capture of a stream, `streams`
- * of them (0: 8; 9 MB each at head size 64, 17 at 128): calls on different streams, and graphs, may run at the same
- * time. What is enqueued on one stream, or captured on one stream in one capture, shares a
+ * of them (0: 8; 9 MB each at head size 64, 17 at 128): calls on different streams, and graphs,
+ * may run at the same time (hipStreamPerThread, a different stream in each thread, is refused). What is enqueued on one stream, or captured on one stream in one capture, shares a
  * workspace: such a graph is instantiated once. A call that would need one more is refused;
  * ill_paged_release, called when nothing that the handle has enqueued or captured will run any
  * more, makes all of them free again. */
@@ -313,14 +313,16 @@ ILL_API int ill_paged_release(ill_paged* p);
 
 /* A batch. lens, table and row0 are device arrays that the kernels read when they run, so a
  * captured call follows what they then hold. lens [seqs]: the positions of each sequence, its
- * new rows included (below 0 counts as 0). table [seqs][table_stride], table_width entries used: the page of positions
- * i * page_size .. in entry i; entries behind a sequence's last position are not read. row0
+ * new rows included (below 0 counts as 0). table [seqs][table_stride], table_width entries used:
+ * the page of positions i * page_size .. in entry i; entries behind a sequence's last position
+ * are not read. row0
  * [seqs + 1]: ascending; sequence s has the new rows row0[s] .. row0[s + 1] - 1, which stand at
- * its last positions; NULL: row s is sequence s's only one. rows: rows of the buffers (the ones behind
- * the last sequence's are left alone). max_rows: the most new rows that a sequence has, if
+ * its last positions; NULL: row s is sequence s's only one. rows: rows of the buffers (the ones
+ * behind the last sequence's are left alone). max_rows: the most new rows that a sequence has, if
  * known (0: unknown; a hint for the launch only). pages: pages of the cache. A page number
  * outside 0 .. pages - 1 is not followed: its positions are neither written nor seen, and so are
- * positions past table_width pages or below 0. Pages may be shared for reading. */
+ * positions past table_width pages or below 0. Pages may be shared for reading. rows x heads is
+ * at most 2^26, seqs x heads at most 2^22. */
 typedef struct {
   int32_t seqs, table_width;
   int64_t table_stride, rows, max_rows, pages;

@@ -337,7 +337,7 @@ struct PgFinder {
       work += lds.work[i];
     }
     part = pg_part(work, c);
-    units = (int)tiles;   // of uncut sequences: a unit for each
+    units = (int)min(tiles, (int64_t)PG_MOST);   // of uncut sequences: a unit for each. (As many only where row0 does not ascend.)
     int u = 0;
     for (s = threadIdx.x; s - (int)threadIdx.x < b.seqs; s += NT) {
       if (b.seqs > NT) look(s);
@@ -741,7 +741,7 @@ __global__ __launch_bounds__(64 * NW, 2) void pg_step_kernel(PgStep p) {
   if ((int)blockIdx.x >= __builtin_amdgcn_readfirstlane(finder.units)) return;
   const PgUnit un = pg_uniform(finder.find(blockIdx.x));
   if (un.seq.n == 0) return;
-  const int G = c.G, flat = un.seq.n * G, f0 = 16 * un.q, live = min(16, flat - f0);   // (n G is at most 2^30)
+  const int G = c.G, flat = un.seq.n * G, f0 = 16 * un.q, live = min(16, flat - f0);   // (n G is at most 2^26)
   const uint32_t f = min(f0 + n, flat - 1), at_row = f / c.G;
   const int row = un.seq.first + at_row, head = un.head * G + (f - at_row * c.G);
   const int pos = un.seq.p0 + at_row, p0 = __builtin_amdgcn_readlane(pos, 0), p1 = __builtin_amdgcn_readlane(pos, 15);
@@ -975,7 +975,7 @@ __global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
   if ((int)blockIdx.x >= __builtin_amdgcn_readfirstlane(finder.units)) return;
   const PgUnit un = pg_uniform(finder.find(blockIdx.x));
   if (un.seq.n == 0) return;
-  const int G = c.G, flat = un.seq.n * G, f0 = M * un.q, live = min(M, flat - f0);   // (n G is at most 2^30)
+  const int G = c.G, flat = un.seq.n * G, f0 = M * un.q, live = min(M, flat - f0);   // (n G is at most 2^26)
   const uint32_t f = min(f0 + 32 * w + n, flat - 1), at_row = f / c.G;
   const int row = un.seq.first + at_row, head = un.head * G + (f - at_row * c.G);
   const int pos = un.seq.p0 + at_row, w0 = __builtin_amdgcn_readlane(pos, 0), w1 = __builtin_amdgcn_readlane(pos, 31);   // of the wave's rows

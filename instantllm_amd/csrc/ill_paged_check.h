@@ -10,7 +10,8 @@
 
 namespace illp {
 
-constexpr int64_t kMost = 1 << 30;
+constexpr int64_t kMost = 1 << 30;                          // positions, strides
+constexpr int64_t kMostRows = 1 << 26, kMostSeqs = 1 << 22;   // times heads: a launch has fewer than 2^24 workgroups of 256 threads
 
 inline bool aligned(const void* p, int n) { return ((uintptr_t)p & (uintptr_t)(n - 1)) == 0; }
 
@@ -62,8 +63,8 @@ inline int check_desc(ill_paged_desc& d) {
 
 inline int check_batch(const ill_paged_desc& d, const ill_paged_batch* b) {
   if (!b) return fail(ILL_E_ARG, "paged: null batch");
-  if (b->seqs < 0 || b->rows < 0 || b->rows > kMost / d.heads || b->seqs > kMost / d.heads)
-    return fail(ILL_E_ARG, "paged: %d sequences, %lld rows (rows x heads up to 2^30)", b->seqs, (long long)b->rows);
+  if (b->seqs < 0 || b->rows < 0 || b->rows > kMostRows / d.heads || b->seqs > kMostSeqs / d.heads)
+    return fail(ILL_E_ARG, "paged: %d sequences, %lld rows (rows x heads up to 2^26, sequences x heads up to 2^22)", b->seqs, (long long)b->rows);
   if (b->pages < 1 || b->pages > INT32_MAX || b->table_width < 1 || b->table_width > kMost / d.page_size || b->table_stride < b->table_width ||
       b->table_stride > kMost)
     return fail(ILL_E_ARG, "paged: %lld pages, table of %d entries, %lld apart (positions up to 2^30)", (long long)b->pages, b->table_width,

@@ -63,7 +63,6 @@ PgWork work_of(uint8_t* at, int log, int M, int D) {
 
 // The workspace of the stream, or of its capture.
 int workspace(ill_paged* p, hipStream_t st, uint8_t** out) {
-  if (st == hipStreamPerThread) return fail(ILL_E_ARG, "paged: the per-thread default stream is several streams; pass a stream of your own");
   unsigned long long id = 0;
   if (st && st != hipStreamLegacy) {
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
@@ -203,6 +202,8 @@ int ill_paged_attend(ill_paged* p, const ill_paged_batch* batch, const void* q, 
   if (!p) return fail(ILL_E_ARG, "paged: null handle");
   const ill_paged_desc& d = p->d;
   if (int rc = illp::check_attend(d, batch, q, q_stride, k_cache, v_cache, window, sinks, out, out_stride, out_dtype)) return rc;
+  hipStream_t st = (hipStream_t)stream;
+  if (st == hipStreamPerThread) return fail(ILL_E_ARG, "paged: the per-thread default stream is several streams; pass a stream of your own");
   if (!batch->seqs || !batch->rows) return ILL_OK;
   PgAttend a{};
   a.b = illp::batch_of(p, *batch);
@@ -223,7 +224,6 @@ int ill_paged_attend(ill_paged* p, const ill_paged_batch* batch, const void* q, 
   a.scale = d.scale;
   illp::OnDevice on(p->device);
   if (on.rc) return on.rc;
-  hipStream_t st = (hipStream_t)stream;
   // One of the kernels where the sizes that the host knows say which, else both: the sequences are divided by pg_share.
   const int64_t G = d.heads / d.kv_heads, most = !a.b.row0 ? 1 : std::min<int64_t>(a.b.rows, batch->max_rows ? batch->max_rows : a.b.rows);
   PgStep parts[2] = {{a, illp::step_cut(d, a.window, a.sinks), {}}, {a, illp::prompt_cut(d, a.window, a.sinks), {}}};
@@ -238,7 +238,7 @@ int ill_paged_attend(ill_paged* p, const ill_paged_batch* batch, const void* q, 
   for (int i = 0; i < 2; i++) {
     if (!(i ? prompts : both || !prompts)) continue;
     PgStep& s = parts[i];
-    const int64_t grid = pg_grid(a.b.seqs, a.b.rows, !a.b.row0, cap, s.c);   // (below 2^31: rows x heads are at most 2^30)
+    const int64_t grid = pg_grid(a.b.seqs, a.b.rows, !a.b.row0, cap, s.c);   // (below 2^24: rows x heads are at most 2^26, sequences x heads 2^22)
     if (!grid) continue;
     if (work) s.w = illp::work_of(work, s.c.log, s.c.M, d.head_dim);
     if (d.dtype == ILL_F16) {

@@ -94,7 +94,7 @@ PG_FN void pg_share(PgCut& c, int64_t tiles) {
 }
 
 PG_FN int pg_qtiles(int n, const PgCut& c) {
-  const uint32_t f = (uint32_t)n * c.G;   // (rows x heads: at most 2^30)
+  const uint32_t f = (uint32_t)n * c.G;   // (rows x heads: at most 2^26)
   return f > (uint32_t)c.lo && f <= (uint32_t)c.hi ? (int)((f + c.M - 1) / (uint32_t)c.M) : 0;
 }
 

@@ -162,6 +162,10 @@ APPEND = [
     (dict(seqs=[(2, 5), (0, 2), (-7, 1), (0, 0), (18, 4)], pad=1), dict(norm=True)),
     # many sequences, so that a row's sequence is found over several steps
     (dict(seqs=[(i % 50 + 1, i % 4) for i in range(200)], heads=2, kv=1, dim=64), dict(x="f16")),
+    (dict(seqs=[(i % 50 + 1, i % 4) for i in range(300)], heads=2, kv=2, dim=128, dtype="bf16", pad=3), dict(norm=True)),
+    # prompts of which a workgroup takes several rows, the last one fewer
+    (dict(seqs=[(1500, 1300), (2901, 2901)], heads=2, kv=1, pad=2), dict(norm=True, bias=True)),
+    (dict(seqs=[(1031, 1031), (40, 1), (7, 9)], heads=3, kv=1, dim=128, dtype="bf16"), dict(x="f32")),
 ]
 
 
@@ -301,6 +305,12 @@ ATTEND = [
     # many sequences
     (dict(seqs=[(3 * i % 190, i % 3) for i in range(150)], heads=2, kv=1), dict(window=30, sinks=2)),
     (dict(seqs=[(7 * i % 300, 1) for i in range(130)], one_row=True, heads=4, kv=2, dim=128, scale=0.3), dict()),
+    # more than a workgroup has threads, one of them in parts
+    (dict(seqs=[(7 * i % 90, 1) if i != 290 else (6000, 1) for i in range(301)], one_row=True, heads=4, kv=2), dict()),
+    (dict(seqs=[(25 + i % 9, 20) if i != 270 else (3000, 30) for i in range(280)] + [(9, 2), (70, 1)], heads=4, kv=2, pad=2), dict(sinks=2, window=2000)),
+    # scores that leave only a few weights, with the greatest anywhere
+    (dict(seqs=[(700, 1), (90, 5), (65, 1)], heads=4, kv=2, scale=4.0), dict()),
+    (dict(seqs=[(300, 130), (129, 128)], heads=112, kv=112, dtype="bf16", scale=4.0), dict()),
 ]
 
 
@@ -501,6 +511,38 @@ def test_an_attention_block_with_the_stand_alone_product(hip):
         ref = mats[1][1] @ att.reshape(-1)
         # the decode step's tolerance: products in 16-bit fixed point, queries, keys and values rounded to f16
         assert np.linalg.norm(y - ref) <= 1e-2 * np.linalg.norm(ref), t
+
+
+@pytest.mark.parametrize("max_rows", [1, 3, 1 << 40])
+def test_a_wrong_hint_of_the_most_rows(hip, max_rows):
+    """max_rows only chooses kernels: too small or too large, every row is evaluated."""
+    s = Setup(hip, [(200, 129), (64, 64), (31, 40), (1, 1)], heads=64, kv=64, max_rows=max_rows)
+    s.attend()
+
+
+def test_workspaces_run_out_and_are_released(hip):
+    from instantllm_amd.engine import ILL_E_ARG, IllError
+    s = Setup(hip, [(9000, 1)], one_row=True, streams=2)
+    s.upload()
+    st = [hip.stream() for _ in range(2)]
+    dq, do = hip.put(s.random_bits(1, 896)), hip.alloc(2 * 896)
+    for stream in (st[0], None, st[0]):
+        s.op.attend(s.batch, s.kc, s.vc, dq, do, stream=stream)
+    with pytest.raises(IllError, match="ill_paged_release") as e:
+        s.op.attend(s.batch, s.kc, s.vc, dq, do, stream=st[1])
+    assert e.value.code == ILL_E_ARG
+    hip.sync()
+    s.op.release()
+    s.op.attend(s.batch, s.kc, s.vc, dq, do, stream=st[1])
+    s.attend(stream=st[0])
+
+
+def test_the_per_thread_stream_is_refused(hip):
+    from instantllm_amd.engine import IllError
+    s = Setup(hip, [(3, 1)], one_row=True)
+    s.upload()
+    with pytest.raises(IllError, match="per-thread"):
+        s.op.attend(s.batch, s.kc, s.vc, s.kc, s.vc, stream=2)
 
 
 def test_nothing_to_do(hip):

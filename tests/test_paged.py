@@ -90,7 +90,8 @@ def test_descriptions_refused(checks, kw, code):
 
 
 @pytest.mark.parametrize("kw", [
-    dict(seqs=-1), dict(rows=-1), dict(rows=2), dict(rows=1 << 27), dict(seqs=1 << 30, rows=1 << 30), dict(table_width=0), dict(table_stride=4),
+    dict(seqs=-1), dict(rows=-1), dict(rows=2), dict(rows=1 << 27), dict(rows=(1 << 26) // 14 + 1),
+    dict(seqs=(1 << 22) // 14 + 1, rows=1 << 20), dict(seqs=1 << 30, rows=1 << 30), dict(table_width=0), dict(table_stride=4),
     dict(table_width=1 << 27, table_stride=1 << 27), dict(pages=0), dict(pages=1 << 31), dict(max_rows=-1), dict(lens=None), dict(table=None),
     dict(lens=P16 + 2), dict(row0=P16 + 1)])
 def test_batches_refused(checks, kw):

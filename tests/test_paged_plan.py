@@ -98,6 +98,27 @@ int main() {
     CHECK(units <= pg_grid(seqs, rows, false, cap, c));
     if (most_rows <= 1 && rows == seqs) CHECK(units <= pg_grid(seqs, rows, true, cap, c));
   }
+  // rows of sequences in any order (which is not allowed): nothing is cut where the units are more than the launch has, and
+  // else the workspace holds the parts
+  for (int i = 0; i < 20000; i++) {
+    PgCut c{};
+    c.G = draw(1, 20); c.kv = draw(1, 4); c.M = draw(0, 1) ? 16 : 128; c.KT = 64;
+    c.log = draw(0, 6); c.least = draw(1, 5); c.hi = PG_MOST;
+    const int seqs = draw(1, 6), rows = draw(1, 200), cap = 16 * draw(1, 40);
+    long long work = 0, parts = 0, cut = 0;
+    std::vector<PgSeq> seq(seqs);
+    for (auto& q : seq) {
+      q = pg_seq(draw(-5, 220), draw(-5, 220), draw(-10, 700), rows);
+      work += (long long)pg_qtiles(q.n, c) * c.kv * pg_most(q.p0 + q.n, cap, c);
+    }
+    const int part = pg_part(work, c);
+    for (auto& q : seq) {
+      const int t = pg_qtiles(q.n, c) * (int)c.kv, most = pg_most(q.p0 + q.n, cap, c);
+      if (pg_splits(most, part) > 1) { parts += (long long)t * pg_splits(most, part); cut += t; }
+      CHECK(pg_splits(most, PG_MOST) == 1);
+    }
+    CHECK(parts <= 2ll << c.log && cut <= 1ll << c.log);
+  }
   // two kernels: every sequence with rows is exactly one's
   for (int i = 0; i < 20000; i++) {
     PgCut step{}, prompt{};

@@ -294,7 +294,7 @@ ILL_API int ill_gemv_destroy(ill_gemv* g);
  * when it was created; one thread at a time calls on it.
  * Attention that is split over the keys joins its parts through a workspace that the handle
  * holds, one for each stream that calls come on and one for each capture of a stream, `streams`
- * of them (0: 8; 9 MB each at head size 64, 17 at 128): calls on different streams, and graphs,
+ * of them (0: 8; 11 MB each at head size 64, 22 at 128): calls on different streams, and graphs,
  * may run at the same time (hipStreamPerThread, a different stream in each thread, is refused). What is enqueued on one stream, or captured on one stream in one capture, shares a
  * workspace: such a graph is instantiated once. A call that would need one more is refused;
  * ill_paged_release, called when nothing that the handle has enqueued or captured will run any

@@ -269,6 +269,7 @@ struct PgFinder {
   const PgBatch& b;
   PgCut c;
   int part, units;   // tiles of keys in a part; units of work in all
+  const int grid;    // workgroups that the launch has for them
   struct Lds {
     int64_t tiles[NW], work[NW];
     int units[NW], parts[NW], cut[NW];
@@ -293,7 +294,7 @@ struct PgFinder {
     for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
     return v;
   }
-  __device__ __forceinline__ PgFinder(const PgBatch& b_, const PgCut& c_, Lds& lds_) : b(b_), c(c_), lds(lds_) {
+  __device__ __forceinline__ PgFinder(const PgBatch& b_, const PgCut& c_, int grid_, Lds& lds_) : b(b_), c(c_), grid(grid_), lds(lds_) {
     if (b.seqs == 1) {   // (one sequence is one kernel's: shared is 0)
       look(0);
       part = pg_part((int64_t)n * most, c);
@@ -352,7 +353,7 @@ struct PgFinder {
   }
   // The launch has a workgroup for each unit if row0 ascends. If not, nothing is cut: no part waits in vain for another.
   __device__ __forceinline__ void whole_if_more() {
-    if (units > (int)gridDim.x) part = PG_MOST;
+    if (units > grid) part = PG_MOST;
   }
 
   // Unit u of sequence s: u is counted from the sequence's first, parts and tiles are what the sequences before it have.
@@ -698,14 +699,19 @@ struct PgStep {
 // + r: key 32 (b / 2) + 8 g + 4 (b % 2) + r). Values are transposed by the LDS read. The waves' states are
 // joined in LDS; a tile of rows whose keys are in several parts is joined by the workgroup that ends last, in
 // the parts' order.
+template <int NW>
+struct PgStepLds {
+  __attribute__((aligned(16))) uint4 lds[NW][1024];
+  float smx[NW][16], sls[NW][16];
+  int last;
+  typename PgFinder<NW>::Lds found;
+};
 template <int TC, int D, bool FINE, int NW>   // FINE: weights in two parts (float32 outputs)
-__global__ __launch_bounds__(64 * NW, 2) void pg_step_kernel(PgStep p) {
+__device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, PgStepLds<NW>& shared) {
   constexpr int KT = D == 64 ? 64 : 32, UPR = D / 8, KPI = 64 / UPR, NB = KT / 16, KS = D / 32, ND = D / 16, NS = KT / 32, NG = KT / 16;
   constexpr int RF = D + 4;   // floats between the rows of a state in LDS
-  __shared__ __attribute__((aligned(16))) uint4 lds[NW][1024];
-  __shared__ float smx[NW][16], sls[NW][16];
-  __shared__ int last;
-  __shared__ typename PgFinder<NW>::Lds found;
+  auto &lds = shared.lds;
+  auto &smx = shared.smx, &sls = shared.sls;
   const PgAttend& a = p.a;
   PgCut c = p.c;
   c.M = 16;   // (as the host has them, for the compiler)
@@ -725,7 +731,7 @@ __global__ __launch_bounds__(64 * NW, 2) void pg_step_kernel(PgStep p) {
 #pragma unroll
   for (int d = 0; d < ND; d++) va[d] = pg_values_at<D>(8 * kg, 16 * d, n);
   const float sc2 = a.scale * 1.4426950408889634f;
-  PgFinder<NW> finder(a.b, c, found);
+  PgFinder<NW> finder(a.b, c, grid, shared.found);
   auto over_kg = [](float v, auto op) {   // over the lanes of the same row
     const auto x = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
     v = op(__int_as_float((int)x[0]), __int_as_float((int)x[1]));
@@ -738,8 +744,8 @@ __global__ __launch_bounds__(64 * NW, 2) void pg_step_kernel(PgStep p) {
     const int key = KPI * i + lane / UPR;
     lane_off[i] = 2 * ((uint32_t)(key & 15) * (uint32_t)a.slot_stride + 8 * ((lane % UPR) ^ pg_swz<D>(key)));
   }
-  if ((int)blockIdx.x >= __builtin_amdgcn_readfirstlane(finder.units)) return;
-  const PgUnit un = pg_uniform(finder.find(blockIdx.x));
+  if (block >= __builtin_amdgcn_readfirstlane(finder.units)) return;
+  const PgUnit un = pg_uniform(finder.find(block));
   if (un.seq.n == 0) return;
   const int G = c.G, flat = un.seq.n * G, f0 = 16 * un.q, live = min(16, flat - f0);   // (n G is at most 2^26)
   const uint32_t f = min(f0 + n, flat - 1), at_row = f / c.G;
@@ -919,7 +925,7 @@ __global__ __launch_bounds__(64 * NW, 2) void pg_step_kernel(PgStep p) {
       pg_put_part<D, 16>(p.w, un.part_at + un.split, r, d, m, l, o);
     }
   }
-  if (un.splits > 1) pg_finish<TC, D, 16, NW>(a, c, p.w, un, f0, live, (LAS float*)lds, &last);
+  if (un.splits > 1) pg_finish<TC, D, 16, NW>(a, c, p.w, un, f0, live, (LAS float*)lds, &shared.last);
 }
 
 template <int TC>
@@ -935,12 +941,17 @@ __device__ __forceinline__ v16f pg_mfma32(uint4 a, uint4 b, v16f c) {   // 32 x 
 // stand (row m of block b: key 32 b + m with bits 2 and 3 of m swapped).
 // What a row does not see must not reach it as 0 x inf either: in a tile that some row does not see whole, infinities and
 // NaN among the values are replaced by 0 in LDS, and added afterwards to the rows that see them.
+template <int D>
+struct PgPromptLds {
+  __attribute__((aligned(16))) uint4 lds[2][2][8 * D];   // [buffer][keys, values]
+  int last, tamed;   // tamed: 1 + the last tile whose values were changed
+  PgFinder<4>::Lds found;
+};
 template <int TC, int D, bool FINE>   // FINE: weights in two parts (float32 outputs)
-__global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
+__device__ __forceinline__ void pg_prompt(const PgStep& p, int block, int grid, PgPromptLds<D>& shared) {
   constexpr int M = 128, KT = 64, UPR = D / 8, KS = D / 16, ND = D / 32, T = KT * UPR, LOADS = T / 256;   // LOADS: of keys, and of values, per wave and tile
-  __shared__ __attribute__((aligned(16))) uint4 lds[2][2][T];   // [buffer][keys, values]
-  __shared__ int last, tamed;   // tamed: 1 + the last tile whose values were changed
-  __shared__ PgFinder<4>::Lds found;
+  auto& lds = shared.lds;
+  int& tamed = shared.tamed;
   const PgAttend& a = p.a;
   PgCut c = p.c;
   c.M = M;   // (as the host has them, for the compiler)
@@ -948,7 +959,7 @@ __global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 31, h = lane >> 5;
   const int cap = pg_cap(a.b), pmask = (1 << a.b.page_log) - 1;
   const float sc2 = a.scale * 1.4426950408889634f;
-  PgFinder<4> finder(a.b, c, found);
+  PgFinder<4> finder(a.b, c, grid, shared.found);
   auto over_h = [](float v, auto op) {   // over the two lanes of a row
     const auto x = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
     return op(__int_as_float((int)x[0]), __int_as_float((int)x[1]));
@@ -972,8 +983,8 @@ __global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
   for (int d = 0; d < ND; d++)
 #pragma unroll
     for (int t = 0; t < 2; t++) va[d][t] = pg_values_at<D>(16 * t + 8 * h, 32 * d + 16 * ((lane >> 4) & 1), lane & 15);
-  if ((int)blockIdx.x >= __builtin_amdgcn_readfirstlane(finder.units)) return;
-  const PgUnit un = pg_uniform(finder.find(blockIdx.x));
+  if (block >= __builtin_amdgcn_readfirstlane(finder.units)) return;
+  const PgUnit un = pg_uniform(finder.find(block));
   if (un.seq.n == 0) return;
   const int G = c.G, flat = un.seq.n * G, f0 = M * un.q, live = min(M, flat - f0);   // (n G is at most 2^26)
   const uint32_t f = min(f0 + 32 * w + n, flat - 1), at_row = f / c.G;
@@ -1180,5 +1191,33 @@ __global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
         else pg_put_part<D, M>(p.w, un.part_at + un.split, r, dim, Mx, Ls, o);
       }
   }
-  if (un.splits > 1) pg_finish<TC, D, M, 4>(a, c, p.w, un, f0, live, (LAS float*)lds, &last);
+  if (un.splits > 1) pg_finish<TC, D, M, 4>(a, c, p.w, un, f0, live, (LAS float*)lds, &shared.last);
+}
+
+template <int TC, int D, bool FINE>
+__global__ __launch_bounds__(256, 2) void pg_step_kernel(PgStep p) {
+  __shared__ PgStepLds<4> lds;
+  pg_step<TC, D, FINE, 4>(p, blockIdx.x, gridDim.x, lds);
+}
+template <int TC, int D, bool FINE>
+__global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
+  __shared__ PgPromptLds<D> lds;
+  pg_prompt<TC, D, FINE>(p, blockIdx.x, gridDim.x, lds);
+}
+// Both in one launch: prompts in its first workgroups, and what waits for memory beside them.
+struct PgBoth {
+  PgAttend a;
+  PgCut prompt, step;
+  PgWork prompt_work, step_work;
+  int32_t prompts;   // workgroups
+};
+template <int TC, int D, bool FINE>
+__global__ __launch_bounds__(256, 2) void pg_both_kernel(PgBoth p) {
+  __shared__ union Lds {
+    PgStepLds<4> step;
+    PgPromptLds<D> prompt;
+    __device__ Lds() {}
+  } lds;
+  if ((int)blockIdx.x < p.prompts) pg_prompt<TC, D, FINE>({p.a, p.prompt, p.prompt_work}, blockIdx.x, p.prompts, lds.prompt);
+  else pg_step<TC, D, FINE, 4>({p.a, p.step, p.step_work}, blockIdx.x - p.prompts, gridDim.x - p.prompts, lds.step);
 }

@@ -51,7 +51,7 @@ PgCut prompt_cut(const ill_paged_desc& d, int window, int sinks) {
 
 // Bytes of a workspace where 2^log parts are wanted, over tiles of M rows.
 size_t counters(int log) { return al256(((size_t)(PG_MAXSPLIT / PG_FAN + 1) << log) * 4); }
-size_t work_size(int log, int M, int D) { return ((size_t)M * (D + 2) * 4 << (log + 1)) + counters(log); }
+size_t work_size(int log, int M, int D) { return al256((size_t)M * (D + 2) * 4 << (log + 1)) + counters(log); }
 
 PgWork work_of(uint8_t* at, int log, int M, int D) {
   PgWork w;
@@ -82,15 +82,17 @@ int workspace(ill_paged* p, hipStream_t st, uint8_t** out) {
   return ILL_OK;
 }
 
+// `steps`, `prompts`: workgroups of each kind.
+template <int TC, int D, bool FINE>
+void launch_attend(const PgBoth& s, int64_t steps, hipStream_t st) {
+  if (!s.prompts) hipLaunchKernelGGL((pg_step_kernel<TC, D, FINE>), dim3(steps), dim3(256), 0, st, PgStep{s.a, s.step, s.step_work});
+  else if (!steps) hipLaunchKernelGGL((pg_prompt_kernel<TC, D, FINE>), dim3(s.prompts), dim3(256), 0, st, PgStep{s.a, s.prompt, s.prompt_work});
+  else hipLaunchKernelGGL((pg_both_kernel<TC, D, FINE>), dim3(s.prompts + steps), dim3(256), 0, st, s);
+}
 template <int TC, int D>
-void launch_attend(const PgStep& s, int64_t grid, hipStream_t st) {
-  if (s.c.M == 16) {
-    if (s.a.out_f32) hipLaunchKernelGGL((pg_step_kernel<TC, D, true, 4>), dim3(grid), dim3(256), 0, st, s);
-    else hipLaunchKernelGGL((pg_step_kernel<TC, D, false, 4>), dim3(grid), dim3(256), 0, st, s);
-  } else {
-    if (s.a.out_f32) hipLaunchKernelGGL((pg_prompt_kernel<TC, D, true>), dim3(grid), dim3(256), 0, st, s);
-    else hipLaunchKernelGGL((pg_prompt_kernel<TC, D, false>), dim3(grid), dim3(256), 0, st, s);
-  }
+void launch_attend(const PgBoth& s, int64_t steps, hipStream_t st) {
+  if (s.a.out_f32) launch_attend<TC, D, true>(s, steps, st);
+  else launch_attend<TC, D, false>(s, steps, st);
 }
 
 template <int TX, int TC>
@@ -131,8 +133,7 @@ int ill_paged_create(const ill_paged_desc* desc, ill_paged** out) {
   for (int i = 0; i < d.rotary_dim / 2; i++) freq[i] = std::pow(d.rope_base, -2.0 * i / d.rotary_dim) / (2 * M_PI);
   if (hipMalloc(&p->freq, sizeof freq) != hipSuccess || hipMemcpy(p->freq, freq, sizeof freq, hipMemcpyHostToDevice) != hipSuccess)
     return bad(fail(ILL_E_HIP, "paged: buffer allocation failed"));
-  p->work_bytes = al256(illp::work_size(illp::prompt_cut(d, 0, 0).log, 128, d.head_dim));   // (the step kernel's is smaller)
-  static_assert((16 << 8) <= (128 << 7), "rows of the step kernel's parts");
+  for (const PgCut& c : {illp::step_cut(d, 0, 0), illp::prompt_cut(d, 0, 0)}) p->work_bytes += illp::work_size(c.log, c.M, d.head_dim);
   if (hipMalloc(&p->work, p->work_bytes * d.streams) != hipSuccess || hipMemset(p->work, 0, p->work_bytes * d.streams) != hipSuccess ||
       hipDeviceSynchronize() != hipSuccess)
     return bad(fail(ILL_E_HIP, "paged: %d workspaces of %zu bytes cannot be allocated", d.streams, p->work_bytes));
@@ -224,30 +225,30 @@ int ill_paged_attend(ill_paged* p, const ill_paged_batch* batch, const void* q, 
   a.scale = d.scale;
   illp::OnDevice on(p->device);
   if (on.rc) return on.rc;
-  // One of the kernels where the sizes that the host knows say which, else both: the sequences are divided by pg_share.
+  // One of the kernels where the sizes that the host knows say which, else both in one launch: the sequences are divided by pg_share.
   const int64_t G = d.heads / d.kv_heads, most = !a.b.row0 ? 1 : std::min<int64_t>(a.b.rows, batch->max_rows ? batch->max_rows : a.b.rows);
-  PgStep parts[2] = {{a, illp::step_cut(d, a.window, a.sinks), {}}, {a, illp::prompt_cut(d, a.window, a.sinks), {}}};
+  PgBoth s{a, illp::prompt_cut(d, a.window, a.sinks), illp::step_cut(d, a.window, a.sinks), {}, {}, 0};
   const int cap = pg_cap(a.b);
   const bool prompts = most * G > PG_FEW && std::min((a.b.rows * G / 128 + a.b.seqs), (most * G + 127) / 128 * a.b.seqs) * d.kv_heads >= PG_MANY;
   const bool both = prompts && a.b.seqs > 1;
-  parts[0].c.shared = parts[1].c.shared = both;
-  uint8_t* work = nullptr;
-  for (int i = 0; i < 2; i++)
-    if ((i ? prompts : both || !prompts) && !work && pg_splits(pg_most(cap, cap, parts[i].c), parts[i].c.least) > 1)
-      if (int rc = illp::workspace(p, st, &work)) return rc;
-  for (int i = 0; i < 2; i++) {
-    if (!(i ? prompts : both || !prompts)) continue;
-    PgStep& s = parts[i];
-    const int64_t grid = pg_grid(a.b.seqs, a.b.rows, !a.b.row0, cap, s.c);   // (below 2^24: rows x heads are at most 2^26, sequences x heads 2^22)
-    if (!grid) continue;
-    if (work) s.w = illp::work_of(work, s.c.log, s.c.M, d.head_dim);
-    if (d.dtype == ILL_F16) {
-      if (d.head_dim == 64) illp::launch_attend<PG_F16, 64>(s, grid, st);
-      else illp::launch_attend<PG_F16, 128>(s, grid, st);
-    } else {
-      if (d.head_dim == 64) illp::launch_attend<PG_BF16, 64>(s, grid, st);
-      else illp::launch_attend<PG_BF16, 128>(s, grid, st);
-    }
+  s.prompt.shared = s.step.shared = both;
+  auto cuts = [&](const PgCut& c) { return pg_splits(pg_most(cap, cap, c), c.least) > 1; };
+  if ((prompts && cuts(s.prompt)) || ((both || !prompts) && cuts(s.step))) {
+    uint8_t* work = nullptr;
+    if (int rc = illp::workspace(p, st, &work)) return rc;
+    s.step_work = illp::work_of(work, s.step.log, s.step.M, d.head_dim);
+    s.prompt_work = illp::work_of(work + illp::work_size(s.step.log, s.step.M, d.head_dim), s.prompt.log, s.prompt.M, d.head_dim);
+  }
+  // (below 2^24 workgroups: rows x heads are at most 2^26, sequences x heads 2^22)
+  const int64_t steps = both || !prompts ? pg_grid(a.b.seqs, a.b.rows, !a.b.row0, cap, s.step) : 0;
+  s.prompts = prompts ? (int)pg_grid(a.b.seqs, a.b.rows, !a.b.row0, cap, s.prompt) : 0;
+  if (!s.prompts && !steps) return ILL_OK;
+  if (d.dtype == ILL_F16) {
+    if (d.head_dim == 64) illp::launch_attend<PG_F16, 64>(s, steps, st);
+    else illp::launch_attend<PG_F16, 128>(s, steps, st);
+  } else {
+    if (d.head_dim == 64) illp::launch_attend<PG_BF16, 64>(s, steps, st);
+    else illp::launch_attend<PG_BF16, 128>(s, steps, st);
   }
   HCK(hipGetLastError());
   return ILL_OK;

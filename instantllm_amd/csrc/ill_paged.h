@@ -45,6 +45,20 @@ __device__ __forceinline__ uint32_t pg_pack2(float a, float b) {   // (as a pair
   if constexpr (T == PG_BF16) return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){a, b}, v2bf));
   else return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){a, b}, v2h));
 }
+// A pair of floats in parts of type T, each the rest of the one before: two parts of f16 keep 22 bits, three of bf16 24.
+template <int T>
+constexpr int PG_PARTS = T == PG_BF16 ? 3 : 2;
+template <int T, int N>
+__device__ __forceinline__ void pg_parts2(float a, float b, uint32_t* part) {
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    part[i] = pg_pack2<T>(a, b);
+    float y[2];
+    pg_unpack2<T>(part[i], y);
+    a -= y[0];
+    b -= y[1];
+  }
+}
 template <int T>
 __device__ __forceinline__ uint4 pg_pack8(const float* x) {
   return {pg_pack2<T>(x[0], x[1]), pg_pack2<T>(x[2], x[3]), pg_pack2<T>(x[4], x[5]), pg_pack2<T>(x[6], x[7])};
@@ -558,13 +572,6 @@ __device__ __forceinline__ v4f pg_shared(const float* p) {
   return (v4f){__uint_as_float((uint32_t)x), __uint_as_float((uint32_t)(x >> 32)), __uint_as_float((uint32_t)y), __uint_as_float((uint32_t)(y >> 32))};
 }
 
-// The same number, which the compiler does not know to be: what is computed from it is computed here, and not ahead of
-// the loops, where every workgroup would wait for what only the last ones need (8.8 against 8.0 us for a sequence of 500).
-__device__ __forceinline__ int pg_late(int v) {
-  asm volatile("" : "+v"(v));
-  return v;
-}
-
 // Whether this is the last of `count` workgroups to come here, whose parts it then sees (the same for every thread). The
 // counter is left at 0 for the next call.
 __device__ __forceinline__ bool pg_last(int32_t* counter, int count, int* lds) {
@@ -587,13 +594,14 @@ __device__ __forceinline__ void pg_put_part(const PgWork& w, int part, int r, in
   pg_share(w.o + at * D + d, o);
 }
 
+static_assert(PG_FAN * PG_FAN >= PG_MAXSPLIT, "two steps");
 // Joins `count` <= PG_FAN parts (from part `first` on, every step-th) of a tile of rows in their order, by one workgroup
 // of NW waves: into the output, or into the first of them. lds: PG_FAN x M x 2 + 2 M floats and, behind them, NW x 64 states.
 template <int TC, int D, int M, int NW>
 __device__ __forceinline__ void pg_join(const PgAttend& a, const PgCut& c, const PgWork& pw, const PgUnit& un, int first, int step, int count, bool out,
                                         int f0, int live, LAS float* lds) {
   constexpr int NT = 64 * NW, T = NT / M >= 64 ? 64 : NT / M < 1 ? 1 : NT / M;   // T threads of a row, neighbours in a wave
-  const int tid = pg_late(threadIdx.x);
+  const int tid = threadIdx.x;
   LAS float *wt = lds, *ls = lds + PG_FAN * M, *rows = ls + PG_FAN * M;
   // few items (four dims of a row): `groups` threads each, every groups-th part to one of them, its values fetched along
   // with the statistics
@@ -706,9 +714,10 @@ struct PgStepLds {
   int last;
   typename PgFinder<NW>::Lds found;
 };
-template <int TC, int D, bool FINE, int NW>   // FINE: weights in two parts (float32 outputs)
+template <int TC, int D, bool FINE, int NW>   // FINE: weights in parts that keep float32 (float32 outputs)
 __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, PgStepLds<NW>& shared) {
   constexpr int KT = D == 64 ? 64 : 32, UPR = D / 8, KPI = 64 / UPR, NB = KT / 16, KS = D / 32, ND = D / 16, NS = KT / 32, NG = KT / 16;
+  constexpr int N = FINE ? PG_PARTS<TC> : 1;   // parts of a weight
   constexpr int RF = D + 4;   // floats between the rows of a state in LDS
   auto &lds = shared.lds;
   auto &smx = shared.smx, &sls = shared.sls;
@@ -844,7 +853,7 @@ __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, Pg
       for (int d = 0; d < ND; d++) O[d] *= up;
     }
     const float ref = Mx == -INFINITY ? 0.f : Mx;
-    gu32x4 ph[NS], pl[NS];
+    gu32x4 ph[N][NS];
 #pragma unroll
     for (int b = 0; b < NB; b++) {
       float e[4];
@@ -855,13 +864,10 @@ __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, Pg
       }
 #pragma unroll
       for (int r = 0; r < 4; r += 2) {
-        const uint32_t x = pg_pack2<TC>(e[r], e[r + 1]);
-        ph[b >> 1][2 * (b & 1) + r / 2] = x;
-        if constexpr (FINE) {
-          float y[2];
-          pg_unpack2<TC>(x, y);
-          pl[b >> 1][2 * (b & 1) + r / 2] = pg_pack2<TC>(e[r] - y[0], e[r + 1] - y[1]);
-        }
+        uint32_t x[N];
+        pg_parts2<TC, N>(e[r], e[r + 1], x);
+#pragma unroll
+        for (int i = 0; i < N; i++) ph[i][b >> 1][2 * (b & 1) + r / 2] = x[i];
       }
     }
     if (more) PG_WAIT(8);   // the values; the 8 loads after them are the next keys
@@ -876,8 +882,8 @@ __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, Pg
         for (int t = 0; t < NS; t++) {
           uint4 marks;
           const uint4 v = pg_tamed<TC>(pg_values<D>(vl + va[d] + 32 * t * 2 * D), marks);
-          O[d] = pg_mfma16<TC>(v, __builtin_bit_cast(uint4, ph[t]), O[d]);
-          if constexpr (FINE) O[d] = pg_mfma16<TC>(v, __builtin_bit_cast(uint4, pl[t]), O[d]);
+#pragma unroll
+          for (int i = 0; i < N; i++) O[d] = pg_mfma16<TC>(v, __builtin_bit_cast(uint4, ph[i][t]), O[d]);
           m = pg_mfma16<TC>(marks, pg_ones<TC>(seen >> (8 * t)), m);
         }
 #pragma unroll
@@ -889,8 +895,8 @@ __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, Pg
 #pragma unroll
       for (int t = 0; t < NS; t++) {
         const uint4 v = pg_values<D>(vl + va[d] + 32 * t * 2 * D);
-        O[d] = pg_mfma16<TC>(v, __builtin_bit_cast(uint4, ph[t]), O[d]);
-        if constexpr (FINE) O[d] = pg_mfma16<TC>(v, __builtin_bit_cast(uint4, pl[t]), O[d]);
+#pragma unroll
+        for (int i = 0; i < N; i++) O[d] = pg_mfma16<TC>(v, __builtin_bit_cast(uint4, ph[i][t]), O[d]);
       }
     }
     PG_WAIT_LDS();   // the values have been read
@@ -906,7 +912,7 @@ __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, Pg
     sls[w][n] = Ls;
   }
   __syncthreads();
-  for (int i = pg_late(tid); i < live * (D / 4); i += 64 * NW) {
+  for (int i = tid; i < live * (D / 4); i += 64 * NW) {
     const int r = i / (D / 4), d = 4 * (i % (D / 4));
     float m = smx[0][r];
 #pragma unroll
@@ -947,8 +953,9 @@ struct PgPromptLds {
   int last, tamed;   // tamed: 1 + the last tile whose values were changed
   PgFinder<4>::Lds found;
 };
-template <int TC, int D, bool FINE>   // FINE: weights in two parts (float32 outputs)
+template <int TC, int D, bool FINE>   // FINE: weights in parts that keep float32 (float32 outputs)
 __device__ __forceinline__ void pg_prompt(const PgStep& p, int block, int grid, PgPromptLds<D>& shared) {
+  constexpr int N = FINE ? PG_PARTS<TC> : 1;   // parts of a weight
   constexpr int M = 128, KT = 64, UPR = D / 8, KS = D / 16, ND = D / 32, T = KT * UPR, LOADS = T / 256;   // LOADS: of keys, and of values, per wave and tile
   auto& lds = shared.lds;
   int& tamed = shared.tamed;
@@ -1124,7 +1131,16 @@ __device__ __forceinline__ void pg_prompt(const PgStep& p, int block, int grid, 
       for (int d = 0; d < ND; d++) O[d] *= up;
     }
     const float ref = Mx == -INFINITY ? 0.f : Mx;
-    gu32x4 ph[4], pl[4];   // weights of 16 keys each
+    gu32x4 ph[4][N];   // weights of 16 keys each; in parts only where they are used, and until then in the scores' place
+    auto parts = [&](int t) {
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        uint32_t x[N];
+        pg_parts2<TC, N>(s[t >> 1][8 * (t & 1) + i], s[t >> 1][8 * (t & 1) + i + 1], x);
+#pragma unroll
+        for (int n = 0; n < N; n++) ph[t][n][i >> 1] = x[n];
+      }
+    };
 #pragma unroll
     for (int t = 0; t < 4; t++) {
       float sum = 0.f;
@@ -1132,24 +1148,20 @@ __device__ __forceinline__ void pg_prompt(const PgStep& p, int block, int grid, 
       for (int i = 0; i < 8; i += 2) {
         const float e0 = __builtin_amdgcn_exp2f(fmaf(s[t >> 1][8 * (t & 1) + i], sc2, -ref)), e1 = __builtin_amdgcn_exp2f(fmaf(s[t >> 1][8 * (t & 1) + i + 1], sc2, -ref));
         sum += e0 + e1;
-        const uint32_t x = pg_pack2<TC>(e0, e1);
-        ph[t][i >> 1] = x;
-        if constexpr (FINE) {
-          float y[2];
-          pg_unpack2<TC>(x, y);
-          pl[t][i >> 1] = pg_pack2<TC>(e0 - y[0], e1 - y[1]);
-        }
+        s[t >> 1][8 * (t & 1) + i] = e0;
+        s[t >> 1][8 * (t & 1) + i + 1] = e1;
       }
       Ls += sum;
+      if constexpr (!FINE) parts(t);
     }
 #pragma unroll
     for (int t = 0; t < 4; t++) {
       if (t < 3) values(t + 1);
+      if constexpr (FINE) parts(t);
 #pragma unroll
-      for (int d = 0; d < ND; d++) {
-        O[d] = pg_mfma32<TC>(vf[t & 1][d], __builtin_bit_cast(uint4, ph[t]), O[d]);
-        if constexpr (FINE) O[d] = pg_mfma32<TC>(vf[t & 1][d], __builtin_bit_cast(uint4, pl[t]), O[d]);
-      }
+      for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int n = 0; n < N; n++) O[d] = pg_mfma32<TC>(vf[t & 1][d], __builtin_bit_cast(uint4, ph[t][n]), O[d]);
       __builtin_amdgcn_sched_barrier(0);
     }
     if (!all && __builtin_amdgcn_readfirstlane(tamed) == k + 1) {   // the values as they were, from memory

@@ -10,7 +10,7 @@
 
 #define PG_MOST (1 << 30)    // positions, rows x heads, windows and sinks: at most this many
 #define PG_MAXSPLIT 256      // parts that the keys of a tile of rows are cut into at most
-#define PG_FAN 16            // of which so many are joined at a time, in two steps (131071 keys in 256 parts: 24.4 us; 32: 26.2, 64: 31.4, 128: 39.6)
+#define PG_FAN 16            // of which so many are joined at a time, in two steps (131071 keys in 256 parts: 20.1 us; 32: 21.7)
 
 // A batch as the kernels read it (ill_paged_batch with the handle's geometry).
 struct PgBatch {
@@ -76,10 +76,10 @@ struct PgCut {
 
 // Two kernels evaluate a batch. Sequences of up to PG_FEW flat rows are always the step kernel's (16 flat rows to a tile);
 // the others are the prompt kernel's (128) if they have PG_MANY tiles of 128 in all, times key/value heads, about one for
-// each CU, and the step kernel's otherwise. (Step against prompt kernel, us, 14 / 2 heads of 64: 512 rows, 56 tiles, 8.7 against
-// 24; 1024 rows behind 4000, 112 tiles, 56.3 against 56.7; 2048 rows, 224 tiles, 39.7 against 36.2; 8 x 512 rows, 448 tiles, 63
-// against 33. 32 / 8 heads of 128: 512 rows behind 4000, 128 tiles, 84 against 81; 4 x 256, 256 tiles, 38.5 against 26.7; but 32 x
-// 8 rows, 256 tiles of 32 flat rows, 28 against 36.)
+// each CU, and the step kernel's otherwise. (Step against prompt kernel, us, 14 / 2 heads of 64: 512 rows, 56 tiles, 7.1 against
+// 21.5; 1024 rows behind 4000, 112 tiles, 55 against 51; 2048 rows, 224 tiles, 35.8 against 34.0; 8 x 512 rows, 448 tiles, 58
+// against 20. 32 / 8 heads of 128: 512 rows behind 4000, 128 tiles, 84 against 90; 4 x 256, 256 tiles, 36 against 16; but 64 x
+// 2 rows behind 1000, 512 tiles of 8 flat rows, 44 against 50.)
 #define PG_FEW 32
 #define PG_MANY 224
 PG_FN int pg_prompt_tiles(int n, uint32_t G, uint32_t kv) {

@@ -7,8 +7,8 @@ append: the result is rounded once, h |y|, from float32 arithmetic on values of 
   at 2^30 positions 3 u. Together below 32 u z. Below the least normal number half a step is half of the smallest subnormal.
 attend: scores are sums of D products in float32, off by at most D u times d, the greatest sum of |q k| scale; scale, the change to
   powers of 2 and the exponential add at most 8 u d + 2^-21. A softmax weight is off by at most twice that relative to itself, and sums of N
-  weights and values by N u each. Weights are rounded for the product with the values to the cache's type (two parts for float32
-  outputs: f16 2^-22, bf16 2^-16). All of these are relative to z, the weighted sum of the values' sizes. The output is rounded once, h |y|.
+  weights and values by N u each. Weights are rounded for the product with the values to the cache's type (for float32
+  outputs in parts: two of f16 2^-22, three of bf16 2^-24). All of these are relative to z, the weighted sum of the values' sizes. The output is rounded once, h |y|.
 These are bounds; the errors are nearly independent, so all values together are off by less than 1.5 h (the output's and the weights'
   rounding, uniform, are h / sqrt 3 each), and in float32 by less than 1e-5.
 """
@@ -125,7 +125,7 @@ class Setup:
         val = O.from_bits(got[:, :w], out_dtype) if out_dtype != "f32" else got[:, :w].view(np.float32).astype(np.float64)
         off2 = ref2 = 0.0
         h = O.HALF_STEP[out_dtype]
-        weight = {"f16": 2.0 ** -22, "bf16": 2.0 ** -16}[self.dtype] if out_dtype == "f32" else O.HALF_STEP[self.dtype]
+        weight = {"f16": 2.0 ** -22, "bf16": 2.0 ** -24}[self.dtype] if out_dtype == "f32" else O.HALF_STEP[self.dtype]
         n = int(self.lens.max(initial=1))
         for r in ref:
             y, g = ref[r], val[r].reshape(self.heads, self.dim)

@@ -110,7 +110,8 @@ __device__ __forceinline__ void pg_floats8(const float* p, float* y) {
 // neighbouring lanes. The angles' sines and cosines are computed once per row and pair, from turns
 // in float64 (a position of 2^20 has to keep 2^-20 of a turn and more), and shared through LDS. A thread's
 // first values are on their way while the rows' places and angles are found, the next ones while it
-// computes: one row waits for three loads one after the other, many rows for memory.
+// computes. One row waits for three loads one after the other (a kernel of 3.5 us), many rows for memory: 343 MB of
+// bf16 heads of 128 in 73 us, 4.7 TB/s, where a large copy reaches 5.1.
 template <int TX, int TC, int D>
 __global__ __launch_bounds__(256) void pg_append_kernel(PgAppend a, int R) {
   extern __shared__ __attribute__((aligned(16))) uint8_t pg_lds[];
@@ -707,6 +708,9 @@ struct PgStep {
 // + r: key 32 (b / 2) + 8 g + 4 (b % 2) + r). Values are transposed by the LDS read. The waves' states are
 // joined in LDS; a tile of rows whose keys are in several parts is joined by the workgroup that ends last, in
 // the parts' order.
+// Bound by memory where there is enough of it: 64 sequences of 100 to 9000 positions, 32 / 8 heads of 128, 432 MB in 97 us,
+// 4.4 TB/s (a large copy: 5.1). One sequence of 131071, 14 / 2 heads of 64, 67 MB in 20 us: 13 at the copy's rate, the rest the
+// launch, three dependent loads at the start (3) and the join (4). One of 500: 6.5 us, all latency.
 template <int NW>
 struct PgStepLds {
   __attribute__((aligned(16))) uint4 lds[NW][1024];
@@ -947,6 +951,9 @@ __device__ __forceinline__ v16f pg_mfma32(uint4 a, uint4 b, v16f c) {   // 32 x 
 // stand (row m of block b: key 32 b + m with bits 2 and 3 of m swapped).
 // What a row does not see must not reach it as 0 x inf either: in a tile that some row does not see whole, infinities and
 // NaN among the values are replaced by 0 in LDS, and added afterwards to the rows that see them.
+// One prompt of 8000 rows, 28 / 4 heads of 128, bf16: 442 to 458 us, 1.0 PFLOP/s, 0.86 to 0.89 of a large matrix product's rate here;
+// the card lowers its clock in both. With heads of 64 a score costs as many exponentials and sums for half the products: 4096 rows
+// of 14 / 2 heads in a window of 1024 take 36 us, 0.42 PFLOP/s, with 1.75 workgroups to a CU; a third of the waves' cycles are waits.
 template <int D>
 struct PgPromptLds {
   __attribute__((aligned(16))) uint4 lds[2][2][8 * D];   // [buffer][keys, values]

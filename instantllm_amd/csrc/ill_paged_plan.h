@@ -48,7 +48,7 @@ PG_FN bool pg_sees(int p, int j, int window, int sinks) { return j >= 0 && j <= 
 
 // Rows of a workgroup of the append kernel, whose 256 threads take `items` pieces of each row: as few as fill the threads'
 // turns to four fifths, up to 8, and fewer where there would be less than two workgroups for each CU. (64 rows of 384 pieces
-// at 4 rows to a workgroup, 16 workgroups of six turns: 10.2 us.)
+// at 4 rows to a workgroup, 16 workgroups of six turns: 10.2 us; at one row 6.9.)
 PG_FN int pg_append_rows(int rows, int items) {
   int best = 1;
   for (int r = 1; r <= 8; r++) {

@@ -456,6 +456,40 @@ def test_graphs_follow_lengths_and_tables(hip):
     assert np.array_equal(hip.get(s.kc, s.k_bits), hip.get(twin.kc, s.k_bits))
 
 
+def test_graphs_at_once(hip):
+    """Two graphs of a batch that both kernels and split keys take part in, and an eager call, at a time and again."""
+    s = Setup(hip, [(6000, 40)] + [(100 + i, 40) for i in range(7)] + [(900, 1), (64, 1), (0, 1), (5, 9), (70, 0)], heads=64, kv=32)
+    s.upload()
+    w = s.heads * s.dim
+    qs = [s.random_bits(s.rows, w) for _ in range(3)]
+    want = [s.attend(q=q) for q in qs]
+    st = [hip.stream(), hip.stream(), None]
+    dq, do = [hip.put(q) for q in qs], [hip.alloc(2 * s.rows * w) for _ in st]
+    calls = [lambda i=i: s.op.attend(s.batch, s.kc, s.vc, dq[i], do[i], stream=st[i]) for i in range(3)]
+    graphs = [hip.capture(st[i], calls[i]) for i in range(2)]
+    for turn in range(5):
+        for i in range(3):
+            hip.write(do[i], np.zeros_like(want[i]))
+        hip.sync()
+        for _ in range(2):
+            for i in range(2):
+                hip.launch(graphs[i], st[i])
+            calls[2]()
+        for i in range(3):
+            assert np.array_equal(hip.get(do[i], want[i]), want[i]), (turn, i)
+
+
+def test_rows_before_the_first_sequence(hip):
+    """Rows in front of row0[0] are no sequence's: neither call writes them."""
+    s = Setup(hip, [(70, 3), (5, 0), (300, 40)], pad=1)
+    s.row0 += 2
+    s.rows += 2
+    hip.write(s.d_row0, s.row0)
+    s.batch = s.op.batch(s.d_lens, s.d_table, s.width, s.pages, 3, rows=s.rows, row0=s.d_row0, table_stride=s.width + 2)
+    _append(s, bias=True)
+    s.attend()
+
+
 def test_streams_at_once(hip):
     """Calls of one handle on several streams at a time keep apart."""
     s = Setup(hip, [(9000, 1)], one_row=True)

@@ -315,14 +315,13 @@ ILL_API int ill_paged_release(ill_paged* p);
  * captured call follows what they then hold. lens [seqs]: the positions of each sequence, its
  * new rows included (below 0 counts as 0). table [seqs][table_stride], table_width entries used:
  * the page of positions i * page_size .. in entry i; entries behind a sequence's last position
- * are not read. row0
- * [seqs + 1]: ascending; sequence s has the new rows row0[s] .. row0[s + 1] - 1, which stand at
- * its last positions; NULL: row s is sequence s's only one. rows: rows of the buffers (the ones
- * behind the last sequence's are left alone). max_rows: the most new rows that a sequence has, if
- * known (0: unknown; a hint for the launch only). pages: pages of the cache. A page number
- * outside 0 .. pages - 1 is not followed: its positions are neither written nor seen, and so are
- * positions past table_width pages or below 0. Pages may be shared for reading. rows x heads is
- * at most 2^26, seqs x heads at most 2^22. */
+ * are not read. row0 [seqs + 1]: ascending; sequence s has the new rows row0[s] ..
+ * row0[s + 1] - 1, which stand at its last positions; NULL: row s is sequence s's only one.
+ * rows: rows of the buffers (the ones that are no sequence's are left alone). max_rows: the most
+ * new rows that a sequence has, if known (0: unknown; a hint for the launch only). pages: pages
+ * of the cache. A page number outside 0 .. pages - 1 is not followed: its positions are neither
+ * written nor seen, and so are positions past table_width pages or below 0. Pages may be shared
+ * for reading. rows x heads is at most 2^26, seqs x heads at most 2^22. */
 typedef struct {
   int32_t seqs, table_width;
   int64_t table_stride, rows, max_rows, pages;

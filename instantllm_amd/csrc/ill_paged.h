@@ -895,13 +895,13 @@ __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, Pg
       }
     } else {
 #pragma unroll
-    for (int d = 0; d < ND; d++)
+      for (int d = 0; d < ND; d++)
 #pragma unroll
-      for (int t = 0; t < NS; t++) {
-        const uint4 v = pg_values<D>(vl + va[d] + 32 * t * 2 * D);
+        for (int t = 0; t < NS; t++) {
+          const uint4 v = pg_values<D>(vl + va[d] + 32 * t * 2 * D);
 #pragma unroll
-        for (int i = 0; i < N; i++) O[d] = pg_mfma16<TC>(v, __builtin_bit_cast(uint4, ph[i][t]), O[d]);
-      }
+          for (int i = 0; i < N; i++) O[d] = pg_mfma16<TC>(v, __builtin_bit_cast(uint4, ph[i][t]), O[d]);
+        }
     }
     PG_WAIT_LDS();   // the values have been read
     if (more) load(a.vc, VALUES, k + 1);
@@ -951,7 +951,7 @@ __device__ __forceinline__ v16f pg_mfma32(uint4 a, uint4 b, v16f c) {   // 32 x 
 // stand (row m of block b: key 32 b + m with bits 2 and 3 of m swapped).
 // What a row does not see must not reach it as 0 x inf either: in a tile that some row does not see whole, infinities and
 // NaN among the values are replaced by 0 in LDS, and added afterwards to the rows that see them.
-// One prompt of 8000 rows, 28 / 4 heads of 128, bf16: 442 to 458 us, 1.0 PFLOP/s, 0.86 to 0.89 of a large matrix product's rate here;
+// One prompt of 8000 rows, 28 / 4 heads of 128, bf16: 442 to 461 us, 1.0 PFLOP/s, 0.85 to 0.89 of a large matrix product's rate here;
 // the card lowers its clock in both. With heads of 64 a score costs as many exponentials and sums for half the products: 4096 rows
 // of 14 / 2 heads in a window of 1024 take 36 us, 0.42 PFLOP/s, with 1.75 workgroups to a CU; a third of the waves' cycles are waits.
 template <int D>
@@ -1153,10 +1153,11 @@ __device__ __forceinline__ void pg_prompt(const PgStep& p, int block, int grid, 
       float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; i += 2) {
-        const float e0 = __builtin_amdgcn_exp2f(fmaf(s[t >> 1][8 * (t & 1) + i], sc2, -ref)), e1 = __builtin_amdgcn_exp2f(fmaf(s[t >> 1][8 * (t & 1) + i + 1], sc2, -ref));
+        const int r = 8 * (t & 1) + i;
+        const float e0 = __builtin_amdgcn_exp2f(fmaf(s[t >> 1][r], sc2, -ref)), e1 = __builtin_amdgcn_exp2f(fmaf(s[t >> 1][r + 1], sc2, -ref));
         sum += e0 + e1;
-        s[t >> 1][8 * (t & 1) + i] = e0;
-        s[t >> 1][8 * (t & 1) + i + 1] = e1;
+        s[t >> 1][r] = e0;
+        s[t >> 1][r + 1] = e1;
       }
       Ls += sum;
       if constexpr (!FINE) parts(t);

@@ -122,8 +122,9 @@ PG_FN int pg_most(int end, int cap, const PgCut& c) {
   return pg_min(some, all);
 }
 
-// Tiles of keys in a part, from the sum over the sequences of qtiles x kv x most. A sequence is cut into parts if its `most` is over that; the parts of all cut ones are
-// then at most 2 x 2^log (most / part + 1 <= 2 most / part each), their tiles of rows at most 2^log.
+// Tiles of keys in a part, from the sum over the sequences of qtiles x kv x most. A sequence is cut into parts if its
+// `most` is over that; the parts of all cut ones are then at most 2 x 2^log (most / part + 1 <= 2 most / part each), their
+// tiles of rows at most 2^log.
 PG_FN int pg_part(int64_t work, const PgCut& c) {
   const int64_t p = (work + (1ll << c.log) - 1) >> c.log;
   return p < c.least ? c.least : p < PG_MOST ? (int)p : PG_MOST;

@@ -533,6 +533,21 @@ __device__ __forceinline__ uint4 pg_ones(uint32_t seen) {
   for (int i = 0; i < 4; i++) y[i] = (seen >> (2 * i) & 1 ? ONE : 0u) | (seen >> (2 * i + 1) & 1 ? ONE << 16 : 0u);
   return {y[0], y[1], y[2], y[3]};
 }
+// Tiles that all rows see go to the product as they are. An infinity or NaN there makes its sums infinite or NaN, whatever
+// its weight is, but not the right one: a weight's lesser parts may be 0 or negative, and a small weight rounds to 0. So a wave
+// (the prompt kernel: a workgroup) that ends with such a sum evaluates its keys once more, and then sets them aside in every tile.
+// Finite values pay for the look at the sums and a barrier: 8000 rows of 28 / 4 heads of 128, 449 -> 454 us; 200 single rows
+// in a window 24.2 -> 24.4.
+template <int N, class V>
+__device__ __forceinline__ bool pg_any_wild(const V* sums) {   // of the wave's
+  float z[4] = {};
+#pragma unroll
+  for (int d = 0; d < N; d++)
+#pragma unroll
+    for (int r = 0; r < (int)(sizeof(V) / 4); r++) z[r & 3] = fmaf(sums[d][r], 0.f, z[r & 3]);
+  const float y = (z[0] + z[1]) + (z[2] + z[3]);
+  return __any(y != y);
+}
 __device__ __forceinline__ float pg_wild_sum(float marks) {
   const int n = (int)marks;
   float y = n & 127 ? INFINITY : 0.f;
@@ -797,114 +812,119 @@ __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, Pg
       });
     });
   };
-  float Mx = -INFINITY, Ls = 0.f;   // Ls: this lane's keys only
+  float Mx, Ls;   // Ls: this lane's keys only
   v4f O[ND];
+  for (bool careful = false;; careful = true) {   // (twice only for infinities and NaN, pg_any_wild)
+    Mx = -INFINITY;
+    Ls = 0.f;
 #pragma unroll
-  for (int d = 0; d < ND; d++) O[d] = (v4f){0.f, 0.f, 0.f, 0.f};
-  groups(0);
-  PG_WAIT_OWN();
-  if (mine > 0) {
-    load(a.kc, KEYS, 0);
-    load(a.vc, VALUES, 0);
-  }
-  for (int k = 0; k < mine; k++) {
-    const int kt = pg_key_tile(range, c0 + w + NW * k) * KT;
-    const bool more = k + 1 < mine;
-    int good = 0;   // groups of 16 keys whose pages are there
-#pragma unroll
-    for (int g = 0; g < NG; g++) good |= (__builtin_amdgcn_readlane((int)(group >> 32), (k * NG + g) & 63) >= 0) << g;
-    PG_WAIT(8);   // the keys; the 8 loads after them are the values
-    v4f s[NB];
-#pragma unroll
-    for (int b = 0; b < NB; b++) {
-      s[b] = (v4f){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int ks = 0; ks < KS; ks++) s[b] = pg_mfma16<TC>(pg_get(kl + ka[ks] + (32 * (b >> 1) + 4 * (b & 1)) * 2 * D), qf[ks], s[b]);
+    for (int d = 0; d < ND; d++) O[d] = (v4f){0.f, 0.f, 0.f, 0.f};
+    groups(0);
+    PG_WAIT_OWN();
+    if (mine > 0) {
+      load(a.kc, KEYS, 0);
+      load(a.vc, VALUES, 0);
     }
-    PG_WAIT_LDS();   // the keys have been read
-    if (more) {
-      if (((k + 1) & (64 / NG - 1)) == 0) groups(k + 1);
-      load(a.kc, KEYS, k + 1);
-    }
-    // every row sees the whole tile, or the rows' masks (wave-uniform)
-    const bool whole = good == (1 << NG) - 1 && kt + KT - 1 <= p0 && kt + KT <= end && (c.window == 0 || kt > p1 - c.window || kt + KT <= c.sinks);
-    uint32_t seen = ~0u;
-    if (!whole) {
-      seen = 0;
+    for (int k = 0; k < mine; k++) {
+      const int kt = pg_key_tile(range, c0 + w + NW * k) * KT;
+      const bool more = k + 1 < mine;
+      int good = 0;   // groups of 16 keys whose pages are there
+#pragma unroll
+      for (int g = 0; g < NG; g++) good |= (__builtin_amdgcn_readlane((int)(group >> 32), (k * NG + g) & 63) >= 0) << g;
+      PG_WAIT(8);   // the keys; the 8 loads after them are the values
+      v4f s[NB];
+#pragma unroll
+      for (int b = 0; b < NB; b++) {
+        s[b] = (v4f){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) s[b] = pg_mfma16<TC>(pg_get(kl + ka[ks] + (32 * (b >> 1) + 4 * (b & 1)) * 2 * D), qf[ks], s[b]);
+      }
+      PG_WAIT_LDS();   // the keys have been read
+      if (more) {
+        if (((k + 1) & (64 / NG - 1)) == 0) groups(k + 1);
+        load(a.kc, KEYS, k + 1);
+      }
+      // every row sees the whole tile, or the rows' masks (wave-uniform)
+      const bool whole = good == (1 << NG) - 1 && kt + KT - 1 <= p0 && kt + KT <= end && (c.window == 0 || kt > p1 - c.window || kt + KT <= c.sinks);
+      uint32_t seen = ~0u;
+      if (!whole) {
+        seen = 0;
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            const int key = 32 * (b >> 1) + 8 * kg + 4 * (b & 1) + r, j = kt + key;
+            // pg_sees. (Without branches: the compiler has lost the stores of `if (!on) s[b][r] = ..` behind && and ||.)
+            const bool on = j < cap & j <= pos & (c.window == 0 | j > pos - c.window | j < c.sinks) & (good >> (key >> 4) & 1);
+            s[b][r] = on ? s[b][r] : -INFINITY;
+            seen |= (uint32_t)on << (4 * b + r);
+          }
+      }
+      float mc = s[0][0];
 #pragma unroll
       for (int b = 0; b < NB; b++)
 #pragma unroll
+        for (int r = 0; r < 4; r++) mc = fmaxf(mc, s[b][r]);
+      mc *= sc2;
+      if (__any(mc > Mx + (PG_UP + PG_SLACK))) {
+        mc = over_kg(mc, OpMaxF{});
+        const float mn = mc == -INFINITY ? Mx : fmaxf(mc - PG_UP, Mx), up = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(Mx - mn);
+        Mx = mn;
+        Ls *= up;
+#pragma unroll
+        for (int d = 0; d < ND; d++) O[d] *= up;
+      }
+      const float ref = Mx == -INFINITY ? 0.f : Mx;
+      gu32x4 ph[N][NS];
+#pragma unroll
+      for (int b = 0; b < NB; b++) {
+        float e[4];
+#pragma unroll
         for (int r = 0; r < 4; r++) {
-          const int key = 32 * (b >> 1) + 8 * kg + 4 * (b & 1) + r, j = kt + key;
-          // pg_sees. (Without branches: the compiler has lost the stores of `if (!on) s[b][r] = ..` behind && and ||.)
-          const bool on = j < cap & j <= pos & (c.window == 0 | j > pos - c.window | j < c.sinks) & (good >> (key >> 4) & 1);
-          s[b][r] = on ? s[b][r] : -INFINITY;
-          seen |= (uint32_t)on << (4 * b + r);
-        }
-    }
-    float mc = s[0][0];
-#pragma unroll
-    for (int b = 0; b < NB; b++)
-#pragma unroll
-      for (int r = 0; r < 4; r++) mc = fmaxf(mc, s[b][r]);
-    mc *= sc2;
-    if (__any(mc > Mx + (PG_UP + PG_SLACK))) {
-      mc = over_kg(mc, OpMaxF{});
-      const float mn = mc == -INFINITY ? Mx : fmaxf(mc - PG_UP, Mx), up = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(Mx - mn);
-      Mx = mn;
-      Ls *= up;
-#pragma unroll
-      for (int d = 0; d < ND; d++) O[d] *= up;
-    }
-    const float ref = Mx == -INFINITY ? 0.f : Mx;
-    gu32x4 ph[N][NS];
-#pragma unroll
-    for (int b = 0; b < NB; b++) {
-      float e[4];
-#pragma unroll
-      for (int r = 0; r < 4; r++) {
-        e[r] = __builtin_amdgcn_exp2f(fmaf(s[b][r], sc2, -ref));
-        Ls += e[r];
-      }
-#pragma unroll
-      for (int r = 0; r < 4; r += 2) {
-        uint32_t x[N];
-        pg_parts2<TC, N>(e[r], e[r + 1], x);
-#pragma unroll
-        for (int i = 0; i < N; i++) ph[i][b >> 1][2 * (b & 1) + r / 2] = x[i];
-      }
-    }
-    if (more) PG_WAIT(8);   // the values; the 8 loads after them are the next keys
-    else PG_WAIT(0);
-    bool wild = false;
-    if (!whole) wild = pg_wild_tile<TC, KT * UPR>(vl, lane);   // what a row does not see must not reach it as 0 x inf
-    if (wild) {
-#pragma unroll
-      for (int d = 0; d < ND; d++) {
-        v4f m = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int t = 0; t < NS; t++) {
-          uint4 marks;
-          const uint4 v = pg_tamed<TC>(pg_values<D>(vl + va[d] + 32 * t * 2 * D), marks);
-#pragma unroll
-          for (int i = 0; i < N; i++) O[d] = pg_mfma16<TC>(v, __builtin_bit_cast(uint4, ph[i][t]), O[d]);
-          m = pg_mfma16<TC>(marks, pg_ones<TC>(seen >> (8 * t)), m);
+          e[r] = __builtin_amdgcn_exp2f(fmaf(s[b][r], sc2, -ref));
+          Ls += e[r];
         }
 #pragma unroll
-        for (int r = 0; r < 4; r++) O[d][r] += pg_wild_sum(m[r]);
-      }
-    } else {
+        for (int r = 0; r < 4; r += 2) {
+          uint32_t x[N];
+          pg_parts2<TC, N>(e[r], e[r + 1], x);
 #pragma unroll
-      for (int d = 0; d < ND; d++)
-#pragma unroll
-        for (int t = 0; t < NS; t++) {
-          const uint4 v = pg_values<D>(vl + va[d] + 32 * t * 2 * D);
-#pragma unroll
-          for (int i = 0; i < N; i++) O[d] = pg_mfma16<TC>(v, __builtin_bit_cast(uint4, ph[i][t]), O[d]);
+          for (int i = 0; i < N; i++) ph[i][b >> 1][2 * (b & 1) + r / 2] = x[i];
         }
+      }
+      if (more) PG_WAIT(8);   // the values; the 8 loads after them are the next keys
+      else PG_WAIT(0);
+      bool wild = false;
+      if (!whole || careful) wild = pg_wild_tile<TC, KT * UPR>(vl, lane);   // what a row does not see must not reach it as 0 x inf
+      if (wild) {
+#pragma unroll
+        for (int d = 0; d < ND; d++) {
+          v4f m = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int t = 0; t < NS; t++) {
+            uint4 marks;
+            const uint4 v = pg_tamed<TC>(pg_values<D>(vl + va[d] + 32 * t * 2 * D), marks);
+#pragma unroll
+            for (int i = 0; i < N; i++) O[d] = pg_mfma16<TC>(v, __builtin_bit_cast(uint4, ph[i][t]), O[d]);
+            m = pg_mfma16<TC>(marks, pg_ones<TC>(seen >> (8 * t)), m);
+          }
+#pragma unroll
+          for (int r = 0; r < 4; r++) O[d][r] += pg_wild_sum(m[r]);
+        }
+      } else {
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+          for (int t = 0; t < NS; t++) {
+            const uint4 v = pg_values<D>(vl + va[d] + 32 * t * 2 * D);
+#pragma unroll
+            for (int i = 0; i < N; i++) O[d] = pg_mfma16<TC>(v, __builtin_bit_cast(uint4, ph[i][t]), O[d]);
+          }
+      }
+      PG_WAIT_LDS();   // the values have been read
+      if (more) load(a.vc, VALUES, k + 1);
     }
-    PG_WAIT_LDS();   // the values have been read
-    if (more) load(a.vc, VALUES, k + 1);
+    if (careful || !pg_any_wild<ND>(O)) break;
   }
   // the waves' states, each in its own LDS
   Ls = over_kg(Ls, OpAddF{});
@@ -957,7 +977,7 @@ __device__ __forceinline__ v16f pg_mfma32(uint4 a, uint4 b, v16f c) {   // 32 x 
 template <int D>
 struct PgPromptLds {
   __attribute__((aligned(16))) uint4 lds[2][2][8 * D];   // [buffer][keys, values]
-  int last, tamed;   // tamed: 1 + the last tile whose values were changed
+  int last, tamed, wild;   // tamed: 1 + the last tile whose values were changed; wild: a wave has infinite sums or NaN
   PgFinder<4>::Lds found;
 };
 template <int TC, int D, bool FINE>   // FINE: weights in parts that keep float32 (float32 outputs)
@@ -1016,7 +1036,8 @@ __device__ __forceinline__ void pg_prompt(const PgStep& p, int block, int grid, 
     const int page = gld(a.b.table + un.s * a.b.table_stride + (min(key, end - 1) >> a.b.page_log));
     return page >= 0 && page < a.b.pages ? page * a.page_stride + (key & pmask) * a.slot_stride + un.head * a.head_stride : -1;
   };
-  const int all_hi = min(p0 + 1, end) - KT, all_lo = c.window ? p1 - c.window : -1, mine_hi = min(w0 + 1, wend) - KT, mine_lo = c.window ? w1 - c.window : -1;
+  int all_hi = min(p0 + 1, end) - KT;
+  const int all_lo = c.window ? p1 - c.window : -1, mine_hi = min(w0 + 1, wend) - KT, mine_lo = c.window ? w1 - c.window : -1;
   int64_t group = -1;   // of the next 16 tiles, 16 keys a lane
   uint64_t there = 0;   // which of them have a place
   auto groups = [&](int k) {
@@ -1042,17 +1063,8 @@ __device__ __forceinline__ void pg_prompt(const PgStep& p, int block, int grid, 
                                                                 mine_lds);
   };
   const auto B0 = std::integral_constant<int, 0>{};
-  float Mx = -INFINITY, Ls = 0.f;   // Ls: this lane's keys only
+  float Mx, Ls;   // Ls: this lane's keys only
   v16f O[ND];
-#pragma unroll
-  for (int d = 0; d < ND; d++) O[d] = (v16f){};
-  if (tid == 0) tamed = 0;
-  groups(0);
-  PG_WAIT_OWN();
-  if (count > 0) {
-    next(0);
-    pg_each<2 * LOADS>([&](auto i) { load(i, B0); });
-  }
   auto tile = [&](int k, auto buffer) {   // buffer: k % 2
     constexpr int BUF = decltype(buffer)::value;
     constexpr std::integral_constant<int, 1 - BUF> OTHER{};
@@ -1192,11 +1204,30 @@ __device__ __forceinline__ void pg_prompt(const PgStep& p, int block, int grid, 
       }
     }
   };
-  for (int k = 0; k < count; k += 2) {
-    tile(k, std::integral_constant<int, 0>{});
-    if (k + 1 < count) tile(k + 1, std::integral_constant<int, 1>{});
+  if (tid == 0) shared.wild = 0;
+  for (bool careful = false;; careful = true) {   // (twice only for infinities and NaN, pg_any_wild)
+    Mx = -INFINITY;
+    Ls = 0.f;
+#pragma unroll
+    for (int d = 0; d < ND; d++) O[d] = (v16f){};
+    if (tid == 0) tamed = 0;
+    groups(0);
+    PG_WAIT_OWN();
+    if (count > 0) {
+      next(0);
+      pg_each<2 * LOADS>([&](auto i) { load(i, B0); });
+    }
+    for (int k = 0; k < count; k += 2) {
+      tile(k, std::integral_constant<int, 0>{});
+      if (k + 1 < count) tile(k + 1, std::integral_constant<int, 1>{});
+    }
+    PG_WAIT(0);   // (a load behind the last tile)
+    if (careful || count == 0) break;
+    if (pg_any_wild<ND>(O) && lane == 0) shared.wild = 1;   // (set to 0 before the first tile's barrier)
+    __syncthreads();
+    if (!__builtin_amdgcn_readfirstlane(shared.wild)) break;
+    all_hi = -KT;   // no tile counts as seen whole by all rows
   }
-  PG_WAIT(0);   // (a load behind the last tile)
   Ls = over_h(Ls, OpAddF{});
   const int r = 32 * w + n;
   if (r < live) {

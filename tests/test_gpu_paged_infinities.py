@@ -1,0 +1,98 @@
+"""GPU tests of the paged-cache attention where rows see infinities and NaN among the values: an output is NaN, +inf or -inf
+exactly where the definition says, wherever the value lies in its tile and however the keys are cut. A softmax weight is
+positive, so a row that sees +inf (-inf) in a dim has +inf (-inf) there, and NaN if it sees both, or a NaN; the other dims are finite
+and are held to the float64 restatement by the tolerances of test_gpu_paged.py."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from hip_buffers import Hip
+from oracle import paged as O
+from test_gpu_paged import Setup
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture()
+def hip():
+    h = Hip()
+    yield h
+    h.close()
+
+
+def check_kinds(s, got, window, sinks, out_dtype):
+    """The kinds of all outputs, from the kinds of the values that their rows see (no weights in this)."""
+    val = (O.from_bits(got, out_dtype) if out_dtype != "f32" else got.view(np.float32)).reshape(s.rows, s.heads, s.dim)
+    v = O.from_bits(s.view(s.v_bits), s.dtype)
+    kinds = np.stack([np.isposinf(v), np.isneginf(v), np.isnan(v)])   # [3][pages][slots][kv][dim]
+    wild = 0
+    for r, seq, p in O.rows_of(s.lens, s.row0, s.rows):
+        seen = [O.slot(s.table[:, :s.width], s.pages, s.page, seq, j) for j in range(max(p + 1, 0)) if window == 0 or j > p - window or j < sinks]
+        seen = [x for x in seen if x is not None]
+        pg, sl = np.array(seen, int).reshape(-1, 2).T
+        up, down, nan = np.repeat(kinds[:, pg, sl].any(1), s.heads // s.kv, axis=1)   # [heads][dim] each
+        nan = nan | (up & down)
+        want = np.where(nan, 3, np.where(up, 1, np.where(down, 2, 0)))
+        g = val[r]
+        have = np.where(np.isnan(g), 3, np.where(np.isposinf(g), 1, np.where(np.isneginf(g), 2, 0)))
+        bad = want != have
+        assert not bad.any(), (f"row {r} at {p}", np.argwhere(bad)[:4], "want, have (1 inf, 2 -inf, 3 nan)", want[bad][:4], have[bad][:4])
+        wild += int((want > 0).sum())
+    return wild
+
+
+def put(s, seq, t, head, dims):
+    """dims: {dim: value} of the value at position t of a sequence."""
+    pg, sl = O.slot(s.table[:, :s.width], s.pages, s.page, seq, t)
+    for d, x in dims.items():
+        s.view(s.v_bits)[pg, sl, head, d] = O.to_bits(np.array([x], np.float32), s.dtype)[0]
+
+
+def attend(s, window=0, sinks=0, out_dtype=None, **kw):
+    with np.errstate(invalid="ignore", over="ignore"):   # (the restatement's own comparison of infinities)
+        got = s.attend(window=window, sinks=sinks, out_dtype=out_dtype, **kw)
+    return check_kinds(s, got, window, sinks, out_dtype or s.dtype)
+
+
+INF, NAN = np.inf, np.nan
+SHAPES = [(1, 6, 2), (3, 6, 2), (40, 6, 2), (150, 112, 112)]
+
+
+@pytest.mark.parametrize("out_dtype", [None, "f32"], ids=["narrow", "f32"])
+@pytest.mark.parametrize("dim,dtype", [(64, "f16"), (128, "f16"), (64, "bf16"), (128, "bf16")])
+@pytest.mark.parametrize("rows,heads,kv", SHAPES, ids=["1", "3", "40", "150-prompt-kernel"])
+def test_infinities_that_every_row_sees(hip, rows, heads, kv, dim, dtype, out_dtype):
+    """In tiles that are seen whole, in the last one, and in several tiles of one dim."""
+    s = Setup(hip, [(300, rows), (260, min(rows, 60)), (16, 1)], heads=heads, kv=kv, dim=dim, dtype=dtype)
+    for t in (5, 70, 140):   # (all rows of the first sequence are behind position 149)
+        put(s, 0, t, 0, {1: INF, 2: -INF, 40: INF})
+    put(s, 0, 20, 0, {3: INF, 4: -INF, 5: INF})
+    put(s, 0, 100, 0, {3: INF, 4: -INF, 5: -INF, 6: NAN})
+    put(s, 0, 149, 1, {0: INF, dim - 1: -INF})
+    put(s, 0, 299, 0, {7: INF, 2: INF})        # seen by the last row alone: -inf and +inf make NaN
+    put(s, 1, 9, 1, {11: -INF, 12: NAN})
+    put(s, 2, 15, 0, {13: INF})
+    assert attend(s, out_dtype=out_dtype) > 0
+    assert attend(s, window=250, sinks=7, out_dtype=out_dtype) > 0
+    assert attend(s, window=30, sinks=6, out_dtype=out_dtype) > 0
+
+
+@pytest.mark.parametrize("rows,heads,kv", [(1, 4, 2), (150, 112, 112)], ids=["step", "prompt-kernel"])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_rows_whose_scores_are_all_minus_infinity_are_zeros(hip, rows, heads, kv, dtype):
+    """Whatever the values are; and NaN scores make all of a row NaN."""
+    s = Setup(hip, [(300, rows)], heads=heads, kv=kv, dtype=dtype)
+    s.view(s.k_bits)[..., 0] = O.to_bits(np.array([-INF], np.float32), dtype)[0]
+    put(s, 0, 5, 0, {1: INF, 2: NAN})
+    put(s, 0, 299, 1, {1: INF, 2: NAN})
+    q = np.abs(s.rng.standard_normal((s.rows, heads * 64), dtype=np.float32)) + 0.5
+    for out_dtype in (s.dtype, "f32"):
+        got = s.attend(q=O.to_bits(q, dtype), out_dtype=out_dtype, check=False)
+        assert not got.any()
+    s.kc = None
+    pg, sl = O.slot(s.table, s.pages, s.page, 0, 8)
+    s.view(s.k_bits)[pg, sl, 0, 0] = O.to_bits(np.array([NAN], np.float32), dtype)[0]
+    got = s.attend(q=O.to_bits(q, dtype), out_dtype="f32", check=False).view(np.float32).reshape(s.rows, heads, 64)
+    assert np.isnan(got[:, :heads // kv]).all()
+    assert not got[:, heads // kv:].any()

@@ -353,7 +353,10 @@ ILL_API int ill_paged_append(ill_paged* p, const ill_paged_batch* batch, const i
  * j < sinks. out [rows][heads x head_dim], row r at r * out_stride, of type out_dtype (the
  * cache's, or ILL_F32): the values weighted by the softmax of the scaled scores; zeros for a row
  * that sees nothing (or whose scores are all -inf). q [rows][heads x head_dim] is of the
- * cache's type. What a row does not see never reaches it, infinities and NaN included. */
+ * cache's type. What a row does not see never reaches it, infinities and NaN included. A value
+ * that is infinite or NaN reaches every row that sees it, however small its weight: the output
+ * is that infinity, or NaN where the row also sees a NaN or the other one; unless all of the
+ * row's scores are -inf, or one is +inf or NaN (the row is then NaN). */
 ILL_API int ill_paged_attend(ill_paged* p, const ill_paged_batch* batch, const void* q, int64_t q_stride, const void* k_cache,
                              const void* v_cache, int window, int sinks, void* out, int64_t out_stride, int out_dtype, void* stream);
 

@@ -548,6 +548,11 @@ __device__ __forceinline__ bool pg_any_wild(const V* sums) {   // of the wave's
   const float y = (z[0] + z[1]) + (z[2] + z[3]);
   return __any(y != y);
 }
+// The factor by which sums to reference `from` are moved to `to`, which is not below it; never 0, so that infinite sums stay
+// what they are where it underflows. (The exponential ends at 2^-126: 2^-149, the least number, is no further off.)
+__device__ __forceinline__ float pg_moved(float from, float to) {
+  return to == -INFINITY ? 1.f : fmaxf(__builtin_amdgcn_exp2f(from - to), 0x1p-149f);
+}
 __device__ __forceinline__ float pg_wild_sum(float marks) {
   const int n = (int)marks;
   float y = n & 127 ? INFINITY : 0.f;
@@ -643,7 +648,7 @@ __device__ __forceinline__ void pg_join(const PgAttend& a, const PgCut& c, const
 #pragma unroll
     for (int k = 1; k < T; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
     for (int x = j; x < count; x += T) {
-      const float e = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(wt[x * M + r] - m);
+      const float e = pg_moved(wt[x * M + r], m);
       wt[x * M + r] = e;
       l += ls[x * M + r] * e;
     }
@@ -662,17 +667,10 @@ __device__ __forceinline__ void pg_join(const PgAttend& a, const PgCut& c, const
       if (groups > 1) {
 #pragma unroll
         for (int u = 0; u < PG_FAN / 2; u++)
-          if (g + u * groups < count) {
-            const float e = wt[(g + u * groups) * M + r];
-            if (e != 0.f) y += ahead[u] * e;
-          }
+          if (g + u * groups < count) y += ahead[u] * wt[(g + u * groups) * M + r];
       } else {
 #pragma unroll 8
-        for (int x = 0; x < count; x++) {
-          const float e = wt[x * M + r];
-          const v4f v = pg_shared(part_of(i, x));
-          if (e != 0.f) y += v * e;
-        }
+        for (int x = 0; x < count; x++) y += pg_shared(part_of(i, x)) * wt[x * M + r];
       }
     }
     if (groups > 1) {   // (items <= width: once)
@@ -868,7 +866,7 @@ __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, Pg
       mc *= sc2;
       if (__any(mc > Mx + (PG_UP + PG_SLACK))) {
         mc = over_kg(mc, OpMaxF{});
-        const float mn = mc == -INFINITY ? Mx : fmaxf(mc - PG_UP, Mx), up = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(Mx - mn);
+        const float mn = mc == -INFINITY ? Mx : fmaxf(mc - PG_UP, Mx), up = pg_moved(Mx, mn);
         Mx = mn;
         Ls *= up;
 #pragma unroll
@@ -945,9 +943,9 @@ __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, Pg
     v4f o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int x = 0; x < NW; x++) {
-      const float e = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(smx[x][r] - m);
+      const float e = pg_moved(smx[x][r], m);
       l += sls[x][r] * e;
-      if (e != 0.f) o += *(const LAS v4f*)((const LAS float*)lds[x] + r * RF + d) * e;
+      o += *(const LAS v4f*)((const LAS float*)lds[x] + r * RF + d) * e;
     }
     if (un.splits == 1) {
       pg_store<TC>(a, un.seq.first + (uint32_t)(f0 + r) / c.G, un.head * c.G + (uint32_t)(f0 + r) % c.G, d, D, l == 0.f ? (v4f){0.f, 0.f, 0.f, 0.f} : o / l);
@@ -1143,7 +1141,7 @@ __device__ __forceinline__ void pg_prompt(const PgStep& p, int block, int grid, 
     mc *= sc2;
     if (__any(mc > Mx + (PG_UP + PG_SLACK))) {
       mc = over_h(mc, OpMaxF{});
-      const float mn = mc == -INFINITY ? Mx : fmaxf(mc - PG_UP, Mx), up = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(Mx - mn);
+      const float mn = mc == -INFINITY ? Mx : fmaxf(mc - PG_UP, Mx), up = pg_moved(Mx, mn);
       Mx = mn;
       Ls *= up;
 #pragma unroll

@@ -78,6 +78,34 @@ def test_infinities_that_every_row_sees(hip, rows, heads, kv, dim, dtype, out_dt
     assert attend(s, window=30, sinks=6, out_dtype=out_dtype) > 0
 
 
+@pytest.mark.parametrize("out_dtype", [None, "f32"], ids=["narrow", "f32"])
+@pytest.mark.parametrize("dim,dtype", [(64, "f16"), (128, "bf16")])
+@pytest.mark.parametrize("seqs,heads,kv", [([(9000, 1)], 4, 2), ([(9000, 20)], 4, 1), ([(6000, 40)] + [(100 + i, 40) for i in range(7)], 64, 32)],
+                         ids=["1", "20", "both"])
+def test_infinities_with_weights_of_next_to_nothing(hip, seqs, heads, kv, dim, dtype, out_dtype):
+    """A few keys' scores lie 110 to 400 above the others', whose weights underflow in float32: the infinities among the others' values
+    reach the rows all the same, from tiles before and behind those keys, and from other parts of the keys. (Up to 700 the float64
+    restatement's weights do not underflow.)"""
+    s = Setup(hip, seqs, heads=heads, kv=kv, dim=dim, dtype=dtype)
+    w = s.heads * s.dim
+    q = s.rng.standard_normal((s.rows, w), dtype=np.float32)
+    q[:, ::dim] = 30.0                       # dim 0 of every head
+    keys = s.view(s.k_bits)
+    scale = 30 * s.scale
+    keys[..., 0] = 0
+    for t, score in ((3000, 110.0), (3001, 250.0), (5200, 400.0)):
+        pg, sl = O.slot(s.table, s.pages, s.page, 0, t)
+        keys[pg, sl, :, 0] = O.to_bits(np.array([score / scale], np.float32), dtype)[0]
+    put(s, 0, 17, 0, {1: INF, 2: -INF, 3: INF})
+    put(s, 0, 2990, 0, {4: INF, 3: -INF})
+    put(s, 0, 3064, 0, {5: -INF})
+    put(s, 0, 5000, kv - 1, {6: INF, 7: NAN})
+    put(s, 0, 5900, 0, {8: -INF, 9: INF})
+    if seqs[0][0] > 8000:
+        put(s, 0, 8000, 0, {10: INF, 1: -INF})
+    assert attend(s, out_dtype=out_dtype, q=O.to_bits(q, dtype)) > 0
+
+
 @pytest.mark.parametrize("rows,heads,kv", [(1, 4, 2), (150, 112, 112)], ids=["step", "prompt-kernel"])
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 def test_rows_whose_scores_are_all_minus_infinity_are_zeros(hip, rows, heads, kv, dtype):

@@ -352,7 +352,8 @@ ILL_API int ill_paged_append(ill_paged* p, const ill_paged_batch* batch, const i
  * row at position p sees the positions j <= p with j > p - window (window 0: all of them) or
  * j < sinks. out [rows][heads x head_dim], row r at r * out_stride, of type out_dtype (the
  * cache's, or ILL_F32): the values weighted by the softmax of the scaled scores; zeros for a row
- * that sees nothing (or whose scores are all -inf). q [rows][heads x head_dim] is of the
+ * that sees nothing (or whose scores are all -inf). Sums are float32, of weights of at most 1 for a
+ * bf16 cache (an f16 cache's values cannot overflow them). q [rows][heads x head_dim] is of the
  * cache's type. What a row does not see never reaches it, infinities and NaN included. A value
  * that is infinite or NaN reaches every row that sees it, however small its weight: the output
  * is that infinity, or NaN where the row also sees a NaN or the other one; unless all of the

@@ -561,10 +561,13 @@ __device__ __forceinline__ float pg_wild_sum(float marks) {
 }
 
 // The exponents' reference of a row follows its greatest score, PG_UP below it, and is moved only when a score
-// passes it by more than PG_UP + PG_SLACK: weights then stay below 2^15, in f16's range, and their rounding
-// keeps its 11 bits down to 2^-24 of the greatest one.
-#define PG_UP 10.f
+// passes it by more than PG_UP + PG_SLACK. For f16 weights then stay below 2^15, in its range: one rounding keeps their 11 bits
+// down to 2^-24 of the greatest one, two parts (float32 outputs) 22 bits down to 2^-13 of it, and 2^-35 of it below that. bf16
+// has float32's range: weights up to 1, so that sums overflow only where a softmax with its greatest weight at 1 does too (with
+// the greatest at 2^10, 34 even values of 1e34 overflowed).
 #define PG_SLACK 5.f
+template <int TC>
+constexpr float PG_UP = TC == PG_BF16 ? -PG_SLACK : 10.f;
 
 struct PgWork {        // a call's share of the handle's workspace
   float2* ml;          // [2 x 2^log][M] reference and sum of a part's rows
@@ -864,9 +867,9 @@ __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, Pg
 #pragma unroll
         for (int r = 0; r < 4; r++) mc = fmaxf(mc, s[b][r]);
       mc *= sc2;
-      if (__any(mc > Mx + (PG_UP + PG_SLACK))) {
+      if (__any(mc > Mx + (PG_UP<TC> + PG_SLACK))) {
         mc = over_kg(mc, OpMaxF{});
-        const float mn = mc == -INFINITY ? Mx : fmaxf(mc - PG_UP, Mx), up = pg_moved(Mx, mn);
+        const float mn = mc == -INFINITY ? Mx : fmaxf(mc - PG_UP<TC>, Mx), up = pg_moved(Mx, mn);
         Mx = mn;
         Ls *= up;
 #pragma unroll
@@ -1139,9 +1142,9 @@ __device__ __forceinline__ void pg_prompt(const PgStep& p, int block, int grid, 
 #pragma unroll
       for (int r = 0; r < 16; r++) mc = fmaxf(mc, s[b][r]);
     mc *= sc2;
-    if (__any(mc > Mx + (PG_UP + PG_SLACK))) {
+    if (__any(mc > Mx + (PG_UP<TC> + PG_SLACK))) {
       mc = over_h(mc, OpMaxF{});
-      const float mn = mc == -INFINITY ? Mx : fmaxf(mc - PG_UP, Mx), up = pg_moved(Mx, mn);
+      const float mn = mc == -INFINITY ? Mx : fmaxf(mc - PG_UP<TC>, Mx), up = pg_moved(Mx, mn);
       Mx = mn;
       Ls *= up;
 #pragma unroll

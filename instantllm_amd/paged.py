@@ -31,7 +31,15 @@ class _Rows(C.Structure):
                [(n, C.c_void_p) for n in ("bias", "q_norm", "k_norm", "positions")] + [("dtype", C.c_int32), ("reserved", C.c_int32)]
 
 
-_pack_rows = struct.Struct("PPPPqqqqPPPPii").pack   # a _Rows, at a third of the time
+# a Batch and a _Rows, faster than field by field; numbers that do not fit are an error (ctypes cuts them off)
+_pack_batch = struct.Struct("iiqqqqPPP").pack
+_pack_rows = struct.Struct("PPPPqqqqPPPPii").pack
+
+
+def _fits(bits: int, **values: int):
+    for name, v in values.items():
+        if not -1 << bits - 1 <= v < 1 << bits - 1:
+            raise ValueError(f"{name} {v}: more than {bits} bits")
 
 
 def _dtype(name: str) -> int:
@@ -52,6 +60,8 @@ class PagedAttention:
         self.lib = load_library()
         self.heads, self.kv_heads, self.head_dim, self.dtype, self.type = heads, kv_heads, head_dim, dtype, _dtype(dtype)
         self.q_width, self.kv_width = heads * head_dim, kv_heads * head_dim
+        _fits(32, heads=heads, kv_heads=kv_heads, head_dim=head_dim, page_size=page_size, rotary_dim=rotary_dim or 0, streams=streams)
+        _fits(64, **dict(zip(("page_stride", "slot_stride", "head_stride"), strides or ())))
         d = _Desc(self.type, heads, kv_heads, head_dim, page_size, head_dim if rotary_dim is None else rotary_dim, int(interleaved), streams,
                   *(strides or (0, 0, 0)), rope_base, norm_eps, scale or 0.0)
         h = C.c_void_p()
@@ -65,8 +75,11 @@ class PagedAttention:
     def batch(self, lens: int, table: int, table_width: int, pages: int, seqs: int, rows: int | None = None, row0: int | None = None,
               max_rows: int = 0, table_stride: int | None = None) -> Batch:
         """lens [seqs], table [seqs][table_stride], row0 [seqs + 1] (None: one row each): device addresses of int32 arrays."""
-        return Batch(seqs, table_width, table_width if table_stride is None else table_stride, seqs if rows is None else rows, max_rows, pages,
-                     lens, table, row0)
+        try:
+            return Batch.from_buffer_copy(_pack_batch(seqs, table_width, table_width if table_stride is None else table_stride, seqs if rows is None else rows,
+                                                      max_rows, pages, lens or 0, table or 0, row0 or 0))
+        except struct.error as e:
+            raise ValueError(f"a batch's sizes and addresses: {e}") from None
 
     def append(self, batch: Batch, k_cache: int, v_cache: int, k: int, v: int, q: int | None = None, q_out: int | None = None,
                x_dtype: str | None = None, x_stride: int | None = None, q_stride: int | None = None, k_stride: int | None = None,
@@ -77,9 +90,12 @@ class PagedAttention:
         qw, kw = self.q_width, self.kv_width
         if x_stride is not None:
             qw = kw = x_stride
-        x = _pack_rows(q or 0, k or 0, v or 0, q_out or 0, qw if q_stride is None else q_stride, kw if k_stride is None else k_stride,
-                       kw if v_stride is None else v_stride, self.q_width if q_out_stride is None else q_out_stride, bias or 0, q_norm or 0,
-                       k_norm or 0, positions or 0, self.type if x_dtype is None else _dtype(x_dtype), 0)
+        try:
+            x = _pack_rows(q or 0, k or 0, v or 0, q_out or 0, qw if q_stride is None else q_stride, kw if k_stride is None else k_stride,
+                           kw if v_stride is None else v_stride, self.q_width if q_out_stride is None else q_out_stride, bias or 0, q_norm or 0,
+                           k_norm or 0, positions or 0, self.type if x_dtype is None else _dtype(x_dtype), 0)
+        except struct.error as e:
+            raise ValueError(f"strides and addresses of rows: {e}") from None
         rc = self.lib.ill_paged_append(self.h, C.byref(batch), x, k_cache, v_cache, stream)
         if rc:
             self._check(rc)
@@ -87,8 +103,12 @@ class PagedAttention:
     def attend(self, batch: Batch, k_cache: int, v_cache: int, q: int, out: int, out_dtype: str | None = None, window: int = 0, sinks: int = 0,
                q_stride: int | None = None, out_stride: int | None = None, stream: int | None = None):
         """Attention of the new rows over the cache, all earlier positions or the last `window` and the first `sinks`."""
-        rc = self.lib.ill_paged_attend(self.h, C.byref(batch), q, self.q_width if q_stride is None else q_stride, k_cache, v_cache, window, sinks,
-                                       out, self.q_width if out_stride is None else out_stride, self.type if out_dtype is None else _dtype(out_dtype), stream)
+        q_stride, out_stride = self.q_width if q_stride is None else q_stride, self.q_width if out_stride is None else out_stride
+        if (window | sinks) >> 31 or (q_stride | out_stride) >> 31:   # (negative ones are the library's to refuse)
+            _fits(32, window=window, sinks=sinks)
+            _fits(64, q_stride=q_stride, out_stride=out_stride)
+        rc = self.lib.ill_paged_attend(self.h, C.byref(batch), q, q_stride, k_cache, v_cache, window, sinks, out, out_stride,
+                                       self.type if out_dtype is None else _dtype(out_dtype), stream)
         if rc:
             self._check(rc)
 

@@ -292,13 +292,20 @@ ILL_API int ill_gemv_destroy(ill_gemv* g);
  * with interleaved != 0 dims 2 i and 2 i + 1. norm_eps belongs to the head norms; scale
  * multiplies the scores (0: 1 / sqrt(head_dim)). A handle belongs to the GPU that was current
  * when it was created; one thread at a time calls on it.
- * Attention that is split over the keys joins its parts through a workspace that the handle
- * holds, one for each stream that calls come on and one for each capture of a stream, `streams`
- * of them (0: 8; 11 MB each at head size 64, 22 at 128): calls on different streams, and graphs,
- * may run at the same time (hipStreamPerThread, a different stream in each thread, is refused). What is enqueued on one stream, or captured on one stream in one capture, shares a
- * workspace: such a graph is instantiated once. A call that would need one more is refused;
- * ill_paged_release, called when nothing that the handle has enqueued or captured will run any
- * more, makes all of them free again. */
+ * Attention that is split over the keys joins its parts through a workspace, one of `streams`
+ * that the handle holds (0: 8; 11 MB each at head size 64, 22 at 128). Each stream that calls
+ * come on takes one, and so does each capture of a stream: calls on different streams, and
+ * graphs, may run at the same time. (hipStreamPerThread, a different stream in each thread, is
+ * refused.) What is enqueued on one stream, or captured on one stream in one capture, shares a
+ * workspace: such a graph is instantiated once. A call that would need one more is refused.
+ * ill_paged_bind makes a stream's calls, captured or not, take workspace 0 .. streams - 1
+ * from now on: a program that launches its graphs in order captures all of them on streams
+ * bound to one workspace. What was enqueued or captured on streams of one workspace must not
+ * run at the same time. A workspace that an unbound stream's calls hold is refused, and a
+ * second one for a stream. Workspace -1: the stream is bound no more, and the workspaces that its calls and captures have taken
+ * are free; called when nothing that came on the stream will run any more, also before a
+ * stream is destroyed (a later one may get its address). ill_paged_release does so for all
+ * streams. */
 enum { ILL_F32 = 0, ILL_F16 = 1, ILL_BF16 = 2 };
 typedef struct ill_paged ill_paged;
 typedef struct {
@@ -309,6 +316,7 @@ typedef struct {
 } ill_paged_desc;
 ILL_API int ill_paged_create(const ill_paged_desc* desc, ill_paged** out);
 ILL_API int ill_paged_destroy(ill_paged* p);
+ILL_API int ill_paged_bind(ill_paged* p, void* stream, int workspace);
 ILL_API int ill_paged_release(ill_paged* p);
 
 /* A batch. lens, table and row0 are device arrays that the kernels read when they run, so a

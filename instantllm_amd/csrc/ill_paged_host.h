@@ -3,20 +3,15 @@
 #pragma once
 #include "ill_paged.h"
 #include "ill_paged_check.h"
+#include "ill_paged_claims.h"
 
 struct ill_paged {
   ill_paged_desc d{};
   int device = 0, page_log = 0;
   double* freq = nullptr;   // [rotary_dim / 2] turns per position
-  // Workspaces of attention parts: one for each stream, and for each capture of a stream, that calls have come on. What
-  // runs on one stream, or in one captured graph's branch, is in order; two of them never share a workspace.
-  uint8_t* work = nullptr;
+  uint8_t* work = nullptr;   // workspaces of attention parts
   size_t work_bytes = 0;
-  struct Claim {
-    hipStream_t stream;
-    unsigned long long capture;   // 0: not captured
-  };
-  std::vector<Claim> claims;
+  illp::Workspaces workspaces;
 };
 
 namespace illp {
@@ -63,22 +58,21 @@ PgWork work_of(uint8_t* at, int log, int M, int D) {
 
 // The workspace of the stream, or of its capture.
 int workspace(ill_paged* p, hipStream_t st, uint8_t** out) {
-  unsigned long long id = 0;
-  if (st && st != hipStreamLegacy) {
-    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    HCK(hipStreamGetCaptureInfo(st, &status, &id));
-    if (status == hipStreamCaptureStatusNone) id = 0;
-  } else {
-    st = nullptr;
+  if (st == hipStreamLegacy) st = nullptr;
+  int w = p->workspaces.bound_to(st);
+  if (w < 0) {
+    unsigned long long id = 0;
+    if (st) {
+      hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+      HCK(hipStreamGetCaptureInfo(st, &status, &id));
+      if (status == hipStreamCaptureStatusNone) id = 0;
+    }
+    w = p->workspaces.claim(st, id);
   }
-  size_t i = 0;
-  while (i < p->claims.size() && !(p->claims[i].stream == st && p->claims[i].capture == id)) i++;
-  if (i == p->claims.size()) {
-    if ((int)i == p->d.streams)
-      return fail(ILL_E_ARG, "paged: calls have come on %d streams and captures, as many as the handle has workspaces for (ill_paged_release)", (int)i);
-    p->claims.push_back({st, id});
-  }
-  *out = p->work + i * p->work_bytes;
+  if (w < 0)
+    return fail(ILL_E_ARG, "paged: calls have come on as many streams and captures as the handle has workspaces for, %d (ill_paged_bind, ill_paged_release)",
+                p->d.streams);
+  *out = p->work + w * p->work_bytes;
   return ILL_OK;
 }
 
@@ -137,8 +131,9 @@ int ill_paged_create(const ill_paged_desc* desc, ill_paged** out) {
   if (hipMalloc(&p->work, p->work_bytes * d.streams) != hipSuccess || hipMemset(p->work, 0, p->work_bytes * d.streams) != hipSuccess ||
       hipDeviceSynchronize() != hipSuccess)
     return bad(fail(ILL_E_HIP, "paged: %d workspaces of %zu bytes cannot be allocated", d.streams, p->work_bytes));
+  p->workspaces.count = d.streams;
   try {
-    p->claims.reserve(d.streams);
+    p->workspaces.claims.reserve(d.streams);
   } catch (const std::exception&) {
     return bad(fail(ILL_E_ARG, "paged: out of host memory"));
   }
@@ -148,7 +143,29 @@ int ill_paged_create(const ill_paged_desc* desc, ill_paged** out) {
 
 int ill_paged_release(ill_paged* p) {
   if (!p) return fail(ILL_E_ARG, "paged: null handle");
-  p->claims.clear();
+  p->workspaces.clear();
+  return ILL_OK;
+}
+
+int ill_paged_bind(ill_paged* p, void* stream, int workspace) {
+  if (!p) return fail(ILL_E_ARG, "paged: null handle");
+  hipStream_t st = (hipStream_t)stream;
+  if (st == hipStreamPerThread) return fail(ILL_E_ARG, "paged: the per-thread default stream is several streams; pass a stream of your own");
+  if (st == hipStreamLegacy) st = nullptr;
+  if (workspace < -1 || workspace >= p->d.streams) return fail(ILL_E_ARG, "paged: workspace %d of %d", workspace, p->d.streams);
+  if (workspace < 0) {
+    p->workspaces.forget(st);
+    return ILL_OK;
+  }
+  try {
+    if (!p->workspaces.bind(st, workspace)) {
+      const int now = p->workspaces.bound_to(st);
+      if (now >= 0) return fail(ILL_E_ARG, "paged: the stream is bound to workspace %d", now);
+      return fail(ILL_E_ARG, "paged: workspace %d is held by the calls of a stream that is not bound", workspace);
+    }
+  } catch (const std::exception&) {
+    return fail(ILL_E_ARG, "paged: out of host memory");
+  }
   return ILL_OK;
 }
 

@@ -119,6 +119,7 @@ def load_library(path: str | os.PathLike | None = None) -> C.CDLL:
         "ill_gemv_run_noalloc": (C.c_int, [P, C.c_int, P, P, P, P, P]),
         "ill_paged_create": (C.c_int, [P, C.POINTER(P)]),
         "ill_paged_destroy": (C.c_int, [P]),
+        "ill_paged_bind": (C.c_int, [P, P, C.c_int]),
         "ill_paged_release": (C.c_int, [P]),
         "ill_paged_append": (C.c_int, [P, P, P, P, P, P]),
         "ill_paged_attend": (C.c_int, [P, P, P, C.c_int64, P, P, C.c_int, C.c_int, P, C.c_int64, C.c_int, P]),

@@ -112,6 +112,14 @@ class PagedAttention:
         if rc:
             self._check(rc)
 
+    def bind(self, stream: int | None, workspace: int | None):
+        """Calls on the stream, captured or not, take this of the `streams` workspaces from now on: streams that never run at the same
+        time, and graphs launched in order, may share one. None: the stream's workspaces are free (when nothing that came on
+        it will run any more, and before it is destroyed)."""
+        w = -1 if workspace is None else workspace
+        _fits(32, workspace=w)
+        self._check(self.lib.ill_paged_bind(self.h, stream, w))
+
     def release(self):
         """Frees the workspaces of all streams and captures (when nothing enqueued or captured will run any more)."""
         self._check(self.lib.ill_paged_release(self.h))

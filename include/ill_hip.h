@@ -329,7 +329,8 @@ ILL_API int ill_paged_release(ill_paged* p);
  * new rows that a sequence has, if known (0: unknown; a hint for the launch only). pages: pages
  * of the cache. A page number outside 0 .. pages - 1 is not followed: its positions are neither
  * written nor seen, and so are positions past table_width pages or below 0. Pages may be shared
- * for reading. rows x heads is at most 2^26, seqs x heads at most 2^22. */
+ * for reading. rows x heads is at most 2^26, seqs x heads at most 2^22, seqs at most 2^14 (from
+ * a thousand on a call's time grows with their square: 1024 with 2 key/value heads 42 us, 4096 320). */
 typedef struct {
   int32_t seqs, table_width;
   int64_t table_stride, rows, max_rows, pages;

@@ -11,7 +11,11 @@
 namespace illp {
 
 constexpr int64_t kMost = 1 << 30;                          // positions, strides
-constexpr int64_t kMostRows = 1 << 26, kMostSeqs = 1 << 22;   // times heads: a launch has fewer than 2^24 workgroups of 256 threads
+constexpr int64_t kMostRows = 1 << 26, kMostSeqHeads = 1 << 22;   // times heads: a launch has fewer than 2^24 workgroups of 256 threads
+// Every workgroup of attention, and of append with row0 every row's wave, looks at all sequences: time grows with their square.
+// Single rows behind 100 positions, 14 / 2 heads of 64: 1024 sequences 42 us, 4096 0.32 ms, 16384 4.1 ms (without a hint of max_rows
+// 11); 256 key/value heads are 128 times as many workgroups.
+constexpr int64_t kMostSeqs = 1 << 14;
 
 inline bool aligned(const void* p, int n) { return ((uintptr_t)p & (uintptr_t)(n - 1)) == 0; }
 
@@ -63,8 +67,9 @@ inline int check_desc(ill_paged_desc& d) {
 
 inline int check_batch(const ill_paged_desc& d, const ill_paged_batch* b) {
   if (!b) return fail(ILL_E_ARG, "paged: null batch");
-  if (b->seqs < 0 || b->rows < 0 || b->rows > kMostRows / d.heads || b->seqs > kMostSeqs / d.heads)
-    return fail(ILL_E_ARG, "paged: %d sequences, %lld rows (rows x heads up to 2^26, sequences x heads up to 2^22)", b->seqs, (long long)b->rows);
+  if (b->seqs < 0 || b->rows < 0 || b->rows > kMostRows / d.heads || b->seqs > kMostSeqHeads / d.heads || b->seqs > kMostSeqs)
+    return fail(ILL_E_ARG, "paged: %d sequences, %lld rows (up to 2^14 sequences, rows x heads up to 2^26, sequences x heads up to 2^22)", b->seqs,
+                (long long)b->rows);
   if (b->pages < 1 || b->pages > INT32_MAX || b->table_width < 1 || b->table_width > kMost / d.page_size || b->table_stride < b->table_width ||
       b->table_stride > kMost)
     return fail(ILL_E_ARG, "paged: %lld pages, table of %d entries, %lld apart (positions up to 2^30)", (long long)b->pages, b->table_width,

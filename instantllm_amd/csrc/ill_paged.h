@@ -277,10 +277,12 @@ __device__ __forceinline__ PgUnit pg_uniform(const PgUnit& u) {
   return {one(u.s), one(u.head), one(u.q), one(u.split), one(u.splits), one(u.part_at), one(u.tile_at), {one(u.seq.first), one(u.seq.n), one(u.seq.p0)}};
 }
 
-// The division of a call's work, found by every workgroup of NW waves from the lengths: sequence s is thread s % NT's.
-template <int NW>
+// Workgroups of attention: waves and threads, for the kernels and their launches.
+constexpr int PG_WAVES = 4, PG_THREADS = 64 * PG_WAVES;
+
+// The division of a call's work, found by every workgroup from the lengths: sequence s is thread s % NT's.
 struct PgFinder {
-  static constexpr int NT = 64 * NW;
+  static constexpr int NW = PG_WAVES, NT = PG_THREADS;
   const PgBatch& b;
   PgCut c;
   int part, units;   // tiles of keys in a part; units of work in all
@@ -619,12 +621,12 @@ __device__ __forceinline__ void pg_put_part(const PgWork& w, int part, int r, in
 }
 
 static_assert(PG_FAN * PG_FAN >= PG_MAXSPLIT, "two steps");
-// Joins `count` <= PG_FAN parts (from part `first` on, every step-th) of a tile of rows in their order, by one workgroup
-// of NW waves: into the output, or into the first of them. lds: PG_FAN x M x 2 + 2 M floats and, behind them, NW x 64 states.
-template <int TC, int D, int M, int NW>
+// Joins `count` <= PG_FAN parts (from part `first` on, every step-th) of a tile of rows in their order, by one workgroup:
+// into the output, or into the first of them. lds: PG_FAN x M x 2 + 2 M floats and, behind them, PG_THREADS states.
+template <int TC, int D, int M>
 __device__ __forceinline__ void pg_join(const PgAttend& a, const PgCut& c, const PgWork& pw, const PgUnit& un, int first, int step, int count, bool out,
                                         int f0, int live, LAS float* lds) {
-  constexpr int NT = 64 * NW, T = NT / M >= 64 ? 64 : NT / M < 1 ? 1 : NT / M;   // T threads of a row, neighbours in a wave
+  constexpr int NT = PG_THREADS, T = NT / M >= 64 ? 64 : NT / M < 1 ? 1 : NT / M;   // T threads of a row, neighbours in a wave
   const int tid = threadIdx.x;
   LAS float *wt = lds, *ls = lds + PG_FAN * M, *rows = ls + PG_FAN * M;
   // few items (four dims of a row): `groups` threads each, every groups-th part to one of them, its values fetched along
@@ -692,7 +694,7 @@ __device__ __forceinline__ void pg_join(const PgAttend& a, const PgCut& c, const
 }
 
 // What follows a part of several: the last workgroup of PG_FAN parts joins them, and the last of those joins theirs.
-template <int TC, int D, int M, int NW>
+template <int TC, int D, int M>
 __device__ __forceinline__ void pg_finish(const PgAttend& a, const PgCut& c, const PgWork& w, const PgUnit& un, int f0, int live, LAS float* lds, int* last) {
   const int g = un.split / PG_FAN, groups = pg_up(un.splits, PG_FAN);
   int32_t* joined = w.joined + un.tile_at * (PG_MAXSPLIT / PG_FAN + 1);
@@ -700,7 +702,7 @@ __device__ __forceinline__ void pg_finish(const PgAttend& a, const PgCut& c, con
   int32_t* counter = joined + 1 + g;
   for (bool out = groups == 1;; out = true) {   // (once or twice)
     if (!pg_last(counter, count, last)) return;
-    pg_join<TC, D, M, NW>(a, c, w, un, first, step, count, out, f0, live, lds);
+    pg_join<TC, D, M>(a, c, w, un, first, step, count, out, f0, live, lds);
     if (out) return;
     first = un.part_at;
     step = PG_FAN;
@@ -727,16 +729,15 @@ struct PgStep {
 // Bound by memory where there is enough of it: 64 sequences of 100 to 9000 positions, 32 / 8 heads of 128, 432 MB in 97 us,
 // 4.4 TB/s (a large copy: 5.1). One sequence of 131071, 14 / 2 heads of 64, 67 MB in 20 us: 13 at the copy's rate, the rest the
 // launch, three dependent loads at the start (3) and the join (4). One of 500: 6.5 us, all latency.
-template <int NW>
 struct PgStepLds {
-  __attribute__((aligned(16))) uint4 lds[NW][1024];
-  float smx[NW][16], sls[NW][16];
+  __attribute__((aligned(16))) uint4 lds[PG_WAVES][1024];
+  float smx[PG_WAVES][16], sls[PG_WAVES][16];
   int last;
-  typename PgFinder<NW>::Lds found;
+  PgFinder::Lds found;
 };
-template <int TC, int D, bool FINE, int NW>   // FINE: weights in parts that keep float32 (float32 outputs)
-__device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, PgStepLds<NW>& shared) {
-  constexpr int KT = D == 64 ? 64 : 32, UPR = D / 8, KPI = 64 / UPR, NB = KT / 16, KS = D / 32, ND = D / 16, NS = KT / 32, NG = KT / 16;
+template <int TC, int D, bool FINE>   // FINE: weights in parts that keep float32 (float32 outputs)
+__device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, PgStepLds& shared) {
+  constexpr int NW = PG_WAVES, KT = D == 64 ? 64 : 32, UPR = D / 8, KPI = 64 / UPR, NB = KT / 16, KS = D / 32, ND = D / 16, NS = KT / 32, NG = KT / 16;
   constexpr int N = FINE ? PG_PARTS<TC> : 1;   // parts of a weight
   constexpr int RF = D + 4;   // floats between the rows of a state in LDS
   auto &lds = shared.lds;
@@ -760,7 +761,7 @@ __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, Pg
 #pragma unroll
   for (int d = 0; d < ND; d++) va[d] = pg_values_at<D>(8 * kg, 16 * d, n);
   const float sc2 = a.scale * 1.4426950408889634f;
-  PgFinder<NW> finder(a.b, c, grid, shared.found);
+  PgFinder finder(a.b, c, grid, shared.found);
   auto over_kg = [](float v, auto op) {   // over the lanes of the same row
     const auto x = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
     v = op(__int_as_float((int)x[0]), __int_as_float((int)x[1]));
@@ -937,7 +938,7 @@ __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, Pg
     sls[w][n] = Ls;
   }
   __syncthreads();
-  for (int i = tid; i < live * (D / 4); i += 64 * NW) {
+  for (int i = tid; i < live * (D / 4); i += PG_THREADS) {
     const int r = i / (D / 4), d = 4 * (i % (D / 4));
     float m = smx[0][r];
 #pragma unroll
@@ -956,7 +957,7 @@ __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, Pg
       pg_put_part<D, 16>(p.w, un.part_at + un.split, r, d, m, l, o);
     }
   }
-  if (un.splits > 1) pg_finish<TC, D, 16, NW>(a, c, p.w, un, f0, live, (LAS float*)lds, &shared.last);
+  if (un.splits > 1) pg_finish<TC, D, 16>(a, c, p.w, un, f0, live, (LAS float*)lds, &shared.last);
 }
 
 template <int TC>
@@ -979,12 +980,12 @@ template <int D>
 struct PgPromptLds {
   __attribute__((aligned(16))) uint4 lds[2][2][8 * D];   // [buffer][keys, values]
   int last, tamed, wild;   // tamed: 1 + the last tile whose values were changed; wild: a wave has infinite sums or NaN
-  PgFinder<4>::Lds found;
+  PgFinder::Lds found;
 };
 template <int TC, int D, bool FINE>   // FINE: weights in parts that keep float32 (float32 outputs)
 __device__ __forceinline__ void pg_prompt(const PgStep& p, int block, int grid, PgPromptLds<D>& shared) {
   constexpr int N = FINE ? PG_PARTS<TC> : 1;   // parts of a weight
-  constexpr int M = 128, KT = 64, UPR = D / 8, KS = D / 16, ND = D / 32, T = KT * UPR, LOADS = T / 256;   // LOADS: of keys, and of values, per wave and tile
+  constexpr int M = 128, KT = 64, UPR = D / 8, KS = D / 16, ND = D / 32, T = KT * UPR, LOADS = T / PG_THREADS;   // LOADS: of keys, and of values, per wave and tile
   auto& lds = shared.lds;
   int& tamed = shared.tamed;
   const PgAttend& a = p.a;
@@ -994,7 +995,7 @@ __device__ __forceinline__ void pg_prompt(const PgStep& p, int block, int grid, 
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 31, h = lane >> 5;
   const int cap = pg_cap(a.b), pmask = (1 << a.b.page_log) - 1;
   const float sc2 = a.scale * 1.4426950408889634f;
-  PgFinder<4> finder(a.b, c, grid, shared.found);
+  PgFinder finder(a.b, c, grid, shared.found);
   auto over_h = [](float v, auto op) {   // over the two lanes of a row
     const auto x = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
     return op(__int_as_float((int)x[0]), __int_as_float((int)x[1]));
@@ -1007,6 +1008,7 @@ __device__ __forceinline__ void pg_prompt(const PgStep& p, int block, int grid, 
     const int key = 16 * w + 8 * i + lane / UPR;
     lane_off[i] = 2 * ((uint32_t)(key & 15) * (uint32_t)a.slot_stride + 8 * ((lane % UPR) ^ pg_swz<D>(key)));
   }
+  static_assert(M == 32 * PG_WAVES && KT == 16 * PG_WAVES, "a wave has 32 rows, and loads 16 keys");
   static_assert(LOADS == 2 || LOADS == 4, "two or four keys x 16 bytes x lanes");
   const uint32_t mine_lds = pg_lds_at(&lds[0][0][64 * LOADS * w]);
   // this lane's operands in a tile: of the keys for each 16 dims, of the values for each 32 and for even and odd 16 keys;
@@ -1081,7 +1083,7 @@ __device__ __forceinline__ void pg_prompt(const PgStep& p, int block, int grid, 
     LAS uint8_t* vl = (LAS uint8_t*)lds[BUF][1];
     if (!all) {
 #pragma unroll 1
-      for (int i = tid; i < T; i += 256) {
+      for (int i = tid; i < T; i += PG_THREADS) {
         uint4 marks;
         const uint4 v = pg_get(vl + 16 * i);
         if (pg_wild<TC>(v)) {
@@ -1243,16 +1245,16 @@ __device__ __forceinline__ void pg_prompt(const PgStep& p, int block, int grid, 
         else pg_put_part<D, M>(p.w, un.part_at + un.split, r, dim, Mx, Ls, o);
       }
   }
-  if (un.splits > 1) pg_finish<TC, D, M, 4>(a, c, p.w, un, f0, live, (LAS float*)lds, &shared.last);
+  if (un.splits > 1) pg_finish<TC, D, M>(a, c, p.w, un, f0, live, (LAS float*)lds, &shared.last);
 }
 
 template <int TC, int D, bool FINE>
-__global__ __launch_bounds__(256, 2) void pg_step_kernel(PgStep p) {
-  __shared__ PgStepLds<4> lds;
-  pg_step<TC, D, FINE, 4>(p, blockIdx.x, gridDim.x, lds);
+__global__ __launch_bounds__(PG_THREADS, 2) void pg_step_kernel(PgStep p) {
+  __shared__ PgStepLds lds;
+  pg_step<TC, D, FINE>(p, blockIdx.x, gridDim.x, lds);
 }
 template <int TC, int D, bool FINE>
-__global__ __launch_bounds__(256, 2) void pg_prompt_kernel(PgStep p) {
+__global__ __launch_bounds__(PG_THREADS, 2) void pg_prompt_kernel(PgStep p) {
   __shared__ PgPromptLds<D> lds;
   pg_prompt<TC, D, FINE>(p, blockIdx.x, gridDim.x, lds);
 }
@@ -1264,12 +1266,12 @@ struct PgBoth {
   int32_t prompts;   // workgroups
 };
 template <int TC, int D, bool FINE>
-__global__ __launch_bounds__(256, 2) void pg_both_kernel(PgBoth p) {
+__global__ __launch_bounds__(PG_THREADS, 2) void pg_both_kernel(PgBoth p) {
   __shared__ union Lds {
-    PgStepLds<4> step;
+    PgStepLds step;
     PgPromptLds<D> prompt;
     __device__ Lds() {}
   } lds;
   if ((int)blockIdx.x < p.prompts) pg_prompt<TC, D, FINE>({p.a, p.prompt, p.prompt_work}, blockIdx.x, p.prompts, lds.prompt);
-  else pg_step<TC, D, FINE, 4>({p.a, p.step, p.step_work}, blockIdx.x - p.prompts, gridDim.x - p.prompts, lds.step);
+  else pg_step<TC, D, FINE>({p.a, p.step, p.step_work}, blockIdx.x - p.prompts, gridDim.x - p.prompts, lds.step);
 }

@@ -79,9 +79,9 @@ int workspace(ill_paged* p, hipStream_t st, uint8_t** out) {
 // `steps`, `prompts`: workgroups of each kind.
 template <int TC, int D, bool FINE>
 void launch_attend(const PgBoth& s, int64_t steps, hipStream_t st) {
-  if (!s.prompts) hipLaunchKernelGGL((pg_step_kernel<TC, D, FINE>), dim3(steps), dim3(256), 0, st, PgStep{s.a, s.step, s.step_work});
-  else if (!steps) hipLaunchKernelGGL((pg_prompt_kernel<TC, D, FINE>), dim3(s.prompts), dim3(256), 0, st, PgStep{s.a, s.prompt, s.prompt_work});
-  else hipLaunchKernelGGL((pg_both_kernel<TC, D, FINE>), dim3(s.prompts + steps), dim3(256), 0, st, s);
+  if (!s.prompts) hipLaunchKernelGGL((pg_step_kernel<TC, D, FINE>), dim3(steps), dim3(PG_THREADS), 0, st, PgStep{s.a, s.step, s.step_work});
+  else if (!steps) hipLaunchKernelGGL((pg_prompt_kernel<TC, D, FINE>), dim3(s.prompts), dim3(PG_THREADS), 0, st, PgStep{s.a, s.prompt, s.prompt_work});
+  else hipLaunchKernelGGL((pg_both_kernel<TC, D, FINE>), dim3(s.prompts + steps), dim3(PG_THREADS), 0, st, s);
 }
 template <int TC, int D>
 void launch_attend(const PgBoth& s, int64_t steps, hipStream_t st) {

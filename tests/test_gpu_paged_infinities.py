@@ -124,3 +124,62 @@ def test_rows_whose_scores_are_all_minus_infinity_are_zeros(hip, rows, heads, kv
     got = s.attend(q=O.to_bits(q, dtype), out_dtype="f32", check=False).view(np.float32).reshape(s.rows, heads, 64)
     assert np.isnan(got[:, :heads // kv]).all()
     assert not got[:, heads // kv:].any()
+
+
+@pytest.mark.parametrize("rows,heads,kv", [(1, 4, 2), (40, 4, 2), (150, 112, 112)], ids=["step", "40", "prompt-kernel"])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_infinite_scores_and_queries_stay_in_their_rows(hip, rows, heads, kv, dtype):
+    """A key with +inf, and queries with infinities and NaN, make whole rows NaN, and no other row."""
+    s = Setup(hip, [(300, rows), (200, 1)], heads=heads, kv=kv, dtype=dtype)
+    q = np.abs(s.rng.standard_normal((s.rows, heads, 64), dtype=np.float32)) + 0.5
+    plain = {t: s.attend(q=O.to_bits(q.reshape(s.rows, -1), dtype), out_dtype=t) for t in (dtype, "f32")}
+    wild = q.copy()
+    wild[0, 0, 3], wild[-1, -1, 5] = NAN, INF
+    v = s.view(s.k_bits)
+    seen = [O.slot(s.table[:, :s.width], s.pages, s.page, 0, t) for t in range(300)]
+    assert all((O.from_bits(v[p, t, 0, 5], dtype) != 0).all() for p, t in seen)
+    for t, before in plain.items():
+        got = s.attend(q=O.to_bits(wild.reshape(s.rows, -1), dtype), out_dtype=t, check=False).reshape(s.rows, heads, 64)
+        val = got.view(np.float32) if t == "f32" else O.from_bits(got, t)
+        want = before.reshape(got.shape)
+        for r in range(s.rows):
+            for h in range(heads):
+                if (r, h) in ((0, 0), (s.rows - 1, heads - 1)):
+                    assert np.isnan(val[r, h]).all(), (r, h)
+                else:
+                    assert np.array_equal(got[r, h], want[r, h]), (r, h)
+    pg, sl = seen[70]
+    v[pg, sl, 0, 9] = O.to_bits(np.array([INF], np.float32), dtype)[0]
+    s.kc = None
+    for t, before in plain.items():
+        got = s.attend(q=O.to_bits(q.reshape(s.rows, -1), dtype), out_dtype=t, check=False).reshape(s.rows, heads, 64)
+        val, want, group = got.view(np.float32) if t == "f32" else O.from_bits(got, t), before.reshape(got.shape), heads // kv
+        assert np.isnan(val[:rows, :group]).all()
+        assert np.array_equal(got[:rows, group:], want[:rows, group:]) and np.array_equal(got[rows:], want[rows:])
+
+
+@pytest.mark.parametrize("length,rows,heads,kv", [(9000, 1, 4, 2), (400, 150, 112, 112)], ids=["step", "prompt-kernel"])
+def test_graphs_follow_values_that_become_infinite(hip, length, rows, heads, kv):
+    """One graph over finite values, over infinities and over finite ones again."""
+    s = Setup(hip, [(length, rows), (200, rows)], heads=heads, kv=kv)
+    s.upload()
+    clean, w = s.v_bits.copy(), heads * 64
+    q = s.random_bits(s.rows, w)
+    put(s, 0, 100, 0, {1: INF, 2: -INF})
+    put(s, 1, 20, 1, {3: NAN})
+    dirty = s.v_bits.copy()
+    st = hip.stream()
+    dq, do = hip.put(q), hip.alloc(2 * s.rows * w)
+    graph = hip.capture(st, lambda: s.op.attend(s.batch, s.kc, s.vc, dq, do, stream=st))
+    for turn in range(5):
+        s.v_bits[...] = dirty if turn % 2 else clean
+        hip.write(s.vc, s.v_bits)
+        with np.errstate(invalid="ignore"):
+            want = s.attend(q=q, check=turn < 2)
+        hip.write(do, np.zeros_like(want))
+        hip.sync()
+        for _ in range(2):
+            hip.launch(graph, st)
+        got = hip.get(do, want)
+        assert np.array_equal(got, want), turn
+        assert (check_kinds(s, got, 0, 0, "f16") > 0) == (turn % 2 == 1)

@@ -288,8 +288,8 @@ ILL_API int ill_gemv_destroy(ill_gemv* g);
  * (page, slot, head, dim) of either cache is at page * page_stride + slot * slot_stride +
  * head * head_stride + dim elements (all 0: [pages][page_size][kv_heads][head_dim]); strides are
  * multiples of 8, slot_stride at most 2^24. The rotation turns the first `rotary_dim` dims of a
- * head (a multiple of 16; 0: none) by position * rope_base^(-2 i / rotary_dim), pairing dim i with i + rotary_dim / 2, or
- * with interleaved != 0 dims 2 i and 2 i + 1. norm_eps belongs to the head norms; scale
+ * head (a multiple of 16; 0: none) by position * rope_base^(-2 i / rotary_dim), pairing dim i
+ * with i + rotary_dim / 2, or with interleaved != 0 dims 2 i and 2 i + 1. norm_eps belongs to the head norms; scale
  * multiplies the scores (0: 1 / sqrt(head_dim)). A handle belongs to the GPU that was current
  * when it was created; one thread at a time calls on it.
  * Attention that is split over the keys joins its parts through a workspace, one of `streams`
@@ -326,8 +326,9 @@ ILL_API int ill_paged_release(ill_paged* p);
  * are not read. row0 [seqs + 1]: ascending; sequence s has the new rows row0[s] ..
  * row0[s + 1] - 1, which stand at its last positions; NULL: row s is sequence s's only one.
  * rows: rows of the buffers (the ones that are no sequence's are left alone). max_rows: the most
- * new rows that a sequence has, if known (0: unknown; a hint for the launch only). pages: pages
- * of the cache. A page number outside 0 .. pages - 1 is not followed: its positions are neither
+ * new rows that a sequence has, if known (0: unknown; a hint for the launch only: without it
+ * single rows that come with row0 are launched with prompts' workgroups too, which end at once;
+ * 200 rows in a window 27.5 in place of 24.3 us). pages: pages of the cache. A page number outside 0 .. pages - 1 is not followed: its positions are neither
  * written nor seen, and so are positions past table_width pages or below 0. Pages may be shared
  * for reading. rows x heads is at most 2^26, seqs x heads at most 2^22, seqs at most 2^14 (from
  * a thousand on a call's time grows with their square: 1024 with 2 key/value heads 42 us, 4096 320). */
@@ -344,7 +345,8 @@ typedef struct {
  * q_norm (k_norm) [head_dim], then the rotation by the row's position (positions [rows]: by
  * these instead), computed in float32 from angles in float64 and rounded once. NULL leaves a
  * step out. Keys and values go to their slots, queries to q_out (the cache's type; q itself
- * will do where type and stride agree). Two rows of one batch must not share a slot. Buffers
+ * will do where type and stride agree). Two rows of one batch must not share a slot, and
+ * q_out and the caches overlap nothing else that the call reads. Buffers
  * and caches are aligned to 16 bytes, strides are multiples of 8 elements (float32: 4). */
 typedef struct {
   const void *q, *k, *v;
@@ -363,7 +365,7 @@ ILL_API int ill_paged_append(ill_paged* p, const ill_paged_batch* batch, const i
  * cache's, or ILL_F32): the values weighted by the softmax of the scaled scores; zeros for a row
  * that sees nothing (or whose scores are all -inf). Sums are float32, of weights of at most 1 for a
  * bf16 cache (an f16 cache's values cannot overflow them). q [rows][heads x head_dim] is of the
- * cache's type. What a row does not see never reaches it, infinities and NaN included. A value
+ * cache's type; out overlaps nothing that the call reads. What a row does not see never reaches it, infinities and NaN included. A value
  * that is infinite or NaN reaches every row that sees it, however small its weight: the output
  * is that infinity, or NaN where the row also sees a NaN or the other one; unless all of the
  * row's scores are -inf, or one is +inf or NaN (the row is then NaN). */

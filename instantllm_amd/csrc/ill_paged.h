@@ -45,7 +45,10 @@ __device__ __forceinline__ uint32_t pg_pack2(float a, float b) {   // (as a pair
   if constexpr (T == PG_BF16) return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){a, b}, v2bf));
   else return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){a, b}, v2h));
 }
-// A pair of floats in parts of type T, each the rest of the one before: two parts of f16 keep 22 bits, three of bf16 24.
+// A pair of floats in parts of type T, each the rest of the one before: two parts of f16 keep 22 bits, three of bf16 24. Weights
+// go to the product with the values as such parts for float32 outputs. For 16-bit outputs they are rounded once, to the cache's
+// type: against float64 the outputs are then off by 0.0020 (8000 rows of 28 / 4 heads of 128, bf16), of which their own rounding alone is
+// 0.0017; in three parts the call takes 795 us in place of 469.
 template <int T>
 constexpr int PG_PARTS = T == PG_BF16 ? 3 : 2;
 template <int T, int N>
@@ -727,8 +730,8 @@ struct PgStep {
 // joined in LDS; a tile of rows whose keys are in several parts is joined by the workgroup that ends last, in
 // the parts' order.
 // Bound by memory where there is enough of it: 64 sequences of 100 to 9000 positions, 32 / 8 heads of 128, 432 MB in 97 us,
-// 4.4 TB/s (a large copy: 5.1). One sequence of 131071, 14 / 2 heads of 64, 67 MB in 20 us: 13 at the copy's rate, the rest the
-// launch, three dependent loads at the start (3) and the join (4). One of 500: 6.5 us, all latency.
+// 4.4 TB/s (a large copy: 5.1). One sequence of 131071, 14 / 2 heads of 64, 67 MB in 19.6 us: 13 at the copy's rate, the rest the
+// launch, three dependent loads at the start (3) and the join. One of 500: 6.5 us, all latency.
 struct PgStepLds {
   __attribute__((aligned(16))) uint4 lds[PG_WAVES][1024];
   float smx[PG_WAVES][16], sls[PG_WAVES][16];
@@ -856,7 +859,7 @@ __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, Pg
 #pragma unroll
           for (int r = 0; r < 4; r++) {
             const int key = 32 * (b >> 1) + 8 * kg + 4 * (b & 1) + r, j = kt + key;
-            // pg_sees. (Without branches: the compiler has lost the stores of `if (!on) s[b][r] = ..` behind && and ||.)
+            // pg_sees, by selects
             const bool on = j < cap & j <= pos & (c.window == 0 | j > pos - c.window | j < c.sinks) & (good >> (key >> 4) & 1);
             s[b][r] = on ? s[b][r] : -INFINITY;
             seen |= (uint32_t)on << (4 * b + r);
@@ -973,9 +976,11 @@ __device__ __forceinline__ v16f pg_mfma32(uint4 a, uint4 b, v16f c) {   // 32 x 
 // stand (row m of block b: key 32 b + m with bits 2 and 3 of m swapped).
 // What a row does not see must not reach it as 0 x inf either: in a tile that some row does not see whole, infinities and
 // NaN among the values are replaced by 0 in LDS, and added afterwards to the rows that see them.
-// One prompt of 8000 rows, 28 / 4 heads of 128, bf16: 442 to 461 us, 1.0 PFLOP/s, 0.85 to 0.89 of a large matrix product's rate here;
-// the card lowers its clock in both. With heads of 64 a score costs as many exponentials and sums for half the products: 4096 rows
-// of 14 / 2 heads in a window of 1024 take 36 us, 0.42 PFLOP/s, with 1.75 workgroups to a CU; a third of the waves' cycles are waits.
+// One prompt of 8000 rows, 28 / 4 heads of 128, bf16: 454 to 471 us on several cards, 0.97 to 1.01 PFLOP/s, 0.83 to 0.87 of a large matrix
+// product's rate; the card lowers its clock in both. With heads of 64 a score costs as many exponentials and sums for half the
+// products: 4096 rows of 14 / 2 heads in a window of 1024 take 35 to 37 us, 0.41 to 0.43 PFLOP/s. By the counters vector
+// instructions take 13 and the matrix units 7 us of it: a wave's scores, exponentials and weighted values follow each other, and
+// the one other wave of a SIMD does not fill its waits. Heads of 128 use all 256 registers and spill 19 outside the loop over tiles.
 template <int D>
 struct PgPromptLds {
   __attribute__((aligned(16))) uint4 lds[2][2][8 * D];   // [buffer][keys, values]

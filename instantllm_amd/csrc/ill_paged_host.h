@@ -36,7 +36,8 @@ PgBatch batch_of(const ill_paged* p, const ill_paged_batch& b) {
 // A call's parts. The step kernel cuts the keys into about a part for each CU (2^8), of 8 tiles of keys at least, two for each
 // wave: with 2^9 parts or 4 tiles the joining cost more than it gave (us, 2^8 / 2^9: one sequence of 131071 20.3 / 21.1, 200
 // through a window of 1024 25.1 / 33.7, but 64 ragged ones 97.7 / 95; 8 / 4 tiles: one of 500 6.8 / 8.3). The prompt kernel cuts
-// only what is over twice the average share of a CU (2^7): 2^8 is no faster, with twice the workspace.
+// a tile of rows whose keys are over 2^-7 of the call's work; a prompt alone, with PG_MANY tiles at least, never is. More parts, for the 512
+// workgroups that run at a time, have not been measured on batches that they would cut.
 PgCut step_cut(const ill_paged_desc& d, int window, int sinks) {
   return {(uint32_t)(d.heads / d.kv_heads), (uint32_t)d.kv_heads, 16, d.head_dim == 64 ? 64 : 32, window, sinks, 8, 8, 0, PG_MOST, 0};
 }

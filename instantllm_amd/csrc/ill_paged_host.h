@@ -77,24 +77,29 @@ int workspace(ill_paged* p, hipStream_t st, uint8_t** out) {
   return ILL_OK;
 }
 
+// Enqueues a kernel and returns this launch's error (hipGetLastError may hold one of the program's own calls).
+template <class... P>
+hipError_t launch(void (*kernel)(P...), int64_t blocks, int threads, int lds, hipStream_t st, std::common_type_t<P>... args) {
+  void* p[] = {&args...};
+  return hipLaunchKernel((const void*)kernel, dim3(blocks), dim3(threads), p, lds, st);
+}
+
 // `steps`, `prompts`: workgroups of each kind.
 template <int TC, int D, bool FINE>
-void launch_attend(const PgBoth& s, int64_t steps, hipStream_t st) {
-  if (!s.prompts) hipLaunchKernelGGL((pg_step_kernel<TC, D, FINE>), dim3(steps), dim3(PG_THREADS), 0, st, PgStep{s.a, s.step, s.step_work});
-  else if (!steps) hipLaunchKernelGGL((pg_prompt_kernel<TC, D, FINE>), dim3(s.prompts), dim3(PG_THREADS), 0, st, PgStep{s.a, s.prompt, s.prompt_work});
-  else hipLaunchKernelGGL((pg_both_kernel<TC, D, FINE>), dim3(s.prompts + steps), dim3(PG_THREADS), 0, st, s);
+hipError_t launch_attend(const PgBoth& s, int64_t steps, hipStream_t st) {
+  if (!s.prompts) return launch(pg_step_kernel<TC, D, FINE>, steps, PG_THREADS, 0, st, PgStep{s.a, s.step, s.step_work});
+  if (!steps) return launch(pg_prompt_kernel<TC, D, FINE>, s.prompts, PG_THREADS, 0, st, PgStep{s.a, s.prompt, s.prompt_work});
+  return launch(pg_both_kernel<TC, D, FINE>, s.prompts + steps, PG_THREADS, 0, st, s);
 }
 template <int TC, int D>
-void launch_attend(const PgBoth& s, int64_t steps, hipStream_t st) {
-  if (s.a.out_f32) launch_attend<TC, D, true>(s, steps, st);
-  else launch_attend<TC, D, false>(s, steps, st);
+hipError_t launch_attend(const PgBoth& s, int64_t steps, hipStream_t st) {
+  return s.a.out_f32 ? launch_attend<TC, D, true>(s, steps, st) : launch_attend<TC, D, false>(s, steps, st);
 }
 
 template <int TX, int TC>
-void launch_append(const PgAppend& a, int D, int R, int lds, hipStream_t st) {
-  const dim3 grid((a.b.rows + R - 1) / R);
-  if (D == 64) hipLaunchKernelGGL((pg_append_kernel<TX, TC, 64>), grid, dim3(256), lds, st, a, R);
-  else hipLaunchKernelGGL((pg_append_kernel<TX, TC, 128>), grid, dim3(256), lds, st, a, R);
+hipError_t launch_append(const PgAppend& a, int D, int R, int lds, hipStream_t st) {
+  const int64_t blocks = ((int64_t)a.b.rows + R - 1) / R;
+  return D == 64 ? launch(pg_append_kernel<TX, TC, 64>, blocks, 256, lds, st, a, R) : launch(pg_append_kernel<TX, TC, 128>, blocks, 256, lds, st, a, R);
 }
 
 }  // namespace illp
@@ -205,14 +210,13 @@ int ill_paged_append(ill_paged* p, const ill_paged_batch* batch, const ill_paged
   const int R = pg_append_rows(a.b.rows, ((a.q ? d.heads : 0) + 2 * d.kv_heads) * d.head_dim / 16), lds = R * 8 + (R + 1) / 2 * 8 + R * (d.rotary_dim / 2) * 8;
   hipStream_t st = (hipStream_t)stream;
   if (x->dtype == ILL_F32) {
-    if (d.dtype == ILL_F16) illp::launch_append<PG_F32, PG_F16>(a, d.head_dim, R, lds, st);
-    else illp::launch_append<PG_F32, PG_BF16>(a, d.head_dim, R, lds, st);
+    if (d.dtype == ILL_F16) HCK((illp::launch_append<PG_F32, PG_F16>(a, d.head_dim, R, lds, st)));
+    else HCK((illp::launch_append<PG_F32, PG_BF16>(a, d.head_dim, R, lds, st)));
   } else if (d.dtype == ILL_F16) {
-    illp::launch_append<PG_F16, PG_F16>(a, d.head_dim, R, lds, st);
+    HCK((illp::launch_append<PG_F16, PG_F16>(a, d.head_dim, R, lds, st)));
   } else {
-    illp::launch_append<PG_BF16, PG_BF16>(a, d.head_dim, R, lds, st);
+    HCK((illp::launch_append<PG_BF16, PG_BF16>(a, d.head_dim, R, lds, st)));
   }
-  HCK(hipGetLastError());
   return ILL_OK;
 }
 
@@ -262,13 +266,12 @@ int ill_paged_attend(ill_paged* p, const ill_paged_batch* batch, const void* q, 
   s.prompts = prompts ? (int)pg_grid(a.b.seqs, a.b.rows, !a.b.row0, cap, s.prompt) : 0;
   if (!s.prompts && !steps) return ILL_OK;
   if (d.dtype == ILL_F16) {
-    if (d.head_dim == 64) illp::launch_attend<PG_F16, 64>(s, steps, st);
-    else illp::launch_attend<PG_F16, 128>(s, steps, st);
+    if (d.head_dim == 64) HCK((illp::launch_attend<PG_F16, 64>(s, steps, st)));
+    else HCK((illp::launch_attend<PG_F16, 128>(s, steps, st)));
   } else {
-    if (d.head_dim == 64) illp::launch_attend<PG_BF16, 64>(s, steps, st);
-    else illp::launch_attend<PG_BF16, 128>(s, steps, st);
+    if (d.head_dim == 64) HCK((illp::launch_attend<PG_BF16, 64>(s, steps, st)));
+    else HCK((illp::launch_attend<PG_BF16, 128>(s, steps, st)));
   }
-  HCK(hipGetLastError());
   return ILL_OK;
 }
 

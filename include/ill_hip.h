@@ -372,6 +372,33 @@ ILL_API int ill_paged_append(ill_paged* p, const ill_paged_batch* batch, const i
 ILL_API int ill_paged_attend(ill_paged* p, const ill_paged_batch* batch, const void* q, int64_t q_stride, const void* k_cache,
                              const void* v_cache, int window, int sinks, void* out, int64_t out_stride, int out_dtype, void* stream);
 
+/* ---- Microscaled rows: quantisation and products for batches (no counterpart in the reference) ----
+ * A microscaled row is blocks of 32 values that share a power of two. A block's byte e stands for 2^(e - 127), 255
+ * for a block of NaN. Codes are e4m3 (ILL_MXF8: one byte, up to 448) or e2m1 (ILL_MXF4: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their
+ * negatives; two to a byte, the first in the low four bits). A matrix of rows is two arrays: codes [rows][cols or cols / 2] and powers
+ * [rows][cols / 32], both without gaps and aligned to 16 bytes; cols is a multiple of 32.
+ * Like the calls on a paged cache these take device pointers, enqueue on `stream` (a hipStream_t; NULL: the current device's
+ * default stream), allocate nothing, wait for nothing, keep nothing and can be captured into a graph. They run on the GPU that the stream belongs to.
+ *
+ * ill_mx_quantize: x [rows][cols] of type `dtype`, row r at r * x_stride elements (a multiple of 8, float32: 4; x aligned to 16
+ * bytes). A block's power is floor(log2(the largest size in it)) - 8 (ILL_MXF4: - 2), at least 2^-127; its values divided by it
+ * are rounded to nearest, ties to even, and end at +-448 (+-6). A block that holds an infinity or NaN becomes NaN (codes 0).
+ * ill_mx_dequantize: the values, rounded to `dtype` where they have no exact place in it. Up to 2^34 values a call. */
+enum { ILL_MXF8 = 8, ILL_MXF4 = 16 };
+ILL_API int ill_mx_quantize(int format, int dtype, const void* x, int64_t x_stride, int64_t rows, int64_t cols, void* codes, void* powers, void* stream);
+ILL_API int ill_mx_dequantize(int format, int dtype, const void* codes, const void* powers, int64_t rows, int64_t cols, void* y, int64_t y_stride,
+                              void* stream);
+
+/* y[r][c] = the sum over k of x[r][k] w[c][k], plus bias[c] (NULL: none): x [rows][inner] of format x_format, the matrix w
+ * [cols][inner] of format ILL_MXF4, both as ill_mx_quantize writes them. y: row r at r * y_stride elements of type y_dtype, rounded
+ * once. inner: a multiple of 32 up to 2^20 (multiples of 128 take the fast path of many rows); cols up to 2^24, rows up to 2^26, rows x cols up to 2^32. Sums are
+ * float32's. With x of format ILL_MXF8 and a 16-bit y they are the matrix units' own, which drop parts of a product far below the
+ * largest of its group: 4e-6 of the sums' size for normal values, 5e-5 for codes of evenly spread exponents; the sums for a float32 y are not
+ * cut. The result does not depend on which other rows or columns are computed with it only as far as the same kernel takes them. y overlaps nothing
+ * that the call reads. A NaN block makes every output that it belongs to NaN. */
+ILL_API int ill_mx_product(int x_format, const void* x, const void* x_powers, const void* w, const void* w_powers, int64_t rows, int64_t cols,
+                           int64_t inner, const float* bias, int y_dtype, void* y, int64_t y_stride, void* stream);
+
 /* The converter's quantizers (Converter.quantizeQ4Raw / quantGroup and quantizeQ8,
  * Sources/Engine/Convert.swift:252-370), host code that needs no GPU. w is a row-major
  * float32 [rows][cols] matrix; `threads` CPU threads split the rows (any count gives the

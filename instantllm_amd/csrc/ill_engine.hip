@@ -2133,4 +2133,15 @@ int ill_tok_encode_cb(void* user, const char* text, int32_t* ids, int cap) {
 
 }  // extern "C"
 
+// The other translation units' errors (ill_error.h).
+namespace illerr {
+int keep(int code, const char* text) noexcept {
+  try {
+    g_err = text;
+  } catch (const std::exception&) {   // (no memory for the message: the last one stays)
+  }
+  return code;
+}
+}  // namespace illerr
+
 #include "ill_paged_host.h"

@@ -1,0 +1,302 @@
+// Kernels of the microscaled operators (ill_mx_* in include/ill_hip.h): rows of blocks of 32 values that share a power of two.
+#pragma once
+#include "ill_lds.h"
+#include "ill_values.h"
+
+enum MxFormat { MX_F8 = 0, MX_F4 = 4 };   // as the matrix instructions name their operands' types: e4m3, e2m1
+
+typedef int v8i __attribute__((ext_vector_type(8)));
+typedef short v2s __attribute__((ext_vector_type(2)));
+
+// A block's power of two as a float, which the conversions read the exponent of only: 0 is 2^-127, 255 NaN.
+__device__ __forceinline__ float mx_power(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+// Bytes of `n` codes.
+template <int F>
+constexpr int mx_bytes(int n) { return F == MX_F8 ? n : n / 2; }
+
+// The power's byte of a block whose largest size has these bits (0: no value; from 0x7F800000 on: an infinity or NaN).
+template <int F>
+__device__ __forceinline__ uint32_t mx_power_of(uint32_t most) {
+  const int e = (int)(most >> 23);
+  return e == 255 ? 255 : (uint32_t)max(e - (F == MX_F8 ? 8 : 2), 0);
+}
+// Eight values of a block as codes, rounded to nearest, ties to even. The conversion to e4m3 makes what rounds past 448 a NaN: its operands end there.
+template <int F>
+__device__ __forceinline__ uint2 mx_codes(const float* x, uint32_t byte) {
+  const float p = mx_power(byte);
+  if constexpr (F == MX_F4) {
+    uint32_t c = 0;
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[0], x[1], p, 0);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[2], x[3], p, 1);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[4], x[5], p, 2);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[6], x[7], p, 3);
+    return {byte == 255 ? 0 : c, 0};
+  } else {
+    const float most = __uint_as_float((byte + 8) << 23 | 0x600000);   // 448 2^(byte - 127)
+    v2s c[2] = {};
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) y[i] = __builtin_amdgcn_fmed3f(x[i], -most, most);
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      c[i] = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c[i], y[4 * i], y[4 * i + 1], p, false);
+      c[i] = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c[i], y[4 * i + 2], y[4 * i + 3], p, true);
+    }
+    const uint2 r = __builtin_bit_cast(uint2, c);
+    return {byte == 255 ? 0 : r.x, byte == 255 ? 0 : r.y};
+  }
+}
+// Eight values of codes (mxf8: eight bytes, mxf4: the first four).
+template <int F>
+__device__ __forceinline__ void mx_values(uint2 c, uint32_t byte, float* x) {
+  typedef float v2f __attribute__((ext_vector_type(2)));
+  const float p = mx_power(byte);
+  v2f y[4];
+  if constexpr (F == MX_F4) {
+    y[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c.x, p, 0);
+    y[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c.x, p, 1);
+    y[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c.x, p, 2);
+    y[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c.x, p, 3);
+  } else {
+    y[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c.x, p, false);
+    y[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c.x, p, true);
+    y[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c.y, p, false);
+    y[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c.y, p, true);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; i++) x[i] = y[i / 2][i & 1];
+}
+
+// ---- rows to microscaled ones, and back ----------------------------------------------------
+struct MxRows {
+  uint8_t* x;            // values, row r at r * stride elements
+  uint8_t *codes, *powers;
+  int64_t stride;
+  uint32_t items, per;   // eight values each: in all, and in a row
+};
+
+__device__ __forceinline__ int64_t mx_at(const MxRows& a, uint32_t i) {   // the element that item i begins with
+  if (a.stride == 8 * (int64_t)a.per) return 8 * (int64_t)i;
+  const uint32_t r = i / a.per;
+  return r * a.stride + 8 * (int64_t)(i - r * a.per);
+}
+// A thread takes eight values at a time, so that four neighbours have a block.
+template <int T, int F>
+__global__ __launch_bounds__(256) void mx_quantize_kernel(MxRows a) {
+  constexpr int EB = T == PG_F32 ? 4 : 2;
+  for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < a.items; i += gridDim.x * 256) {   // (a block's threads agree: items are a multiple of four)
+    const uint8_t* src = a.x + EB * mx_at(a, i);
+    uint4 raw[EB / 2];
+#pragma unroll
+    for (int n = 0; n < EB / 2; n++) raw[n] = gld((const uint4*)src + n);
+    float x[8];
+    pg_unpack<T>(raw, x);
+    uint32_t most = 0;
+#pragma unroll
+    for (int n = 0; n < 8; n++) most = max(most, __float_as_uint(x[n]) & 0x7FFFFFFFu);   // (infinities and NaN are the largest)
+    most = max(most, (uint32_t)__shfl_xor((int)most, 1));
+    most = max(most, (uint32_t)__shfl_xor((int)most, 2));
+    const uint32_t byte = mx_power_of<F>(most);
+    const uint2 c = mx_codes<F>(x, byte);
+    if constexpr (F == MX_F8) gst((gu32x2*)a.codes + i, (gu32x2){c.x, c.y});
+    else gst((uint32_t*)a.codes + i, c.x);
+    if ((i & 3) == 0) gst(a.powers + i / 4, (uint8_t)byte);
+  }
+}
+template <int T, int F>
+__global__ __launch_bounds__(256) void mx_dequantize_kernel(MxRows a) {
+  constexpr int EB = T == PG_F32 ? 4 : 2;
+  for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < a.items; i += gridDim.x * 256) {
+    uint2 c = {0, 0};
+    if constexpr (F == MX_F8) c = gld((const uint2*)a.codes + i);
+    else c.x = gld((const uint32_t*)a.codes + i);
+    float x[8];
+    mx_values<F>(c, gld(a.powers + i / 4), x);
+    uint8_t* dst = a.x + EB * mx_at(a, i);
+    if constexpr (T == PG_F32) {
+      gst((gu32x4*)dst, *(gu32x4*)x);
+      gst((gu32x4*)dst + 1, *(gu32x4*)(x + 4));
+    } else {
+      const uint4 z = pg_pack8<T>(x);
+      gst((gu32x4*)dst, (gu32x4){z.x, z.y, z.z, z.w});
+    }
+  }
+}
+
+// ---- products ------------------------------------------------------------------------------
+// y[r][c] = sum over k of x[r][k] w[c][k], plus bias[c]: rows x microscaled in format F, the matrix w in mxf4.
+struct MxProduct {
+  const uint8_t *x, *xp, *w, *wp;   // codes and powers
+  const float* bias;                // null: none
+  void* y;
+  int64_t stride;                   // of y's rows, in elements
+  int32_t rows, cols, inner;        // inner: a multiple of 32
+  int32_t type, wide;               // of y; whether four neighbouring columns from a multiple of four on may be stored at once
+};
+
+__device__ __forceinline__ v4f mx_bias4(const MxProduct& p, int c) {
+  v4f b = {0.f, 0.f, 0.f, 0.f};
+  if (p.bias) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) b[i] = gld(p.bias + min(c + i, p.cols - 1));
+  }
+  return b;
+}
+// Columns c .. c + 3 of a row, those that there are.
+__device__ __forceinline__ void mx_store4(const MxProduct& p, int r, int c, v4f v) {
+  const int64_t at = r * p.stride + c;
+  if (p.type == PG_F32) {
+    float* y = (float*)p.y + at;
+    if (p.wide && c + 4 <= p.cols) gst((gu32x4*)y, __builtin_bit_cast(gu32x4, v));
+    else
+      for (int i = 0; i < 4; i++)
+        if (c + i < p.cols) gst(y + i, v[i]);
+    return;
+  }
+  const uint32_t a = p.type == PG_BF16 ? pg_pack2<PG_BF16>(v[0], v[1]) : pg_pack2<PG_F16>(v[0], v[1]);
+  const uint32_t b = p.type == PG_BF16 ? pg_pack2<PG_BF16>(v[2], v[3]) : pg_pack2<PG_F16>(v[2], v[3]);
+  uint16_t* y = (uint16_t*)p.y + at;
+  if (p.wide && c + 4 <= p.cols) gst((gu32x2*)y, (gu32x2){a, b});
+  else
+    for (int i = 0; i < 4; i++)
+      if (c + i < p.cols) gst(y + i, (uint16_t)((i < 2 ? a : b) >> 16 * (i & 1)));
+}
+
+// Eight codes as bf16 values: every power and code has an exact one (but below 2^-133 and above its range).
+template <int F>
+__device__ __forceinline__ uint4 mx_bf16(uint2 c, uint32_t byte) {
+  typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+  const float p = mx_power(byte);
+  v2bf y[4];
+  if constexpr (F == MX_F4) {
+    y[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c.x, p, 0);
+    y[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c.x, p, 1);
+    y[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c.x, p, 2);
+    y[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c.x, p, 3);
+  } else {
+    y[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c.x, p, false);
+    y[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c.x, p, true);
+    y[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c.y, p, false);
+    y[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c.y, p, true);
+  }
+  return __builtin_bit_cast(uint4, y);
+}
+
+// 32 codes of a lane, as a matrix instruction takes them.
+struct MxOperand {
+  uint4 lo, hi;   // mxf4: lo
+};
+template <int F>
+__device__ __forceinline__ v8i mx_operand(const MxOperand& o) {
+  if constexpr (F == MX_F4) return (v8i){(int)o.lo.x, (int)o.lo.y, (int)o.lo.z, (int)o.lo.w, 0, 0, 0, 0};
+  else return (v8i){(int)o.lo.x, (int)o.lo.y, (int)o.lo.z, (int)o.lo.w, (int)o.hi.x, (int)o.hi.y, (int)o.hi.z, (int)o.hi.w};
+}
+// Codes 8 i .. 8 i + 7 of them.
+template <int F, int I>
+__device__ __forceinline__ uint2 mx_eight(const MxOperand& o) {
+  const uint32_t v[8] = {o.lo.x, o.lo.y, o.lo.z, o.lo.w, o.hi.x, o.hi.y, o.hi.z, o.hi.w};
+  if constexpr (F == MX_F4) return {v[I], 0};
+  else return {v[2 * I], v[2 * I + 1]};
+}
+
+// The scaled matrix instructions multiply the codes and the powers exactly and add up in float32, but of codes that are not both e2m1 they
+// drop what lies far below the largest product of a group: normal values are off by 4e-6 (2-norm), codes of evenly spread exponents by
+// 5e-5, where rounding to f16 alone is 2e-4. So for 16-bit outputs mxf8 rows go to them as they are; for float32 outputs (FINE) both operands
+// become bf16 values, whose products and sums are float32's.
+template <int F, bool FINE>
+__device__ __forceinline__ v4f mx_mfma16(const MxOperand& w, uint32_t wp, const MxOperand& x, uint32_t xp, v4f c) {   // 16 x 16 x 128
+  if constexpr (!FINE) return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand<MX_F4>(w), mx_operand<F>(x), c, MX_F4, F, 0, wp, 0, xp);
+  pg_each<4>([&](auto i) {
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, mx_bf16<MX_F4>(mx_eight<MX_F4, i>(w), wp)),
+                                                __builtin_bit_cast(v8bf, mx_bf16<F>(mx_eight<F, i>(x), xp)), c, 0, 0, 0);
+  });
+  return c;
+}
+
+// Few rows, or an inner size that is no multiple of 128. A wave multiplies 16 columns by 16 R rows over its share of the inner size: 128 at a
+// time, straight from memory (a lane's 32 codes of a column are 16 bytes; of an mxf8 row 16 + 16, as the instruction divides them, or 32
+// together where they become bf16). KS waves share the inner size of the same columns and are joined in LDS, in their order.
+template <int F, bool FINE, int R, int KS>
+__global__ __launch_bounds__(256) void mx_few_kernel(MxProduct p, int tiles) {   // tiles: workgroups for the columns
+  constexpr int U = R == 4 ? 2 : 4;   // steps whose loads are in flight together
+  __shared__ __attribute__((aligned(16))) v4f part[KS > 1 ? 4 : 1][R][64];
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int row_tile = blockIdx.x / (uint32_t)tiles, tile = blockIdx.x - row_tile * tiles, r0 = 16 * R * row_tile, c0 = 16 * (KS == 1 ? tile * 4 + w : tile);
+  const int blocks = p.inner >> 5, steps = (blocks + 3) >> 2, each = (steps + KS - 1) / KS;
+  const int s0 = KS == 1 ? 0 : min(each * w, steps), s1 = KS == 1 ? steps : min(s0 + each, steps);
+  if (KS == 1 && c0 >= p.cols) return;
+  const int64_t wc = min(c0 + n, p.cols - 1);
+  const uint8_t *wr = p.w + wc * (p.inner / 2), *wpr = p.wp + wc * blocks;
+  const uint8_t *xr[R], *xpr[R];
+#pragma unroll
+  for (int i = 0; i < R; i++) {
+    const int64_t r = min(r0 + 16 * i + n, p.rows - 1);
+    xr[i] = p.x + r * mx_bytes<F>(p.inner);
+    xpr[i] = p.xp + r * blocks;
+  }
+  v4f acc[R] = {};
+  const uint4 none = {0, 0, 0, 0};
+  for (int s = s0; s < s1; s += U) {
+    MxOperand a[U], b[U][R];
+    uint32_t ap[U], bp[U][R];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int at = min(s + u, s1 - 1), block = 4 * at + g, first = min(block, blocks - 1);   // (blocks behind the last are not read)
+      a[u].lo = gld((const uint4*)(wr + 16 * first));
+      ap[u] = gld(wpr + first);
+#pragma unroll
+      for (int i = 0; i < R; i++) {
+        bp[u][i] = gld(xpr[i] + first);
+        if constexpr (F == MX_F4) {
+          b[u][i].lo = gld((const uint4*)(xr[i] + 16 * first));
+        } else if constexpr (FINE) {
+          b[u][i].lo = gld((const uint4*)(xr[i] + 32 * first));
+          b[u][i].hi = gld((const uint4*)(xr[i] + 32 * first + 16));
+        } else {
+          b[u][i].lo = gld((const uint4*)(xr[i] + 32 * min(4 * at + (g >> 1), blocks - 1) + 16 * (g & 1)));
+          b[u][i].hi = gld((const uint4*)(xr[i] + 32 * min(4 * at + 2 + (g >> 1), blocks - 1) + 16 * (g & 1)));
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      if (s + u >= s1) break;
+      if (4 * (s + u) + 4 > blocks) {   // zeros for the blocks behind the last
+        const int block = 4 * (s + u) + g;
+        if (block >= blocks) {
+          a[u].lo = none;
+          ap[u] = 127;
+        }
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+          const bool apart = F == MX_F8 && !FINE;
+          if (block >= blocks) bp[u][i] = 127;
+          if ((apart ? 4 * (s + u) + (g >> 1) : block) >= blocks) b[u][i].lo = none;
+          if ((apart ? 4 * (s + u) + 2 + (g >> 1) : block) >= blocks) b[u][i].hi = none;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < R; i++) acc[i] = mx_mfma16<F, FINE>(a[u], ap[u], b[u][i], bp[u][i], acc[i]);
+    }
+  }
+  if constexpr (KS > 1) {
+#pragma unroll
+    for (int i = 0; i < R; i++) part[w][i][lane] = acc[i];
+    __syncthreads();
+    for (int i = w; i < R; i += 4) {
+      v4f y = part[0][i][lane];
+#pragma unroll
+      for (int k = 1; k < KS; k++) y += part[k][i][lane];
+      const int r = r0 + 16 * i + n, c = c0 + 4 * g;
+      if (r < p.rows && c < p.cols) mx_store4(p, r, c, y + mx_bias4(p, c));
+    }
+  } else {
+    const int c = c0 + 4 * g;
+    if (c >= p.cols) return;
+    const v4f b = mx_bias4(p, c);
+#pragma unroll
+    for (int i = 0; i < R; i++)
+      if (r0 + 16 * i + n < p.rows) mx_store4(p, r0 + 16 * i + n, c, acc[i] + b);
+  }
+}

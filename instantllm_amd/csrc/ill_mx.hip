@@ -1,0 +1,90 @@
+// The microscaled operators (ill_mx_* in include/ill_hip.h): entry points and launches.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "ill_error.h"
+#include "ill_launch.h"
+#include "ill_mx.h"
+#include "ill_mx_check.h"
+
+namespace illm {
+namespace {
+
+using illp::launch;
+
+// The GPU that a stream belongs to; of the default streams the current one.
+int device_of(hipStream_t st, int* dev) {
+  if (!st || st == hipStreamLegacy || st == hipStreamPerThread) HCK(hipGetDevice(dev));
+  else HCK(hipStreamGetDevice(st, dev));
+  return ILL_OK;
+}
+
+template <int T, int F>
+hipError_t launch_rows(bool back, const MxRows& a, hipStream_t st) {
+  const int64_t blocks = std::min<int64_t>((a.items + 255ll) / 256, 1 << 16);
+  return back ? launch(mx_dequantize_kernel<T, F>, blocks, 256, 0, st, a) : launch(mx_quantize_kernel<T, F>, blocks, 256, 0, st, a);
+}
+template <int F>
+hipError_t launch_rows(bool back, int dtype, const MxRows& a, hipStream_t st) {
+  return dtype == ILL_F32 ? launch_rows<PG_F32, F>(back, a, st) : dtype == ILL_F16 ? launch_rows<PG_F16, F>(back, a, st) : launch_rows<PG_BF16, F>(back, a, st);
+}
+
+int rows(bool back, int format, int dtype, const void* x, int64_t stride, int64_t rows, int64_t cols, const void* codes, const void* powers, void* stream) {
+  if (int rc = check_rows(format, dtype, x, stride, rows, cols, codes, powers)) return rc;
+  if (!rows) return ILL_OK;
+  hipStream_t st = (hipStream_t)stream;
+  int dev = 0;
+  if (int rc = device_of(st, &dev)) return rc;
+  illp::OnDevice on(dev);
+  if (on.rc) return on.rc;
+  const MxRows a{(uint8_t*)x, (uint8_t*)codes, (uint8_t*)powers, stride, (uint32_t)(rows * cols / 8), (uint32_t)(cols / 8)};
+  HCK(format == ILL_MXF8 ? launch_rows<MX_F8>(back, dtype, a, st) : launch_rows<MX_F4>(back, dtype, a, st));
+  return ILL_OK;
+}
+
+template <int F, bool FINE, int R, int KS>
+hipError_t launch_few(const MxProduct& p, hipStream_t st) {
+  const int cols = KS == 1 ? 64 : 16, tiles = (p.cols + cols - 1) / cols;
+  return launch(mx_few_kernel<F, FINE, R, KS>, (int64_t)((p.rows + 16 * R - 1) / (16 * R)) * tiles, 256, 0, st, p, tiles);
+}
+template <int F, bool FINE>
+hipError_t launch_product(const MxProduct& p, hipStream_t st) {
+  const bool split = p.cols < 16 * 1024;
+  if (p.rows <= 16) return split ? launch_few<F, FINE, 1, 4>(p, st) : launch_few<F, FINE, 1, 1>(p, st);
+  if (p.rows <= 32) return split ? launch_few<F, FINE, 2, 4>(p, st) : launch_few<F, FINE, 2, 1>(p, st);
+  return split ? launch_few<F, FINE, 4, 4>(p, st) : launch_few<F, FINE, 4, 1>(p, st);
+}
+
+}  // namespace
+}  // namespace illm
+
+extern "C" {
+
+int ill_mx_quantize(int format, int dtype, const void* x, int64_t x_stride, int64_t rows, int64_t cols, void* codes, void* powers, void* stream) {
+  return illm::rows(false, format, dtype, x, x_stride, rows, cols, codes, powers, stream);
+}
+
+int ill_mx_dequantize(int format, int dtype, const void* codes, const void* powers, int64_t rows, int64_t cols, void* y, int64_t y_stride, void* stream) {
+  return illm::rows(true, format, dtype, y, y_stride, rows, cols, codes, powers, stream);
+}
+
+int ill_mx_product(int x_format, const void* x, const void* x_powers, const void* w, const void* w_powers, int64_t rows, int64_t cols, int64_t inner,
+                   const float* bias, int y_dtype, void* y, int64_t y_stride, void* stream) {
+  if (int rc = illm::check_product(x_format, x, x_powers, w, w_powers, bias, y, y_stride, y_dtype, rows, cols, inner)) return rc;
+  if (!rows) return ILL_OK;
+  hipStream_t st = (hipStream_t)stream;
+  int dev = 0;
+  if (int rc = illm::device_of(st, &dev)) return rc;
+  illp::OnDevice on(dev);
+  if (on.rc) return on.rc;
+  const bool wide = y_stride % 4 == 0 && illm::aligned(y, y_dtype == ILL_F32 ? 16 : 8);
+  const MxProduct p{(const uint8_t*)x, (const uint8_t*)x_powers, (const uint8_t*)w, (const uint8_t*)w_powers, bias, y, y_stride,
+                    (int)rows, (int)cols, (int)inner, y_dtype, wide};
+  if (x_format == ILL_MXF4) HCK((illm::launch_product<MX_F4, false>(p, st)));
+  else if (y_dtype == ILL_F32) HCK((illm::launch_product<MX_F8, true>(p, st)));
+  else HCK((illm::launch_product<MX_F8, false>(p, st)));
+  return ILL_OK;
+}
+
+}  // extern "C"

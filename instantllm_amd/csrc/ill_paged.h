@@ -7,44 +7,10 @@
 #include <type_traits>
 #include <utility>
 #include "ill_device.h"
+#include "ill_lds.h"
 #include "ill_paged_plan.h"
+#include "ill_values.h"
 
-enum PgType { PG_F32 = 0, PG_F16 = 1, PG_BF16 = 2 };   // ILL_F32, ILL_F16, ILL_BF16
-
-typedef float v16f __attribute__((ext_vector_type(16)));
-typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
-#define LAS __attribute__((address_space(3)))   // LDS: named, as GAS is, or an access counts as one to memory too
-
-// 16-bit values as floats, and back with one rounding to nearest, ties to even.
-template <int T>
-__device__ __forceinline__ void pg_unpack2(uint32_t w, float* x) {
-  if constexpr (T == PG_BF16) {
-    x[0] = __uint_as_float(w << 16);
-    x[1] = __uint_as_float(w & 0xFFFF0000u);
-  } else {
-    x[0] = (float)__builtin_bit_cast(_Float16, (uint16_t)w);
-    x[1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w >> 16));
-  }
-}
-template <int T>
-__device__ __forceinline__ void pg_unpack(const uint4* p, float* x) {   // eight values of type T
-  if constexpr (T == PG_F32) {
-    *(uint4*)x = p[0];
-    *(uint4*)(x + 4) = p[1];
-  } else {
-    const uint32_t w[4] = {p->x, p->y, p->z, p->w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) pg_unpack2<T>(w[i], x + 2 * i);
-  }
-}
-template <int T>
-__device__ __forceinline__ uint32_t pg_pack2(float a, float b) {   // (as a pair: one instruction)
-  typedef float v2f __attribute__((ext_vector_type(2)));
-  typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
-  typedef _Float16 v2h __attribute__((ext_vector_type(2)));
-  if constexpr (T == PG_BF16) return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){a, b}, v2bf));
-  else return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){a, b}, v2h));
-}
 // A pair of floats in parts of type T, each the rest of the one before: two parts of f16 keep 22 bits, three of bf16 24. Weights
 // go to the product with the values as such parts for float32 outputs. For 16-bit outputs they are rounded once, to the cache's
 // type: against float64 the outputs are then off by 0.0020 (8000 rows of 28 / 4 heads of 128, bf16), of which their own rounding alone is
@@ -61,10 +27,6 @@ __device__ __forceinline__ void pg_parts2(float a, float b, uint32_t* part) {
     a -= y[0];
     b -= y[1];
   }
-}
-template <int T>
-__device__ __forceinline__ uint4 pg_pack8(const float* x) {
-  return {pg_pack2<T>(x[0], x[1]), pg_pack2<T>(x[2], x[3]), pg_pack2<T>(x[4], x[5]), pg_pack2<T>(x[6], x[7])};
 }
 // ---- new rows into the cache -------------------------------------------------------------
 struct PgAppend {
@@ -435,35 +397,6 @@ __device__ __forceinline__ v4f pg_mfma16(uint4 a, uint4 b, v4f c) {   // 16 x 16
   if constexpr (TC == PG_BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
   else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
-
-// 16 bytes from base + each lane's offset into LDS, lane i's at lds + 16 i. In inline assembly, because the
-// compiler cannot tell the buffers apart and would wait for every load in flight before each LDS read;
-// the kernels wait themselves (PG_WAIT), and extra loads of the compiler's own only make that wait longer.
-// `base` may have been written by a vector instruction just before (v_readlane, also from a spill): a load may read it five
-// wait states later, which the compiler, not seeing the load, does not ensure.
-template <int AT>
-__device__ __forceinline__ void pg_dma16(const void* base, uint32_t off, uint32_t lds) {   // to lds + AT + 16 i; base and lds: the same for every lane
-  asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base), "n"(AT) : "memory", "scc", "m0");
-}
-__device__ __forceinline__ uint32_t pg_lds_at(const void* p) {   // an LDS address, as every lane's
-  return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const LAS uint8_t*)p);
-}
-// Calls f with the constants 0 .. N - 1.
-template <int N, class F>
-__device__ __forceinline__ void pg_each(F&& f) {
-  [&]<int... I>(std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }(std::make_integer_sequence<int, N>{});
-}
-// The compiler's own loads so far have arrived, and it knows it (else it would wait for them, and with them for every later
-// load of pg_dma16, where it first uses them inside a loop).
-#define PG_WAIT_OWN() __builtin_amdgcn_s_waitcnt(0x0F70)   // vmcnt(0)
-#define PG_WAIT(n) asm volatile("s_waitcnt vmcnt(" #n ")" ::: "memory")
-#define PG_TURN()                                                        \
-  do { /* a barrier that waits for no loads, and that no work moves over */ \
-    __builtin_amdgcn_sched_barrier(0);                                   \
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");      \
-    __builtin_amdgcn_sched_barrier(0);                                   \
-  } while (0)
-#define PG_WAIT_LDS() asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory")
 
 // Where the 16-byte unit u of key `key` of a tile lies in LDS, in units: a key's units in a row, permuted so that the
 // eight keys of an eighth of an operand read, and the 4 keys x 64 bytes of half a transposed read, are on different banks.

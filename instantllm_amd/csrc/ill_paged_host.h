@@ -1,6 +1,7 @@
 // Host side of the paged-cache operators: argument checks and launches (ill_paged_* in
 // include/ill_hip.h). Included by ill_engine.hip after its error helpers.
 #pragma once
+#include "ill_launch.h"
 #include "ill_paged.h"
 #include "ill_paged_check.h"
 #include "ill_paged_claims.h"
@@ -15,19 +16,6 @@ struct ill_paged {
 };
 
 namespace illp {
-
-// The current device is the handle's while this lives.
-struct OnDevice {
-  int was = -1, rc = ILL_OK;
-  explicit OnDevice(int dev) {
-    if (hipGetDevice(&was) != hipSuccess) rc = fail(ILL_E_HIP, "no HIP device");
-    else if (was != dev && hipSetDevice(dev) != hipSuccess) rc = fail(ILL_E_HIP, "device %d cannot be made current", dev);
-    if (was == dev || rc) was = -1;
-  }
-  ~OnDevice() {
-    if (was >= 0) hipSetDevice(was);
-  }
-};
 
 PgBatch batch_of(const ill_paged* p, const ill_paged_batch& b) {
   return {b.lens, b.table, b.row0, b.table_stride, b.pages, b.seqs, (int)b.rows, b.table_width, p->page_log};
@@ -75,13 +63,6 @@ int workspace(ill_paged* p, hipStream_t st, uint8_t** out) {
                 p->d.streams);
   *out = p->work + w * p->work_bytes;
   return ILL_OK;
-}
-
-// Enqueues a kernel and returns this launch's error (hipGetLastError may hold one of the program's own calls).
-template <class... P>
-hipError_t launch(void (*kernel)(P...), int64_t blocks, int threads, int lds, hipStream_t st, std::common_type_t<P>... args) {
-  void* p[] = {&args...};
-  return hipLaunchKernel((const void*)kernel, dim3(blocks), dim3(threads), p, lds, st);
 }
 
 // `steps`, `prompts`: workgroups of each kind.

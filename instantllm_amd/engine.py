@@ -123,6 +123,9 @@ def load_library(path: str | os.PathLike | None = None) -> C.CDLL:
         "ill_paged_release": (C.c_int, [P]),
         "ill_paged_append": (C.c_int, [P, P, P, P, P, P]),
         "ill_paged_attend": (C.c_int, [P, P, P, C.c_int64, P, P, C.c_int, C.c_int, P, C.c_int64, C.c_int, P]),
+        "ill_mx_quantize": (C.c_int, [C.c_int, C.c_int, P, C.c_int64, C.c_int64, C.c_int64, P, P, P]),
+        "ill_mx_dequantize": (C.c_int, [C.c_int, C.c_int, P, P, C.c_int64, C.c_int64, P, C.c_int64, P]),
+        "ill_mx_product": (C.c_int, [C.c_int, P, P, P, P, C.c_int64, C.c_int64, C.c_int64, P, C.c_int, P, C.c_int64, P]),
         "ill_quantize_q4": (C.c_int, [C.POINTER(F32), C.c_int64, C.c_int, C.POINTER(C.c_uint8), C.POINTER(C.c_uint16), C.c_int]),
         "ill_quantize_q8": (C.c_int, [C.POINTER(F32), C.c_int64, C.c_int, C.c_int, C.POINTER(C.c_int8), C.POINTER(C.c_uint16), C.c_int]),
         "ill_ildraft_open": (P, [C.c_char_p]),

@@ -17,6 +17,10 @@ template <int AT>
 __device__ __forceinline__ void pg_dma16(const void* base, uint32_t off, uint32_t lds) {   // to lds + AT + 16 i; base and lds: the same for every lane
   asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base), "n"(AT) : "memory", "scc", "m0");
 }
+template <int AT>
+__device__ __forceinline__ void pg_dma4(const void* base, uint32_t off, uint32_t lds) {   // four bytes of each lane, to lds + AT + 4 i
+  asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 3\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(off), "s"(base), "n"(AT) : "memory", "scc", "m0");
+}
 __device__ __forceinline__ uint32_t pg_lds_at(const void* p) {   // an LDS address, as every lane's
   return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const LAS uint8_t*)p);
 }

@@ -300,3 +300,133 @@ __global__ __launch_bounds__(256) void mx_few_kernel(MxProduct p, int tiles) {  
       if (r0 + 16 * i + n < p.rows) mx_store4(p, r0 + 16 * i + n, c, acc[i] + b);
   }
 }
+
+template <int F, bool FINE, class J>
+__device__ __forceinline__ v16f mx_mfma32(const MxOperand& w, uint32_t wp, const MxOperand& x, uint32_t xp, v16f c, J) {   // 32 x 32 x 64
+  constexpr int AT = 2 * J::value;   // the powers: this byte of each lane's word
+  if constexpr (!FINE) return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand<MX_F4>(w), mx_operand<F>(x), c, MX_F4, F, AT, wp, AT, xp);
+  pg_each<4>([&](auto i) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, mx_bf16<MX_F4>(mx_eight<MX_F4, i>(w), wp >> 8 * AT & 255)),
+                                                __builtin_bit_cast(v8bf, mx_bf16<F>(mx_eight<F, i>(x), xp >> 8 * AT & 255)), c, 0, 0, 0);
+  });
+  return c;
+}
+
+// Many rows, an inner size that is a multiple of 128. A workgroup of 2 x 2 waves computes a tile of 64 TC columns x 64 TR rows, a wave
+// TC x TR products of 32 x 32 x 64. 128 of the inner size are a stage: their codes and powers go straight into LDS, S - 1 stages ahead.
+// A stage's codes lie there as rows of 64 bytes, 16 bytes a unit (mxf8 rows twice, 64 codes each); a row's units are permuted so that the
+// 16 rows of a quarter of an operand read are on different banks.
+template <int F, int TC, int TR, int S>
+struct MxTile {
+  static constexpr int C = 64 * TC, R = 64 * TR, SLABS = F == MX_F8 ? 2 : 1;   // columns, rows; slabs of the rows' codes
+  static constexpr int X = 64 * C, WP = X + 64 * R * SLABS, XP = WP + 4 * C, STAGE = XP + 4 * R;   // where the rows, the powers are
+  static constexpr int LOADS = (TC + TR * SLABS) + (TC + TR + 3) / 4;          // of a wave and stage
+  static constexpr int LDS = S * STAGE;
+};
+__device__ __forceinline__ int mx_unit(int row, int unit) { return 16 * (4 * row + (unit ^ (row >> 2 & 3))); }
+
+template <int F, bool FINE, int TC, int TR, int S>
+__global__ __launch_bounds__(256, TC* TR > 8 ? 1 : 2) void mx_many_kernel(MxProduct p, int tiles_c, int tiles) {
+  using T = MxTile<F, TC, TR, S>;
+  __shared__ __attribute__((aligned(16))) uint8_t mx_lds[T::LDS];
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 31, g = lane >> 5;
+  // an XCD has every eighth workgroup: it takes neighbouring tiles, eight rows of tiles at a time down each column
+  const int per = (tiles + 7) / 8, at = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per || at >= tiles) return;
+  const int tiles_r = tiles / tiles_c, band = at / (8 * tiles_c), high = min(8, tiles_r - 8 * band), in = at - 8 * band * tiles_c;
+  const int r0 = (8 * band + in % high) * T::R, c0 = in / high * T::C;
+  const int stages = p.inner >> 7, blocks = p.inner >> 5;
+  const uint32_t wrow = p.inner / 2, xrow = mx_bytes<F>(p.inner);
+  // what this lane loads of 16 rows: 16 bytes, its row's unit that lies where the load puts the lane's
+  const int sub = lane >> 2, unit = (lane & 3) ^ (sub >> 2 & 3);
+  uint32_t woff[TC], xoff[TR];
+#pragma unroll
+  for (int i = 0; i < TC; i++) woff[i] = (uint32_t)(min(c0 + 16 * (4 * i + w) + sub, p.cols - 1) - c0) * wrow + 16 * unit;
+#pragma unroll
+  for (int i = 0; i < TR; i++) xoff[i] = (uint32_t)(min(r0 + 16 * (4 * i + w) + sub, p.rows - 1) - r0) * xrow + 16 * unit;
+  // and of 64 rows' powers: a word
+  constexpr int PL = (TC + TR + 3) / 4;
+  uint32_t poff[PL], pto[PL];
+  bool of_w[PL];
+#pragma unroll
+  for (int i = 0; i < PL; i++) {
+    const int u = min(4 * i + w, TC + TR - 1);   // (one group twice where they do not come out even)
+    of_w[i] = u < TC;
+    const int row = of_w[i] ? min(c0 + 64 * u + lane, p.cols - 1) - c0 : min(r0 + 64 * (u - TC) + lane, p.rows - 1) - r0;
+    poff[i] = (uint32_t)row * blocks;
+    pto[i] = 256 * u;
+  }
+  const uint8_t *wb = p.w + (int64_t)c0 * wrow, *xb = p.x + (int64_t)r0 * xrow, *wpb = p.wp + (int64_t)c0 * blocks, *xpb = p.xp + (int64_t)r0 * blocks;
+  const uint32_t lds = pg_lds_at(mx_lds);
+  auto load = [&](int k, int buffer) {   // stage k (behind the last: the last once more, which nobody reads)
+    k = min(k, stages - 1);
+    const uint32_t to = lds + buffer * T::STAGE + 1024 * w;
+    const uint8_t *wk = wb + 64 * k, *xk = xb + 64 * T::SLABS * k;
+    pg_each<TC>([&](auto i) { pg_dma16<4096 * i>(wk, woff[i], to); });
+    pg_each<T::SLABS>([&](auto s) {
+      pg_each<TR>([&](auto i) { pg_dma16<T::X + 64 * T::R * s + 4096 * i>(xk + 64 * s, xoff[i], to); });
+    });
+    pg_each<PL>([&](auto i) { pg_dma4<T::WP>((of_w[i] ? wpb : xpb) + 4 * k, poff[i], lds + buffer * T::STAGE + pto[i]); });
+  };
+  const int wc = w & 1, wr = w >> 1;   // the wave's place in the tile
+  // this lane's operands in a stage: unit 2 step + g of a column's 64 bytes; of an mxf8 row's slab `step` units g and 2 + g, or 2 g and 2 g + 1
+  int wa[2], xa[2];
+#pragma unroll
+  for (int j = 0; j < 2; j++) {
+    wa[j] = mx_unit(32 * TC * wc + n, 2 * j + g);
+    xa[j] = T::X + mx_unit(32 * TR * wr + n, F == MX_F4 ? 2 * j + g : FINE ? 2 * g + j : 2 * j + g);
+  }
+  v16f acc[TC][TR] = {};
+  PG_WAIT_OWN();
+#pragma unroll
+  for (int k = 0; k < S - 1; k++) load(k, k);
+  int buffer = 0;
+  for (int k = 0; k < stages; k++) {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * T::LOADS) : "memory");
+    __syncthreads();   // the stage is there, and every wave is done with the buffer filled next
+    load(k + S - 1, buffer == 0 ? S - 1 : buffer - 1);
+    const LAS uint8_t* b = (const LAS uint8_t*)mx_lds + buffer * T::STAGE;
+    uint32_t wp[TC], xp[TR];
+#pragma unroll
+    for (int i = 0; i < TC; i++) wp[i] = *(const LAS uint32_t*)(b + T::WP + 4 * (32 * (TC * wc + i) + n)) >> 8 * g;
+#pragma unroll
+    for (int i = 0; i < TR; i++) xp[i] = *(const LAS uint32_t*)(b + T::XP + 4 * (32 * (TR * wr + i) + n)) >> 8 * g;
+    pg_each<2>([&](auto j) {
+      MxOperand wo[TC], xo[TR];
+      auto get = [](const LAS uint8_t* q) {
+        const gu32x4 v = *(const LAS gu32x4*)q;
+        return uint4{v[0], v[1], v[2], v[3]};
+      };
+#pragma unroll
+      for (int i = 0; i < TC; i++) wo[i].lo = get(b + wa[j] + 2048 * i);
+#pragma unroll
+      for (int i = 0; i < TR; i++) {
+        if constexpr (F == MX_F4) {
+          xo[i].lo = get(b + xa[j] + 2048 * i);
+        } else {
+          xo[i].lo = get(b + xa[0] + 64 * T::R * j + 2048 * i);
+          xo[i].hi = get(b + xa[1] + 64 * T::R * j + 2048 * i);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < TC; c++)
+#pragma unroll
+        for (int r = 0; r < TR; r++) acc[c][r] = mx_mfma32<F, FINE>(wo[c], wp[c], xo[r], xp[r], acc[c][r], j);
+    });
+    buffer = buffer == S - 1 ? 0 : buffer + 1;
+  }
+  PG_WAIT(0);   // (loads behind the last stage)
+#pragma unroll
+  for (int c = 0; c < TC; c++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int col = c0 + 32 * (TC * wc + c) + 8 * i + 4 * g;
+      if (col >= p.cols) continue;
+      const v4f bias = mx_bias4(p, col);
+#pragma unroll
+      for (int r = 0; r < TR; r++) {
+        const int row = r0 + 32 * (TR * wr + r) + n;
+        if (row < p.rows) mx_store4(p, row, col, (v4f){acc[c][r][4 * i], acc[c][r][4 * i + 1], acc[c][r][4 * i + 2], acc[c][r][4 * i + 3]} + bias);
+      }
+    }
+}

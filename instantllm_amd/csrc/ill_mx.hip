@@ -48,8 +48,18 @@ hipError_t launch_few(const MxProduct& p, hipStream_t st) {
   const int cols = KS == 1 ? 64 : 16, tiles = (p.cols + cols - 1) / cols;
   return launch(mx_few_kernel<F, FINE, R, KS>, (int64_t)((p.rows + 16 * R - 1) / (16 * R)) * tiles, 256, 0, st, p, tiles);
 }
+template <int F, bool FINE, int TC, int TR, int S>
+hipError_t launch_many(const MxProduct& p, hipStream_t st) {
+  using T = MxTile<F, TC, TR, S>;
+  const int tiles_c = (p.cols + T::C - 1) / T::C, tiles = tiles_c * ((p.rows + T::R - 1) / T::R);
+  return launch(mx_many_kernel<F, FINE, TC, TR, S>, (tiles + 7) / 8 * 8ll, 256, 0, st, p, tiles_c, tiles);
+}
 template <int F, bool FINE>
 hipError_t launch_product(const MxProduct& p, hipStream_t st) {
+  if (p.rows > 64 && p.inner % 128 == 0) {
+    if (!FINE && (int64_t)p.rows * p.cols >= 1 << 23) return launch_many<F, FINE, 4, 4, 3>(p, st);
+    return launch_many<F, FINE, 2, 2, 3>(p, st);
+  }
   const bool split = p.cols < 16 * 1024;
   if (p.rows <= 16) return split ? launch_few<F, FINE, 1, 4>(p, st) : launch_few<F, FINE, 1, 1>(p, st);
   if (p.rows <= 32) return split ? launch_few<F, FINE, 2, 4>(p, st) : launch_few<F, FINE, 2, 1>(p, st);

@@ -306,7 +306,7 @@ ILL_API int ill_gemv_destroy(ill_gemv* g);
  * are free; called when nothing that came on the stream will run any more, also before a
  * stream is destroyed (a later one may get its address). ill_paged_release does so for all
  * streams. */
-enum { ILL_F32 = 0, ILL_F16 = 1, ILL_BF16 = 2 };
+enum { ILL_F32 = 0, ILL_F16 = 1, ILL_BF16 = 2, ILL_MXF8 = 8, ILL_MXF4 = 16 };
 typedef struct ill_paged ill_paged;
 typedef struct {
   int32_t dtype, heads, kv_heads, head_dim, page_size, rotary_dim, interleaved, streams;
@@ -372,6 +372,13 @@ ILL_API int ill_paged_append(ill_paged* p, const ill_paged_batch* batch, const i
 ILL_API int ill_paged_attend(ill_paged* p, const ill_paged_batch* batch, const void* q, int64_t q_stride, const void* k_cache,
                              const void* v_cache, int window, int sinks, void* out, int64_t out_stride, int out_dtype, void* stream);
 
+/* The batch's rows out of the cache, where ill_paged_append would put them: keys to k, values to v, rows of kv_heads x head_dim
+ * values, row r at r * stride, of type out_dtype (the handle's, or ILL_F32), as the cache holds them. With row0 over all of a sequence's
+ * positions that is the whole sequence. Zeros for a row without a place in the cache; rows that are no sequence's are left alone.
+ * k and v are aligned to 16 bytes, strides multiples of 8 elements (float32: 4); they overlap nothing else that the call reads or writes. */
+ILL_API int ill_paged_read(ill_paged* p, const ill_paged_batch* batch, const void* k_cache, const void* v_cache, void* k, int64_t k_stride,
+                           void* v, int64_t v_stride, int out_dtype, void* stream);
+
 /* ---- Microscaled rows: quantisation and products for batches (no counterpart in the reference) ----
  * A microscaled row is blocks of 32 values that share a power of two. A block's byte e stands for 2^(e - 127), 255
  * for a block of NaN. Codes are e4m3 (ILL_MXF8: one byte, up to 448) or e2m1 (ILL_MXF4: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their
@@ -384,7 +391,6 @@ ILL_API int ill_paged_attend(ill_paged* p, const ill_paged_batch* batch, const v
  * bytes). A block's power is floor(log2(the largest size in it)) - 8 (ILL_MXF4: - 2), at least 2^-127; its values divided by it
  * are rounded to nearest, ties to even, and end at +-448 (+-6). A block that holds an infinity or NaN becomes NaN (codes 0).
  * ill_mx_dequantize: the values, rounded to `dtype` where they have no exact place in it. Up to 2^34 values a call. */
-enum { ILL_MXF8 = 8, ILL_MXF4 = 16 };
 ILL_API int ill_mx_quantize(int format, int dtype, const void* x, int64_t x_stride, int64_t rows, int64_t cols, void* codes, void* powers, void* stream);
 ILL_API int ill_mx_dequantize(int format, int dtype, const void* codes, const void* powers, int64_t rows, int64_t cols, void* y, int64_t y_stride,
                               void* stream);

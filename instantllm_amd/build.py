@@ -14,7 +14,7 @@ from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
-SRCS = [HERE / "csrc" / f"{name}.hip" for name in ("ill_engine", "ill_mx")]
+SRCS = [HERE / "csrc" / f"{name}.hip" for name in ("ill_engine", "ill_mx", "ill_paged_mx")]
 OUT = HERE / "libillhip.so"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 

@@ -3,11 +3,16 @@
 // A cache is two arrays of pages of 2^page_log positions, keys and values; position t of sequence
 // s is slot t % page_size of page table[s][t / page_size]. A batch's new rows are the last ones
 // of their sequences. Page numbers outside 0 .. pages - 1 are never followed.
+//
+// MX: a cache of microscaled e4m3 codes. A page holds [kv heads][page size][D] codes and, `powers_at` bytes on, [kv heads][page size][D / 32]
+// powers, so that neighbouring positions of a head are neighbours in memory; page_stride is in bytes. TC is then the
+// type that keys and values are multiplied in, the queries'.
 #pragma once
 #include <type_traits>
 #include <utility>
 #include "ill_device.h"
 #include "ill_lds.h"
+#include "ill_mx_codes.h"
 #include "ill_paged_plan.h"
 #include "ill_values.h"
 
@@ -40,6 +45,7 @@ struct PgAppend {
   const int32_t* positions;                         // null: the positions in the sequence
   int32_t heads, kv, rot, interleaved;
   float eps;
+  int64_t powers_at;   // MX
 };
 
 // The sequence of new row r: the last one whose first row is at most r. One wave; every lane
@@ -77,7 +83,7 @@ __device__ __forceinline__ void pg_floats8(const float* p, float* y) {
 // first values are on their way while the rows' places and angles are found, the next ones while it
 // computes. One row waits for three loads one after the other (a kernel of 3.5 us), many rows for memory: 343 MB of
 // bf16 heads of 128 in 73 us, 4.7 TB/s, where a large copy reaches 5.1.
-template <int TX, int TC, int D>
+template <int TX, int TC, int D, bool MX = false>
 __global__ __launch_bounds__(256) void pg_append_kernel(PgAppend a, int R) {
   extern __shared__ __attribute__((aligned(16))) uint8_t pg_lds[];
   constexpr int C = D / 16, EB = TX == PG_F32 ? 4 : 2;   // threads of a head; bytes of a value
@@ -85,6 +91,7 @@ __global__ __launch_bounds__(256) void pg_append_kernel(PgAppend a, int R) {
   int64_t* place = (int64_t*)pg_lds;             // [R] element offset of the row's slot; -1: no sequence's row; -2: it has no place
   int* angle_of = (int*)(place + R);             // [R] position that turns the row
   float2* cs = (float2*)(angle_of + (R + 1) / 2 * 2);   // [R][half]
+  int* slot_of = (int*)(cs + R * half);                 // MX: [R]
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, first = blockIdx.x * R;
   const int h0 = a.q ? 0 : a.heads, nh = a.heads + 2 * a.kv - h0, items = R * nh * C;
   struct Item {
@@ -120,7 +127,7 @@ __global__ __launch_bounds__(256) void pg_append_kernel(PgAppend a, int R) {
   for (int i = w; i < R; i += 4) {
     const int r = first + i;
     int64_t off = -1;
-    int at = 0;
+    int at = 0, slot = 0;
     const int s = r >= a.b.rows ? -1 : a.b.row0 ? pg_seq_of(a.b, r, lane) : r;
     if (s >= 0 && s < a.b.seqs) {
       const PgSeq q = pg_seq_at(a.b, s);
@@ -129,10 +136,12 @@ __global__ __launch_bounds__(256) void pg_append_kernel(PgAppend a, int R) {
       off = -2;   // (a row without a place in the cache: its query is turned all the same)
       if (t >= 0 && t < pg_cap(a.b)) {
         const int page = gld(a.b.table + s * a.b.table_stride + (t >> a.b.page_log));
-        if (page >= 0 && page < a.b.pages) off = page * a.page_stride + (t & ((1 << a.b.page_log) - 1)) * a.slot_stride;
+        slot = t & ((1 << a.b.page_log) - 1);
+        if (page >= 0 && page < a.b.pages) off = page * a.page_stride + (MX ? 0 : slot * a.slot_stride);
       }
     }
     if (lane == 0) {
+      if constexpr (MX) slot_of[i] = slot;
       place[i] = off;
       angle_of[i] = at;
     }
@@ -209,12 +218,116 @@ __global__ __launch_bounds__(256) void pg_append_kernel(PgAppend a, int R) {
         }
       }
     }
+    if constexpr (MX) {
+      if (y.kind > 0) {
+        // the largest size of each of the head's blocks, over its lanes: each run of eight is part of one block
+        uint32_t most[2] = {0, 0}, byte[D / 32];
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int n = 0; n < 8; n++) most[u] = max(most[u], __float_as_uint(v[u][n]) & 0x7FFFFFFFu);
+#pragma unroll
+        for (int b = 0; b < D / 32; b++) {
+          uint32_t m = max(y.d[0] >> 5 == b ? most[0] : 0, y.d[1] >> 5 == b ? most[1] : 0);
+#pragma unroll
+          for (int i = 1; i < C; i <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, i));
+          byte[b] = mx_power_of<MX_F8>(m);
+        }
+        uint8_t* page = (y.kind == 1 ? a.kc : a.vc) + at;
+        const int row = (y.hk << a.b.page_log) + slot_of[y.i];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          uint32_t own = byte[0];
+#pragma unroll
+          for (int b = 1; b < D / 32; b++) own = y.d[u] >> 5 == b ? byte[b] : own;
+          const uint2 z = mx_codes<MX_F8>(v[u], own);
+          gst((gu32x2*)(page + row * D + y.d[u]), (gu32x2){z.x, z.y});
+        }
+        if ((it & (C - 1)) == 0) {
+          uint8_t* powers = page + a.powers_at + row * (D / 32);
+          if constexpr (D == 64) gst((uint16_t*)powers, (uint16_t)(byte[0] | byte[1] << 8));
+          else gst((uint32_t*)powers, byte[0] | byte[1] << 8 | byte[2] << 16 | byte[D / 32 - 1] << 24);
+        }
+        continue;
+      }
+    }
     uint16_t* dst = y.kind == 0 ? (uint16_t*)a.qo + y.r * a.qos + (int64_t)y.hk * D
                                 : (uint16_t*)(y.kind == 1 ? a.kc : a.vc) + at + y.hk * a.head_stride;
 #pragma unroll
     for (int u = 0; u < 2; u++) {
       const uint4 z = pg_pack8<TC>(v[u]);
       gst((gu32x4*)(dst + y.d[u]), (gu32x4){z.x, z.y, z.z, z.w});
+    }
+  }
+}
+
+// ---- rows out of the cache -----------------------------------------------------------------
+struct PgRead {
+  PgBatch b;
+  const uint8_t *kc, *vc;
+  void *k, *v;
+  int64_t ks, vs;                                           // row strides in elements
+  int64_t page_stride, slot_stride, head_stride, powers_at;   // as PgAppend's
+  int32_t kv;
+};
+
+// The batch's rows as append would place them: their keys and values as the cache holds them, zeros where a row has no place. A workgroup
+// takes R rows, a thread eight values at a time, neighbours the same row's.
+template <int TO, int TC, bool MX, int D>
+__global__ __launch_bounds__(256) void pg_read_kernel(PgRead a, int R) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t pg_lds[];
+  int64_t* place = (int64_t*)pg_lds;   // [R] offset of the row's slot (MX: of its page); -1: no sequence's row; -2: it has no place
+  int* slot_of = (int*)(place + R);    // [R]
+  const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, first = blockIdx.x * R;
+  for (int i = w; i < R; i += 4) {
+    const int r = first + i;
+    int64_t off = -1;
+    int slot = 0;
+    const int s = r >= a.b.rows ? -1 : a.b.row0 ? pg_seq_of(a.b, r, lane) : r;
+    if (s >= 0 && s < a.b.seqs) {
+      const PgSeq q = pg_seq_at(a.b, s);
+      const int t = q.p0 + (r - q.first);
+      off = -2;
+      if (t >= 0 && t < pg_cap(a.b)) {
+        const int page = gld(a.b.table + s * a.b.table_stride + (t >> a.b.page_log));
+        slot = t & ((1 << a.b.page_log) - 1);
+        if (page >= 0 && page < a.b.pages) off = page * a.page_stride + (MX ? 0 : slot * a.slot_stride);
+      }
+    }
+    if (lane == 0) {
+      place[i] = off;
+      slot_of[i] = slot;
+    }
+  }
+  __syncthreads();
+  constexpr int C = D / 8;
+  const uint32_t each = 2 * a.kv * C;   // of a row: keys, then values
+  for (uint32_t it = tid; it < R * each; it += 256) {
+    const uint32_t i = it / each, x = it - i * each, head = x / C, d = 8 * (x - head * C);   // (of both, keys' heads first)
+    const int64_t at = place[i];
+    if (at == -1) continue;
+    const bool value = head >= (uint32_t)a.kv;
+    const int h = head - (value ? a.kv : 0);
+    const uint8_t* cache = value ? a.vc : a.kc;
+    float y[8] = {};
+    uint4 raw = {0, 0, 0, 0};
+    if (at >= 0) {
+      if constexpr (MX) {
+        const int row = (h << a.b.page_log) + slot_of[i];
+        mx_values<MX_F8>(gld((const uint2*)(cache + at + row * D + d)), gld(cache + at + a.powers_at + row * (D / 32) + (d >> 5)), y);
+      } else {
+        raw = gld((const uint4*)((const uint16_t*)cache + at + h * a.head_stride + d));
+        pg_unpack<TC>(&raw, y);
+      }
+    }
+    const int64_t to = (int64_t)(first + i) * (value ? a.vs : a.ks) + h * D + d;
+    void* out = value ? a.v : a.k;
+    if constexpr (TO == PG_F32) {
+      gst((gu32x4*)((float*)out + to), (gu32x4){__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3])});
+      gst((gu32x4*)((float*)out + to + 4), (gu32x4){__float_as_uint(y[4]), __float_as_uint(y[5]), __float_as_uint(y[6]), __float_as_uint(y[7])});
+    } else {
+      const uint4 z = MX ? pg_pack8<TO>(y) : raw;   // (a 16-bit cache's values in its own type: as they are)
+      gst((gu32x4*)((uint16_t*)out + to), (gu32x4){z.x, z.y, z.z, z.w});
     }
   }
 }
@@ -228,6 +341,7 @@ struct PgAttend {
   int64_t page_stride, slot_stride, head_stride;
   int32_t heads, kv, window, sinks, out_f32;
   float scale;
+  int64_t powers_at;   // MX
 };
 
 // What the unit of work u is: a part of the keys for a tile of rows of one key/value head.
@@ -671,7 +785,7 @@ struct PgStepLds {
   int last;
   PgFinder::Lds found;
 };
-template <int TC, int D, bool FINE>   // FINE: weights in parts that keep float32 (float32 outputs)
+template <int TC, int D, bool FINE, bool MX>   // FINE: weights in parts that keep float32 (float32 outputs)
 __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, PgStepLds& shared) {
   constexpr int NW = PG_WAVES, KT = D == 64 ? 64 : 32, UPR = D / 8, KPI = 64 / UPR, NB = KT / 16, KS = D / 32, ND = D / 16, NS = KT / 32, NG = KT / 16;
   constexpr int N = FINE ? PG_PARTS<TC> : 1;   // parts of a weight
@@ -722,7 +836,7 @@ __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, Pg
   const int end = min(p1 + 1, cap);
   uint4 qf[KS];
 #pragma unroll
-  for (int ks = 0; ks < KS; ks++) qf[ks] = gld((const uint4*)(a.q + row * a.qs + (int64_t)head * D + 32 * ks + 8 * kg));
+  for (int ks = 0; ks < KS; ks++) qf[ks] = gld((const uint4*)(a.q + row * a.qs + (int64_t)head * D + (MX ? 64 * (ks >> 1) + 16 * kg + 8 * (ks & 1) : 32 * ks + 8 * kg)));
   const int mine = c0 + w < c1 ? (c1 - c0 - w + NW - 1) / NW : 0;   // this wave's tiles
   // where the keys of the wave's next 64 / NG tiles are, 16 of them a lane: elements from the cache's begin; -1: not there
   int64_t group = -1;
@@ -732,7 +846,7 @@ __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, Pg
     if (t < c1) {
       const int g = pg_key_tile(range, t) * KT + 16 * (lane % NG), key = min(g, end - 1);
       const int page = gld(a.b.table + un.s * a.b.table_stride + (key >> a.b.page_log));
-      if (page >= 0 && page < a.b.pages) group = page * a.page_stride + (g & pmask) * a.slot_stride + un.head * a.head_stride;
+      if (page >= 0 && page < a.b.pages) group = page * a.page_stride + (MX ? 0 : (g & pmask) * a.slot_stride + un.head * a.head_stride);
     }
   };
   auto group_at = [&](int k, int g) {   // (the same for every lane)
@@ -750,6 +864,55 @@ __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, Pg
       });
     });
   };
+  // MX: a tile's codes and powers come through registers, the next tile's as soon as this one's have been used. A lane's keys are its score
+  // products' (16 dims of 64 at a time: the products' dims are dealt the same way to queries and keys), its values any 16 bytes.
+  uint4 kreg[NB][D / 64], vreg[4];
+  uint32_t kpow[NB], vpow[4];
+  auto mx_page = [&](int k, int g) {   // the page of a group of the wave's tile k (behind the last: the first one, which is there)
+    const int64_t at = group_at(k, g);
+    return k < mine && at > 0 ? at : 0;
+  };
+  auto mx_slot = [&](int k, int g) {   // where in its page: keys from the page's begin, of all heads
+    return (un.head << a.b.page_log) + (k < mine ? (pg_key_tile(range, c0 + w + NW * k) * KT + 16 * g) & pmask : 0);
+  };
+  auto mx_keys = [&](int k) {
+    const uint8_t* cache = (const uint8_t*)a.kc;
+    pg_each<NB / 2>([&](auto i) {
+      const int64_t p0 = mx_page(k, 2 * i), p1 = mx_page(k, 2 * i + 1);
+      const uint8_t* page = cache + (n & 8 ? p1 : p0);
+      const int first = n & 8 ? mx_slot(k, 2 * i + 1) : mx_slot(k, 2 * i);
+#pragma unroll
+      for (int odd = 0; odd < 2; odd++) {
+        const int b = 2 * i + odd, row = first + ((8 * (n >> 2) + 4 * odd + (n & 3)) & 15);
+#pragma unroll
+        for (int j = 0; j < D / 64; j++) kreg[b][j] = gld((const uint4*)(page + row * D + 64 * j + 16 * kg));
+        if constexpr (D == 64) kpow[b] = gld(page + a.powers_at + 2 * row + (kg >> 1));
+        else kpow[b] = gld((const uint32_t*)(page + a.powers_at + 4 * row)) >> 8 * (kg >> 1);   // bytes 0 and 2
+      }
+    });
+  };
+  constexpr int VL = 16 * D / 1024, LPK = D / 16;   // loads of a group's values; lanes of a key
+  auto mx_vals = [&](int k) {
+    pg_each<NG>([&](auto g) {
+      const uint8_t* page = (const uint8_t*)a.vc + mx_page(k, g);
+      const int first = mx_slot(k, g);
+#pragma unroll
+      for (int j = 0; j < VL; j++) {
+        const int row = first + 64 / LPK * j + lane / LPK;
+        vreg[VL * g + j] = gld((const uint4*)(page + row * D + 16 * (lane % LPK)));
+        vpow[VL * g + j] = gld(page + a.powers_at + (D / 32) * row + (lane % LPK >> 1));
+      }
+    });
+  };
+  auto mx_put = [&] {   // the values into LDS, as the other caches' come there
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int key = 64 / LPK * i + lane / LPK, u = 2 * (lane % LPK);
+      const uint4 lo = mx_16<TC, MX_F8>({vreg[i].x, vreg[i].y}, vpow[i]), hi = mx_16<TC, MX_F8>({vreg[i].z, vreg[i].w}, vpow[i]);
+      *(pg_lds4*)(vl + 16 * pg_unit_at<D>(key, u)) = (gu32x4){lo.x, lo.y, lo.z, lo.w};
+      *(pg_lds4*)(vl + 16 * pg_unit_at<D>(key, u + 1)) = (gu32x4){hi.x, hi.y, hi.z, hi.w};
+    }
+  };
   float Mx, Ls;   // Ls: this lane's keys only
   v4f O[ND];
   for (bool careful = false;; careful = true) {   // (twice only for infinities and NaN, pg_any_wild)
@@ -759,7 +922,10 @@ __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, Pg
     for (int d = 0; d < ND; d++) O[d] = (v4f){0.f, 0.f, 0.f, 0.f};
     groups(0);
     PG_WAIT_OWN();
-    if (mine > 0) {
+    if constexpr (MX) {
+      mx_keys(0);
+      mx_vals(0);
+    } else if (mine > 0) {
       load(a.kc, KEYS, 0);
       load(a.vc, VALUES, 0);
     }
@@ -769,18 +935,32 @@ __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, Pg
       int good = 0;   // groups of 16 keys whose pages are there
 #pragma unroll
       for (int g = 0; g < NG; g++) good |= (__builtin_amdgcn_readlane((int)(group >> 32), (k * NG + g) & 63) >= 0) << g;
-      PG_WAIT(8);   // the keys; the 8 loads after them are the values
+      if constexpr (!MX) PG_WAIT(8);   // the keys; the 8 loads after them are the values
       v4f s[NB];
 #pragma unroll
       for (int b = 0; b < NB; b++) {
         s[b] = (v4f){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++) s[b] = pg_mfma16<TC>(pg_get(kl + ka[ks] + (32 * (b >> 1) + 4 * (b & 1)) * 2 * D), qf[ks], s[b]);
+        for (int ks = 0; ks < KS; ks++) {
+          if constexpr (MX) {
+            const uint4 c = kreg[b][ks / 2];
+            s[b] = pg_mfma16<TC>(mx_16<TC, MX_F8>(ks & 1 ? uint2{c.z, c.w} : uint2{c.x, c.y}, kpow[b] >> 16 * (ks / 2) & 255), qf[ks], s[b]);
+          } else {
+            s[b] = pg_mfma16<TC>(pg_get(kl + ka[ks] + (32 * (b >> 1) + 4 * (b & 1)) * 2 * D), qf[ks], s[b]);
+          }
+        }
       }
-      PG_WAIT_LDS();   // the keys have been read
-      if (more) {
+      if constexpr (MX) {
+        mx_put();   // (before the groups: these are this tile's)
         if (((k + 1) & (64 / NG - 1)) == 0) groups(k + 1);
-        load(a.kc, KEYS, k + 1);
+        mx_keys(k + 1);
+        mx_vals(k + 1);
+      } else {
+        PG_WAIT_LDS();   // the keys have been read
+        if (more) {
+          if (((k + 1) & (64 / NG - 1)) == 0) groups(k + 1);
+          load(a.kc, KEYS, k + 1);
+        }
       }
       // every row sees the whole tile, or the rows' masks (wave-uniform)
       const bool whole = good == (1 << NG) - 1 && kt + KT - 1 <= p0 && kt + KT <= end && (c.window == 0 || kt > p1 - c.window || kt + KT <= c.sinks);
@@ -830,8 +1010,10 @@ __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, Pg
           for (int i = 0; i < N; i++) ph[i][b >> 1][2 * (b & 1) + r / 2] = x[i];
         }
       }
-      if (more) PG_WAIT(8);   // the values; the 8 loads after them are the next keys
-      else PG_WAIT(0);
+      if constexpr (!MX) {
+        if (more) PG_WAIT(8);   // the values; the 8 loads after them are the next keys
+        else PG_WAIT(0);
+      }
       bool wild = false;
       if (!whole || careful) wild = pg_wild_tile<TC, KT * UPR>(vl, lane);   // what a row does not see must not reach it as 0 x inf
       if (wild) {
@@ -859,8 +1041,10 @@ __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, Pg
             for (int i = 0; i < N; i++) O[d] = pg_mfma16<TC>(v, __builtin_bit_cast(uint4, ph[i][t]), O[d]);
           }
       }
-      PG_WAIT_LDS();   // the values have been read
-      if (more) load(a.vc, VALUES, k + 1);
+      if constexpr (!MX) {
+        PG_WAIT_LDS();   // the values have been read
+        if (more) load(a.vc, VALUES, k + 1);
+      }
     }
     if (careful || !pg_any_wild<ND>(O)) break;
   }
@@ -914,16 +1098,18 @@ __device__ __forceinline__ v16f pg_mfma32(uint4 a, uint4 b, v16f c) {   // 32 x 
 // products: 4096 rows of 14 / 2 heads in a window of 1024 take 35 to 37 us, 0.41 to 0.43 PFLOP/s. By the counters vector
 // instructions take 13 and the matrix units 7 us of it: a wave's scores, exponentials and weighted values follow each other, and
 // the one other wave of a SIMD does not fill its waits. Heads of 128 use all 256 registers and spill 19 outside the loop over tiles.
-template <int D>
+template <int D, bool MX>
 struct PgPromptLds {
-  __attribute__((aligned(16))) uint4 lds[2][2][8 * D];   // [buffer][keys, values]
+  static constexpr int BUFFERS = MX ? 1 : 2;
+  __attribute__((aligned(16))) uint4 lds[BUFFERS][2][8 * D];   // [buffer][keys, values]
+  __attribute__((aligned(16))) uint8_t raw[MX ? 2 * (64 * D + 1024) : 16];   // MX: keys and values, each codes [64][D], then the powers of 16 keys in 256 bytes
   int last, tamed, wild;   // tamed: 1 + the last tile whose values were changed; wild: a wave has infinite sums or NaN
   PgFinder::Lds found;
 };
-template <int TC, int D, bool FINE>   // FINE: weights in parts that keep float32 (float32 outputs)
-__device__ __forceinline__ void pg_prompt(const PgStep& p, int block, int grid, PgPromptLds<D>& shared) {
+template <int TC, int D, bool FINE, bool MX>   // FINE: weights in parts that keep float32 (float32 outputs)
+__device__ __forceinline__ void pg_prompt(const PgStep& p, int block, int grid, PgPromptLds<D, MX>& shared) {
   constexpr int N = FINE ? PG_PARTS<TC> : 1;   // parts of a weight
-  constexpr int M = 128, KT = 64, UPR = D / 8, KS = D / 16, ND = D / 32, T = KT * UPR, LOADS = T / PG_THREADS;   // LOADS: of keys, and of values, per wave and tile
+  constexpr int M = 128, KT = 64, UPR = D / 8, KS = D / 16, ND = D / 32, T = KT * UPR, LOADS = MX ? D / 64 + 1 : T / PG_THREADS;   // LOADS: of keys, and of values, per wave and tile
   auto& lds = shared.lds;
   int& tamed = shared.tamed;
   const PgAttend& a = p.a;
@@ -947,8 +1133,9 @@ __device__ __forceinline__ void pg_prompt(const PgStep& p, int block, int grid, 
     lane_off[i] = 2 * ((uint32_t)(key & 15) * (uint32_t)a.slot_stride + 8 * ((lane % UPR) ^ pg_swz<D>(key)));
   }
   static_assert(M == 32 * PG_WAVES && KT == 16 * PG_WAVES, "a wave has 32 rows, and loads 16 keys");
-  static_assert(LOADS == 2 || LOADS == 4, "two or four keys x 16 bytes x lanes");
-  const uint32_t mine_lds = pg_lds_at(&lds[0][0][64 * LOADS * w]);
+  static_assert(MX || LOADS == 2 || LOADS == 4, "two or four keys x 16 bytes x lanes");
+  constexpr int RAW = 64 * D + 1024;   // MX: bytes of a tile's keys, or values
+  const uint32_t mine_lds = MX ? pg_lds_at(shared.raw) : pg_lds_at(&lds[0][0][64 * LOADS * w]);
   // this lane's operands in a tile: of the keys for each 16 dims, of the values for each 32 and for even and odd 16 keys;
   // others are whole multiples of 32 rows further
   int ka[KS], va[ND][2];
@@ -975,8 +1162,9 @@ __device__ __forceinline__ void pg_prompt(const PgStep& p, int block, int grid, 
   // where the 16 keys from `key` on are: elements from the cache's begin; -1: not there
   auto place = [&](int key) -> int64_t {
     const int page = gld(a.b.table + un.s * a.b.table_stride + (min(key, end - 1) >> a.b.page_log));
-    return page >= 0 && page < a.b.pages ? page * a.page_stride + (key & pmask) * a.slot_stride + un.head * a.head_stride : -1;
+    return page >= 0 && page < a.b.pages ? page * a.page_stride + (MX ? 0 : (key & pmask) * a.slot_stride + un.head * a.head_stride) : -1;
   };
+  auto mx_slot = [&](int key) { return (un.head << a.b.page_log) + (key & pmask); };   // MX: a key's place among all of its page
   int all_hi = min(p0 + 1, end) - KT;
   const int all_lo = c.window ? p1 - c.window : -1, mine_hi = min(w0 + 1, wend) - KT, mine_lo = c.window ? w1 - c.window : -1;
   int64_t group = -1;   // of the next 16 tiles, 16 keys a lane
@@ -990,17 +1178,30 @@ __device__ __forceinline__ void pg_prompt(const PgStep& p, int block, int grid, 
   // Loads of a tile, 2 x LOADS of them, one at a time between the products of the tile before: together, right behind the
   // barrier, they held every wave up for 900 cycles (D 128), a quarter of a tile. A tile behind the last is the first page.
   const uint16_t *next_k, *next_v;
+  int64_t next_powers;   // MX: bytes from the codes to their powers
   auto next = [&](int k) {
     const int at = (4 * k + w) & 63;
     const int64_t e = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)group, at) |
                                 (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(group >> 32), at) << 32);
     const int64_t off = k < count && e > 0 ? e : 0;   // (where there is none, the first page is loaded, and masked)
-    next_k = a.kc + off;
-    next_v = a.vc + off;
+    if constexpr (MX) {
+      const int slot = mx_slot(k < count ? pg_key_tile(range, c0 + k) * KT + 16 * w : 0);
+      next_k = (const uint16_t*)((const uint8_t*)a.kc + off + slot * D);
+      next_v = (const uint16_t*)((const uint8_t*)a.vc + off + slot * D);
+      next_powers = a.powers_at - slot * (D - D / 32);
+    } else {
+      next_k = a.kc + off;
+      next_v = a.vc + off;
+    }
   };
   auto load = [&](auto i, auto buffer) {
     constexpr int I = i % LOADS;
-    pg_dma16<32 * T * buffer + (i < LOADS ? 0 : 16 * T) + 1024 * I>((i < LOADS ? next_k : next_v) + (LOADS == 4 && (I & 1) ? 4 * a.slot_stride : 0), lane_off[I * 2 / LOADS],
+    if constexpr (MX) {   // 16 keys of the wave's: D / 64 loads of codes, one of powers (which the lanes read several times)
+      const uint8_t* from = (const uint8_t*)(i < LOADS ? next_k : next_v);
+      constexpr int AT = i < LOADS ? 0 : RAW;
+      if constexpr (I < D / 64) pg_dma16<AT + 1024 * I>(from + 1024 * I, 16 * lane, mine_lds + 16 * D * w);
+      else pg_dma4<AT + 64 * D>(from + next_powers, 4 * (lane % (D / 8)), mine_lds + 256 * w);
+    } else pg_dma16<32 * T * buffer + (i < LOADS ? 0 : 16 * T) + 1024 * I>((i < LOADS ? next_k : next_v) + (LOADS == 4 && (I & 1) ? 4 * a.slot_stride : 0), lane_off[I * 2 / LOADS],
                                                                 mine_lds);
   };
   const auto B0 = std::integral_constant<int, 0>{};
@@ -1019,7 +1220,28 @@ __device__ __forceinline__ void pg_prompt(const PgStep& p, int block, int grid, 
     __syncthreads();   // the tile is there, and every wave is done with the buffer filled next
     const LAS uint8_t* kl = (const LAS uint8_t*)lds[BUF][0];
     LAS uint8_t* vl = (LAS uint8_t*)lds[BUF][1];
-    if (!all) {
+    if constexpr (MX) {   // codes and powers as 16-bit values where the other caches' loads put them
+      const LAS uint8_t* raw = (const LAS uint8_t*)shared.raw;
+#pragma unroll
+      for (int x = 0; x < 2; x++)
+#pragma unroll
+        for (int j = 0; j < D / 64; j++) {
+          const int i = tid + PG_THREADS * j, key = i / (D / 16), u = i % (D / 16);
+          const uint4 c = pg_get(raw + RAW * x + 16 * i);
+          const uint32_t byte = raw[RAW * x + 64 * D + 256 * (key >> 4) + (D / 32) * (key & 15) + (u >> 1)];
+#pragma unroll
+          for (int half = 0; half < 2; half++) {
+            uint4 y = mx_16<TC, MX_F8>(half ? uint2{c.z, c.w} : uint2{c.x, c.y}, byte);
+            if (x == 1 && !all && pg_wild<TC>(y)) {
+              uint4 marks;
+              y = pg_tamed<TC>(y, marks);
+              tamed = k + 1;
+            }
+            *(pg_lds4*)((x ? vl : (LAS uint8_t*)lds[BUF][0]) + 16 * pg_unit_at<D>(key, 2 * u + half)) = (gu32x4){y.x, y.y, y.z, y.w};
+          }
+        }
+      PG_TURN();
+    } else if (!all) {
 #pragma unroll 1
       for (int i = tid; i < T; i += PG_THREADS) {
         uint4 marks;
@@ -1053,7 +1275,10 @@ __device__ __forceinline__ void pg_prompt(const PgStep& p, int block, int grid, 
       for (int i = 0; i < 2; i++)
 #pragma unroll
         for (int b = 0; b < 2; b++) s[b] = pg_mfma32<TC>(kf[g & 1][i][b], qf[2 * g + i], s[b]);
-      pg_each<4 * LOADS / KS>([&](auto i) { load(std::integral_constant<int, 4 * LOADS / KS * g + i>{}, OTHER); });
+      constexpr int PER = (4 * LOADS + KS - 1) / KS;
+      pg_each<PER>([&](auto i) {
+        if constexpr (PER * g + i < 2 * LOADS) load(std::integral_constant<int, PER * g + i>{}, OTHER);
+      });
       __builtin_amdgcn_sched_barrier(0);
     });
     uint4 vf[2][ND];   // [group's turn][32 dims]: the values of 16 keys
@@ -1132,10 +1357,18 @@ __device__ __forceinline__ void pg_prompt(const PgStep& p, int block, int grid, 
 #pragma unroll 1
         for (int t = 0; t < 4; t++) {
           const int64_t at = place(kt + 16 * t);
-          const uint16_t* v = a.vc + (at < 0 ? 0 : at) + 8 * h * a.slot_stride + 32 * d + n;
           uint32_t x[4];
+          if constexpr (MX) {
+            const uint8_t* page = (const uint8_t*)a.vc + (at < 0 ? 0 : at);
+            const int first = mx_slot(kt + 16 * t) + 8 * h;
+            auto value = [&](int i) { return mx_16<TC, MX_F8>({gld(page + (first + i) * D + 32 * d + n), 0}, gld(page + a.powers_at + (first + i) * (D / 32) + d)).x & 0xFFFF; };
 #pragma unroll
-          for (int i = 0; i < 4; i++) x[i] = gld(v + 2 * i * a.slot_stride) | (uint32_t)gld(v + (2 * i + 1) * a.slot_stride) << 16;
+            for (int i = 0; i < 4; i++) x[i] = value(2 * i) | value(2 * i + 1) << 16;
+          } else {
+            const uint16_t* v = a.vc + (at < 0 ? 0 : at) + 8 * h * a.slot_stride + 32 * d + n;
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] = gld(v + 2 * i * a.slot_stride) | (uint32_t)gld(v + (2 * i + 1) * a.slot_stride) << 16;
+          }
           uint4 marks;
           pg_tamed<TC>(make_uint4(x[0], x[1], x[2], x[3]), marks);
           m = pg_mfma32<TC>(marks, pg_ones<TC>(seen >> (8 * t)), m);
@@ -1158,9 +1391,13 @@ __device__ __forceinline__ void pg_prompt(const PgStep& p, int block, int grid, 
       next(0);
       pg_each<2 * LOADS>([&](auto i) { load(i, B0); });
     }
-    for (int k = 0; k < count; k += 2) {
-      tile(k, std::integral_constant<int, 0>{});
-      if (k + 1 < count) tile(k + 1, std::integral_constant<int, 1>{});
+    if constexpr (MX) {
+      for (int k = 0; k < count; k++) tile(k, B0);
+    } else {
+      for (int k = 0; k < count; k += 2) {
+        tile(k, std::integral_constant<int, 0>{});
+        if (k + 1 < count) tile(k + 1, std::integral_constant<int, 1>{});
+      }
     }
     PG_WAIT(0);   // (a load behind the last tile)
     if (careful || count == 0) break;
@@ -1186,15 +1423,15 @@ __device__ __forceinline__ void pg_prompt(const PgStep& p, int block, int grid, 
   if (un.splits > 1) pg_finish<TC, D, M>(a, c, p.w, un, f0, live, (LAS float*)lds, &shared.last);
 }
 
-template <int TC, int D, bool FINE>
+template <int TC, int D, bool FINE, bool MX>
 __global__ __launch_bounds__(PG_THREADS, 2) void pg_step_kernel(PgStep p) {
   __shared__ PgStepLds lds;
-  pg_step<TC, D, FINE>(p, blockIdx.x, gridDim.x, lds);
+  pg_step<TC, D, FINE, MX>(p, blockIdx.x, gridDim.x, lds);
 }
-template <int TC, int D, bool FINE>
+template <int TC, int D, bool FINE, bool MX>
 __global__ __launch_bounds__(PG_THREADS, 2) void pg_prompt_kernel(PgStep p) {
-  __shared__ PgPromptLds<D> lds;
-  pg_prompt<TC, D, FINE>(p, blockIdx.x, gridDim.x, lds);
+  __shared__ PgPromptLds<D, MX> lds;
+  pg_prompt<TC, D, FINE, MX>(p, blockIdx.x, gridDim.x, lds);
 }
 // Both in one launch: prompts in its first workgroups, and what waits for memory beside them.
 struct PgBoth {
@@ -1203,13 +1440,13 @@ struct PgBoth {
   PgWork prompt_work, step_work;
   int32_t prompts;   // workgroups
 };
-template <int TC, int D, bool FINE>
+template <int TC, int D, bool FINE, bool MX>
 __global__ __launch_bounds__(PG_THREADS, 2) void pg_both_kernel(PgBoth p) {
   __shared__ union Lds {
     PgStepLds step;
-    PgPromptLds<D> prompt;
+    PgPromptLds<D, MX> prompt;
     __device__ Lds() {}
   } lds;
-  if ((int)blockIdx.x < p.prompts) pg_prompt<TC, D, FINE>({p.a, p.prompt, p.prompt_work}, blockIdx.x, p.prompts, lds.prompt);
-  else pg_step<TC, D, FINE>({p.a, p.step, p.step_work}, blockIdx.x - p.prompts, gridDim.x - p.prompts, lds.step);
+  if ((int)blockIdx.x < p.prompts) pg_prompt<TC, D, FINE, MX>({p.a, p.prompt, p.prompt_work}, blockIdx.x, p.prompts, lds.prompt);
+  else pg_step<TC, D, FINE, MX>({p.a, p.step, p.step_work}, blockIdx.x - p.prompts, gridDim.x - p.prompts, lds.step);
 }

@@ -35,9 +35,16 @@ inline bool nested(int64_t dim, int64_t s0, int64_t n0, int64_t s1, int64_t n1, 
   return true;
 }
 
+// A handle's type of queries and outputs, and of a 16-bit cache; and whether its cache is microscaled.
+inline int type_of(const ill_paged_desc& d) { return d.dtype & ~ILL_MXF8; }
+inline bool microscaled(const ill_paged_desc& d) { return d.dtype & ILL_MXF8; }
+// Bytes of a microscaled page's codes, which its powers follow.
+inline int64_t mx_codes_of(const ill_paged_desc& d) { return (int64_t)d.page_size * d.kv_heads * d.head_dim; }
+
 // Checks a description and fills in what it leaves at 0.
 inline int check_desc(ill_paged_desc& d) {
-  if (d.dtype != ILL_F16 && d.dtype != ILL_BF16) return fail(ILL_E_FORMAT, "paged: cache type %d (ILL_F16 or ILL_BF16)", d.dtype);
+  if (type_of(d) != ILL_F16 && type_of(d) != ILL_BF16)
+    return fail(ILL_E_FORMAT, "paged: cache type %d (ILL_F16 or ILL_BF16, or one of them | ILL_MXF8)", d.dtype);
   if (d.kv_heads < 1 || d.heads < d.kv_heads || d.heads % d.kv_heads || d.heads > 1024)
     return fail(ILL_E_ARG, "paged: %d query heads over %d key/value heads (a multiple, at most 1024)", d.heads, d.kv_heads);
   if (d.head_dim != 64 && d.head_dim != 128) return fail(ILL_E_ARG, "paged: head size %d (64 or 128)", d.head_dim);
@@ -51,6 +58,14 @@ inline int check_desc(ill_paged_desc& d) {
   if (!(d.scale > 0 && std::isfinite(d.scale))) return fail(ILL_E_ARG, "paged: scale %g", d.scale);
   if (d.streams == 0) d.streams = 8;
   if (d.streams < 1 || d.streams > 256) return fail(ILL_E_ARG, "paged: %d streams (up to 256)", d.streams);
+  if (microscaled(d)) {
+    const int64_t bytes = mx_codes_of(d) + mx_codes_of(d) / 32;
+    if (d.slot_stride || d.head_stride) return fail(ILL_E_ARG, "paged: slot and head strides of a microscaled cache (0: its pages have one layout)");
+    if (!d.page_stride) d.page_stride = bytes;
+    if (d.page_stride < bytes || d.page_stride % 16)
+      return fail(ILL_E_ARG, "paged: microscaled pages %lld bytes apart (at least %lld, a multiple of 16)", (long long)d.page_stride, (long long)bytes);
+    return d.page_stride <= INT64_MAX / 8 ? ILL_OK : fail(ILL_E_ARG, "paged: page stride %lld", (long long)d.page_stride);
+  }
   if (!d.page_stride && !d.slot_stride && !d.head_stride) {
     d.head_stride = d.head_dim;
     d.slot_stride = (int64_t)d.kv_heads * d.head_dim;
@@ -79,7 +94,9 @@ inline int check_batch(const ill_paged_desc& d, const ill_paged_batch* b) {
   if (!b->row0 && b->rows < b->seqs) return fail(ILL_E_ARG, "paged: %lld rows for %d sequences of one row each", (long long)b->rows, b->seqs);
   if (!aligned(b->lens, 4) || !aligned(b->table, 4) || !aligned(b->row0, 4))
     return fail(ILL_E_ARG, "paged: lens, table and row0 are arrays of 4-byte values");
-  if (!nested(d.head_dim, d.page_stride, b->pages, d.slot_stride, d.page_size, d.head_stride, d.kv_heads))
+  if (microscaled(d)) {
+    if (d.page_stride > INT64_MAX / 8 / b->pages) return fail(ILL_E_ARG, "paged: %lld pages, %lld bytes apart", (long long)b->pages, (long long)d.page_stride);
+  } else if (!nested(d.head_dim, d.page_stride, b->pages, d.slot_stride, d.page_size, d.head_stride, d.kv_heads))
     return fail(ILL_E_ARG, "paged: cache strides %lld, %lld, %lld overlap for %lld pages", (long long)d.page_stride, (long long)d.slot_stride,
                 (long long)d.head_stride, (long long)b->pages);
   return ILL_OK;
@@ -101,12 +118,12 @@ inline int check_caches(const void* k, const void* v) {
 inline int check_append(const ill_paged_desc& d, const ill_paged_batch* b, const ill_paged_rows* x, const void* kc, const void* vc) {
   if (int rc = check_batch(d, b)) return rc;
   if (!x) return fail(ILL_E_ARG, "paged: null rows");
-  if (x->dtype != ILL_F32 && x->dtype != d.dtype) return fail(ILL_E_FORMAT, "paged: rows of type %d (ILL_F32 or the cache's)", x->dtype);
+  if (x->dtype != ILL_F32 && x->dtype != type_of(d)) return fail(ILL_E_FORMAT, "paged: rows of type %d (ILL_F32 or the handle's)", x->dtype);
   const int64_t qw = (int64_t)d.heads * d.head_dim, kw = (int64_t)d.kv_heads * d.head_dim;
   if (x->q) {
     if (int rc = check_rows("q", x->q, x->q_stride, qw, x->dtype)) return rc;
-    if (int rc = check_rows("q_out", x->q_out, x->q_out_stride, qw, d.dtype)) return rc;
-    if (x->q_out == x->q && (x->dtype != d.dtype || x->q_stride != x->q_out_stride))
+    if (int rc = check_rows("q_out", x->q_out, x->q_out_stride, qw, type_of(d))) return rc;
+    if (x->q_out == x->q && (x->dtype != type_of(d) || x->q_stride != x->q_out_stride))
       return fail(ILL_E_ARG, "paged: q_out is q, of another type or stride");
   }
   if (int rc = check_rows("k", x->k, x->k_stride, kw, x->dtype)) return rc;
@@ -119,12 +136,23 @@ inline int check_append(const ill_paged_desc& d, const ill_paged_batch* b, const
 inline int check_attend(const ill_paged_desc& d, const ill_paged_batch* b, const void* q, int64_t q_stride, const void* kc, const void* vc, int window,
                         int sinks, const void* out, int64_t out_stride, int out_dtype) {
   if (int rc = check_batch(d, b)) return rc;
-  if (out_dtype != ILL_F32 && out_dtype != d.dtype) return fail(ILL_E_FORMAT, "paged: output of type %d (ILL_F32 or the cache's)", out_dtype);
+  if (out_dtype != ILL_F32 && out_dtype != type_of(d)) return fail(ILL_E_FORMAT, "paged: output of type %d (ILL_F32 or the handle's)", out_dtype);
   const int64_t w = (int64_t)d.heads * d.head_dim;
-  if (int rc = check_rows("q", q, q_stride, w, d.dtype)) return rc;
+  if (int rc = check_rows("q", q, q_stride, w, type_of(d))) return rc;
   if (int rc = check_rows("out", out, out_stride, w, out_dtype)) return rc;
   if (out == q) return fail(ILL_E_ARG, "paged: out is q");
   if (window < 0 || sinks < 0) return fail(ILL_E_ARG, "paged: window %d, sinks %d", window, sinks);
+  return check_caches(kc, vc);
+}
+
+inline int check_read(const ill_paged_desc& d, const ill_paged_batch* b, const void* kc, const void* vc, const void* k, int64_t k_stride, const void* v,
+                      int64_t v_stride, int out_dtype) {
+  if (int rc = check_batch(d, b)) return rc;
+  if (out_dtype != ILL_F32 && out_dtype != type_of(d)) return fail(ILL_E_FORMAT, "paged: output of type %d (ILL_F32 or the handle's)", out_dtype);
+  const int64_t w = (int64_t)d.kv_heads * d.head_dim;
+  if (int rc = check_rows("k", k, k_stride, w, out_dtype)) return rc;
+  if (int rc = check_rows("v", v, v_stride, w, out_dtype)) return rc;
+  if (k == v) return fail(ILL_E_ARG, "paged: k is v");
   return check_caches(kc, vc);
 }
 

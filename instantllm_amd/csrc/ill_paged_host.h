@@ -1,8 +1,7 @@
 // Host side of the paged-cache operators: argument checks and launches (ill_paged_* in
 // include/ill_hip.h). Included by ill_engine.hip after its error helpers.
 #pragma once
-#include "ill_launch.h"
-#include "ill_paged.h"
+#include "ill_paged_launch.h"
 #include "ill_paged_check.h"
 #include "ill_paged_claims.h"
 
@@ -65,22 +64,15 @@ int workspace(ill_paged* p, hipStream_t st, uint8_t** out) {
   return ILL_OK;
 }
 
-// `steps`, `prompts`: workgroups of each kind.
-template <int TC, int D, bool FINE>
-hipError_t launch_attend(const PgBoth& s, int64_t steps, hipStream_t st) {
-  if (!s.prompts) return launch(pg_step_kernel<TC, D, FINE>, steps, PG_THREADS, 0, st, PgStep{s.a, s.step, s.step_work});
-  if (!steps) return launch(pg_prompt_kernel<TC, D, FINE>, s.prompts, PG_THREADS, 0, st, PgStep{s.a, s.prompt, s.prompt_work});
-  return launch(pg_both_kernel<TC, D, FINE>, s.prompts + steps, PG_THREADS, 0, st, s);
-}
-template <int TC, int D>
-hipError_t launch_attend(const PgBoth& s, int64_t steps, hipStream_t st) {
-  return s.a.out_f32 ? launch_attend<TC, D, true>(s, steps, st) : launch_attend<TC, D, false>(s, steps, st);
+hipError_t append_16(int x_type, int type, const PgAppend& a, int D, int R, hipStream_t st) { return launch_append<false>(x_type, type, a, D, R, st); }
+
+hipError_t read_16(int out_type, int type, const PgRead& a, int D, int R, hipStream_t st) {
+  if (type == ILL_F16) return out_type == ILL_F32 ? launch_read<PG_F32, PG_F16, false>(a, D, R, st) : launch_read<PG_F16, PG_F16, false>(a, D, R, st);
+  return out_type == ILL_F32 ? launch_read<PG_F32, PG_BF16, false>(a, D, R, st) : launch_read<PG_BF16, PG_BF16, false>(a, D, R, st);
 }
 
-template <int TX, int TC>
-hipError_t launch_append(const PgAppend& a, int D, int R, int lds, hipStream_t st) {
-  const int64_t blocks = ((int64_t)a.b.rows + R - 1) / R;
-  return D == 64 ? launch(pg_append_kernel<TX, TC, 64>, blocks, 256, lds, st, a, R) : launch(pg_append_kernel<TX, TC, 128>, blocks, 256, lds, st, a, R);
+hipError_t attend_16(int type, int D, const PgBoth& s, int64_t steps, hipStream_t st) {
+  return type == ILL_F16 ? launch_attend<PG_F16, false>(D, s, steps, st) : launch_attend<PG_BF16, false>(D, s, steps, st);
 }
 
 }  // namespace illp
@@ -186,18 +178,28 @@ int ill_paged_append(ill_paged* p, const ill_paged_batch* batch, const ill_paged
   a.rot = d.rotary_dim;
   a.interleaved = d.interleaved != 0;
   a.eps = d.norm_eps;
+  a.powers_at = illp::mx_codes_of(d);
   illp::OnDevice on(p->device);
   if (on.rc) return on.rc;
-  const int R = pg_append_rows(a.b.rows, ((a.q ? d.heads : 0) + 2 * d.kv_heads) * d.head_dim / 16), lds = R * 8 + (R + 1) / 2 * 8 + R * (d.rotary_dim / 2) * 8;
+  const int R = pg_append_rows(a.b.rows, ((a.q ? d.heads : 0) + 2 * d.kv_heads) * d.head_dim / 16);
   hipStream_t st = (hipStream_t)stream;
-  if (x->dtype == ILL_F32) {
-    if (d.dtype == ILL_F16) HCK((illp::launch_append<PG_F32, PG_F16>(a, d.head_dim, R, lds, st)));
-    else HCK((illp::launch_append<PG_F32, PG_BF16>(a, d.head_dim, R, lds, st)));
-  } else if (d.dtype == ILL_F16) {
-    HCK((illp::launch_append<PG_F16, PG_F16>(a, d.head_dim, R, lds, st)));
-  } else {
-    HCK((illp::launch_append<PG_BF16, PG_BF16>(a, d.head_dim, R, lds, st)));
-  }
+  HCK(illp::microscaled(d) ? illp::append_mx(x->dtype, illp::type_of(d), a, d.head_dim, R, st) : illp::append_16(x->dtype, d.dtype, a, d.head_dim, R, st));
+  return ILL_OK;
+}
+
+int ill_paged_read(ill_paged* p, const ill_paged_batch* batch, const void* k_cache, const void* v_cache, void* k, int64_t k_stride, void* v, int64_t v_stride,
+                   int out_dtype, void* stream) {
+  if (!p) return fail(ILL_E_ARG, "paged: null handle");
+  const ill_paged_desc& d = p->d;
+  if (int rc = illp::check_read(d, batch, k_cache, v_cache, k, k_stride, v, v_stride, out_dtype)) return rc;
+  if (!batch->seqs || !batch->rows) return ILL_OK;
+  const PgRead a{illp::batch_of(p, *batch), (const uint8_t*)k_cache, (const uint8_t*)v_cache, k, v, k_stride, v_stride,
+                 d.page_stride, d.slot_stride, d.head_stride, illp::mx_codes_of(d), d.kv_heads};
+  illp::OnDevice on(p->device);
+  if (on.rc) return on.rc;
+  const int R = pg_append_rows(a.b.rows, 2 * d.kv_heads * d.head_dim / 8);
+  hipStream_t st = (hipStream_t)stream;
+  HCK(illp::microscaled(d) ? illp::read_mx(out_dtype, a, d.head_dim, R, st) : illp::read_16(out_dtype, d.dtype, a, d.head_dim, R, st));
   return ILL_OK;
 }
 
@@ -226,6 +228,7 @@ int ill_paged_attend(ill_paged* p, const ill_paged_batch* batch, const void* q, 
   a.sinks = (int)std::min<int64_t>(sinks, illp::kMost);
   a.out_f32 = out_dtype == ILL_F32;
   a.scale = d.scale;
+  a.powers_at = illp::mx_codes_of(d);
   illp::OnDevice on(p->device);
   if (on.rc) return on.rc;
   // One of the kernels where the sizes that the host knows say which, else both in one launch: the sequences are divided by pg_share.
@@ -246,13 +249,7 @@ int ill_paged_attend(ill_paged* p, const ill_paged_batch* batch, const void* q, 
   const int64_t steps = both || !prompts ? pg_grid(a.b.seqs, a.b.rows, !a.b.row0, cap, s.step) : 0;
   s.prompts = prompts ? (int)pg_grid(a.b.seqs, a.b.rows, !a.b.row0, cap, s.prompt) : 0;
   if (!s.prompts && !steps) return ILL_OK;
-  if (d.dtype == ILL_F16) {
-    if (d.head_dim == 64) HCK((illp::launch_attend<PG_F16, 64>(s, steps, st)));
-    else HCK((illp::launch_attend<PG_F16, 128>(s, steps, st)));
-  } else {
-    if (d.head_dim == 64) HCK((illp::launch_attend<PG_BF16, 64>(s, steps, st)));
-    else HCK((illp::launch_attend<PG_BF16, 128>(s, steps, st)));
-  }
+  HCK(illp::microscaled(d) ? illp::attend_mx(illp::type_of(d), d.head_dim, s, steps, st) : illp::attend_16(d.dtype, d.head_dim, s, steps, st));
   return ILL_OK;
 }
 

@@ -123,6 +123,7 @@ def load_library(path: str | os.PathLike | None = None) -> C.CDLL:
         "ill_paged_release": (C.c_int, [P]),
         "ill_paged_append": (C.c_int, [P, P, P, P, P, P]),
         "ill_paged_attend": (C.c_int, [P, P, P, C.c_int64, P, P, C.c_int, C.c_int, P, C.c_int64, C.c_int, P]),
+        "ill_paged_read": (C.c_int, [P, P, P, P, P, C.c_int64, P, C.c_int64, C.c_int, P]),
         "ill_mx_quantize": (C.c_int, [C.c_int, C.c_int, P, C.c_int64, C.c_int64, C.c_int64, P, P, P]),
         "ill_mx_dequantize": (C.c_int, [C.c_int, C.c_int, P, P, C.c_int64, C.c_int64, P, C.c_int64, P]),
         "ill_mx_product": (C.c_int, [C.c_int, P, P, P, P, C.c_int64, C.c_int64, C.c_int64, P, C.c_int, P, C.c_int64, P]),

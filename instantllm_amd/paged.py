@@ -12,6 +12,7 @@ import struct
 from .engine import ILL_OK, IllError, load_library
 
 DTYPES = {"f32": 0, "f16": 1, "bf16": 2}
+MXF8 = 8   # ILL_MXF8: a cache of microscaled 8-bit values, beside the type of queries and outputs
 
 
 class _Desc(C.Structure):
@@ -51,18 +52,30 @@ def _dtype(name: str) -> int:
 class PagedAttention:
     """A model's head geometry and cache layout. `strides`: (page, slot, head) strides of the
     caches in elements (None: [pages][page_size][kv_heads][head_dim]); `rotary_dim` None: the
-    whole head; `streams`: how many streams, and captures of streams, attention calls may come on."""
+    whole head; `streams`: how many streams, and captures of streams, attention calls may come on.
+
+    `cache` "mxf8": the caches hold microscaled 8-bit values (as `mx.quantize` makes them), `dtype` is the type of queries and
+    outputs. A page is `page_bytes` bytes: [kv_heads][page_size][head_dim] codes, then [kv_heads][page_size][head_dim / 32] powers.
+    `page_stride`: bytes from one page to the next (None: none between them)."""
 
     def __init__(self, heads: int, kv_heads: int, head_dim: int, page_size: int = 16, dtype: str = "f16", rotary_dim: int | None = None,
                  rope_base: float = 1e6, interleaved: bool = False, norm_eps: float = 1e-6, scale: float | None = None,
-                 strides: tuple[int, int, int] | None = None, streams: int = 8):
+                 strides: tuple[int, int, int] | None = None, streams: int = 8, cache: str | None = None, page_stride: int | None = None):
         self.h = None
         self.lib = load_library()
+        if cache not in (None, "mxf8"):
+            raise ValueError(f"cache {cache!r}: None (of the handle's type) or 'mxf8'")
+        if cache is None and page_stride is not None or cache and strides is not None:
+            raise ValueError("strides are a 16-bit cache's, page_stride a microscaled one's")
         self.heads, self.kv_heads, self.head_dim, self.dtype, self.type = heads, kv_heads, head_dim, dtype, _dtype(dtype)
         self.q_width, self.kv_width = heads * head_dim, kv_heads * head_dim
         _fits(32, heads=heads, kv_heads=kv_heads, head_dim=head_dim, page_size=page_size, rotary_dim=rotary_dim or 0, streams=streams)
         _fits(64, **dict(zip(("page_stride", "slot_stride", "head_stride"), strides or ())))
-        d = _Desc(self.type, heads, kv_heads, head_dim, page_size, head_dim if rotary_dim is None else rotary_dim, int(interleaved), streams,
+        if cache:
+            self.page_bytes = page_size * kv_heads * (head_dim + head_dim // 32)
+            _fits(64, page_stride=page_stride or 0)
+            strides = (page_stride or 0, 0, 0)
+        d = _Desc(self.type | (MXF8 if cache else 0), heads, kv_heads, head_dim, page_size, head_dim if rotary_dim is None else rotary_dim, int(interleaved), streams,
                   *(strides or (0, 0, 0)), rope_base, norm_eps, scale or 0.0)
         h = C.c_void_p()
         self._check(self.lib.ill_paged_create(C.byref(d), C.byref(h)))
@@ -109,6 +122,15 @@ class PagedAttention:
             _fits(64, q_stride=q_stride, out_stride=out_stride)
         rc = self.lib.ill_paged_attend(self.h, C.byref(batch), q, q_stride, k_cache, v_cache, window, sinks, out, out_stride,
                                        self.type if out_dtype is None else _dtype(out_dtype), stream)
+        if rc:
+            self._check(rc)
+
+    def read(self, batch: Batch, k_cache: int, v_cache: int, k: int, v: int, dtype: str | None = None, k_stride: int | None = None,
+             v_stride: int | None = None, stream: int | None = None):
+        """The batch's rows out of the cache: keys to k, values to v, of type dtype (None: the handle's) or "f32"."""
+        k_stride, v_stride = self.kv_width if k_stride is None else k_stride, self.kv_width if v_stride is None else v_stride
+        _fits(64, k_stride=k_stride, v_stride=v_stride)
+        rc = self.lib.ill_paged_read(self.h, C.byref(batch), k_cache, v_cache, k, k_stride, v, v_stride, self.type if dtype is None else _dtype(dtype), stream)
         if rc:
             self._check(rc)
 

@@ -45,3 +45,15 @@ def values(held: np.ndarray, powers: np.ndarray, fmt: str) -> np.ndarray:
     scale = np.where(powers == 255, np.nan, np.ldexp(1.0, powers.astype(np.int64) - 127))
     with np.errstate(invalid="ignore"):
         return (y * scale[..., None]).reshape(codes.shape)
+
+
+def held_as(y: np.ndarray, powers: np.ndarray, fmt: str) -> np.ndarray:
+    """The values that y [..., n] is held as in blocks of these power bytes [..., n / 32]: nearest, ties to the even code."""
+    sizes = SIZES[fmt]
+    scale = np.ldexp(1.0, powers.astype(np.int64) - 127)[..., None]
+    z = np.minimum(np.abs(np.asarray(y, np.float64).reshape(*powers.shape, 32)) / scale, sizes[-1])
+    hi = np.minimum(np.searchsorted(sizes, z), len(sizes) - 1)
+    lo = np.maximum(hi - 1, 0)
+    below, above = z - sizes[lo], sizes[hi] - z
+    code = np.where((below < above) | ((below == above) & (lo % 2 == 0)), lo, hi)
+    return (np.copysign(sizes[code], np.reshape(y, (*powers.shape, 32))) * scale).reshape(np.shape(y))

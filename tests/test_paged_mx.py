@@ -81,9 +81,9 @@ def test_batches_and_types(checks):
         assert checks.append(C.byref(d), C.byref(_batch()), C.byref(_Rows(**rows, dtype=t)), P16, P16) == code
         assert checks.attend(C.byref(d), C.byref(_batch()), P16, 896, P16, P16, 0, 0, 2 * P16, 896, t) == code
         assert checks.read(C.byref(d), C.byref(_batch()), P16, P16, P16, 128, 2 * P16, 128, t) == code
-    far, _ = _desc(checks, page_stride=1 << 59)
-    assert checks.attend(C.byref(far), C.byref(_batch(pages=2)), P16, 896, P16, P16, 0, 0, 2 * P16, 896, F16) == ILL_OK
-    assert checks.attend(C.byref(far), C.byref(_batch(pages=3)), P16, 896, P16, P16, 0, 0, 2 * P16, 896, F16) == ILL_E_ARG
+    far, _ = _desc(checks, page_stride=1 << 58)
+    assert checks.attend(C.byref(far), C.byref(_batch(pages=3)), P16, 896, P16, P16, 0, 0, 2 * P16, 896, F16) == ILL_OK
+    assert checks.attend(C.byref(far), C.byref(_batch(pages=4)), P16, 896, P16, P16, 0, 0, 2 * P16, 896, F16) == ILL_E_ARG
 
 
 READ = dict(kc=P16, vc=P16, k=P16, k_stride=128, v=2 * P16, v_stride=128, t=F16)

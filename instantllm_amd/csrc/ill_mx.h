@@ -70,7 +70,7 @@ struct MxProduct {
   void* y;
   int64_t stride;                   // of y's rows, in elements
   int32_t rows, cols, inner;        // inner: a multiple of 32
-  int32_t type, wide;               // of y; whether four neighbouring columns from a multiple of four on may be stored at once
+  int32_t type, wide;               // of y; whether its columns from a multiple of four on may be stored four at once (1), or 16 bytes (2)
 };
 
 __device__ __forceinline__ v4f mx_bias4(const MxProduct& p, int c) {
@@ -231,20 +231,71 @@ __device__ __forceinline__ v16f mx_mfma32(const MxOperand& w, uint32_t wp, const
 }
 
 // Many rows, an inner size that is a multiple of 128. A workgroup of 2 x 2 waves computes a tile of 64 TC columns x 64 TR rows, a wave
-// TC x TR products of 32 x 32 x 64. 128 of the inner size are a stage: their codes and powers go straight into LDS, S - 1 stages ahead.
+// TC x TR products of 32 x 32 x 64. 128 of the inner size are a stage: their codes go straight into LDS, S stages ahead.
 // A stage's codes lie there as rows of 64 bytes, 16 bytes a unit (mxf8 rows twice, 64 codes each); a row's units are permuted so that the
-// 16 rows of a quarter of an operand read are on different banks.
+// 16 rows of a quarter of an operand read are on different banks. Powers come for four stages at once (a row's 16 bytes): a
+// stage's four bytes of a row at a time are as many requests as the codes are.
 template <int F, int TC, int TR, int S>
 struct MxTile {
   static constexpr int C = 64 * TC, R = 64 * TR, SLABS = F == MX_F8 ? 2 : 1;   // columns, rows; slabs of the rows' codes
-  static constexpr int X = 64 * C, WP = X + 64 * R * SLABS, XP = WP + 4 * C, STAGE = XP + 4 * R;   // where the rows, the powers are
-  static constexpr int LOADS = (TC + TR * SLABS) + (TC + TR + 3) / 4;          // of a wave and stage
-  static constexpr int LDS = S * STAGE;
+  static constexpr int X = 64 * C, STAGE = X + 64 * R * SLABS;                 // where the rows are; bytes of a stage
+  static constexpr int POWERS = S * STAGE, SLOT = 16 * (C + R);                // powers: of four stages, columns and rows, twice
+  static constexpr int LOADS = TC + TR * SLABS;                                // of a wave and stage
+  static constexpr int LDS = POWERS + 2 * SLOT;
+  static constexpr bool ALONE = LDS > 80 << 10;   // one workgroup for a CU: the compiler then holds the sums in accumulation registers
+  static_assert(4 * 32 * (32 * TC * 4 + 16) <= LDS, "outputs go through it");
 };
 __device__ __forceinline__ int mx_unit(int row, int unit) { return 16 * (4 * row + (unit ^ (row >> 2 & 3))); }
 
+template <int TC>
+constexpr int MX_OUT = 32 * (32 * TC * 4 + 16);   // bytes of LDS for a wave's outputs: 32 rows, of float32 at most
+// 16 bytes of a row's columns from c on, those that there are.
+template <int T>
+__device__ __forceinline__ void mx_store16(const MxProduct& p, int r, int c, gu32x4 v) {
+  constexpr int N = T == PG_F32 ? 4 : 8;
+  const int64_t at = r * p.stride + c;
+  if (p.wide == 2 && c + N <= p.cols) {
+    gst((gu32x4*)((uint8_t*)p.y + (16 / N) * at), v);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < N; i++)
+    if (c + i < p.cols) {
+      if constexpr (T == PG_F32) gst((uint32_t*)p.y + at + i, (uint32_t)v[i]);
+      else gst((uint16_t*)p.y + at + i, (uint16_t)(v[i / 2] >> 16 * (i & 1)));
+    }
+}
+template <int T, int TC, int TR>
+__device__ __forceinline__ void mx_put(const MxProduct& p, const v16f (&acc)[TC][TR], LAS uint8_t* lds, int r0, int c0, int lane) {
+  constexpr int B = T == PG_F32 ? 4 : 2, N = 16 / B, UNITS = 32 * TC / N, ROW = 32 * TC * B + 16;   // units of 16 bytes in a row
+  const int n = lane & 31, g = lane >> 5;
+  v4f bias[TC][4];
+#pragma unroll
+  for (int c = 0; c < TC; c++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) bias[c][i] = mx_bias4(p, min(c0 + 32 * c + 8 * i + 4 * g, p.cols - 1));
+#pragma unroll
+  for (int r = 0; r < TR; r++) {
+#pragma unroll
+    for (int c = 0; c < TC; c++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const v4f y = (v4f){acc[c][r][4 * i], acc[c][r][4 * i + 1], acc[c][r][4 * i + 2], acc[c][r][4 * i + 3]} + bias[c][i];
+        LAS uint8_t* at = lds + n * ROW + B * (32 * c + 8 * i + 4 * g);
+        if constexpr (T == PG_F32) *(LAS gu32x4*)at = __builtin_bit_cast(gu32x4, y);
+        else *(LAS gu32x2*)at = (gu32x2){pg_pack2<T>(y[0], y[1]), pg_pack2<T>(y[2], y[3])};
+      }
+#pragma unroll
+    for (int i = 0; i < 32 * UNITS / 64; i++) {
+      const int u = 64 * i + lane, row = u / UNITS, col = u % UNITS;
+      const gu32x4 v = *(const LAS gu32x4*)(lds + row * ROW + 16 * col);
+      if (r0 + 32 * r + row < p.rows && c0 + N * col < p.cols) mx_store16<T>(p, r0 + 32 * r + row, c0 + N * col, v);
+    }
+  }
+}
+
 template <int F, bool FINE, int TC, int TR, int S>
-__global__ __launch_bounds__(256, TC* TR > 8 ? 1 : 2) void mx_many_kernel(MxProduct p, int tiles_c, int tiles) {
+__global__ __launch_bounds__(256, (MxTile<F, TC, TR, S>::ALONE ? 1 : 2)) void mx_many_kernel(MxProduct p, int tiles_c, int tiles) {
   using T = MxTile<F, TC, TR, S>;
   __shared__ __attribute__((aligned(16))) uint8_t mx_lds[T::LDS];
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 31, g = lane >> 5;
@@ -252,7 +303,8 @@ __global__ __launch_bounds__(256, TC* TR > 8 ? 1 : 2) void mx_many_kernel(MxProd
   const int per = (tiles + 7) / 8, at = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
   if ((int)(blockIdx.x >> 3) >= per || at >= tiles) return;
   const int tiles_r = tiles / tiles_c, band = at / (8 * tiles_c), high = min(8, tiles_r - 8 * band), in = at - 8 * band * tiles_c;
-  const int r0 = (8 * band + in % high) * T::R, c0 = in / high * T::C;
+  // (every lane's: the compiler divides in vector registers, and the loads' addresses have to be in scalar ones)
+  const int r0 = __builtin_amdgcn_readfirstlane((8 * band + in % high) * T::R), c0 = __builtin_amdgcn_readfirstlane(in / high * T::C);
   const int stages = p.inner >> 7, blocks = p.inner >> 5;
   const uint32_t wrow = p.inner / 2, xrow = mx_bytes<F>(p.inner);
   // what this lane loads of 16 rows: 16 bytes, its row's unit that lies where the load puts the lane's
@@ -262,30 +314,32 @@ __global__ __launch_bounds__(256, TC* TR > 8 ? 1 : 2) void mx_many_kernel(MxProd
   for (int i = 0; i < TC; i++) woff[i] = (uint32_t)(min(c0 + 16 * (4 * i + w) + sub, p.cols - 1) - c0) * wrow + 16 * unit;
 #pragma unroll
   for (int i = 0; i < TR; i++) xoff[i] = (uint32_t)(min(r0 + 16 * (4 * i + w) + sub, p.rows - 1) - r0) * xrow + 16 * unit;
-  // and of 64 rows' powers: a word
-  constexpr int PL = (TC + TR + 3) / 4;
-  uint32_t poff[PL], pto[PL];
-  bool of_w[PL];
-#pragma unroll
-  for (int i = 0; i < PL; i++) {
-    const int u = min(4 * i + w, TC + TR - 1);   // (one group twice where they do not come out even)
-    of_w[i] = u < TC;
-    const int row = of_w[i] ? min(c0 + 64 * u + lane, p.cols - 1) - c0 : min(r0 + 64 * (u - TC) + lane, p.rows - 1) - r0;
-    poff[i] = (uint32_t)row * blocks;
-    pto[i] = 256 * u;
-  }
   const uint8_t *wb = p.w + (int64_t)c0 * wrow, *xb = p.x + (int64_t)r0 * xrow, *wpb = p.wp + (int64_t)c0 * blocks, *xpb = p.xp + (int64_t)r0 * blocks;
   const uint32_t lds = pg_lds_at(mx_lds);
-  auto load = [&](int k, int buffer) {   // stage k (behind the last: the last once more, which nobody reads)
+  // 16 rows' powers of four stages: a lane loads a row's word of a stage (behind the last: the last one's)
+  uint32_t poff[TC + TR];
+#pragma unroll
+  for (int i = 0; i < TC + TR; i++) {
+    const int row = 16 * (4 * (i < TC ? i : i - TC) + w) + (lane >> 2);
+    poff[i] = (uint32_t)(i < TC ? min(row, p.cols - 1 - c0) : min(row, p.rows - 1 - r0)) * blocks + 4 * (lane & 3);
+  }
+  auto powers = [&](int q) {   // of stages 4 q .. 4 q + 3
+    const uint32_t to = lds + (q & 1) * T::SLOT + 256 * w, back = 4 * max((int)(lane & 3) - (stages - 1 - 4 * q), 0);
+    pg_each<TC + TR>([&](auto i) { pg_dma4<T::POWERS + 1024 * i>((i < TC ? wpb : xpb) + 16 * q, poff[i] - back, to); });
+  };
+  // Part i of TC of stage k's loads (behind the last stage: the last once more, which nobody reads).
+  auto load = [&](int k, int buffer, auto part) {
+    constexpr int I = decltype(part)::value;
     k = min(k, stages - 1);
     const uint32_t to = lds + buffer * T::STAGE + 1024 * w;
-    const uint8_t *wk = wb + 64 * k, *xk = xb + 64 * T::SLABS * k;
-    pg_each<TC>([&](auto i) { pg_dma16<4096 * i>(wk, woff[i], to); });
-    pg_each<T::SLABS>([&](auto s) {
-      pg_each<TR>([&](auto i) { pg_dma16<T::X + 64 * T::R * s + 4096 * i>(xk + 64 * s, xoff[i], to); });
+    pg_dma16<4096 * I>(wb + 64 * k, woff[I], to);
+    const uint8_t* xk = xb + 64 * T::SLABS * k;
+    pg_each<TR * T::SLABS / TC>([&](auto j) {
+      constexpr int J = I * (TR * T::SLABS / TC) + j, SLAB = J / TR, AT = J % TR;
+      pg_dma16<T::X + 64 * T::R * SLAB + 4096 * AT>(xk + 64 * SLAB, xoff[AT], to);
     });
-    pg_each<PL>([&](auto i) { pg_dma4<T::WP>((of_w[i] ? wpb : xpb) + 4 * k, poff[i], lds + buffer * T::STAGE + pto[i]); });
   };
+  static_assert(TR * T::SLABS % TC == 0, "parts of one size");
   const int wc = w & 1, wr = w >> 1;   // the wave's place in the tile
   // this lane's operands in a stage: unit 2 step + g of a column's 64 bytes; of an mxf8 row's slab `step` units g and 2 + g, or 2 g and 2 g + 1
   int wa[2], xa[2];
@@ -295,56 +349,81 @@ __global__ __launch_bounds__(256, TC* TR > 8 ? 1 : 2) void mx_many_kernel(MxProd
     xa[j] = T::X + mx_unit(32 * TR * wr + n, F == MX_F4 ? 2 * j + g : FINE ? 2 * g + j : 2 * j + g);
   }
   v16f acc[TC][TR] = {};
-  PG_WAIT_OWN();
-#pragma unroll
-  for (int k = 0; k < S - 1; k++) load(k, k);
-  int buffer = 0;
-  for (int k = 0; k < stages; k++) {
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * T::LOADS) : "memory");
-    __syncthreads();   // the stage is there, and every wave is done with the buffer filled next
-    load(k + S - 1, buffer == 0 ? S - 1 : buffer - 1);
+  // operands of a step are read while the products of the step before it run; powers, words of a stage's four, along with its first step's
+  MxOperand wo[2][TC], xo[2][TR];
+  uint32_t wp[TC], xp[TR], wnext[TC], xnext[TR];
+  auto read = [&](int k, int buffer, auto step) {
+    constexpr int J = decltype(step)::value;
     const LAS uint8_t* b = (const LAS uint8_t*)mx_lds + buffer * T::STAGE;
-    uint32_t wp[TC], xp[TR];
+    auto get = [](const LAS uint8_t* q) {
+      const gu32x4 v = *(const LAS gu32x4*)q;
+      return uint4{v[0], v[1], v[2], v[3]};
+    };
+    if constexpr (J == 0) {
+      const LAS uint8_t* q = (const LAS uint8_t*)mx_lds + T::POWERS + (k >> 2 & 1) * T::SLOT + 4 * (k & 3) + 16 * n;
 #pragma unroll
-    for (int i = 0; i < TC; i++) wp[i] = *(const LAS uint32_t*)(b + T::WP + 4 * (32 * (TC * wc + i) + n)) >> 8 * g;
+      for (int i = 0; i < TC; i++) wnext[i] = *(const LAS uint32_t*)(q + 512 * (TC * wc + i));
 #pragma unroll
-    for (int i = 0; i < TR; i++) xp[i] = *(const LAS uint32_t*)(b + T::XP + 4 * (32 * (TR * wr + i) + n)) >> 8 * g;
-    pg_each<2>([&](auto j) {
-      MxOperand wo[TC], xo[TR];
-      auto get = [](const LAS uint8_t* q) {
-        const gu32x4 v = *(const LAS gu32x4*)q;
-        return uint4{v[0], v[1], v[2], v[3]};
-      };
+      for (int i = 0; i < TR; i++) xnext[i] = *(const LAS uint32_t*)(q + 16 * T::C + 512 * (TR * wr + i));
+    }
 #pragma unroll
-      for (int i = 0; i < TC; i++) wo[i].lo = get(b + wa[j] + 2048 * i);
+    for (int i = 0; i < TC; i++) wo[J][i].lo = get(b + wa[J] + 2048 * i);
 #pragma unroll
-      for (int i = 0; i < TR; i++) {
-        if constexpr (F == MX_F4) {
-          xo[i].lo = get(b + xa[j] + 2048 * i);
-        } else {
-          xo[i].lo = get(b + xa[0] + 64 * T::R * j + 2048 * i);
-          xo[i].hi = get(b + xa[1] + 64 * T::R * j + 2048 * i);
-        }
-      }
-#pragma unroll
-      for (int c = 0; c < TC; c++)
-#pragma unroll
-        for (int r = 0; r < TR; r++) acc[c][r] = mx_mfma32<F, FINE>(wo[c], wp[c], xo[r], xp[r], acc[c][r], j);
-    });
-    buffer = buffer == S - 1 ? 0 : buffer + 1;
-  }
-  PG_WAIT(0);   // (loads behind the last stage)
-#pragma unroll
-  for (int c = 0; c < TC; c++)
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int col = c0 + 32 * (TC * wc + c) + 8 * i + 4 * g;
-      if (col >= p.cols) continue;
-      const v4f bias = mx_bias4(p, col);
-#pragma unroll
-      for (int r = 0; r < TR; r++) {
-        const int row = r0 + 32 * (TR * wr + r) + n;
-        if (row < p.rows) mx_store4(p, row, col, (v4f){acc[c][r][4 * i], acc[c][r][4 * i + 1], acc[c][r][4 * i + 2], acc[c][r][4 * i + 3]} + bias);
+    for (int i = 0; i < TR; i++) {
+      if constexpr (F == MX_F4) {
+        xo[J][i].lo = get(b + xa[J] + 2048 * i);
+      } else {
+        xo[J][i].lo = get(b + xa[0] + 64 * T::R * J + 2048 * i);
+        xo[J][i].hi = get(b + xa[1] + 64 * T::R * J + 2048 * i);
       }
     }
+  };
+  // A step's products of 32 columns. The compiler moves products past barriers and loads as it likes: the empty statements, which stay in
+  // their order, keep them where they stand.
+  auto multiply = [&](auto step, auto column) {
+    constexpr int J = decltype(step)::value, K = decltype(column)::value;
+#pragma unroll
+    for (int r = 0; r < TR; r++) {
+      acc[K][r] = mx_mfma32<F, FINE>(wo[J][K], wp[K], xo[J][r], xp[r], acc[K][r], step);
+      if constexpr (T::ALONE) asm volatile("" : "+a"(acc[K][r]));
+      else asm volatile("" : "+v"(acc[K][r]));
+    }
+  };
+  const std::integral_constant<int, 0> FIRST{};
+  const std::integral_constant<int, 1> SECOND{};
+  PG_WAIT_OWN();
+  powers(0);
+  for (int k = 0; k < S; k++) pg_each<TC>([&](auto i) { load(k, k, i); });
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 1) * T::LOADS) : "memory");
+  PG_TURN();
+  read(0, 0, FIRST);
+  int buffer = 0;
+  for (int k = 0; k < stages; k++) {
+#pragma unroll
+    for (int i = 0; i < TC; i++) wp[i] = wnext[i] >> 8 * g;
+#pragma unroll
+    for (int i = 0; i < TR; i++) xp[i] = xnext[i] >> 8 * g;
+    read(k, buffer, SECOND);
+    pg_each<TC>([&](auto c) { multiply(FIRST, c); });
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * T::LOADS) : "memory");
+    PG_TURN();   // the next stage is there, and every wave has read this one
+    const int free = buffer;
+    buffer = buffer == S - 1 ? 0 : buffer + 1;
+    read(k + 1, buffer, FIRST);
+    // (the powers that these replace were last read two turns ago; they are used in four turns, and have arrived when the codes loaded next have)
+    if ((k & 3) == 0 && k + 4 < stages) powers((k >> 2) + 1);
+    __builtin_amdgcn_sched_barrier(0);
+    pg_each<TC>([&](auto c) {
+      multiply(SECOND, c);
+      load(k + S, free, c);
+    });
+  }
+  PG_WAIT(0);   // (loads behind the last stage)
+  PG_TURN();
+  // Outputs go through the wave's own LDS, 32 rows at a time, so that a store has whole runs of a row: straight from the products' lanes, 16 bytes
+  // of 32 rows each, they took 90 of 377 us (8192 x 8192 x 8192 in mxf4).
+  LAS uint8_t* mine = (LAS uint8_t*)mx_lds + w * MX_OUT<TC>;
+  if (p.type == PG_F32) mx_put<PG_F32, TC, TR>(p, acc, mine, r0 + 32 * TR * wr, c0 + 32 * TC * wc, lane);
+  else if (p.type == PG_BF16) mx_put<PG_BF16, TC, TR>(p, acc, mine, r0 + 32 * TR * wr, c0 + 32 * TC * wc, lane);
+  else mx_put<PG_F16, TC, TR>(p, acc, mine, r0 + 32 * TR * wr, c0 + 32 * TC * wc, lane);
 }

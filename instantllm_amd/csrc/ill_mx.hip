@@ -56,9 +56,22 @@ hipError_t launch_many(const MxProduct& p, hipStream_t st) {
 }
 template <int F, bool FINE>
 hipError_t launch_product(const MxProduct& p, hipStream_t st) {
+  // Tiles as large as leave enough of them for 256 CUs. Columns x rows, us. mxf8 rows, 256 x 128 / 128 x 128 / 128 x 64 / 64 x 64: 8192 x 8192 x 8192 449 / 519 / 675 /
+  // 927; 3000 x 5000 x 4096 (480 tiles of 256 x 128) 64 / 71 / 88; 2048 x 2048 x 4096 (128) 38 / 32 / 28 / 34; 5001 x 896 x 4864 (280 of 128 x 128) 45 / 41 / 37 / 48;
+  // 512 x 896 x 4864 (112 of 64 x 64) 34 / 24 / 18 / 15. mxf4, 256 x 256 / 128 x 256 / 128 x 128 / 64 x 64: 8192 x 8192 x 8192 312 / 335 / 407 / 768; 3000 x 5000 x 4096 (240) 48 / 50 / 57;
+  // 8192 x 8192 x 2048 107 / 97 / 108; 2048 x 2048 x 4096 (128 of 128 x 256) 40 / 32 / 22 / 29; 512 x 896 x 4864 - / 27 / 19 / 13.5.
   if (p.rows > 64 && p.inner % 128 == 0) {
-    if (!FINE && (int64_t)p.rows * p.cols >= 1 << 23) return launch_many<F, FINE, 4, 4, 3>(p, st);
-    return launch_many<F, FINE, 2, 2, 3>(p, st);
+    auto tiles = [&](int c, int r) { return (int64_t)((p.cols + c - 1) / c) * ((p.rows + r - 1) / r); };
+    if (tiles(64, 64) <= 512) return launch_many<F, FINE, 1, 1, 3>(p, st);
+    if constexpr (FINE) {
+      return launch_many<F, FINE, 2, 1, 2>(p, st);
+    } else if constexpr (F == MX_F8) {
+      if (tiles(256, 128) >= 384) return launch_many<F, FINE, 4, 2, 2>(p, st);
+      return tiles(128, 128) >= 480 ? launch_many<F, FINE, 2, 2, 2>(p, st) : launch_many<F, FINE, 2, 1, 2>(p, st);
+    } else {
+      if (tiles(256, 256) >= 240 && p.inner >= 4096) return launch_many<F, FINE, 4, 4, 3>(p, st);
+      return tiles(128, 256) >= 512 ? launch_many<F, FINE, 2, 4, 2>(p, st) : launch_many<F, FINE, 2, 2, 2>(p, st);
+    }
   }
   const bool split = p.cols < 16 * 1024;
   if (p.rows <= 16) return split ? launch_few<F, FINE, 1, 4>(p, st) : launch_few<F, FINE, 1, 1>(p, st);
@@ -88,7 +101,8 @@ int ill_mx_product(int x_format, const void* x, const void* x_powers, const void
   if (int rc = illm::device_of(st, &dev)) return rc;
   illp::OnDevice on(dev);
   if (on.rc) return on.rc;
-  const bool wide = y_stride % 4 == 0 && illm::aligned(y, y_dtype == ILL_F32 ? 16 : 8);
+  const int size = y_dtype == ILL_F32 ? 4 : 2;
+  const int wide = y_stride % (16 / size) == 0 && illm::aligned(y, 16) ? 2 : y_stride % 4 == 0 && illm::aligned(y, 4 * size) ? 1 : 0;
   const MxProduct p{(const uint8_t*)x, (const uint8_t*)x_powers, (const uint8_t*)w, (const uint8_t*)w_powers, bias, y, y_stride,
                     (int)rows, (int)cols, (int)inner, y_dtype, wide};
   if (x_format == ILL_MXF4) HCK((illm::launch_product<MX_F4, false>(p, st)));

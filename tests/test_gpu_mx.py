@@ -165,7 +165,9 @@ class Product:
 
 SHAPES = [   # rows, columns, inner size: single rows, batches, prompts; odd sizes; inner sizes that are no multiple of 128
     (1, 1152, 896), (1, 896, 4864), (1, 1, 32), (2, 17, 64), (7, 33, 96), (16, 100, 160), (16, 20001, 256), (17, 1152, 896), (31, 48, 4864), (33, 70, 288),
-    (64, 130, 896), (65, 128, 128), (100, 257, 512), (128, 129, 384), (200, 1000, 2048), (333, 515, 1152), (513, 300, 4864), (1, 17000, 32), (40, 16500, 96), (1025, 1030, 256), (2901, 2950, 256), (8300, 1100, 128)]
+    (64, 130, 896), (65, 128, 128), (100, 257, 512), (128, 129, 384), (200, 1000, 2048), (333, 515, 1152), (513, 300, 4864), (1, 17000, 32), (40, 16500, 96), (1025, 1030, 256),
+    # tiles of every size: 128 x 64, 128 x 128 and 256 x 128 (mxf8), 128 x 128, 128 x 256 and 256 x 256 (mxf4)
+    (1900, 2000, 128), (3001, 2450, 256), (6450, 3850, 128), (4001, 4002, 4096)]
 
 
 @pytest.mark.parametrize("fmt", ["mxf8", "mxf4"])

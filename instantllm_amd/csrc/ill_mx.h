@@ -219,6 +219,102 @@ __global__ __launch_bounds__(256) void mx_few_kernel(MxProduct p, int tiles) {  
   }
 }
 
+// Few rows and many columns: the matrix is read once, as fast as memory gives it. The rows lie in LDS as operands, for every wave of the
+// workgroup and for all of its tiles of 16 columns; a wave holds up to CH steps of a tile and loads the next ones while it multiplies.
+template <int F, bool FINE, int R>
+struct MxWide {
+  static constexpr int PARTS = F == MX_F8 ? 2 : 1, STEP = R * (1024 * PARTS + 64);   // bytes of a step's operands and powers
+  static constexpr int lds(int inner) { return (inner + 127) / 128 * STEP; }
+};
+template <int F, bool FINE, int R>
+__global__ __launch_bounds__(256) void mx_wide_kernel(MxProduct p, int tiles) {
+  constexpr int CH = 8, PARTS = MxWide<F, FINE, R>::PARTS;
+  extern __shared__ __attribute__((aligned(16))) uint8_t mx_rows[];
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int blocks = p.inner >> 5, steps = (blocks + 3) >> 2, stride = gridDim.x * 4;
+  const LAS uint8_t* rows = (const LAS uint8_t*)mx_rows;
+  const LAS uint8_t* powers = rows + steps * R * PARTS * 1024;
+  struct Chunk {
+    uint4 w[CH];
+    uint32_t wp[CH];
+  };
+  auto fetch = [&](Chunk& c, int tile, int s0) {
+    const int64_t col = min(16 * min(tile, tiles - 1) + n, p.cols - 1);
+    const uint8_t *wr = p.w + col * (p.inner / 2), *wpr = p.wp + col * blocks;
+#pragma unroll
+    for (int u = 0; u < CH; u++) {
+      const int block = min(4 * min(s0 + u, steps - 1) + g, blocks - 1);   // (what is behind the last is not read)
+      c.w[u] = gld((const uint4*)(wr + 16 * block));
+      c.wp[u] = gld(wpr + block);
+    }
+  };
+  int tile = blockIdx.x * 4 + w, s0 = 0;
+  Chunk a, b;
+  fetch(a, tile, 0);
+  for (int i = threadIdx.x; i < steps * R * 64; i += 256) {   // a lane's operand of 16 rows and a step
+    const int s = i / (R * 64), part = i / 64 % R, l = i & 63, block = 4 * s + (l >> 4);
+    const int64_t r = min(16 * part + (l & 15), p.rows - 1);
+    const uint8_t* x = p.x + r * mx_bytes<F>(p.inner);
+    const uint4 none = {0, 0, 0, 0};
+    uint4 lo = none, hi = none;
+    if constexpr (F == MX_F4) {
+      if (block < blocks) lo = gld((const uint4*)(x + 16 * block));
+    } else {
+      const int b0 = FINE ? block : 4 * s + (l >> 5), b1 = FINE ? block : b0 + 2, at = FINE ? 0 : 16 * (l >> 4 & 1);
+      if (b0 < blocks) lo = gld((const uint4*)(x + 32 * b0 + at));
+      if (b1 < blocks) hi = gld((const uint4*)(x + 32 * b1 + (FINE ? 16 : at)));
+    }
+    LAS gu32x4* to = (LAS gu32x4*)mx_rows + (s * R + part) * PARTS * 64 + l;
+    to[0] = (gu32x4){lo.x, lo.y, lo.z, lo.w};
+    if constexpr (PARTS == 2) to[64] = (gu32x4){hi.x, hi.y, hi.z, hi.w};
+    ((LAS uint8_t*)mx_rows)[steps * R * PARTS * 1024 + i] = block < blocks ? gld(p.xp + r * blocks + block) : 127;
+  }
+  __syncthreads();
+  v4f acc[R] = {};
+  auto turn = [&](const Chunk& c, Chunk& next) {   // multiplies a chunk; the next one's loads are on their way meanwhile. False: there is none
+    const bool last = s0 + CH >= steps;
+    const int tile1 = last ? tile + stride : tile, s1 = last ? 0 : s0 + CH;
+    fetch(next, tile1, s1);
+#pragma unroll
+    for (int u = 0; u < CH; u++) {
+      if (s0 + u >= steps) break;
+      MxOperand wo{c.w[u], {}};
+      uint32_t wp = c.wp[u];
+      if (4 * (s0 + u) + 4 > blocks && 4 * (s0 + u) + g >= blocks) {   // zeros for the blocks behind the last
+        wo.lo = {0, 0, 0, 0};
+        wp = 127;
+      }
+#pragma unroll
+      for (int i = 0; i < R; i++) {
+        const int at = (s0 + u) * R + i;
+        auto get = [&](int part) {
+          const gu32x4 v = *(const LAS gu32x4*)(rows + (at * PARTS + part) * 1024 + 16 * lane);
+          return uint4{v[0], v[1], v[2], v[3]};
+        };
+        MxOperand x{get(0), {}};
+        if constexpr (PARTS == 2) x.hi = get(1);
+        acc[i] = mx_mfma16<F, FINE>(wo, wp, x, powers[at * 64 + lane], acc[i]);
+      }
+    }
+    if (last) {
+      const int c0 = 16 * tile + 4 * g;
+      if (c0 < p.cols) {
+        const v4f bias = mx_bias4(p, c0);
+#pragma unroll
+        for (int i = 0; i < R; i++)
+          if (16 * i + n < p.rows) mx_store4(p, 16 * i + n, c0, acc[i] + bias);
+      }
+#pragma unroll
+      for (int i = 0; i < R; i++) acc[i] = (v4f){0.f, 0.f, 0.f, 0.f};
+    }
+    tile = tile1;
+    s0 = s1;
+    return tile < tiles;
+  };
+  if (tile >= tiles) return;
+  while (turn(a, b) && turn(b, a)) {}
+}
+
 template <int F, bool FINE, class J>
 __device__ __forceinline__ v16f mx_mfma32(const MxOperand& w, uint32_t wp, const MxOperand& x, uint32_t xp, v16f c, J) {   // 32 x 32 x 64
   constexpr int AT = 2 * J::value;   // the powers: this byte of each lane's word

@@ -48,11 +48,24 @@ hipError_t launch_few(const MxProduct& p, hipStream_t st) {
   const int cols = KS == 1 ? 64 : 16, tiles = (p.cols + cols - 1) / cols;
   return launch(mx_few_kernel<F, FINE, R, KS>, (int64_t)((p.rows + 16 * R - 1) / (16 * R)) * tiles, 256, 0, st, p, tiles);
 }
+// Whether the rows fit into LDS, of which a workgroup may have 64 KB.
+template <int F, bool FINE, int R>
+bool fits_wide(const MxProduct& p) { return MxWide<F, FINE, R>::lds(p.inner) <= 64 << 10; }
+template <int F, bool FINE, int R>
+hipError_t launch_wide(const MxProduct& p, hipStream_t st) {
+  const int tiles = (p.cols + 15) / 16, lds = MxWide<F, FINE, R>::lds(p.inner), each = std::max(1, std::min(4, (160 << 10) / lds));
+  return launch(mx_wide_kernel<F, FINE, R>, std::min(256 * each, (tiles + 3) / 4), 256, lds, st, p, tiles);
+}
 template <int F, bool FINE, int TC, int TR, int S>
 hipError_t launch_many(const MxProduct& p, hipStream_t st) {
   using T = MxTile<F, TC, TR, S>;
   const int tiles_c = (p.cols + T::C - 1) / T::C, tiles = tiles_c * ((p.rows + T::R - 1) / T::R);
   return launch(mx_many_kernel<F, FINE, TC, TR, S>, (tiles + 7) / 8 * 8ll, 256, 0, st, p, tiles_c, tiles);
+}
+template <int F, bool FINE, int R>
+hipError_t launch_few_rows(const MxProduct& p, hipStream_t st) {
+  if (p.cols < 16 * 1024) return launch_few<F, FINE, R, 4>(p, st);
+  return p.rows <= 16 * R && fits_wide<F, FINE, R>(p) ? launch_wide<F, FINE, R>(p, st) : launch_few<F, FINE, R, 1>(p, st);
 }
 template <int F, bool FINE>
 hipError_t launch_product(const MxProduct& p, hipStream_t st) {
@@ -73,10 +86,7 @@ hipError_t launch_product(const MxProduct& p, hipStream_t st) {
       return tiles(128, 256) >= 512 ? launch_many<F, FINE, 2, 4, 2>(p, st) : launch_many<F, FINE, 2, 2, 2>(p, st);
     }
   }
-  const bool split = p.cols < 16 * 1024;
-  if (p.rows <= 16) return split ? launch_few<F, FINE, 1, 4>(p, st) : launch_few<F, FINE, 1, 1>(p, st);
-  if (p.rows <= 32) return split ? launch_few<F, FINE, 2, 4>(p, st) : launch_few<F, FINE, 2, 1>(p, st);
-  return split ? launch_few<F, FINE, 4, 4>(p, st) : launch_few<F, FINE, 4, 1>(p, st);
+  return p.rows <= 16 ? launch_few_rows<F, FINE, 1>(p, st) : p.rows <= 32 ? launch_few_rows<F, FINE, 2>(p, st) : launch_few_rows<F, FINE, 4>(p, st);
 }
 
 }  // namespace

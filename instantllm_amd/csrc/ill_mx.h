@@ -134,16 +134,15 @@ __device__ __forceinline__ v4f mx_mfma16(const MxOperand& w, uint32_t wp, const 
 
 // Few rows, or an inner size that is no multiple of 128. A wave multiplies 16 columns by 16 R rows over its share of the inner size: 128 at a
 // time, straight from memory (a lane's 32 codes of a column are 16 bytes; of an mxf8 row 16 + 16, as the instruction divides them, or 32
-// together where they become bf16). KS waves share the inner size of the same columns and are joined in LDS, in their order.
-template <int F, bool FINE, int R, int KS>
+// together where they become bf16). The four waves of a workgroup share the inner size of a tile and are joined in LDS, in their order.
+template <int F, bool FINE, int R>
 __global__ __launch_bounds__(256) void mx_few_kernel(MxProduct p, int tiles) {   // tiles: workgroups for the columns
   constexpr int U = R == 4 ? 2 : 4;   // steps whose loads are in flight together
-  __shared__ __attribute__((aligned(16))) v4f part[KS > 1 ? 4 : 1][R][64];
+  __shared__ __attribute__((aligned(16))) v4f part[4][R][64];
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-  const int row_tile = blockIdx.x / (uint32_t)tiles, tile = blockIdx.x - row_tile * tiles, r0 = 16 * R * row_tile, c0 = 16 * (KS == 1 ? tile * 4 + w : tile);
-  const int blocks = p.inner >> 5, steps = (blocks + 3) >> 2, each = (steps + KS - 1) / KS;
-  const int s0 = KS == 1 ? 0 : min(each * w, steps), s1 = KS == 1 ? steps : min(s0 + each, steps);
-  if (KS == 1 && c0 >= p.cols) return;
+  const int row_tile = blockIdx.x / (uint32_t)tiles, tile = blockIdx.x - row_tile * tiles, r0 = 16 * R * row_tile, c0 = 16 * tile;
+  const int blocks = p.inner >> 5, steps = (blocks + 3) >> 2, each = (steps + 3) / 4;
+  const int s0 = min(each * w, steps), s1 = min(s0 + each, steps);
   const int64_t wc = min(c0 + n, p.cols - 1);
   const uint8_t *wr = p.w + wc * (p.inner / 2), *wpr = p.wp + wc * blocks;
   const uint8_t *xr[R], *xpr[R];
@@ -198,24 +197,106 @@ __global__ __launch_bounds__(256) void mx_few_kernel(MxProduct p, int tiles) {  
       for (int i = 0; i < R; i++) acc[i] = mx_mfma16<F, FINE>(a[u], ap[u], b[u][i], bp[u][i], acc[i]);
     }
   }
-  if constexpr (KS > 1) {
 #pragma unroll
-    for (int i = 0; i < R; i++) part[w][i][lane] = acc[i];
-    __syncthreads();
-    for (int i = w; i < R; i += 4) {
-      v4f y = part[0][i][lane];
+  for (int i = 0; i < R; i++) part[w][i][lane] = acc[i];
+  __syncthreads();
+  for (int i = w; i < R; i += 4) {
+    v4f y = part[0][i][lane];
 #pragma unroll
-      for (int k = 1; k < KS; k++) y += part[k][i][lane];
-      const int r = r0 + 16 * i + n, c = c0 + 4 * g;
-      if (r < p.rows && c < p.cols) mx_store4(p, r, c, y + mx_bias4(p, c));
+    for (int k = 1; k < 4; k++) y += part[k][i][lane];
+    const int r = r0 + 16 * i + n, c = c0 + 4 * g;
+    if (r < p.rows && c < p.cols) mx_store4(p, r, c, y + mx_bias4(p, c));
+  }
+}
+
+// Up to 16 rows. The inner size is cut into L slices of up to CH steps, one to a wave; a wave holds its slice of the rows in registers and
+// goes from tile to tile of 16 columns, whose next codes are on their way while it multiplies. The slices' sums are joined in LDS, in their order, by
+// each of the waves in turn.
+template <int F, bool FINE, int L>
+__global__ __launch_bounds__(L < 4 ? 256 : 64 * L) void mx_slice_kernel(MxProduct p, int tiles) {
+  constexpr int CH = 8, WAVES = L < 4 ? 4 : L, G = WAVES / L;   // G: tiles that a workgroup computes at a time
+  __shared__ __attribute__((aligned(16))) v4f part[2][L > 1 ? WAVES : 1][64];
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int slice = w % L, group = w / L, blocks = p.inner >> 5, steps = (blocks + 3) >> 2, each = (steps + L - 1) / L;
+  const int s0 = min(slice * each, steps), count = min(each, steps - s0);
+  struct Chunk {
+    uint4 w[CH];
+    uint32_t wp[2];
+  };
+  const int64_t end = (int64_t)p.cols * blocks - 4;
+  auto fetch = [&](Chunk& c, int tile) {
+    const int64_t col = min(16 * min(tile, tiles - 1) + n, p.cols - 1);
+    const uint8_t* wr = p.w + col * (p.inner / 2);
+#pragma unroll
+    for (int u = 0; u < CH; u++) c.w[u] = gld((const uint4*)(wr + 16 * min(4 * min(s0 + u, steps - 1) + g, blocks - 1)));   // (what is behind the last is not read)
+#pragma unroll
+    for (int i = 0; i < 2; i++) {   // a column's powers of two steps, each four bytes: the lanes of the others have them exchanged
+      const int64_t at = col * blocks + 4 * min(s0 + 2 * g + i, steps - 1), from = min(at, max(end, (int64_t)0));
+      typedef uint32_t word __attribute__((aligned(1)));
+      c.wp[i] = end < 0 ? gld(p.wp + at) : *(const GAS word*)(p.wp + from) >> 8 * (int)(at - from);
     }
-  } else {
-    const int c = c0 + 4 * g;
-    if (c >= p.cols) return;
-    const v4f b = mx_bias4(p, c);
+  };
+  int tile = blockIdx.x * G + group, turn = 0;
+  const int stride = gridDim.x * G, turns = (tiles - (int)blockIdx.x * G + stride - 1) / stride;   // (the same for all waves of the workgroup)
+  Chunk a, b;
+  fetch(a, tile);
+  MxOperand x[CH];
+  uint32_t xp[CH];
+  {
+    const int64_t r = min(n, p.rows - 1);
+    const uint8_t *xr = p.x + r * mx_bytes<F>(p.inner), *xpr = p.xp + r * blocks;
+    const uint4 none = {0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < R; i++)
-      if (r0 + 16 * i + n < p.rows) mx_store4(p, r0 + 16 * i + n, c, acc[i] + b);
+    for (int u = 0; u < CH; u++) {   // zeros behind the last block
+      const int s = s0 + u, block = 4 * s + g;
+      xp[u] = u < count && block < blocks ? gld(xpr + block) : 127;
+      if constexpr (F == MX_F4) {
+        x[u] = {u < count && block < blocks ? gld((const uint4*)(xr + 16 * block)) : none, none};
+      } else {
+        const int b0 = FINE ? block : 4 * s + (g >> 1), b1 = FINE ? block : b0 + 2, at = FINE ? 0 : 16 * (g & 1);
+        x[u] = {u < count && b0 < blocks ? gld((const uint4*)(xr + 32 * b0 + at)) : none, u < count && b1 < blocks ? gld((const uint4*)(xr + 32 * b1 + (FINE ? 16 : at))) : none};
+      }
+    }
+  }
+  auto compute = [&](const Chunk& c, Chunk& next, auto more) {   // one tile, while the next one's loads are on their way if there are more
+    if constexpr (decltype(more)::value) fetch(next, tile + stride);
+    if constexpr (FINE) {   // (else the rows' bf16 values are kept from tile to tile: 318 registers)
+#pragma unroll
+      for (int u = 0; u < CH; u++) asm volatile("" : "+v"(x[u].lo.x), "+v"(x[u].lo.y), "+v"(x[u].lo.z), "+v"(x[u].lo.w), "+v"(x[u].hi.x), "+v"(x[u].hi.y), "+v"(x[u].hi.z), "+v"(x[u].hi.w));
+    }
+    v4f acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < CH; u++) {
+      if (u >= count) break;
+      MxOperand wo{c.w[u], {}};
+      uint32_t wp = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * n + 64 * (u >> 1), (int)c.wp[u & 1]) >> 8 * g & 255;
+      if (4 * (s0 + u) + 4 > blocks && 4 * (s0 + u) + g >= blocks) {
+        wo.lo = {0, 0, 0, 0};
+        wp = 127;
+      }
+      acc = mx_mfma16<F, FINE>(wo, wp, x[u], xp[u], acc);
+    }
+    const int c0 = 16 * tile + 4 * g;
+    if constexpr (L > 1) {
+      part[turn & 1][w][lane] = acc;
+      PG_TURN();
+      if (slice == turn % L) {
+        acc = part[turn & 1][group * L][lane];
+#pragma unroll
+        for (int k = 1; k < L; k++) acc += part[turn & 1][group * L + k][lane];
+      }
+    }
+    if ((L == 1 || slice == turn % L) && tile < tiles && n < p.rows && c0 < p.cols) mx_store4(p, n, c0, acc + mx_bias4(p, c0));
+    tile += stride;
+    turn++;
+  };
+  const std::true_type MORE{};
+  const std::false_type LAST{};
+  for (;;) {   // (whether there are more is known where the loads are: behind a branch the compiler waits for all of them)
+    if (turn + 1 == turns) return compute(a, b, LAST);
+    compute(a, b, MORE);
+    if (turn + 1 == turns) return compute(b, a, LAST);
+    compute(b, a, MORE);
   }
 }
 

@@ -13,6 +13,8 @@ namespace {
 
 using illp::launch;
 
+constexpr int SLICE_WAVES = 8;   // of a CU: as many as its registers hold
+
 // The GPU that a stream belongs to; of the default streams the current one.
 int device_of(hipStream_t st, int* dev) {
   if (!st || st == hipStreamLegacy || st == hipStreamPerThread) HCK(hipGetDevice(dev));
@@ -43,15 +45,18 @@ int rows(bool back, int format, int dtype, const void* x, int64_t stride, int64_
   return ILL_OK;
 }
 
-template <int F, bool FINE, int R, int KS>
+template <int F, bool FINE, int R>
 hipError_t launch_few(const MxProduct& p, hipStream_t st) {
-  const int cols = KS == 1 ? 64 : 16, tiles = (p.cols + cols - 1) / cols;
-  return launch(mx_few_kernel<F, FINE, R, KS>, (int64_t)((p.rows + 16 * R - 1) / (16 * R)) * tiles, 256, 0, st, p, tiles);
+  const int tiles = (p.cols + 15) / 16;
+  return launch(mx_few_kernel<F, FINE, R>, (int64_t)((p.rows + 16 * R - 1) / (16 * R)) * tiles, 256, 0, st, p, tiles);
 }
-// Whether the rows fit into LDS, of which a workgroup may have 64 KB.
-template <int F, bool FINE, int R>
-bool fits_wide(const MxProduct& p) { return MxWide<F, FINE, R>::lds(p.inner) <= 64 << 10; }
-template <int F, bool FINE, int R>
+template <int F, bool FINE, int L>
+hipError_t launch_slice(const MxProduct& p, hipStream_t st) {
+  constexpr int waves = L < 4 ? 4 : L;
+  const int tiles = (p.cols + 15) / 16, each = std::max(1, SLICE_WAVES / waves);
+  return launch(mx_slice_kernel<F, FINE, L>, std::min(256 * each, (tiles + waves / L - 1) / (waves / L)), 64 * waves, 0, st, p, tiles);
+}
+template <int F, bool FINE, int R>   // (for rows that take up to 64 KB of LDS)
 hipError_t launch_wide(const MxProduct& p, hipStream_t st) {
   const int tiles = (p.cols + 15) / 16, lds = MxWide<F, FINE, R>::lds(p.inner), each = std::max(1, std::min(4, (160 << 10) / lds));
   return launch(mx_wide_kernel<F, FINE, R>, std::min(256 * each, (tiles + 3) / 4), 256, lds, st, p, tiles);
@@ -62,31 +67,40 @@ hipError_t launch_many(const MxProduct& p, hipStream_t st) {
   const int tiles_c = (p.cols + T::C - 1) / T::C, tiles = tiles_c * ((p.rows + T::R - 1) / T::R);
   return launch(mx_many_kernel<F, FINE, TC, TR, S>, (tiles + 7) / 8 * 8ll, 256, 0, st, p, tiles_c, tiles);
 }
-template <int F, bool FINE, int R>
-hipError_t launch_few_rows(const MxProduct& p, hipStream_t st) {
-  if (p.cols < 16 * 1024) return launch_few<F, FINE, R, 4>(p, st);
-  return p.rows <= 16 * R && fits_wide<F, FINE, R>(p) ? launch_wide<F, FINE, R>(p, st) : launch_few<F, FINE, R, 1>(p, st);
-}
 template <int F, bool FINE>
 hipError_t launch_product(const MxProduct& p, hipStream_t st) {
+  const int steps = (p.inner + 127) / 128;
+  auto tiles = [&](int c, int r) { return (int64_t)((p.cols + c - 1) / c) * ((p.rows + r - 1) / r); };
+  // Up to 16 rows: slices from 512 tiles of 16 columns on (us, against the four waves of a workgroup that share a tile, mxf8 unless said otherwise: 16 x 9728 x 896
+  // 5.2 / 6.3, 16 x 16384 x 4096 14.3 / 19.9, mxf4 16 x 32000 x 8192 37 / 61; but 1 x 896 x 4864 7.8 / 4.7). As bf16 values their rows take too many registers:
+  // 1 x 151936 x 896 23.4, with the rows in LDS 18.6. Up to 32 rows in LDS, against tiles of 64 x 64: 32 x 151936 x 896 22.9 / 28.2.
+  if (p.rows <= 16 && p.cols >= 8192 && steps <= 64) {
+    if constexpr (FINE) {
+      if (steps <= 8) return launch_wide<F, FINE, 1>(p, st);
+    }
+    if (steps <= 8) return launch_slice<F, FINE, 1>(p, st);
+    if (steps <= 16) return launch_slice<F, FINE, 2>(p, st);
+    return steps <= 32 ? launch_slice<F, FINE, 4>(p, st) : launch_slice<F, FINE, 8>(p, st);
+  }
+  if (p.rows <= 16) return launch_few<F, FINE, 1>(p, st);
+  if (p.rows <= 32 && p.cols >= 16384 && MxWide<F, FINE, 2>::lds(p.inner) <= 64 << 10) return launch_wide<F, FINE, 2>(p, st);
+  // Few tiles over a long inner size: 16 rows at a time, as above (64 x 896 x 4864 6.7 us, 14 tiles of 64 x 64 13).
+  if (p.rows <= 64 && tiles(64, 64) < 64 && (steps > 16 || p.inner % 128)) return launch_few<F, FINE, 1>(p, st);
+  if (p.inner % 128) return launch_few<F, FINE, 4>(p, st);
   // Tiles as large as leave enough of them for 256 CUs. Columns x rows, us. mxf8 rows, 256 x 128 / 128 x 128 / 128 x 64 / 64 x 64: 8192 x 8192 x 8192 449 / 519 / 675 /
   // 927; 3000 x 5000 x 4096 (480 tiles of 256 x 128) 64 / 71 / 88; 2048 x 2048 x 4096 (128) 38 / 32 / 28 / 34; 5001 x 896 x 4864 (280 of 128 x 128) 45 / 41 / 37 / 48;
   // 512 x 896 x 4864 (112 of 64 x 64) 34 / 24 / 18 / 15. mxf4, 256 x 256 / 128 x 256 / 128 x 128 / 64 x 64: 8192 x 8192 x 8192 312 / 335 / 407 / 768; 3000 x 5000 x 4096 (240) 48 / 50 / 57;
   // 8192 x 8192 x 2048 107 / 97 / 108; 2048 x 2048 x 4096 (128 of 128 x 256) 40 / 32 / 22 / 29; 512 x 896 x 4864 - / 27 / 19 / 13.5.
-  if (p.rows > 64 && p.inner % 128 == 0) {
-    auto tiles = [&](int c, int r) { return (int64_t)((p.cols + c - 1) / c) * ((p.rows + r - 1) / r); };
-    if (tiles(64, 64) <= 512) return launch_many<F, FINE, 1, 1, 3>(p, st);
-    if constexpr (FINE) {
-      return launch_many<F, FINE, 2, 1, 2>(p, st);
-    } else if constexpr (F == MX_F8) {
-      if (tiles(256, 128) >= 384) return launch_many<F, FINE, 4, 2, 2>(p, st);
-      return tiles(128, 128) >= 480 ? launch_many<F, FINE, 2, 2, 2>(p, st) : launch_many<F, FINE, 2, 1, 2>(p, st);
-    } else {
-      if (tiles(256, 256) >= 240 && p.inner >= 4096) return launch_many<F, FINE, 4, 4, 3>(p, st);
-      return tiles(128, 256) >= 512 ? launch_many<F, FINE, 2, 4, 2>(p, st) : launch_many<F, FINE, 2, 2, 2>(p, st);
-    }
+  if (tiles(64, 64) <= 512 || p.rows <= 64) return launch_many<F, FINE, 1, 1, 3>(p, st);
+  if constexpr (FINE) {
+    return launch_many<F, FINE, 2, 1, 2>(p, st);
+  } else if constexpr (F == MX_F8) {
+    if (tiles(256, 128) >= 384) return launch_many<F, FINE, 4, 2, 2>(p, st);
+    return tiles(128, 128) >= 480 ? launch_many<F, FINE, 2, 2, 2>(p, st) : launch_many<F, FINE, 2, 1, 2>(p, st);
+  } else {
+    if (tiles(256, 256) >= 240 && p.inner >= 4096) return launch_many<F, FINE, 4, 4, 3>(p, st);
+    return tiles(128, 256) >= 512 ? launch_many<F, FINE, 2, 4, 2>(p, st) : launch_many<F, FINE, 2, 2, 2>(p, st);
   }
-  return p.rows <= 16 ? launch_few_rows<F, FINE, 1>(p, st) : p.rows <= 32 ? launch_few_rows<F, FINE, 2>(p, st) : launch_few_rows<F, FINE, 4>(p, st);
 }
 
 }  // namespace

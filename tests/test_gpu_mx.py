@@ -133,7 +133,10 @@ class Product:
         self.hip, self.rows, self.cols, self.inner, self.fmt = hip, rows, cols, inner, fmt
         rng = self.rng = np.random.default_rng([seed, rows, cols, inner])
         self.held = O.quantize(_spread(rng, rows, inner) if x is None else x, fmt)
-        self.w = O.quantize(rng.standard_normal((cols, inner), dtype=np.float32) * 0.05 if w is None else w, "mxf4")
+        if w is None and cols * inner > 1 << 21:   # (quicker: any codes)
+            self.w = (rng.integers(0, 256, (cols, inner // 2), dtype=np.uint8), rng.integers(116, 122, (cols, inner // 32), dtype=np.uint8))
+        else:
+            self.w = O.quantize(rng.standard_normal((cols, inner), dtype=np.float32) * 0.05 if w is None else w, "mxf4")
         self.bias = rng.standard_normal(cols, dtype=np.float32) if bias else None
         self.dev = [hip.put(a) for a in (*self.held, *self.w)]
         self.d_bias = hip.put(self.bias) if bias else None
@@ -166,6 +169,8 @@ class Product:
 SHAPES = [   # rows, columns, inner size: single rows, batches, prompts; odd sizes; inner sizes that are no multiple of 128
     (1, 1152, 896), (1, 896, 4864), (1, 1, 32), (2, 17, 64), (7, 33, 96), (16, 100, 160), (16, 20001, 256), (17, 1152, 896), (31, 48, 4864), (33, 70, 288),
     (64, 130, 896), (65, 128, 128), (100, 257, 512), (128, 129, 384), (200, 1000, 2048), (333, 515, 1152), (513, 300, 4864), (1, 17000, 32), (40, 16500, 96), (1025, 1030, 256),
+    # many columns: slices of the inner size, one to eight, and rows held in LDS
+    (5, 8200, 1504), (16, 8192, 4000), (3, 8300, 8192), (20, 16500, 896), (32, 17000, 96), (1, 8193, 8320),
     # tiles of every size: 128 x 64, 128 x 128 and 256 x 128 (mxf8), 128 x 128, 128 x 256 and 256 x 256 (mxf4)
     (1900, 2000, 128), (3001, 2450, 256), (6450, 3850, 128), (4001, 4002, 4096)]
 

@@ -279,12 +279,24 @@ __global__ __launch_bounds__(256) void pg_read_kernel(PgRead a, int R) {
   int64_t* place = (int64_t*)pg_lds;   // [R] offset of the row's slot (MX: of its page); -1: no sequence's row; -2: it has no place
   int* slot_of = (int*)(place + R);    // [R]
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, first = blockIdx.x * R;
-  for (int i = w; i < R; i += 4) {
-    const int r = first + i;
+  // The sequences of a wave's rows one after the other, then their places side by side (a lane a row).
+  if (w * 64 < R) {
+    const int r = first + w * 64 + lane, rows = min(R - w * 64, 64);
+    int s = a.b.row0 ? -1 : r;
+    if (a.b.row0) {
+      int below = 0;
+      for (int j0 = 0; j0 <= a.b.seqs; j0 += 64) {
+        const int j = j0 + lane, begin = j <= a.b.seqs ? gld(a.b.row0 + j) : 0x7FFFFFFF;
+        for (int i = 0; i < rows; i++) {
+          const int n = __popcll(__ballot(j <= a.b.seqs && begin <= first + w * 64 + i));
+          if (lane == i) below += n;
+        }
+      }
+      s = below - 1;
+    }
     int64_t off = -1;
     int slot = 0;
-    const int s = r >= a.b.rows ? -1 : a.b.row0 ? pg_seq_of(a.b, r, lane) : r;
-    if (s >= 0 && s < a.b.seqs) {
+    if (lane < rows && r < a.b.rows && s >= 0 && s < a.b.seqs) {
       const PgSeq q = pg_seq_at(a.b, s);
       const int t = q.p0 + (r - q.first);
       off = -2;
@@ -294,9 +306,9 @@ __global__ __launch_bounds__(256) void pg_read_kernel(PgRead a, int R) {
         if (page >= 0 && page < a.b.pages) off = page * a.page_stride + (MX ? 0 : slot * a.slot_stride);
       }
     }
-    if (lane == 0) {
-      place[i] = off;
-      slot_of[i] = slot;
+    if (lane < rows) {
+      place[w * 64 + lane] = off;
+      slot_of[w * 64 + lane] = slot;
     }
   }
   __syncthreads();

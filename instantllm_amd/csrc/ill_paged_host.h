@@ -197,7 +197,7 @@ int ill_paged_read(ill_paged* p, const ill_paged_batch* batch, const void* k_cac
                  d.page_stride, d.slot_stride, d.head_stride, illp::mx_codes_of(d), d.kv_heads};
   illp::OnDevice on(p->device);
   if (on.rc) return on.rc;
-  const int R = pg_append_rows(a.b.rows, 2 * d.kv_heads * d.head_dim / 8);
+  const int R = pg_read_rows(a.b.rows);
   hipStream_t st = (hipStream_t)stream;
   HCK(illp::microscaled(d) ? illp::read_mx(out_dtype, a, d.head_dim, R, st) : illp::read_16(out_dtype, d.dtype, a, d.head_dim, R, st));
   return ILL_OK;

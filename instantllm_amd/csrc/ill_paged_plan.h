@@ -143,3 +143,6 @@ PG_FN int64_t pg_grid(int seqs, int rows, bool one_row, int cap, const PgCut& c)
   const int64_t cut = tiles * pg_splits(pg_most(cap, cap, c), c.least);
   return cut < tiles + (1 << c.log) ? cut : tiles + (1 << c.log);
 }
+
+// Rows of a workgroup of the read kernel: up to 16, and fewer where there would be less than four workgroups for each CU.
+PG_FN int pg_read_rows(int rows) { return pg_max(1, pg_min(16, rows / 1024)); }

@@ -382,6 +382,7 @@ struct PgFinder {
     int64_t tiles[NW], work[NW];
     int units[NW], parts[NW], cut[NW];
     PgUnit found;
+    int4 classes[NW];   // units of the waves' sequences, by their keys
   };
   Lds& lds;
 
@@ -509,6 +510,30 @@ struct PgFinder {
         before += x;
         parts += p;
         tiles += t;
+      }
+      if (c.longest && b.seqs <= NT) {   // (then this is the only turn) the units of the most keys first, in four classes
+        const int keys = own.x ? pg_up(most, splits) : 0, of = 2 * keys > part ? 0 : 4 * keys > part ? 1 : 8 * keys > part ? 2 : 3;
+        int4 up = {of == 0 ? own.x : 0, of == 1 ? own.x : 0, of == 2 ? own.x : 0, of == 3 ? own.x : 0};
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) {
+          const int4 o = {__shfl_up(up.x, m), __shfl_up(up.y, m), __shfl_up(up.z, m), __shfl_up(up.w, m)};
+          if (lane >= m) {
+            up.x += o.x;
+            up.y += o.y;
+            up.z += o.z;
+            up.w += o.w;
+          }
+        }
+        if (lane == 63) lds.classes[w] = up;
+        __syncthreads();
+        int4 all = {0, 0, 0, 0}, here = up;   // (here: with the waves before)
+#pragma unroll
+        for (int i = 0; i < NW; i++) {
+          const int4 o = lds.classes[i];
+          all = {all.x + o.x, all.y + o.y, all.z + o.z, all.w + o.w};
+          if (i < w) here = {here.x + o.x, here.y + o.y, here.z + o.z, here.w + o.w};
+        }
+        first = (of == 0 ? here.x : of == 1 ? all.x + here.y : of == 2 ? all.x + all.y + here.z : all.x + all.y + all.z + here.w) - own.x;
       }
       if (u >= first && u < first + own.x) lds.found = unit(u - first, s0 + threadIdx.x, splits, y, z);
       if (u < before) break;
@@ -791,14 +816,16 @@ struct PgStep {
 // Bound by memory where there is enough of it: 64 sequences of 100 to 9000 positions, 32 / 8 heads of 128, 432 MB in 97 us,
 // 4.4 TB/s (a large copy: 5.1). One sequence of 131071, 14 / 2 heads of 64, 67 MB in 19.6 us: 13 at the copy's rate, the rest the
 // launch, three dependent loads at the start (3) and the join. One of 500: 6.5 us, all latency.
+template <bool MX>
 struct PgStepLds {
-  __attribute__((aligned(16))) uint4 lds[PG_WAVES][1024];
+  static constexpr int UNITS = MX ? 544 : 1024;   // of a wave: keys and values of a tile, 8 KB each (MX: values); its state, 16 x (D + 4) floats
+  __attribute__((aligned(16))) uint4 lds[PG_WAVES][UNITS];
   float smx[PG_WAVES][16], sls[PG_WAVES][16];
   int last;
   PgFinder::Lds found;
 };
 template <int TC, int D, bool FINE, bool MX>   // FINE: weights in parts that keep float32 (float32 outputs)
-__device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, PgStepLds& shared) {
+__device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, PgStepLds<MX>& shared) {
   constexpr int NW = PG_WAVES, KT = D == 64 ? 64 : 32, UPR = D / 8, KPI = 64 / UPR, NB = KT / 16, KS = D / 32, ND = D / 16, NS = KT / 32, NG = KT / 16;
   constexpr int N = FINE ? PG_PARTS<TC> : 1;   // parts of a weight
   constexpr int RF = D + 4;   // floats between the rows of a state in LDS
@@ -811,7 +838,7 @@ __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, Pg
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, kg = lane >> 4;
   const int cap = pg_cap(a.b), pmask = (1 << a.b.page_log) - 1;
   LAS uint8_t* kl = (LAS uint8_t*)lds[w];
-  LAS uint8_t* vl = kl + 8192;
+  LAS uint8_t* vl = MX ? kl : kl + 8192;
   const uint32_t mine_lds = pg_lds_at(lds[w]);
   constexpr std::integral_constant<int, 0> KEYS{};
   constexpr std::integral_constant<int, 8192> VALUES{};
@@ -821,7 +848,10 @@ __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, Pg
 #pragma unroll
   for (int ks = 0; ks < KS; ks++) ka[ks] = 16 * pg_unit_at<D>(8 * (n >> 2) + (n & 3), 4 * ks + kg);
 #pragma unroll
-  for (int d = 0; d < ND; d++) va[d] = pg_values_at<D>(8 * kg, 16 * d, n);
+  for (int d = 0; d < ND; d++) {
+    const int key = 4 * kg + (n >> 2), u = 2 * d + (n >> 1 & 1);
+    va[d] = MX ? 16 * (key * UPR + (u ^ (D == 64 ? key & 6 : (key & 7) << 1))) + 8 * (n & 1) : pg_values_at<D>(8 * kg, 16 * d, n);
+  }
   const float sc2 = a.scale * 1.4426950408889634f;
   PgFinder finder(a.b, c, grid, shared.found);
   auto over_kg = [](float v, auto op) {   // over the lanes of the same row
@@ -876,53 +906,55 @@ __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, Pg
       });
     });
   };
-  // MX: a tile's codes and powers come through registers, the next tile's as soon as this one's have been used. A lane's keys are its score
-  // products' (16 dims of 64 at a time: the products' dims are dealt the same way to queries and keys), its values any 16 bytes.
+  // MX: a tile's codes and powers come through registers, the next tile's as soon as this one's have been used; the values go on into LDS as 16-bit
+  // ones. A lane's codes of a key are 16 dims of 64 at a time (the products' dims are dealt the same way to queries and keys), block b's
+  // keys are 16 b + n: a load has neighbouring keys of one page.
   uint4 kreg[NB][D / 64], vreg[4];
   uint32_t kpow[NB], vpow[4];
-  auto mx_page = [&](int k, int g) {   // the page of a group of the wave's tile k (behind the last: the first one, which is there)
-    const int64_t at = group_at(k, g);
-    return k < mine && at > 0 ? at : 0;
-  };
-  auto mx_slot = [&](int k, int g) {   // where in its page: keys from the page's begin, of all heads
-    return (un.head << a.b.page_log) + (k < mine ? (pg_key_tile(range, c0 + w + NW * k) * KT + 16 * g) & pmask : 0);
+  auto mx_group = [&](const void* cache, int k, int g, const uint8_t*& powers) {   // where a group's codes and powers are (behind the last tile: the first page's, which are there)
+    const int64_t at = group_at(k, g), page = k < mine && at > 0 ? at : 0;
+    const int slot = (un.head << a.b.page_log) + (k < mine ? (pg_key_tile(range, c0 + w + NW * k) * KT + 16 * g) & pmask : 0);
+    powers = (const uint8_t*)cache + page + a.powers_at + slot * (D / 32);
+    return (const uint8_t*)cache + page + slot * D;
   };
   auto mx_keys = [&](int k) {
-    const uint8_t* cache = (const uint8_t*)a.kc;
-    pg_each<NB / 2>([&](auto i) {
-      const int64_t p0 = mx_page(k, 2 * i), p1 = mx_page(k, 2 * i + 1);
-      const uint8_t* page = cache + (n & 8 ? p1 : p0);
-      const int first = n & 8 ? mx_slot(k, 2 * i + 1) : mx_slot(k, 2 * i);
+    pg_each<NB>([&](auto b) {
+      const uint8_t *powers, *codes = mx_group(a.kc, k, b, powers);
 #pragma unroll
-      for (int odd = 0; odd < 2; odd++) {
-        const int b = 2 * i + odd, row = first + ((8 * (n >> 2) + 4 * odd + (n & 3)) & 15);
-#pragma unroll
-        for (int j = 0; j < D / 64; j++) kreg[b][j] = gld((const uint4*)(page + row * D + 64 * j + 16 * kg));
-        if constexpr (D == 64) kpow[b] = gld(page + a.powers_at + 2 * row + (kg >> 1));
-        else kpow[b] = gld((const uint32_t*)(page + a.powers_at + 4 * row)) >> 8 * (kg >> 1);   // bytes 0 and 2
-      }
+      for (int j = 0; j < D / 64; j++) kreg[b][j] = gld((const uint4*)(codes + (uint32_t)(D * n + 16 * kg) + 64 * j));
+      if constexpr (D == 64) kpow[b] = gld(powers + (uint32_t)(2 * n + (kg >> 1)));
+      else kpow[b] = gld((const uint32_t*)(powers + (uint32_t)(4 * n)));
     });
   };
   constexpr int VL = 16 * D / 1024, LPK = D / 16;   // loads of a group's values; lanes of a key
   auto mx_vals = [&](int k) {
     pg_each<NG>([&](auto g) {
-      const uint8_t* page = (const uint8_t*)a.vc + mx_page(k, g);
-      const int first = mx_slot(k, g);
+      const uint8_t *powers, *codes = mx_group(a.vc, k, g, powers);
 #pragma unroll
       for (int j = 0; j < VL; j++) {
-        const int row = first + 64 / LPK * j + lane / LPK;
-        vreg[VL * g + j] = gld((const uint4*)(page + row * D + 16 * (lane % LPK)));
-        vpow[VL * g + j] = gld(page + a.powers_at + (D / 32) * row + (lane % LPK >> 1));
+        vreg[VL * g + j] = gld((const uint4*)(codes + (uint32_t)(16 * lane) + 1024 * j));
+        vpow[VL * g + j] = gld(powers + (uint32_t)((D / 32) * (lane / LPK) + (lane % LPK >> 1)) + 32 * j);
       }
     });
   };
-  auto mx_put = [&] {   // the values into LDS, as the other caches' come there
+  // Where the 16 bytes u of a key's values lie: the 16 keys x 32 bytes of a transposed read are on different banks.
+  auto mx_unit = [](int key, int u) { return 16 * (key * UPR + (u ^ (D == 64 ? key & 6 : (key & 7) << 1))); };
+  auto mx_put = [&] {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       const int key = 64 / LPK * i + lane / LPK, u = 2 * (lane % LPK);
       const uint4 lo = mx_16<TC, MX_F8>({vreg[i].x, vreg[i].y}, vpow[i]), hi = mx_16<TC, MX_F8>({vreg[i].z, vreg[i].w}, vpow[i]);
-      *(pg_lds4*)(vl + 16 * pg_unit_at<D>(key, u)) = (gu32x4){lo.x, lo.y, lo.z, lo.w};
-      *(pg_lds4*)(vl + 16 * pg_unit_at<D>(key, u + 1)) = (gu32x4){hi.x, hi.y, hi.z, hi.w};
+      *(pg_lds4*)(vl + mx_unit(key, u)) = (gu32x4){lo.x, lo.y, lo.z, lo.w};
+      *(pg_lds4*)(vl + mx_unit(key, u + 1)) = (gu32x4){hi.x, hi.y, hi.z, hi.w};
+    }
+  };
+  // This lane's operand of 32 keys' values, 16 dims: keys 4 kg .. and 16 + 4 kg .., as its weights are.
+  auto values = [&](int d, int t) {
+    if constexpr (MX) {
+      const uint2 x = pg_tr(vl + va[d] + 32 * t * 2 * D), y = pg_tr(vl + va[d] + (32 * t + 16) * 2 * D);
+      return uint4{x.x, x.y, y.x, y.y};
+    } else {
+      return pg_values<D>(vl + va[d] + 32 * t * 2 * D);
     }
   };
   float Mx, Ls;   // Ls: this lane's keys only
@@ -956,7 +988,7 @@ __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, Pg
         for (int ks = 0; ks < KS; ks++) {
           if constexpr (MX) {
             const uint4 c = kreg[b][ks / 2];
-            s[b] = pg_mfma16<TC>(mx_16<TC, MX_F8>(ks & 1 ? uint2{c.z, c.w} : uint2{c.x, c.y}, kpow[b] >> 16 * (ks / 2) & 255), qf[ks], s[b]);
+            s[b] = pg_mfma16<TC>(mx_16<TC, MX_F8>(ks & 1 ? uint2{c.z, c.w} : uint2{c.x, c.y}, D == 64 ? kpow[b] : kpow[b] >> (8 * (kg >> 1) + 16 * (ks / 2)) & 255), qf[ks], s[b]);
           } else {
             s[b] = pg_mfma16<TC>(pg_get(kl + ka[ks] + (32 * (b >> 1) + 4 * (b & 1)) * 2 * D), qf[ks], s[b]);
           }
@@ -983,7 +1015,7 @@ __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, Pg
         for (int b = 0; b < NB; b++)
 #pragma unroll
           for (int r = 0; r < 4; r++) {
-            const int key = 32 * (b >> 1) + 8 * kg + 4 * (b & 1) + r, j = kt + key;
+            const int key = MX ? 16 * b + 4 * kg + r : 32 * (b >> 1) + 8 * kg + 4 * (b & 1) + r, j = kt + key;
             // pg_sees, by selects
             const bool on = j < cap & j <= pos & (c.window == 0 | j > pos - c.window | j < c.sinks) & (good >> (key >> 4) & 1);
             s[b][r] = on ? s[b][r] : -INFINITY;
@@ -1035,7 +1067,7 @@ __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, Pg
 #pragma unroll
           for (int t = 0; t < NS; t++) {
             uint4 marks;
-            const uint4 v = pg_tamed<TC>(pg_values<D>(vl + va[d] + 32 * t * 2 * D), marks);
+            const uint4 v = pg_tamed<TC>(values(d, t), marks);
 #pragma unroll
             for (int i = 0; i < N; i++) O[d] = pg_mfma16<TC>(v, __builtin_bit_cast(uint4, ph[i][t]), O[d]);
             m = pg_mfma16<TC>(marks, pg_ones<TC>(seen >> (8 * t)), m);
@@ -1048,7 +1080,7 @@ __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, Pg
         for (int d = 0; d < ND; d++)
 #pragma unroll
           for (int t = 0; t < NS; t++) {
-            const uint4 v = pg_values<D>(vl + va[d] + 32 * t * 2 * D);
+            const uint4 v = values(d, t);
 #pragma unroll
             for (int i = 0; i < N; i++) O[d] = pg_mfma16<TC>(v, __builtin_bit_cast(uint4, ph[i][t]), O[d]);
           }
@@ -1437,7 +1469,7 @@ __device__ __forceinline__ void pg_prompt(const PgStep& p, int block, int grid, 
 
 template <int TC, int D, bool FINE, bool MX>
 __global__ __launch_bounds__(PG_THREADS, 2) void pg_step_kernel(PgStep p) {
-  __shared__ PgStepLds lds;
+  __shared__ PgStepLds<MX> lds;
   pg_step<TC, D, FINE, MX>(p, blockIdx.x, gridDim.x, lds);
 }
 template <int TC, int D, bool FINE, bool MX>
@@ -1455,7 +1487,7 @@ struct PgBoth {
 template <int TC, int D, bool FINE, bool MX>
 __global__ __launch_bounds__(PG_THREADS, 2) void pg_both_kernel(PgBoth p) {
   __shared__ union Lds {
-    PgStepLds step;
+    PgStepLds<MX> step;
     PgPromptLds<D, MX> prompt;
     __device__ Lds() {}
   } lds;

@@ -2,6 +2,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <optional>
 
 #include "ill_error.h"
 #include "ill_launch.h"
@@ -15,12 +16,21 @@ using illp::launch;
 
 constexpr int SLICE_WAVES = 8;   // of a CU: as many as its registers hold
 
-// The GPU that a stream belongs to; of the default streams the current one.
-int device_of(hipStream_t st, int* dev) {
-  if (!st || st == hipStreamLegacy || st == hipStreamPerThread) HCK(hipGetDevice(dev));
-  else HCK(hipStreamGetDevice(st, dev));
-  return ILL_OK;
-}
+// While this lives the current device is the one that the stream belongs to (a default stream belongs to the current one).
+struct OnStream {
+  int rc = ILL_OK;
+  std::optional<illp::OnDevice> on;
+  explicit OnStream(hipStream_t st) {
+    if (!st || st == hipStreamLegacy || st == hipStreamPerThread) return;
+    int dev = 0;
+    if (hipStreamGetDevice(st, &dev) != hipSuccess) {
+      rc = fail(ILL_E_HIP, "mx: the stream belongs to no device");
+      return;
+    }
+    on.emplace(dev);
+    rc = on->rc;
+  }
+};
 
 template <int T, int F>
 hipError_t launch_rows(bool back, const MxRows& a, hipStream_t st) {
@@ -36,9 +46,7 @@ int rows(bool back, int format, int dtype, const void* x, int64_t stride, int64_
   if (int rc = check_rows(format, dtype, x, stride, rows, cols, codes, powers)) return rc;
   if (!rows) return ILL_OK;
   hipStream_t st = (hipStream_t)stream;
-  int dev = 0;
-  if (int rc = device_of(st, &dev)) return rc;
-  illp::OnDevice on(dev);
+  OnStream on(st);
   if (on.rc) return on.rc;
   const MxRows a{(uint8_t*)x, (uint8_t*)codes, (uint8_t*)powers, stride, (uint32_t)(rows * cols / 8), (uint32_t)(cols / 8)};
   HCK(format == ILL_MXF8 ? launch_rows<MX_F8>(back, dtype, a, st) : launch_rows<MX_F4>(back, dtype, a, st));
@@ -121,9 +129,7 @@ int ill_mx_product(int x_format, const void* x, const void* x_powers, const void
   if (int rc = illm::check_product(x_format, x, x_powers, w, w_powers, bias, y, y_stride, y_dtype, rows, cols, inner)) return rc;
   if (!rows) return ILL_OK;
   hipStream_t st = (hipStream_t)stream;
-  int dev = 0;
-  if (int rc = illm::device_of(st, &dev)) return rc;
-  illp::OnDevice on(dev);
+  illm::OnStream on(st);
   if (on.rc) return on.rc;
   const int size = y_dtype == ILL_F32 ? 4 : 2;
   const int wide = y_stride % (16 / size) == 0 && illm::aligned(y, 16) ? 2 : y_stride % 4 == 0 && illm::aligned(y, 4 * size) ? 1 : 0;

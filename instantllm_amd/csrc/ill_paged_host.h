@@ -29,7 +29,7 @@ PgCut step_cut(const ill_paged_desc& d, int window, int sinks) {
   return {(uint32_t)(d.heads / d.kv_heads), (uint32_t)d.kv_heads, 16, d.head_dim == 64 ? 64 : 32, window, sinks, 8, microscaled(d) ? 16 : 8, 0, PG_MOST, 0, microscaled(d)};
 }
 PgCut prompt_cut(const ill_paged_desc& d, int window, int sinks) {
-  return {(uint32_t)(d.heads / d.kv_heads), (uint32_t)d.kv_heads, 128, 64, window, sinks, 7, 4, 0, PG_MOST, 0, 0};
+  return {(uint32_t)(d.heads / d.kv_heads), (uint32_t)d.kv_heads, 128, 64, window, sinks, 7, 4, 0, PG_MOST, 0, microscaled(d)};
 }
 
 // Bytes of a workspace where 2^log parts are wanted, over tiles of M rows.

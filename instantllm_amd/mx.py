@@ -19,7 +19,7 @@ def _one_of(what: str, name: str, of: dict[str, int]) -> int:
     return of[name]
 
 
-def _fits(**values: int):
+def _fits(**values: int):   # (ctypes cuts numbers off; asked where one of them is large or negative: those are the library's to refuse)
     for name, v in values.items():
         if not -1 << 63 <= v < 1 << 63:
             raise ValueError(f"{name} {v}: more than 64 bits")
@@ -39,7 +39,8 @@ def quantize(x: int, codes: int, powers: int, rows: int, cols: int, format: str 
              stream: int | None = None):
     """x [rows][cols] of type dtype to codes and powers."""
     x_stride = cols if x_stride is None else x_stride
-    _fits(rows=rows, cols=cols, x_stride=x_stride)
+    if (rows | cols | x_stride) >> 62:
+        _fits(rows=rows, cols=cols, x_stride=x_stride)
     rc = load_library().ill_mx_quantize(_one_of("format", format, FORMATS), _one_of("type", dtype, DTYPES), x, x_stride, rows, cols, codes, powers, stream)
     if rc:
         _check(rc)
@@ -49,7 +50,8 @@ def dequantize(codes: int, powers: int, y: int, rows: int, cols: int, format: st
                stream: int | None = None):
     """codes and powers to values y [rows][cols] of type dtype."""
     y_stride = cols if y_stride is None else y_stride
-    _fits(rows=rows, cols=cols, y_stride=y_stride)
+    if (rows | cols | y_stride) >> 62:
+        _fits(rows=rows, cols=cols, y_stride=y_stride)
     rc = load_library().ill_mx_dequantize(_one_of("format", format, FORMATS), _one_of("type", dtype, DTYPES), codes, powers, rows, cols, y, y_stride, stream)
     if rc:
         _check(rc)
@@ -60,7 +62,8 @@ def product(x: int, x_powers: int, w: int, w_powers: int, y: int, rows: int, col
     """y [rows][cols] of type dtype: microscaled rows x [rows][inner] of the format times the rows of w [cols][inner], of format
     mxf4, plus bias [cols] (float32)."""
     y_stride = cols if y_stride is None else y_stride
-    _fits(rows=rows, cols=cols, inner=inner, y_stride=y_stride)
+    if (rows | cols | inner | y_stride) >> 62:
+        _fits(rows=rows, cols=cols, inner=inner, y_stride=y_stride)
     rc = load_library().ill_mx_product(_one_of("format", format, FORMATS), x, x_powers, w, w_powers, rows, cols, inner, bias,
                                        _one_of("type", dtype, DTYPES), y, y_stride, stream)
     if rc:

@@ -129,7 +129,8 @@ class PagedAttention:
              v_stride: int | None = None, stream: int | None = None):
         """The batch's rows out of the cache: keys to k, values to v, of type dtype (None: the handle's) or "f32"."""
         k_stride, v_stride = self.kv_width if k_stride is None else k_stride, self.kv_width if v_stride is None else v_stride
-        _fits(64, k_stride=k_stride, v_stride=v_stride)
+        if (k_stride | v_stride) >> 31:
+            _fits(64, k_stride=k_stride, v_stride=v_stride)
         rc = self.lib.ill_paged_read(self.h, C.byref(batch), k_cache, v_cache, k, k_stride, v, v_stride, self.type if dtype is None else _dtype(dtype), stream)
         if rc:
             self._check(rc)

@@ -231,9 +231,9 @@ __global__ __launch_bounds__(L < 4 ? 256 : 64 * L) void mx_slice_kernel(MxProduc
     for (int u = 0; u < CH; u++) c.w[u] = gld((const uint4*)(wr + 16 * min(4 * min(s0 + u, steps - 1) + g, blocks - 1)));   // (what is behind the last is not read)
 #pragma unroll
     for (int i = 0; i < 2; i++) {   // a column's powers of two steps, each four bytes: the lanes of the others have them exchanged
-      const int64_t at = col * blocks + 4 * min(s0 + 2 * g + i, steps - 1), from = min(at, max(end, (int64_t)0));
+      const int64_t at = col * blocks + 4 * min(s0 + 2 * g + i, steps - 1), from = min(at, end);   // (behind the matrix nothing is read)
       typedef uint32_t word __attribute__((aligned(1)));
-      c.wp[i] = end < 0 ? gld(p.wp + at) : *(const GAS word*)(p.wp + from) >> 8 * (int)(at - from);
+      c.wp[i] = *(const GAS word*)(p.wp + from) >> 8 * (int)(at - from);
     }
   };
   int tile = blockIdx.x * G + group, turn = 0;

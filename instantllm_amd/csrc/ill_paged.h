@@ -101,8 +101,14 @@ __global__ __launch_bounds__(256) void pg_append_kernel(PgAppend a, int R) {
   auto item = [&](int it) {
     Item x;
     const uint32_t c = (uint32_t)it % C, v = (uint32_t)it / C;
-    x.i = v / (uint32_t)nh;
-    x.head = h0 + v - x.i * nh;
+    if constexpr (MX) {   // queries first, so that few waves have both them and what is quantised
+      const uint32_t qs = R * (uint32_t)(a.heads - h0), nk = 2 * a.kv;
+      x.i = v < qs ? v / (uint32_t)a.heads : (v - qs) / nk;
+      x.head = v < qs ? v - x.i * a.heads : a.heads + (v - qs) - x.i * nk;
+    } else {
+      x.i = v / (uint32_t)nh;
+      x.head = h0 + v - x.i * nh;
+    }
     x.r = first + x.i;
     x.kind = x.head < a.heads ? 0 : x.head < a.heads + a.kv ? 1 : 2;
     x.hk = x.head - (x.kind == 0 ? 0 : x.kind == 1 ? a.heads : a.heads + a.kv);

@@ -292,6 +292,12 @@ ILL_API int ill_gemv_destroy(ill_gemv* g);
  * with i + rotary_dim / 2, or with interleaved != 0 dims 2 i and 2 i + 1. norm_eps belongs to the head norms; scale
  * multiplies the scores (0: 1 / sqrt(head_dim)). A handle belongs to the GPU that was current
  * when it was created; one thread at a time calls on it.
+ * dtype ILL_F16 | ILL_MXF8 or ILL_BF16 | ILL_MXF8: a cache of microscaled 8-bit values (ILL_MXF8 below) for queries and outputs
+ * of the other type, 33 bytes for 32 values. A page is [kv_heads][page_size][head_dim] codes followed by [kv_heads][page_size]
+ * [head_dim / 32] powers; page_stride is the bytes from one page to the next (a multiple of 16; 0: no gap), slot_stride and
+ * head_stride are 0. ill_paged_append quantises each head's blocks of 32 as ill_mx_quantize does, from the float32 values; an infinity
+ * or NaN makes its block NaN. ill_paged_attend takes the cache's values as values of the handle's type: bf16 has an exact place for
+ * all but the least of them, f16 rounds below 2^-14 and is infinite past 65504. Everything else holds for either kind of cache.
  * Attention that is split over the keys joins its parts through a workspace, one of `streams`
  * that the handle holds (0: 8; 11 MB each at head size 64, 22 at 128). Each stream that calls
  * come on takes one, and so does each capture of a stream: calls on different streams, and
@@ -365,7 +371,7 @@ ILL_API int ill_paged_append(ill_paged* p, const ill_paged_batch* batch, const i
  * cache's, or ILL_F32): the values weighted by the softmax of the scaled scores; zeros for a row
  * that sees nothing (or whose scores are all -inf). Sums are float32, of weights of at most 1 for a
  * bf16 cache (an f16 cache's values cannot overflow them). q [rows][heads x head_dim] is of the
- * cache's type; out overlaps nothing that the call reads. What a row does not see never reaches it, infinities and NaN included. A value
+ * handle's type; out overlaps nothing that the call reads. What a row does not see never reaches it, infinities and NaN included. A value
  * that is infinite or NaN reaches every row that sees it, however small its weight: the output
  * is that infinity, or NaN where the row also sees a NaN or the other one; unless all of the
  * row's scores are -inf, or one is +inf or NaN (the row is then NaN). */
@@ -390,18 +396,21 @@ ILL_API int ill_paged_read(ill_paged* p, const ill_paged_batch* batch, const voi
  * ill_mx_quantize: x [rows][cols] of type `dtype`, row r at r * x_stride elements (a multiple of 8, float32: 4; x aligned to 16
  * bytes). A block's power is floor(log2(the largest size in it)) - 8 (ILL_MXF4: - 2), at least 2^-127; its values divided by it
  * are rounded to nearest, ties to even, and end at +-448 (+-6). A block that holds an infinity or NaN becomes NaN (codes 0).
- * ill_mx_dequantize: the values, rounded to `dtype` where they have no exact place in it. Up to 2^34 values a call. */
+ * ill_mx_dequantize: the values, rounded to `dtype` where they have no exact place in it. Up to 2^34 values a call. What a call writes
+ * overlaps nothing that it reads. */
 ILL_API int ill_mx_quantize(int format, int dtype, const void* x, int64_t x_stride, int64_t rows, int64_t cols, void* codes, void* powers, void* stream);
 ILL_API int ill_mx_dequantize(int format, int dtype, const void* codes, const void* powers, int64_t rows, int64_t cols, void* y, int64_t y_stride,
                               void* stream);
 
 /* y[r][c] = the sum over k of x[r][k] w[c][k], plus bias[c] (NULL: none): x [rows][inner] of format x_format, the matrix w
  * [cols][inner] of format ILL_MXF4, both as ill_mx_quantize writes them. y: row r at r * y_stride elements of type y_dtype, rounded
- * once. inner: a multiple of 32 up to 2^20 (multiples of 128 take the fast path of many rows); cols up to 2^24, rows up to 2^26, rows x cols up to 2^32. Sums are
- * float32's. With x of format ILL_MXF8 and a 16-bit y they are the matrix units' own, which drop parts of a product far below the
- * largest of its group: 4e-6 of the sums' size for normal values, 5e-5 for codes of evenly spread exponents; the sums for a float32 y are not
- * cut. The result does not depend on which other rows or columns are computed with it only as far as the same kernel takes them. y overlaps nothing
- * that the call reads. A NaN block makes every output that it belongs to NaN. */
+ * once; aligned to its type (to 16 bytes, with strides of whole 16 bytes, it is stored fastest). inner: a multiple of 32 up to 2^20
+ * (from 17 rows on, multiples of 128 are several times as fast); cols up to 2^24, rows up to 2^26, rows x cols up to 2^32.
+ * Sums are float32's, in an order that depends on the three sizes alone. With x of format ILL_MXF8 and a 16-bit y they are the matrix units' own, which
+ * drop parts of a product far below the largest of its group: 4e-6 of the result (2-norm) for normal values, 5e-5 for codes of evenly spread
+ * exponents. For a float32 y of such x both operands are multiplied as bf16 values: not cut, but values below 2^-126 may count
+ * as 0, and ones past bf16's range as infinite. A NaN block makes every output that it belongs to NaN. y overlaps nothing that the
+ * call reads. */
 ILL_API int ill_mx_product(int x_format, const void* x, const void* x_powers, const void* w, const void* w_powers, int64_t rows, int64_t cols,
                            int64_t inner, const float* bias, int y_dtype, void* y, int64_t y_stride, void* stream);
 

@@ -345,12 +345,12 @@ typedef struct {
 } ill_paged_batch;
 
 /* New rows into the cache. q, k, v: rows of heads x head_dim (kv_heads x head_dim) values of
- * type `dtype` (ILL_F32, or the cache's), row r at r * stride elements; parts of one fused
+ * type `dtype` (ILL_F32, or the handle's), row r at r * stride elements; parts of one fused
  * product will do. q NULL: keys and values only. To each head's x: x + bias (bias [(heads + 2
  * kv_heads) x head_dim], q then k then v), then for q and k x / sqrt(mean(x^2) + norm_eps) *
  * q_norm (k_norm) [head_dim], then the rotation by the row's position (positions [rows]: by
  * these instead), computed in float32 from angles in float64 and rounded once. NULL leaves a
- * step out. Keys and values go to their slots, queries to q_out (the cache's type; q itself
+ * step out. Keys and values go to their slots, queries to q_out (the handle's type; q itself
  * will do where type and stride agree). Two rows of one batch must not share a slot, and
  * q_out and the caches overlap nothing else that the call reads. Buffers
  * and caches are aligned to 16 bytes, strides are multiples of 8 elements (float32: 4). */
@@ -368,7 +368,7 @@ ILL_API int ill_paged_append(ill_paged* p, const ill_paged_batch* batch, const i
 /* Attention of the new rows over the cache (what ill_paged_append has written included): the
  * row at position p sees the positions j <= p with j > p - window (window 0: all of them) or
  * j < sinks. out [rows][heads x head_dim], row r at r * out_stride, of type out_dtype (the
- * cache's, or ILL_F32): the values weighted by the softmax of the scaled scores; zeros for a row
+ * handle's, or ILL_F32): the values weighted by the softmax of the scaled scores; zeros for a row
  * that sees nothing (or whose scores are all -inf). Sums are float32, of weights of at most 1 for a
  * bf16 cache (an f16 cache's values cannot overflow them). q [rows][heads x head_dim] is of the
  * handle's type; out overlaps nothing that the call reads. What a row does not see never reaches it, infinities and NaN included. A value
@@ -405,7 +405,7 @@ ILL_API int ill_mx_dequantize(int format, int dtype, const void* codes, const vo
 /* y[r][c] = the sum over k of x[r][k] w[c][k], plus bias[c] (NULL: none): x [rows][inner] of format x_format, the matrix w
  * [cols][inner] of format ILL_MXF4, both as ill_mx_quantize writes them. y: row r at r * y_stride elements of type y_dtype, rounded
  * once; aligned to its type (to 16 bytes, with strides of whole 16 bytes, it is stored fastest). inner: a multiple of 32 up to 2^20
- * (from 17 rows on, multiples of 128 are several times as fast); cols up to 2^24, rows up to 2^26, rows x cols up to 2^32.
+ * (from 17 rows on, multiples of 128 are up to 1.6 times as fast); cols up to 2^24, rows up to 2^26, rows x cols up to 2^32.
  * Sums are float32's, in an order that depends on the three sizes alone. With x of format ILL_MXF8 and a 16-bit y they are the matrix units' own, which
  * drop parts of a product far below the largest of its group: 4e-6 of the result (2-norm) for normal values, 5e-5 for codes of evenly spread
  * exponents. For a float32 y of such x both operands are multiplied as bf16 values: not cut, but values below 2^-126 may count

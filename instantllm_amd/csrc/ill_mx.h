@@ -19,7 +19,7 @@ __device__ __forceinline__ int64_t mx_at(const MxRows& a, uint32_t i) {   // the
   const uint32_t r = i / a.per;
   return r * a.stride + 8 * (int64_t)(i - r * a.per);
 }
-// A thread takes eight values at a time, so that four neighbours have a block.
+// A thread takes eight values at a time, so that four neighbours have a block. Bound by memory: 4096 x 4864 bf16 values to mxf4, 50 MB, 9.0 to 10.2 us.
 template <int T, int F>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(MxRows a) {
   constexpr int EB = T == PG_F32 ? 4 : 2;
@@ -132,48 +132,38 @@ __device__ __forceinline__ v4f mx_mfma16(const MxOperand& w, uint32_t wp, const 
   return c;
 }
 
-// Few rows, or an inner size that is no multiple of 128. A wave multiplies 16 columns by 16 R rows over its share of the inner size: 128 at a
+// Few tiles: a workgroup multiplies 16 rows by 16 columns, its four waves a share of the inner size each, joined in LDS in their order: 128 at a
 // time, straight from memory (a lane's 32 codes of a column are 16 bytes; of an mxf8 row 16 + 16, as the instruction divides them, or 32
-// together where they become bf16). The four waves of a workgroup share the inner size of a tile and are joined in LDS, in their order.
-template <int F, bool FINE, int R>
+// together where they become bf16). Bound by latency: 1 x 1152 over 896 3.2 us, 1 x 896 over 4864 4.7.
+template <int F, bool FINE>
 __global__ __launch_bounds__(256) void mx_few_kernel(MxProduct p, int tiles) {   // tiles: workgroups for the columns
-  constexpr int U = R == 4 ? 2 : 4;   // steps whose loads are in flight together
-  __shared__ __attribute__((aligned(16))) v4f part[4][R][64];
+  constexpr int U = 4;   // steps whose loads are in flight together
+  __shared__ __attribute__((aligned(16))) v4f part[4][64];
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-  const int row_tile = blockIdx.x / (uint32_t)tiles, tile = blockIdx.x - row_tile * tiles, r0 = 16 * R * row_tile, c0 = 16 * tile;
+  const int row_tile = blockIdx.x / (uint32_t)tiles, r0 = 16 * row_tile, c0 = 16 * (blockIdx.x - row_tile * tiles);
   const int blocks = p.inner >> 5, steps = (blocks + 3) >> 2, each = (steps + 3) / 4;
   const int s0 = min(each * w, steps), s1 = min(s0 + each, steps);
-  const int64_t wc = min(c0 + n, p.cols - 1);
-  const uint8_t *wr = p.w + wc * (p.inner / 2), *wpr = p.wp + wc * blocks;
-  const uint8_t *xr[R], *xpr[R];
-#pragma unroll
-  for (int i = 0; i < R; i++) {
-    const int64_t r = min(r0 + 16 * i + n, p.rows - 1);
-    xr[i] = p.x + r * mx_bytes<F>(p.inner);
-    xpr[i] = p.xp + r * blocks;
-  }
-  v4f acc[R] = {};
+  const int64_t col = min(c0 + n, p.cols - 1), row = min(r0 + n, p.rows - 1);
+  const uint8_t *wr = p.w + col * (p.inner / 2), *wpr = p.wp + col * blocks, *xr = p.x + row * mx_bytes<F>(p.inner), *xpr = p.xp + row * blocks;
+  v4f acc = {0.f, 0.f, 0.f, 0.f};
   const uint4 none = {0, 0, 0, 0};
   for (int s = s0; s < s1; s += U) {
-    MxOperand a[U], b[U][R];
-    uint32_t ap[U], bp[U][R];
+    MxOperand a[U], b[U];
+    uint32_t ap[U], bp[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      const int at = min(s + u, s1 - 1), block = 4 * at + g, first = min(block, blocks - 1);   // (blocks behind the last are not read)
+      const int at = min(s + u, s1 - 1), first = min(4 * at + g, blocks - 1);   // (blocks behind the last are not read)
       a[u].lo = gld((const uint4*)(wr + 16 * first));
       ap[u] = gld(wpr + first);
-#pragma unroll
-      for (int i = 0; i < R; i++) {
-        bp[u][i] = gld(xpr[i] + first);
-        if constexpr (F == MX_F4) {
-          b[u][i].lo = gld((const uint4*)(xr[i] + 16 * first));
-        } else if constexpr (FINE) {
-          b[u][i].lo = gld((const uint4*)(xr[i] + 32 * first));
-          b[u][i].hi = gld((const uint4*)(xr[i] + 32 * first + 16));
-        } else {
-          b[u][i].lo = gld((const uint4*)(xr[i] + 32 * min(4 * at + (g >> 1), blocks - 1) + 16 * (g & 1)));
-          b[u][i].hi = gld((const uint4*)(xr[i] + 32 * min(4 * at + 2 + (g >> 1), blocks - 1) + 16 * (g & 1)));
-        }
+      bp[u] = gld(xpr + first);
+      if constexpr (F == MX_F4) {
+        b[u].lo = gld((const uint4*)(xr + 16 * first));
+      } else if constexpr (FINE) {
+        b[u].lo = gld((const uint4*)(xr + 32 * first));
+        b[u].hi = gld((const uint4*)(xr + 32 * first + 16));
+      } else {
+        b[u].lo = gld((const uint4*)(xr + 32 * min(4 * at + (g >> 1), blocks - 1) + 16 * (g & 1)));
+        b[u].hi = gld((const uint4*)(xr + 32 * min(4 * at + 2 + (g >> 1), blocks - 1) + 16 * (g & 1)));
       }
     }
 #pragma unroll
@@ -181,37 +171,29 @@ __global__ __launch_bounds__(256) void mx_few_kernel(MxProduct p, int tiles) {  
       if (s + u >= s1) break;
       if (4 * (s + u) + 4 > blocks) {   // zeros for the blocks behind the last
         const int block = 4 * (s + u) + g;
+        const bool apart = F == MX_F8 && !FINE;
         if (block >= blocks) {
           a[u].lo = none;
-          ap[u] = 127;
+          ap[u] = bp[u] = 127;
         }
-#pragma unroll
-        for (int i = 0; i < R; i++) {
-          const bool apart = F == MX_F8 && !FINE;
-          if (block >= blocks) bp[u][i] = 127;
-          if ((apart ? 4 * (s + u) + (g >> 1) : block) >= blocks) b[u][i].lo = none;
-          if ((apart ? 4 * (s + u) + 2 + (g >> 1) : block) >= blocks) b[u][i].hi = none;
-        }
+        if ((apart ? 4 * (s + u) + (g >> 1) : block) >= blocks) b[u].lo = none;
+        if ((apart ? 4 * (s + u) + 2 + (g >> 1) : block) >= blocks) b[u].hi = none;
       }
-#pragma unroll
-      for (int i = 0; i < R; i++) acc[i] = mx_mfma16<F, FINE>(a[u], ap[u], b[u][i], bp[u][i], acc[i]);
+      acc = mx_mfma16<F, FINE>(a[u], ap[u], b[u], bp[u], acc);
     }
   }
-#pragma unroll
-  for (int i = 0; i < R; i++) part[w][i][lane] = acc[i];
+  part[w][lane] = acc;
   __syncthreads();
-  for (int i = w; i < R; i += 4) {
-    v4f y = part[0][i][lane];
+  const int r = r0 + n, c = c0 + 4 * g;
+  if (w || r >= p.rows || c >= p.cols) return;
 #pragma unroll
-    for (int k = 1; k < 4; k++) y += part[k][i][lane];
-    const int r = r0 + 16 * i + n, c = c0 + 4 * g;
-    if (r < p.rows && c < p.cols) mx_store4(p, r, c, y + mx_bias4(p, c));
-  }
+  for (int k = 1; k < 4; k++) acc += part[k][lane];
+  mx_store4(p, r, c, acc + mx_bias4(p, c));
 }
 
 // Up to 16 rows. The inner size is cut into L slices of up to CH steps, one to a wave; a wave holds its slice of the rows in registers and
 // goes from tile to tile of 16 columns, whose next codes are on their way while it multiplies. The slices' sums are joined in LDS, in their order, by
-// each of the waves in turn.
+// each of the waves in turn. Bound by memory: 16 x 151936 over 896 16.4 us, 4.7 TB/s, 16 x 32000 over 8192 in mxf4 37 us, 3.8 TB/s.
 template <int F, bool FINE, int L>
 __global__ __launch_bounds__(L < 4 ? 256 : 64 * L) void mx_slice_kernel(MxProduct p, int tiles) {
   constexpr int CH = 8, WAVES = L < 4 ? 4 : L, G = WAVES / L;   // G: tiles that a workgroup computes at a time
@@ -301,7 +283,8 @@ __global__ __launch_bounds__(L < 4 ? 256 : 64 * L) void mx_slice_kernel(MxProduc
 }
 
 // Few rows and many columns: the matrix is read once, as fast as memory gives it. The rows lie in LDS as operands, for every wave of the
-// workgroup and for all of its tiles of 16 columns; a wave holds up to CH steps of a tile and loads the next ones while it multiplies.
+// workgroup and for all of its tiles of 16 columns; a wave holds up to CH steps of a tile and loads the next ones while it multiplies. 32 x 151936 over
+// 896 22.9 us, 3.6 TB/s.
 template <int F, bool FINE, int R>
 struct MxWide {
   static constexpr int PARTS = F == MX_F8 ? 2 : 1, STEP = R * (1024 * PARTS + 64);   // bytes of a step's operands and powers
@@ -407,11 +390,16 @@ __device__ __forceinline__ v16f mx_mfma32(const MxOperand& w, uint32_t wp, const
   return c;
 }
 
-// Many rows, an inner size that is a multiple of 128. A workgroup of 2 x 2 waves computes a tile of 64 TC columns x 64 TR rows, a wave
+// Many rows. A workgroup of 2 x 2 waves computes a tile of 64 TC columns x 64 TR rows, a wave
 // TC x TR products of 32 x 32 x 64. 128 of the inner size are a stage: their codes go straight into LDS, S stages ahead.
 // A stage's codes lie there as rows of 64 bytes, 16 bytes a unit (mxf8 rows twice, 64 codes each); a row's units are permuted so that the
 // 16 rows of a quarter of an operand read are on different banks. Powers come for four stages at once (a row's 16 bytes): a
 // stage's four bytes of a row at a time are as many requests as the codes are.
+// ODD: the inner size is no multiple of 128. Rows' powers then begin at any byte and come through registers (loads into LDS have whole
+// words); in the last stage units behind the rows' ends are loaded from before them, and the rows' operands from there on are zeros. (4096 x 9728
+// over 928 74 us, over 896 46.)
+// Every scaled instruction takes 32 cycles (of 8-bit codes 64) and, issued back to back, 44 to 48: 6.1 PFLOP/s of mxf4 in a loop of nothing else. 8192 x 8192 x 8192: 310 us,
+// 3.5 PFLOP/s, of which the loads cost 60, the operand reads 45 and the outputs 20; mxf8 rows 449 us, 2.4.
 template <int F, int TC, int TR, int S>
 struct MxTile {
   static constexpr int C = 64 * TC, R = 64 * TR, SLABS = F == MX_F8 ? 2 : 1;   // columns, rows; slabs of the rows' codes
@@ -471,7 +459,7 @@ __device__ __forceinline__ void mx_put(const MxProduct& p, const v16f (&acc)[TC]
   }
 }
 
-template <int F, bool FINE, int TC, int TR, int S>
+template <int F, bool FINE, int TC, int TR, int S, bool ODD>
 __global__ __launch_bounds__(256, (MxTile<F, TC, TR, S>::ALONE ? 1 : 2)) void mx_many_kernel(MxProduct p, int tiles_c, int tiles) {
   using T = MxTile<F, TC, TR, S>;
   __shared__ __attribute__((aligned(16))) uint8_t mx_lds[T::LDS];
@@ -482,7 +470,7 @@ __global__ __launch_bounds__(256, (MxTile<F, TC, TR, S>::ALONE ? 1 : 2)) void mx
   const int tiles_r = tiles / tiles_c, band = at / (8 * tiles_c), high = min(8, tiles_r - 8 * band), in = at - 8 * band * tiles_c;
   // (every lane's: the compiler divides in vector registers, and the loads' addresses have to be in scalar ones)
   const int r0 = __builtin_amdgcn_readfirstlane((8 * band + in % high) * T::R), c0 = __builtin_amdgcn_readfirstlane(in / high * T::C);
-  const int stages = p.inner >> 7, blocks = p.inner >> 5;
+  const int blocks = p.inner >> 5, stages = (blocks + 3) >> 2, tail = blocks - 4 * (stages - 1);   // tail: blocks of the last stage
   const uint32_t wrow = p.inner / 2, xrow = mx_bytes<F>(p.inner);
   // what this lane loads of 16 rows: 16 bytes, its row's unit that lies where the load puts the lane's
   const int sub = lane >> 2, unit = (lane & 3) ^ (sub >> 2 & 3);
@@ -501,6 +489,21 @@ __global__ __launch_bounds__(256, (MxTile<F, TC, TR, S>::ALONE ? 1 : 2)) void mx
     poff[i] = (uint32_t)(i < TC ? min(row, p.cols - 1 - c0) : min(row, p.rows - 1 - r0)) * blocks + 4 * (lane & 3);
   }
   auto powers = [&](int q) {   // of stages 4 q .. 4 q + 3
+    if constexpr (ODD) {
+      typedef uint32_t word __attribute__((aligned(1)));
+      const int stage = 4 * q + (lane & 3), over = 4 * (stage - stages + 1);   // (bytes that the word of a stage behind the last is further than the last one's)
+      pg_each<TC + TR>([&](auto i) {
+        const uint8_t *all = i < TC ? p.wp : p.xp, *base = i < TC ? wpb : xpb;
+        const int64_t bytes = (int64_t)(i < TC ? p.cols : p.rows) * blocks, at = (base - all) + (int64_t)poff[i] + 16 * q - max(over, 0), from = min(at, bytes - 4);
+        uint32_t v = 0;   // (behind the matrix nothing is read)
+        if (bytes >= 4) v = *(const GAS word*)(all + from) >> 8 * (int)(at - from);
+        else
+          for (int j = (int)at; j < (int)bytes; j++) v |= (uint32_t)gld(all + j) << 8 * (j - (int)at);
+        if (over >= 0 && tail < 4) v = (v & (1u << 8 * tail) - 1) | 0x7F7F7F7Fu << 8 * tail;   // 1 for the blocks behind the last
+        *(LAS uint32_t*)((LAS uint8_t*)mx_lds + T::POWERS + (q & 1) * T::SLOT + 256 * w + 1024 * i + 4 * lane) = v;
+      });
+      return;
+    }
     const uint32_t to = lds + (q & 1) * T::SLOT + 256 * w, back = 4 * max((int)(lane & 3) - (stages - 1 - 4 * q), 0);
     pg_each<TC + TR>([&](auto i) { pg_dma4<T::POWERS + 1024 * i>((i < TC ? wpb : xpb) + 16 * q, poff[i] - back, to); });
   };
@@ -509,11 +512,13 @@ __global__ __launch_bounds__(256, (MxTile<F, TC, TR, S>::ALONE ? 1 : 2)) void mx
     constexpr int I = decltype(part)::value;
     k = min(k, stages - 1);
     const uint32_t to = lds + buffer * T::STAGE + 1024 * w;
-    pg_dma16<4096 * I>(wb + 64 * k, woff[I], to);
+    const bool cut = ODD && k == stages - 1;   // units behind the rows' ends: the first one instead
+    pg_dma16<4096 * I>(wb + 64 * k, woff[I] - (cut && unit >= tail ? 16 * unit : 0), to);
     const uint8_t* xk = xb + 64 * T::SLABS * k;
     pg_each<TR * T::SLABS / TC>([&](auto j) {
       constexpr int J = I * (TR * T::SLABS / TC) + j, SLAB = J / TR, AT = J % TR;
-      pg_dma16<T::X + 64 * T::R * SLAB + 4096 * AT>(xk + 64 * SLAB, xoff[AT], to);
+      const int there = F == MX_F8 ? 2 * tail - 4 * SLAB : tail, have = there > 0 ? there : 2 * tail;   // units of this slab (none: the first slab instead)
+      pg_dma16<T::X + 64 * T::R * SLAB + 4096 * AT>(xk + (cut && there <= 0 ? 0 : 64 * SLAB), xoff[AT] - (cut && unit >= have ? 16 * unit : 0), to);
     });
   };
   static_assert(TR * T::SLABS % TC == 0, "parts of one size");
@@ -552,6 +557,13 @@ __global__ __launch_bounds__(256, (MxTile<F, TC, TR, S>::ALONE ? 1 : 2)) void mx
       } else {
         xo[J][i].lo = get(b + xa[0] + 64 * T::R * J + 2048 * i);
         xo[J][i].hi = get(b + xa[1] + 64 * T::R * J + 2048 * i);
+      }
+      if constexpr (ODD) {
+        if (k == stages - 1) {   // (the matrix's codes are always numbers)
+          const int lo = 2 * J + (F == MX_F4 || FINE ? g : 0), hi = F == MX_F4 || FINE ? lo : 2 * J + 1;   // their blocks
+          if (lo >= tail) xo[J][i].lo = {0, 0, 0, 0};
+          if (hi >= tail) xo[J][i].hi = {0, 0, 0, 0};
+        }
       }
     }
   };

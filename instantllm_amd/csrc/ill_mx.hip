@@ -53,10 +53,10 @@ int rows(bool back, int format, int dtype, const void* x, int64_t stride, int64_
   return ILL_OK;
 }
 
-template <int F, bool FINE, int R>
+template <int F, bool FINE>
 hipError_t launch_few(const MxProduct& p, hipStream_t st) {
   const int tiles = (p.cols + 15) / 16;
-  return launch(mx_few_kernel<F, FINE, R>, (int64_t)((p.rows + 16 * R - 1) / (16 * R)) * tiles, 256, 0, st, p, tiles);
+  return launch(mx_few_kernel<F, FINE>, (int64_t)((p.rows + 15) / 16) * tiles, 256, 0, st, p, tiles);
 }
 template <int F, bool FINE, int L>
 hipError_t launch_slice(const MxProduct& p, hipStream_t st) {
@@ -69,11 +69,11 @@ hipError_t launch_wide(const MxProduct& p, hipStream_t st) {
   const int tiles = (p.cols + 15) / 16, lds = MxWide<F, FINE, R>::lds(p.inner), each = std::max(1, std::min(4, (160 << 10) / lds));
   return launch(mx_wide_kernel<F, FINE, R>, std::min(256 * each, (tiles + 3) / 4), 256, lds, st, p, tiles);
 }
-template <int F, bool FINE, int TC, int TR, int S>
+template <int F, bool FINE, int TC, int TR, int S, bool ODD = false>
 hipError_t launch_many(const MxProduct& p, hipStream_t st) {
   using T = MxTile<F, TC, TR, S>;
   const int tiles_c = (p.cols + T::C - 1) / T::C, tiles = tiles_c * ((p.rows + T::R - 1) / T::R);
-  return launch(mx_many_kernel<F, FINE, TC, TR, S>, (tiles + 7) / 8 * 8ll, 256, 0, st, p, tiles_c, tiles);
+  return launch(mx_many_kernel<F, FINE, TC, TR, S, ODD>, (tiles + 7) / 8 * 8ll, 256, 0, st, p, tiles_c, tiles);
 }
 template <int F, bool FINE>
 hipError_t launch_product(const MxProduct& p, hipStream_t st) {
@@ -90,11 +90,14 @@ hipError_t launch_product(const MxProduct& p, hipStream_t st) {
     if (steps <= 16) return launch_slice<F, FINE, 2>(p, st);
     return steps <= 32 ? launch_slice<F, FINE, 4>(p, st) : launch_slice<F, FINE, 8>(p, st);
   }
-  if (p.rows <= 16) return launch_few<F, FINE, 1>(p, st);
+  if (p.rows <= 16) return launch_few<F, FINE>(p, st);
   if (p.rows <= 32 && p.cols >= 16384 && MxWide<F, FINE, 2>::lds(p.inner) <= 64 << 10) return launch_wide<F, FINE, 2>(p, st);
   // Few tiles over a long inner size: 16 rows at a time, as above (64 x 896 x 4864 6.7 us, 14 tiles of 64 x 64 13).
-  if (p.rows <= 64 && tiles(64, 64) < 64 && (steps > 16 || p.inner % 128)) return launch_few<F, FINE, 1>(p, st);
-  if (p.inner % 128) return launch_few<F, FINE, 4>(p, st);
+  if (p.rows <= 64 && tiles(64, 64) < 64 && steps > 16) return launch_few<F, FINE>(p, st);
+  if (p.inner % 128) {
+    if (tiles(64, 64) <= 512 || p.rows <= 64) return launch_many<F, FINE, 1, 1, 3, true>(p, st);
+    return launch_many<F, FINE, 2, F == MX_F8 ? 1 : 2, 2, true>(p, st);
+  }
   // Tiles as large as leave enough of them for 256 CUs. Columns x rows, us. mxf8 rows, 256 x 128 / 128 x 128 / 128 x 64 / 64 x 64: 8192 x 8192 x 8192 449 / 519 / 675 /
   // 927; 3000 x 5000 x 4096 (480 tiles of 256 x 128) 64 / 71 / 88; 2048 x 2048 x 4096 (128) 38 / 32 / 28 / 34; 5001 x 896 x 4864 (280 of 128 x 128) 45 / 41 / 37 / 48;
   // 512 x 896 x 4864 (112 of 64 x 64) 34 / 24 / 18 / 15. mxf4, 256 x 256 / 128 x 256 / 128 x 128 / 64 x 64: 8192 x 8192 x 8192 312 / 335 / 407 / 768; 3000 x 5000 x 4096 (240) 48 / 50 / 57;

@@ -169,6 +169,8 @@ class Product:
 SHAPES = [   # rows, columns, inner size: single rows, batches, prompts; odd sizes; inner sizes that are no multiple of 128
     (1, 1152, 896), (1, 896, 4864), (1, 1, 32), (2, 17, 64), (7, 33, 96), (16, 100, 160), (16, 20001, 256), (17, 1152, 896), (31, 48, 4864), (33, 70, 288),
     (64, 130, 896), (65, 128, 128), (100, 257, 512), (128, 129, 384), (200, 1000, 2048), (333, 515, 1152), (513, 300, 4864), (1, 17000, 32), (40, 16500, 96), (1025, 1030, 256),
+    # inner sizes that are no multiple of 128, in tiles: one to three blocks more, one stage and several, one or two columns, the last row alone
+    (17, 1, 32), (18, 3, 96), (65, 2, 64), (129, 200, 32), (64, 65, 160), (193, 130, 1120), (70, 4200, 672), (1100, 2100, 416), (1100, 2100, 1056), (257, 8200, 64),
     # many columns: slices of the inner size, one to eight, and rows held in LDS
     (5, 8200, 1504), (16, 8192, 4000), (3, 8300, 8192), (20, 16500, 896), (32, 17000, 96), (1, 8193, 8320),
     # tiles of every size: 128 x 64, 128 x 128 and 256 x 128 (mxf8), 128 x 128, 128 x 256 and 256 x 256 (mxf4)
@@ -200,7 +202,7 @@ def test_product_of_extreme_powers(hip, rows):
 
 
 @pytest.mark.parametrize("fmt", ["mxf8", "mxf4"])
-@pytest.mark.parametrize("rows,inner", [(2, 96), (40, 256), (200, 256)])
+@pytest.mark.parametrize("rows,inner", [(2, 96), (40, 256), (200, 256), (30, 160), (200, 224)])
 def test_product_of_nan_blocks(hip, fmt, rows, inner):
     """A NaN block reaches the outputs of its row or column, and no other."""
     rng = np.random.default_rng(5)

@@ -253,3 +253,90 @@ def test_streams_and_graphs(hip):
             q = O.values(*O.quantize(V.from_bits(x, "bf16"), "mxf8"), "mxf8")
             wv = O.values(*w, "mxf4")
             assert (np.abs(hip.get(b[3], out) - q @ wv.T) <= (inner + 2) * U * (np.abs(q) @ np.abs(wv).T)).all()
+
+
+@pytest.mark.parametrize("fmt", ["mxf8", "mxf4"])
+@pytest.mark.parametrize("rows,cols,inner", [(3, 40, 96), (5, 8200, 256), (20, 16400, 128), (70, 200, 128), (70, 200, 160)])
+def test_outputs_aligned_to_their_type(hip, fmt, rows, cols, inner):
+    """Outputs from any element on: the same values as from an aligned one, and none beside them."""
+    from instantllm_amd import mx
+    p = Product(hip, rows, cols, inner, fmt)
+    for dtype in ("f32", "bf16"):
+        size = 4 if dtype == "f32" else 2
+        want = p.run(dtype)
+        for off in (1, 4):
+            print("offset", fmt, rows, cols, inner, dtype, off, flush=True)
+            guard = np.full(rows * cols + off + 1, GUARD, want.dtype)
+            dy = hip.put(guard)
+            mx.product(*p.dev, dy + size * off, rows, cols, inner, format=fmt, dtype=dtype)
+            got = hip.get(dy, guard)
+            assert np.array_equal(got[off:-1], want.ravel()) and (got[:off] == GUARD).all() and got[-1] == GUARD
+
+
+def test_rows_past_32_bits(hip):
+    """More than 2^32 values, and rows more than 2^32 bytes apart."""
+    from instantllm_amd import mx
+    rng = np.random.default_rng(8)
+    rows, cols, few = (1 << 16) + 3, 1 << 16, 3
+    bits, x = _bits(_spread(rng, few, cols), "bf16")
+    dx, dc, dp = hip.alloc(2 * rows * cols), hip.alloc(rows * cols), hip.alloc(rows * cols // 32)
+    hip.write(dx + 2 * (rows - few) * cols, bits)
+    for fmt in ("mxf8", "mxf4"):
+        print("rows", fmt, flush=True)
+        mx.quantize(dx, dc, dp, rows, cols, format=fmt, dtype="bf16")
+        want = O.quantize(x, fmt)
+        assert np.array_equal(hip.get(dc + mx.code_bytes(fmt, (rows - few) * cols), want[0]), want[0])
+        assert np.array_equal(hip.get(dp + (rows - few) * cols // 32, want[1]), want[1])
+    stride = (1 << 31) + 8
+    held = O.quantize(x[:2], "mxf8")
+    hip.write(dc, held[0])
+    hip.write(dp, held[1])
+    mx.dequantize(dc, dp, dx, 2, cols, dtype="bf16", y_stride=stride)
+    back = O.values(*held, "mxf8")
+    for r in range(2):
+        assert np.array_equal(V.from_bits(hip.get(dx + 2 * r * stride, bits[0]), "bf16"), back[r])
+    other = [hip.alloc(held[0].nbytes), hip.alloc(held[1].nbytes)]
+    mx.quantize(dx, *other, 2, cols, dtype="bf16", x_stride=stride)
+    assert np.array_equal(O.values(hip.get(other[0], held[0]), hip.get(other[1], held[1]), "mxf8"), back)
+    w = O.quantize(rng.standard_normal((24, 256), dtype=np.float32), "mxf4")
+    dw = [hip.put(a) for a in w]
+    two = O.quantize(x[:2, :256], "mxf8")
+    near = hip.alloc(2 * 24 * 2)
+    d2 = [hip.put(a) for a in two]
+    mx.product(*d2, *dw, near, 2, 24, 256, dtype="bf16")
+    mx.product(*d2, *dw, dx, 2, 24, 256, dtype="bf16", y_stride=stride)
+    want = hip.get(near, np.empty((2, 24), np.uint16))
+    for r in range(2):
+        assert np.array_equal(hip.get(dx + 2 * r * stride, want[r]), want[r])
+
+
+@pytest.mark.parametrize("fmt", ["mxf8", "mxf4"])
+def test_operands_past_32_bits(hip, fmt):
+    """The last columns of a matrix, and the last rows, whose codes are more than 2^32 bytes: as in a product of those alone."""
+    from instantllm_amd import mx
+    rng = np.random.default_rng(9)
+    last, inner, cols = 40, 8192, (1 << 20) + 40
+    w = (rng.integers(0, 256, (last, inner // 2), dtype=np.uint8), rng.integers(116, 122, (last, inner // 32), dtype=np.uint8))
+    big = [hip.alloc(cols * inner // 2), hip.alloc(cols * inner // 32)]   # (what the others hold reaches their outputs only)
+    for d, a in zip(big, w):
+        hip.write(d + (cols - last) * a.shape[1], a)
+    for rows in (3, 40, 300):
+        p = Product(hip, rows, last, inner, fmt, w=np.zeros((last, inner), np.float32))
+        p.w = w
+        dy = hip.alloc(rows * cols * 2)
+        print("columns", fmt, rows, flush=True)
+        mx.product(*p.dev[:2], *big, dy, rows, cols, inner, format=fmt, dtype="f16")
+        got = np.stack([hip.get(dy + 2 * (r * cols + cols - last), np.empty(last, np.uint16)) for r in range(rows)])
+        p.check(got, "f16", norm=False)
+    for inner in (16384, 16384 + 32):
+        rows, cols, last = (1 << 19) + 70, 70, 70
+        p = Product(hip, last, cols, inner, fmt)
+        big = [hip.alloc(rows * a.shape[1]) for a in p.held]
+        for d, a in zip(big, p.held):
+            hip.write(d + (rows - last) * a.shape[1], a)
+        dy = hip.alloc(rows * cols * 4)
+        for dtype in ("f16", "f32"):
+            print("rows", fmt, inner, dtype, flush=True)
+            mx.product(*big, *p.dev[2:], dy, rows, cols, inner, format=fmt, dtype=dtype)
+            size = 4 if dtype == "f32" else 2
+            p.check(hip.get(dy + size * (rows - last) * cols, np.empty((last, cols), np.uint32 if size == 4 else np.uint16)), dtype, norm=False)

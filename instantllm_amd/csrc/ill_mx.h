@@ -390,7 +390,7 @@ __device__ __forceinline__ v16f mx_mfma32(const MxOperand& w, uint32_t wp, const
   return c;
 }
 
-// Many rows. A workgroup of 2 x 2 waves computes a tile of 64 TC columns x 64 TR rows, a wave
+// Many rows. A workgroup of 2 x WR waves computes a tile of 64 TC columns x 32 WR TR rows, a wave
 // TC x TR products of 32 x 32 x 64. 128 of the inner size are a stage: their codes go straight into LDS, S stages ahead.
 // A stage's codes lie there as rows of 64 bytes, 16 bytes a unit (mxf8 rows twice, 64 codes each); a row's units are permuted so that the
 // 16 rows of a quarter of an operand read are on different banks. Powers come for four stages at once (a row's 16 bytes): a
@@ -398,22 +398,20 @@ __device__ __forceinline__ v16f mx_mfma32(const MxOperand& w, uint32_t wp, const
 // ODD: the inner size is no multiple of 128. Rows' powers then begin at any byte and come through registers (loads into LDS have whole
 // words); in the last stage units behind the rows' ends are loaded from before them, and the rows' operands from there on are zeros. (4096 x 9728
 // over 928 74 us, over 896 46.)
-// Every scaled instruction takes 32 cycles (of 8-bit codes 64) and, issued back to back, 44 to 48: 6.1 PFLOP/s of mxf4 in a loop of nothing else. 8192 x 8192 x 8192: 310 us,
-// 3.5 PFLOP/s, of which the loads cost 60, the operand reads 45 and the outputs 20; mxf8 rows 449 us, 2.4.
-template <int F, int TC, int TR, int S>
+// Every scaled instruction takes 32 cycles (of 8-bit codes 64) and, issued back to back, 44 to 48: 6.1 PFLOP/s of mxf4 in a loop of nothing else. 8192 x 8192 x 8192: 306 to
+// 322 us, 3.4 to 3.6 PFLOP/s (with four waves 323 to 347, of which the loads cost 60, the operand reads 45 and the outputs 20); mxf8 rows 449 to 567 us, 1.9 to 2.4.
+template <int TC>
+constexpr int MX_OUT = 32 * (32 * TC * 4 + 16);   // bytes of LDS for a wave's outputs: 32 rows, of float32 at most
+template <int F, int TC, int TR, int S, int WR>
 struct MxTile {
-  static constexpr int C = 64 * TC, R = 64 * TR, SLABS = F == MX_F8 ? 2 : 1;   // columns, rows; slabs of the rows' codes
+  static constexpr int WAVES = 2 * WR, C = 64 * TC, R = 32 * WR * TR, SLABS = F == MX_F8 ? 2 : 1;   // columns, rows; slabs of the rows' codes
   static constexpr int X = 64 * C, STAGE = X + 64 * R * SLABS;                 // where the rows are; bytes of a stage
   static constexpr int POWERS = S * STAGE, SLOT = 16 * (C + R);                // powers: of four stages, columns and rows, twice
-  static constexpr int LOADS = TC + TR * SLABS;                                // of a wave and stage
-  static constexpr int LDS = POWERS + 2 * SLOT;
-  static constexpr bool ALONE = LDS > 80 << 10;   // one workgroup for a CU: the compiler then holds the sums in accumulation registers
-  static_assert(4 * 32 * (32 * TC * 4 + 16) <= LDS, "outputs go through it");
+  static constexpr int LC = 2 * TC / WR, LOADS = LC + TR * SLABS;              // of a wave and stage: of columns, in all
+  static constexpr int USED = POWERS + 2 * SLOT, OUT = WAVES * MX_OUT<TC>, LDS = USED > OUT ? USED : OUT;   // (outputs go through it)
 };
 __device__ __forceinline__ int mx_unit(int row, int unit) { return 16 * (4 * row + (unit ^ (row >> 2 & 3))); }
 
-template <int TC>
-constexpr int MX_OUT = 32 * (32 * TC * 4 + 16);   // bytes of LDS for a wave's outputs: 32 rows, of float32 at most
 // 16 bytes of a row's columns from c on, those that there are.
 template <int T>
 __device__ __forceinline__ void mx_store16(const MxProduct& p, int r, int c, gu32x4 v) {
@@ -459,9 +457,10 @@ __device__ __forceinline__ void mx_put(const MxProduct& p, const v16f (&acc)[TC]
   }
 }
 
-template <int F, bool FINE, int TC, int TR, int S, bool ODD>
-__global__ __launch_bounds__(256, (MxTile<F, TC, TR, S>::ALONE ? 1 : 2)) void mx_many_kernel(MxProduct p, int tiles_c, int tiles) {
-  using T = MxTile<F, TC, TR, S>;
+template <int F, bool FINE, int TC, int TR, int S, bool ODD, int WR>
+__global__ __launch_bounds__((128 * WR), 2) void mx_many_kernel(MxProduct p, int tiles_c, int tiles) {
+  using T = MxTile<F, TC, TR, S, WR>;
+  constexpr int LC = T::LC, NW = T::WAVES;
   __shared__ __attribute__((aligned(16))) uint8_t mx_lds[T::LDS];
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 31, g = lane >> 5;
   // an XCD has every eighth workgroup: it takes neighbouring tiles, eight rows of tiles at a time down each column
@@ -474,54 +473,54 @@ __global__ __launch_bounds__(256, (MxTile<F, TC, TR, S>::ALONE ? 1 : 2)) void mx
   const uint32_t wrow = p.inner / 2, xrow = mx_bytes<F>(p.inner);
   // what this lane loads of 16 rows: 16 bytes, its row's unit that lies where the load puts the lane's
   const int sub = lane >> 2, unit = (lane & 3) ^ (sub >> 2 & 3);
-  uint32_t woff[TC], xoff[TR];
+  uint32_t woff[LC], xoff[TR];
 #pragma unroll
-  for (int i = 0; i < TC; i++) woff[i] = (uint32_t)(min(c0 + 16 * (4 * i + w) + sub, p.cols - 1) - c0) * wrow + 16 * unit;
+  for (int i = 0; i < LC; i++) woff[i] = (uint32_t)(min(c0 + 16 * (NW * i + w) + sub, p.cols - 1) - c0) * wrow + 16 * unit;
 #pragma unroll
-  for (int i = 0; i < TR; i++) xoff[i] = (uint32_t)(min(r0 + 16 * (4 * i + w) + sub, p.rows - 1) - r0) * xrow + 16 * unit;
+  for (int i = 0; i < TR; i++) xoff[i] = (uint32_t)(min(r0 + 16 * (NW * i + w) + sub, p.rows - 1) - r0) * xrow + 16 * unit;
   const uint8_t *wb = p.w + (int64_t)c0 * wrow, *xb = p.x + (int64_t)r0 * xrow, *wpb = p.wp + (int64_t)c0 * blocks, *xpb = p.xp + (int64_t)r0 * blocks;
   const uint32_t lds = pg_lds_at(mx_lds);
   // 16 rows' powers of four stages: a lane loads a row's word of a stage (behind the last: the last one's)
-  uint32_t poff[TC + TR];
+  uint32_t poff[LC + TR];
 #pragma unroll
-  for (int i = 0; i < TC + TR; i++) {
-    const int row = 16 * (4 * (i < TC ? i : i - TC) + w) + (lane >> 2);
-    poff[i] = (uint32_t)(i < TC ? min(row, p.cols - 1 - c0) : min(row, p.rows - 1 - r0)) * blocks + 4 * (lane & 3);
+  for (int i = 0; i < LC + TR; i++) {
+    const int row = 16 * (NW * (i < LC ? i : i - LC) + w) + (lane >> 2);
+    poff[i] = (uint32_t)(i < LC ? min(row, p.cols - 1 - c0) : min(row, p.rows - 1 - r0)) * blocks + 4 * (lane & 3);
   }
   auto powers = [&](int q) {   // of stages 4 q .. 4 q + 3
     if constexpr (ODD) {
       typedef uint32_t word __attribute__((aligned(1)));
       const int stage = 4 * q + (lane & 3), over = 4 * (stage - stages + 1);   // (bytes that the word of a stage behind the last is further than the last one's)
-      pg_each<TC + TR>([&](auto i) {
-        const uint8_t *all = i < TC ? p.wp : p.xp, *base = i < TC ? wpb : xpb;
-        const int64_t bytes = (int64_t)(i < TC ? p.cols : p.rows) * blocks, at = (base - all) + (int64_t)poff[i] + 16 * q - max(over, 0), from = min(at, bytes - 4);
+      pg_each<LC + TR>([&](auto i) {
+        const uint8_t *all = i < LC ? p.wp : p.xp, *base = i < LC ? wpb : xpb;
+        const int64_t bytes = (int64_t)(i < LC ? p.cols : p.rows) * blocks, at = (base - all) + (int64_t)poff[i] + 16 * q - max(over, 0), from = min(at, bytes - 4);
         uint32_t v = 0;   // (behind the matrix nothing is read)
         if (bytes >= 4) v = *(const GAS word*)(all + from) >> 8 * (int)(at - from);
         else
           for (int j = (int)at; j < (int)bytes; j++) v |= (uint32_t)gld(all + j) << 8 * (j - (int)at);
         if (over >= 0 && tail < 4) v = (v & (1u << 8 * tail) - 1) | 0x7F7F7F7Fu << 8 * tail;   // 1 for the blocks behind the last
-        *(LAS uint32_t*)((LAS uint8_t*)mx_lds + T::POWERS + (q & 1) * T::SLOT + 256 * w + 1024 * i + 4 * lane) = v;
+        *(LAS uint32_t*)((LAS uint8_t*)mx_lds + T::POWERS + (q & 1) * T::SLOT + 256 * (w + NW * i) + 4 * lane) = v;
       });
       return;
     }
     const uint32_t to = lds + (q & 1) * T::SLOT + 256 * w, back = 4 * max((int)(lane & 3) - (stages - 1 - 4 * q), 0);
-    pg_each<TC + TR>([&](auto i) { pg_dma4<T::POWERS + 1024 * i>((i < TC ? wpb : xpb) + 16 * q, poff[i] - back, to); });
+    pg_each<LC + TR>([&](auto i) { pg_dma4<T::POWERS + 256 * NW * i>((i < LC ? wpb : xpb) + 16 * q, poff[i] - back, to); });
   };
-  // Part i of TC of stage k's loads (behind the last stage: the last once more, which nobody reads).
+  // Load i of stage k's (behind the last stage: the last once more, which nobody reads).
   auto load = [&](int k, int buffer, auto part) {
     constexpr int I = decltype(part)::value;
     k = min(k, stages - 1);
     const uint32_t to = lds + buffer * T::STAGE + 1024 * w;
     const bool cut = ODD && k == stages - 1;   // units behind the rows' ends: the first one instead
-    pg_dma16<4096 * I>(wb + 64 * k, woff[I] - (cut && unit >= tail ? 16 * unit : 0), to);
-    const uint8_t* xk = xb + 64 * T::SLABS * k;
-    pg_each<TR * T::SLABS / TC>([&](auto j) {
-      constexpr int J = I * (TR * T::SLABS / TC) + j, SLAB = J / TR, AT = J % TR;
+    if constexpr (I < LC) {
+      pg_dma16<1024 * NW * I>(wb + 64 * k, woff[I] - (cut && unit >= tail ? 16 * unit : 0), to);
+    } else {
+      constexpr int SLAB = (I - LC) / TR, AT = (I - LC) % TR;
       const int there = F == MX_F8 ? 2 * tail - 4 * SLAB : tail, have = there > 0 ? there : 2 * tail;   // units of this slab (none: the first slab instead)
-      pg_dma16<T::X + 64 * T::R * SLAB + 4096 * AT>(xk + (cut && there <= 0 ? 0 : 64 * SLAB), xoff[AT] - (cut && unit >= have ? 16 * unit : 0), to);
-    });
+      pg_dma16<T::X + 64 * T::R * SLAB + 1024 * NW * AT>(xb + 64 * T::SLABS * k + (cut && there <= 0 ? 0 : 64 * SLAB), xoff[AT] - (cut && unit >= have ? 16 * unit : 0), to);
+    }
   };
-  static_assert(TR * T::SLABS % TC == 0, "parts of one size");
+  constexpr int PER = (T::LOADS + TC - 1) / TC;   // loads with the products of 32 columns
   const int wc = w & 1, wr = w >> 1;   // the wave's place in the tile
   // this lane's operands in a stage: unit 2 step + g of a column's 64 bytes; of an mxf8 row's slab `step` units g and 2 + g, or 2 g and 2 g + 1
   int wa[2], xa[2];
@@ -574,15 +573,14 @@ __global__ __launch_bounds__(256, (MxTile<F, TC, TR, S>::ALONE ? 1 : 2)) void mx
 #pragma unroll
     for (int r = 0; r < TR; r++) {
       acc[K][r] = mx_mfma32<F, FINE>(wo[J][K], wp[K], xo[J][r], xp[r], acc[K][r], step);
-      if constexpr (T::ALONE) asm volatile("" : "+a"(acc[K][r]));
-      else asm volatile("" : "+v"(acc[K][r]));
+      asm volatile("" : "+v"(acc[K][r]));
     }
   };
   const std::integral_constant<int, 0> FIRST{};
   const std::integral_constant<int, 1> SECOND{};
   PG_WAIT_OWN();
   powers(0);
-  for (int k = 0; k < S; k++) pg_each<TC>([&](auto i) { load(k, k, i); });
+  for (int k = 0; k < S; k++) pg_each<T::LOADS>([&](auto i) { load(k, k, i); });
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 1) * T::LOADS) : "memory");
   PG_TURN();
   read(0, 0, FIRST);
@@ -604,7 +602,9 @@ __global__ __launch_bounds__(256, (MxTile<F, TC, TR, S>::ALONE ? 1 : 2)) void mx
     __builtin_amdgcn_sched_barrier(0);
     pg_each<TC>([&](auto c) {
       multiply(SECOND, c);
-      load(k + S, free, c);
+      pg_each<PER>([&](auto i) {
+        if constexpr (PER * c + i < T::LOADS) load(k + S, free, std::integral_constant<int, PER * c + i>{});
+      });
     });
   }
   PG_WAIT(0);   // (loads behind the last stage)

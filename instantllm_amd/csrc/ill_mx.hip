@@ -69,11 +69,11 @@ hipError_t launch_wide(const MxProduct& p, hipStream_t st) {
   const int tiles = (p.cols + 15) / 16, lds = MxWide<F, FINE, R>::lds(p.inner), each = std::max(1, std::min(4, (160 << 10) / lds));
   return launch(mx_wide_kernel<F, FINE, R>, std::min(256 * each, (tiles + 3) / 4), 256, lds, st, p, tiles);
 }
-template <int F, bool FINE, int TC, int TR, int S, bool ODD = false>
+template <int F, bool FINE, int TC, int TR, int S, bool ODD = false, int WR = 2>
 hipError_t launch_many(const MxProduct& p, hipStream_t st) {
-  using T = MxTile<F, TC, TR, S>;
+  using T = MxTile<F, TC, TR, S, WR>;
   const int tiles_c = (p.cols + T::C - 1) / T::C, tiles = tiles_c * ((p.rows + T::R - 1) / T::R);
-  return launch(mx_many_kernel<F, FINE, TC, TR, S, ODD>, (tiles + 7) / 8 * 8ll, 256, 0, st, p, tiles_c, tiles);
+  return launch(mx_many_kernel<F, FINE, TC, TR, S, ODD, WR>, (tiles + 7) / 8 * 8ll, 128 * WR, 0, st, p, tiles_c, tiles);
 }
 template <int F, bool FINE>
 hipError_t launch_product(const MxProduct& p, hipStream_t st) {
@@ -98,19 +98,24 @@ hipError_t launch_product(const MxProduct& p, hipStream_t st) {
     if (tiles(64, 64) <= 512 || p.rows <= 64) return launch_many<F, FINE, 1, 1, 3, true>(p, st);
     return launch_many<F, FINE, 2, F == MX_F8 ? 1 : 2, 2, true>(p, st);
   }
-  // Tiles as large as leave enough of them for 256 CUs. Columns x rows, us. mxf8 rows, 256 x 128 / 128 x 128 / 128 x 64 / 64 x 64: 8192 x 8192 x 8192 449 / 519 / 675 /
-  // 927; 3000 x 5000 x 4096 (480 tiles of 256 x 128) 64 / 71 / 88; 2048 x 2048 x 4096 (128) 38 / 32 / 28 / 34; 5001 x 896 x 4864 (280 of 128 x 128) 45 / 41 / 37 / 48;
-  // 512 x 896 x 4864 (112 of 64 x 64) 34 / 24 / 18 / 15. mxf4, 256 x 256 / 128 x 256 / 128 x 128 / 64 x 64: 8192 x 8192 x 8192 312 / 335 / 407 / 768; 3000 x 5000 x 4096 (240) 48 / 50 / 57;
-  // 8192 x 8192 x 2048 107 / 97 / 108; 2048 x 2048 x 4096 (128 of 128 x 256) 40 / 32 / 22 / 29; 512 x 896 x 4864 - / 27 / 19 / 13.5.
+  // Tiles as large as leave enough of them for 256 CUs, of four waves or (8) eight: two for each SIMD where a CU has one workgroup. Columns x rows, us (the same
+  // card for the numbers between two semicolons; the largest ones differ by 15% from card to card). mxf8 rows, 256 x 128 / 128 x 128 / 128 x 64 / 64 x 64: 8192 x 8192 x 8192
+  // 449 / 519 / 675 / 927; 3000 x 5000 x 4096 (480 tiles of 256 x 128) 64 / 71 / 88; 512 x 896 x 4864 (112 of 64 x 64) 34 / 24 / 18 / 15. 128 x 128 (8) / 128 x 128 / 128 x 64:
+  // 3000 x 3000 x 4096 (576 of 128 x 128) 50 / 59; 2048 x 2048 x 4096 (256) 22.7 / 32 / 25.5; 4096 x 896 x 4864 (224) 25.5 / - / 28.4; 5001 x 896 x 4864 (280) 39 / 41 / 35; against
+  // 256 x 128: 3000 x 5000 x 4096 75 / 69, 8192 x 8192 x 8192 659 / 567.
+  // mxf4, 256 x 256 (8) / 256 x 256: 8192 x 8192 x 8192 306 / 323; 4096 x 4096 x 4096 43 / 47. 256 x 256 / 128 x 256 / 128 x 128 / 64 x 64: 8192 x 8192 x 8192 312 / 335 / 407 /
+  // 768; 3000 x 5000 x 4096 (240) 48 / 50 / 57; 512 x 896 x 4864 - / 27 / 19 / 13.5. 256 x 256 (8) / 128 x 256: 8192 x 8192 x 2048 94 / 95; 8192 x 8192 x 1024 62 / 59. 128 x 128 (8) / 128 x 128:
+  // 2048 x 2048 x 4096 (256) 17.7 / 22; 4096 x 896 x 4864 (224) 19.5 / 25; 3000 x 3000 x 4096 (576) 41 / 37; 3000 x 5000 x 1024 (960) 21 / 19.3.
   if (tiles(64, 64) <= 512 || p.rows <= 64) return launch_many<F, FINE, 1, 1, 3>(p, st);
   if constexpr (FINE) {
     return launch_many<F, FINE, 2, 1, 2>(p, st);
   } else if constexpr (F == MX_F8) {
     if (tiles(256, 128) >= 384) return launch_many<F, FINE, 4, 2, 2>(p, st);
-    return tiles(128, 128) >= 480 ? launch_many<F, FINE, 2, 2, 2>(p, st) : launch_many<F, FINE, 2, 1, 2>(p, st);
+    return tiles(128, 128) >= 480 || tiles(128, 128) <= 256 ? launch_many<F, FINE, 2, 1, 3, false, 4>(p, st) : launch_many<F, FINE, 2, 1, 2>(p, st);
   } else {
-    if (tiles(256, 256) >= 240 && p.inner >= 4096) return launch_many<F, FINE, 4, 4, 3>(p, st);
-    return tiles(128, 256) >= 512 ? launch_many<F, FINE, 2, 4, 2>(p, st) : launch_many<F, FINE, 2, 2, 2>(p, st);
+    if (tiles(256, 256) >= 240 && p.inner >= 4096) return launch_many<F, FINE, 4, 2, 3, false, 4>(p, st);
+    if (tiles(128, 256) >= 512) return launch_many<F, FINE, 2, 4, 2>(p, st);
+    return tiles(128, 128) <= 256 ? launch_many<F, FINE, 2, 1, 4, false, 4>(p, st) : launch_many<F, FINE, 2, 2, 2>(p, st);
   }
 }
 

@@ -173,8 +173,8 @@ SHAPES = [   # rows, columns, inner size: single rows, batches, prompts; odd siz
     (17, 1, 32), (18, 3, 96), (65, 2, 64), (129, 200, 32), (64, 65, 160), (193, 130, 1120), (70, 4200, 672), (1100, 2100, 416), (1100, 2100, 1056), (257, 8200, 64),
     # many columns: slices of the inner size, one to eight, and rows held in LDS
     (5, 8200, 1504), (16, 8192, 4000), (3, 8300, 8192), (20, 16500, 896), (32, 17000, 96), (1, 8193, 8320),
-    # tiles of every size: 128 x 64, 128 x 128 and 256 x 128 (mxf8), 128 x 128, 128 x 256 and 256 x 256 (mxf4)
-    (1900, 2000, 128), (3001, 2450, 256), (6450, 3850, 128), (4001, 4002, 4096)]
+    # tiles of every size, of four and eight waves: 128 x 128, 128 x 64, 128 x 128 and 256 x 128 (mxf8), 128 x 128 twice, 128 x 256 and 256 x 256 (mxf4)
+    (1900, 2000, 128), (2200, 2300, 384), (3001, 2450, 256), (6450, 3850, 128), (4001, 4002, 4096)]
 
 
 @pytest.mark.parametrize("fmt", ["mxf8", "mxf4"])

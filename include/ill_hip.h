@@ -405,7 +405,7 @@ ILL_API int ill_mx_dequantize(int format, int dtype, const void* codes, const vo
 /* y[r][c] = the sum over k of x[r][k] w[c][k], plus bias[c] (NULL: none): x [rows][inner] of format x_format, the matrix w
  * [cols][inner] of format ILL_MXF4, both as ill_mx_quantize writes them. y: row r at r * y_stride elements of type y_dtype, rounded
  * once; aligned to its type (to 16 bytes, with strides of whole 16 bytes, it is stored fastest). inner: a multiple of 32 up to 2^20
- * (from 17 rows on, multiples of 128 are up to 1.6 times as fast); cols up to 2^24, rows up to 2^26, rows x cols up to 2^32.
+ * (from 17 rows on, multiples of 128 are up to 1.5 times as fast); cols up to 2^24, rows up to 2^26, rows x cols up to 2^32.
  * Sums are float32's, in an order that depends on the sizes and types alone. With x of format ILL_MXF8 and a 16-bit y they are the matrix units' own, which
  * drop parts of a product far below the largest of its group: 4e-6 of the result (2-norm) for normal values, 5e-5 for codes of evenly spread
  * exponents. For a float32 y of such x both operands are multiplied as bf16 values: not cut, but values below 2^-126 may count

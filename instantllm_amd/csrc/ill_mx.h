@@ -397,7 +397,7 @@ __device__ __forceinline__ v16f mx_mfma32(const MxOperand& w, uint32_t wp, const
 // stage's four bytes of a row at a time are as many requests as the codes are.
 // ODD: the inner size is no multiple of 128. Rows' powers then begin at any byte and come through registers (loads into LDS have whole
 // words); in the last stage units behind the rows' ends are loaded from before them, and the rows' operands from there on are zeros. (4096 x 9728
-// over 928 74 us, over 896 46.)
+// over 928 61 us, over 896 44.)
 // Every scaled instruction takes 32 cycles (of 8-bit codes 64) and, issued back to back, 44 to 48: 6.1 PFLOP/s of mxf4 in a loop of nothing else. 8192 x 8192 x 8192: 306 to
 // 322 us, 3.4 to 3.6 PFLOP/s (with four waves 323 to 347, of which the loads cost 60, the operand reads 45 and the outputs 20); mxf8 rows 449 to 567 us, 1.9 to 2.4.
 template <int TC>

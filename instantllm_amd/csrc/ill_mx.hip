@@ -75,29 +75,10 @@ hipError_t launch_many(const MxProduct& p, hipStream_t st) {
   const int tiles_c = (p.cols + T::C - 1) / T::C, tiles = tiles_c * ((p.rows + T::R - 1) / T::R);
   return launch(mx_many_kernel<F, FINE, TC, TR, S, ODD, WR>, (tiles + 7) / 8 * 8ll, 128 * WR, 0, st, p, tiles_c, tiles);
 }
-template <int F, bool FINE>
-hipError_t launch_product(const MxProduct& p, hipStream_t st) {
-  const int steps = (p.inner + 127) / 128;
-  auto tiles = [&](int c, int r) { return (int64_t)((p.cols + c - 1) / c) * ((p.rows + r - 1) / r); };
-  // Up to 16 rows: slices from 512 tiles of 16 columns on (us, against the four waves of a workgroup that share a tile, mxf8 unless said otherwise: 16 x 9728 x 896
-  // 5.2 / 6.3, 16 x 16384 x 4096 14.3 / 19.9, mxf4 16 x 32000 x 8192 37 / 61; but 1 x 896 x 4864 7.8 / 4.7). As bf16 values their rows take too many registers:
-  // 1 x 151936 x 896 23.4, with the rows in LDS 18.6. Up to 32 rows in LDS, against tiles of 64 x 64: 32 x 151936 x 896 22.9 / 28.2.
-  if (p.rows <= 16 && p.cols >= 8192 && steps <= 64) {
-    if constexpr (FINE) {
-      if (steps <= 8) return launch_wide<F, FINE, 1>(p, st);
-    }
-    if (steps <= 8) return launch_slice<F, FINE, 1>(p, st);
-    if (steps <= 16) return launch_slice<F, FINE, 2>(p, st);
-    return steps <= 32 ? launch_slice<F, FINE, 4>(p, st) : launch_slice<F, FINE, 8>(p, st);
-  }
-  if (p.rows <= 16) return launch_few<F, FINE>(p, st);
-  if (p.rows <= 32 && p.cols >= 16384 && MxWide<F, FINE, 2>::lds(p.inner) <= 64 << 10) return launch_wide<F, FINE, 2>(p, st);
-  // Few tiles over a long inner size: 16 rows at a time, as above (64 x 896 x 4864 6.7 us, 14 tiles of 64 x 64 13).
-  if (p.rows <= 64 && tiles(64, 64) < 64 && steps > 16) return launch_few<F, FINE>(p, st);
-  if (p.inner % 128) {
-    if (tiles(64, 64) <= 512 || p.rows <= 64) return launch_many<F, FINE, 1, 1, 3, true>(p, st);
-    return launch_many<F, FINE, 2, F == MX_F8 ? 1 : 2, 2, true>(p, st);
-  }
+inline int64_t mx_tiles(const MxProduct& p, int c, int r) { return (int64_t)((p.cols + c - 1) / c) * ((p.rows + r - 1) / r); }
+template <int F, bool FINE, bool ODD>
+hipError_t launch_tiles(const MxProduct& p, hipStream_t st) {
+  auto tiles = [&](int c, int r) { return mx_tiles(p, c, r); };
   // Tiles as large as leave enough of them for 256 CUs, of four waves or (8) eight: two for each SIMD where a CU has one workgroup. Columns x rows, us (the same
   // card for the numbers between two semicolons; the largest ones differ by 15% from card to card). mxf8 rows, 256 x 128 / 128 x 128 / 128 x 64 / 64 x 64: 8192 x 8192 x 8192
   // 449 / 519 / 675 / 927; 3000 x 5000 x 4096 (480 tiles of 256 x 128) 64 / 71 / 88; 512 x 896 x 4864 (112 of 64 x 64) 34 / 24 / 18 / 15. 128 x 128 (8) / 128 x 128 / 128 x 64:
@@ -106,17 +87,41 @@ hipError_t launch_product(const MxProduct& p, hipStream_t st) {
   // mxf4, 256 x 256 (8) / 256 x 256: 8192 x 8192 x 8192 306 / 323; 4096 x 4096 x 4096 43 / 47. 256 x 256 / 128 x 256 / 128 x 128 / 64 x 64: 8192 x 8192 x 8192 312 / 335 / 407 /
   // 768; 3000 x 5000 x 4096 (240) 48 / 50 / 57; 512 x 896 x 4864 - / 27 / 19 / 13.5. 256 x 256 (8) / 128 x 256: 8192 x 8192 x 2048 94 / 95; 8192 x 8192 x 1024 62 / 59. 128 x 128 (8) / 128 x 128:
   // 2048 x 2048 x 4096 (256) 17.7 / 22; 4096 x 896 x 4864 (224) 19.5 / 25; 3000 x 3000 x 4096 (576) 41 / 37; 3000 x 5000 x 1024 (960) 21 / 19.3.
-  if (tiles(64, 64) <= 512 || p.rows <= 64) return launch_many<F, FINE, 1, 1, 3>(p, st);
+  // ODD, chosen likewise / 128 x 64 (mxf8) and 128 x 128 (mxf4): mxf8 8192 x 8192 x 8160 620 / 876; 3000 x 5000 x 4064 73 / 109; 4096 x 9728 x 928 61.5 / 73.5; 2048 x 2048 x 4064 30.6 / 39.8;
+  // mxf4 8192 x 8192 x 8160 412 / 621; 2048 x 2048 x 4064 25 / 37; 4096 x 9728 x 928 57 / 55.
+  if (tiles(64, 64) <= 512 || p.rows <= 64) return launch_many<F, FINE, 1, 1, 3, ODD>(p, st);
   if constexpr (FINE) {
-    return launch_many<F, FINE, 2, 1, 2>(p, st);
+    return launch_many<F, FINE, 2, 1, 2, ODD>(p, st);
   } else if constexpr (F == MX_F8) {
-    if (tiles(256, 128) >= 384) return launch_many<F, FINE, 4, 2, 2>(p, st);
-    return tiles(128, 128) >= 480 || tiles(128, 128) <= 256 ? launch_many<F, FINE, 2, 1, 3, false, 4>(p, st) : launch_many<F, FINE, 2, 1, 2>(p, st);
+    if (tiles(256, 128) >= 384) return launch_many<F, FINE, 4, 2, 2, ODD>(p, st);
+    return tiles(128, 128) >= 480 || tiles(128, 128) <= 256 ? launch_many<F, FINE, 2, 1, 3, ODD, 4>(p, st) : launch_many<F, FINE, 2, 1, 2, ODD>(p, st);
   } else {
-    if (tiles(256, 256) >= 240 && p.inner >= 4096) return launch_many<F, FINE, 4, 2, 3, false, 4>(p, st);
-    if (tiles(128, 256) >= 512) return launch_many<F, FINE, 2, 4, 2>(p, st);
-    return tiles(128, 128) <= 256 ? launch_many<F, FINE, 2, 1, 4, false, 4>(p, st) : launch_many<F, FINE, 2, 2, 2>(p, st);
+    if (tiles(256, 256) >= 240 && p.inner > 31 * 128) return launch_many<F, FINE, 4, 2, 3, ODD, 4>(p, st);
+    if (tiles(128, 256) >= 512) return launch_many<F, FINE, 2, 4, 2, ODD>(p, st);
+    return tiles(128, 128) <= 256 ? launch_many<F, FINE, 2, 1, 4, ODD, 4>(p, st) : launch_many<F, FINE, 2, 2, 2, ODD>(p, st);
   }
+}
+
+template <int F, bool FINE>
+hipError_t launch_product(const MxProduct& p, hipStream_t st) {
+  const int steps = (p.inner + 127) / 128;
+  // Up to 16 rows: slices from 512 tiles of 16 columns on (us, against the four waves of a workgroup that share a tile, mxf8 unless said otherwise: 16 x 9728 x 896
+  // 5.2 / 6.3, 16 x 16384 x 4096 14.3 / 19.9, mxf4 16 x 32000 x 8192 37 / 61; but 1 x 896 x 4864 7.8 / 4.7). As bf16 values their rows take too many registers:
+  // 1 x 151936 x 896 23.4, with the rows in LDS 18.6. Up to 32 rows in LDS, against tiles of 64 x 64: 32 x 151936 x 896 22.9 / 28.2.
+  if (p.rows <= 16 && p.cols >= 8192 && steps <= 64) {
+    if constexpr (FINE) {
+      if (steps <= 8) return launch_wide<F, FINE, 1>(p, st);
+    } else {
+      if (steps <= 8) return launch_slice<F, FINE, 1>(p, st);
+    }
+    if (steps <= 16) return launch_slice<F, FINE, 2>(p, st);
+    return steps <= 32 ? launch_slice<F, FINE, 4>(p, st) : launch_slice<F, FINE, 8>(p, st);
+  }
+  if (p.rows <= 16) return launch_few<F, FINE>(p, st);
+  if (p.rows <= 32 && p.cols >= 16384 && MxWide<F, FINE, 2>::lds(p.inner) <= 64 << 10) return launch_wide<F, FINE, 2>(p, st);
+  // Few tiles over a long inner size: 16 rows at a time, as above (64 x 896 x 4864 6.7 us, 14 tiles of 64 x 64 13).
+  if (p.rows <= 64 && mx_tiles(p, 64, 64) < 64 && steps > 16) return launch_few<F, FINE>(p, st);
+  return p.inner % 128 ? launch_tiles<F, FINE, true>(p, st) : launch_tiles<F, FINE, false>(p, st);
 }
 
 }  // namespace

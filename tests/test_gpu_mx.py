@@ -174,7 +174,8 @@ SHAPES = [   # rows, columns, inner size: single rows, batches, prompts; odd siz
     # many columns: slices of the inner size, one to eight, and rows held in LDS
     (5, 8200, 1504), (16, 8192, 4000), (3, 8300, 8192), (20, 16500, 896), (32, 17000, 96), (1, 8193, 8320),
     # tiles of every size, of four and eight waves: 128 x 128, 128 x 64, 128 x 128 and 256 x 128 (mxf8), 128 x 128 twice, 128 x 256 and 256 x 256 (mxf4)
-    (1900, 2000, 128), (2200, 2300, 384), (3001, 2450, 256), (6450, 3850, 128), (4001, 4002, 4096)]
+    (1900, 2000, 128), (2200, 2300, 384), (3001, 2450, 256), (6450, 3850, 128), (4001, 4002, 4096),
+    (1900, 2000, 224), (2200, 2300, 352), (2200, 2300, 64), (6450, 3850, 160), (6450, 3850, 96), (4001, 4002, 4064), (4001, 4002, 4128)]
 
 
 @pytest.mark.parametrize("fmt", ["mxf8", "mxf4"])

@@ -379,18 +379,28 @@ __device__ __forceinline__ PgUnit pg_uniform(const PgUnit& u) {
 // Workgroups of attention: waves and threads, for the kernels and their launches.
 constexpr int PG_WAVES = 4, PG_THREADS = 64 * PG_WAVES;
 
-// The division of a call's work, found by every workgroup from the lengths: sequence s is thread s % NT's.
+// What launching the units of many keys first takes in LDS: the units of the waves' sequences, by their keys.
+template <bool LONGEST>
+struct PgClasses {
+  int4 classes[PG_WAVES];
+};
+template <>
+struct PgClasses<false> {};
+
+// The division of a call's work, found by every workgroup from the lengths: sequence s is thread s % NT's. LONGEST: of up to 256 sequences
+// the units of many keys are launched first (microscaled caches: a constant, as asking it of every call costs the kernels of 16-bit ones 3 to
+// 12 spilled scalar registers).
+template <bool LONGEST>
 struct PgFinder {
   static constexpr int NW = PG_WAVES, NT = PG_THREADS;
   const PgBatch& b;
   PgCut c;
   int part, units;   // tiles of keys in a part; units of work in all
   const int grid;    // workgroups that the launch has for them
-  struct Lds {
+  struct Lds : PgClasses<LONGEST> {
     int64_t tiles[NW], work[NW];
     int units[NW], parts[NW], cut[NW];
     PgUnit found;
-    int4 classes[NW];   // units of the waves' sequences, by their keys
   };
   Lds& lds;
 
@@ -519,29 +529,31 @@ struct PgFinder {
         parts += p;
         tiles += t;
       }
-      if (c.longest && b.seqs <= NT) {   // (then this is the only turn) the units of the most keys first, in four classes
-        const int keys = own.x ? pg_up(most, splits) : 0, of = 2 * keys > part ? 0 : 4 * keys > part ? 1 : 8 * keys > part ? 2 : 3;
-        int4 up = {of == 0 ? own.x : 0, of == 1 ? own.x : 0, of == 2 ? own.x : 0, of == 3 ? own.x : 0};
+      if constexpr (LONGEST) {
+        if (b.seqs <= NT) {   // (then this is the only turn) the units of the most keys first, in four classes
+          const int keys = own.x ? pg_up(most, splits) : 0, of = 2 * keys > part ? 0 : 4 * keys > part ? 1 : 8 * keys > part ? 2 : 3;
+          int4 up = {of == 0 ? own.x : 0, of == 1 ? own.x : 0, of == 2 ? own.x : 0, of == 3 ? own.x : 0};
 #pragma unroll
-        for (int m = 1; m < 64; m <<= 1) {
-          const int4 o = {__shfl_up(up.x, m), __shfl_up(up.y, m), __shfl_up(up.z, m), __shfl_up(up.w, m)};
-          if (lane >= m) {
-            up.x += o.x;
-            up.y += o.y;
-            up.z += o.z;
-            up.w += o.w;
+          for (int m = 1; m < 64; m <<= 1) {
+            const int4 o = {__shfl_up(up.x, m), __shfl_up(up.y, m), __shfl_up(up.z, m), __shfl_up(up.w, m)};
+            if (lane >= m) {
+              up.x += o.x;
+              up.y += o.y;
+              up.z += o.z;
+              up.w += o.w;
+            }
           }
-        }
-        if (lane == 63) lds.classes[w] = up;
-        __syncthreads();
-        int4 all = {0, 0, 0, 0}, here = up;   // (here: with the waves before)
+          if (lane == 63) lds.classes[w] = up;
+          __syncthreads();
+          int4 all = {0, 0, 0, 0}, here = up;   // (here: with the waves before)
 #pragma unroll
-        for (int i = 0; i < NW; i++) {
-          const int4 o = lds.classes[i];
-          all = {all.x + o.x, all.y + o.y, all.z + o.z, all.w + o.w};
-          if (i < w) here = {here.x + o.x, here.y + o.y, here.z + o.z, here.w + o.w};
+          for (int i = 0; i < NW; i++) {
+            const int4 o = lds.classes[i];
+            all = {all.x + o.x, all.y + o.y, all.z + o.z, all.w + o.w};
+            if (i < w) here = {here.x + o.x, here.y + o.y, here.z + o.z, here.w + o.w};
+          }
+          first = (of == 0 ? here.x : of == 1 ? all.x + here.y : of == 2 ? all.x + all.y + here.z : all.x + all.y + all.z + here.w) - own.x;
         }
-        first = (of == 0 ? here.x : of == 1 ? all.x + here.y : of == 2 ? all.x + all.y + here.z : all.x + all.y + all.z + here.w) - own.x;
       }
       if (u >= first && u < first + own.x) lds.found = unit(u - first, s0 + threadIdx.x, splits, y, z);
       if (u < before) break;
@@ -833,7 +845,7 @@ struct PgStepLds {
   __attribute__((aligned(16))) uint4 lds[PG_WAVES][UNITS];
   float smx[PG_WAVES][16], sls[PG_WAVES][16];
   int last;
-  PgFinder::Lds found;
+  typename PgFinder<MX>::Lds found;
 };
 template <int TC, int D, bool FINE, bool MX>   // FINE: weights in parts that keep float32 (float32 outputs)
 __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, PgStepLds<MX>& shared) {
@@ -864,7 +876,7 @@ __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, Pg
     va[d] = MX ? 16 * (key * UPR + (u ^ (D == 64 ? key & 6 : (key & 7) << 1))) + 8 * (n & 1) : pg_values_at<D>(8 * kg, 16 * d, n);
   }
   const float sc2 = a.scale * 1.4426950408889634f;
-  PgFinder finder(a.b, c, grid, shared.found);
+  PgFinder<MX> finder(a.b, c, grid, shared.found);
   auto over_kg = [](float v, auto op) {   // over the lanes of the same row
     const auto x = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
     v = op(__int_as_float((int)x[0]), __int_as_float((int)x[1]));
@@ -1161,7 +1173,7 @@ struct PgPromptLds {
   __attribute__((aligned(16))) uint4 lds[BUFFERS][2][8 * D];   // [buffer][keys, values]
   __attribute__((aligned(16))) uint8_t raw[MX ? 2 * (64 * D + 1024) : 16];   // MX: keys and values, each codes [64][D], then the powers of 16 keys in 256 bytes
   int last, tamed, wild;   // tamed: 1 + the last tile whose values were changed; wild: a wave has infinite sums or NaN
-  PgFinder::Lds found;
+  typename PgFinder<MX>::Lds found;
 };
 template <int TC, int D, bool FINE, bool MX>   // FINE: weights in parts that keep float32 (float32 outputs)
 __device__ __forceinline__ void pg_prompt(const PgStep& p, int block, int grid, PgPromptLds<D, MX>& shared) {
@@ -1176,7 +1188,7 @@ __device__ __forceinline__ void pg_prompt(const PgStep& p, int block, int grid, 
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 31, h = lane >> 5;
   const int cap = pg_cap(a.b), pmask = (1 << a.b.page_log) - 1;
   const float sc2 = a.scale * 1.4426950408889634f;
-  PgFinder finder(a.b, c, grid, shared.found);
+  PgFinder<MX> finder(a.b, c, grid, shared.found);
   auto over_h = [](float v, auto op) {   // over the two lanes of a row
     const auto x = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
     return op(__int_as_float((int)x[0]), __int_as_float((int)x[1]));

@@ -26,10 +26,10 @@ PgBatch batch_of(const ill_paged* p, const ill_paged_batch& b) {
 // a tile of rows whose keys are over 2^-7 of the call's work; a prompt alone, with PG_MANY tiles at least, never is. More parts, for the 512
 // workgroups that run at a time, have not been measured on batches that they would cut.
 PgCut step_cut(const ill_paged_desc& d, int window, int sinks) {
-  return {(uint32_t)(d.heads / d.kv_heads), (uint32_t)d.kv_heads, 16, d.head_dim == 64 ? 64 : 32, window, sinks, 8, microscaled(d) ? 16 : 8, 0, PG_MOST, 0, microscaled(d)};
+  return {(uint32_t)(d.heads / d.kv_heads), (uint32_t)d.kv_heads, 16, d.head_dim == 64 ? 64 : 32, window, sinks, 8, microscaled(d) ? 16 : 8, 0, PG_MOST, 0};
 }
 PgCut prompt_cut(const ill_paged_desc& d, int window, int sinks) {
-  return {(uint32_t)(d.heads / d.kv_heads), (uint32_t)d.kv_heads, 128, 64, window, sinks, 7, 4, 0, PG_MOST, 0, microscaled(d)};
+  return {(uint32_t)(d.heads / d.kv_heads), (uint32_t)d.kv_heads, 128, 64, window, sinks, 7, 4, 0, PG_MOST, 0};
 }
 
 // Bytes of a workspace where 2^log parts are wanted, over tiles of M rows.

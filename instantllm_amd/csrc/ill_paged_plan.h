@@ -72,7 +72,6 @@ struct PgCut {
   int32_t least;     // tiles of keys in a part at least
   int32_t lo, hi;    // sequences with lo < n G <= hi are this kernel's
   int32_t shared;    // the other kernel runs too: lo or hi hold as pg_share says
-  int32_t longest;   // units of many keys are launched first (of up to 256 sequences)
 };
 
 // Two kernels evaluate a batch. Sequences of up to PG_FEW flat rows are always the step kernel's (16 flat rows to a tile);

@@ -728,14 +728,20 @@ __device__ __forceinline__ void pg_put_part(const PgWork& w, int part, int r, in
 }
 
 static_assert(PG_FAN * PG_FAN >= PG_MAXSPLIT, "two steps");
+// What pg_join takes of LDS for tiles of M rows, in place of the tiles of keys and values, which nobody reads any more.
+template <int M>
+struct PgJoinLds {
+  __attribute__((aligned(16))) float weights[PG_FAN * M], sums[PG_FAN * M], rows[2 * M];   // of each part's rows; of the rows joined: reference and sum
+  v4f part[PG_THREADS - PG_THREADS / 4];   // states of all groups of threads but the first, up to four groups
+};
 // Joins `count` <= PG_FAN parts (from part `first` on, every step-th) of a tile of rows in their order, by one workgroup:
-// into the output, or into the first of them. lds: PG_FAN x M x 2 + 2 M floats and, behind them, PG_THREADS states.
+// into the output, or into the first of them.
 template <int TC, int D, int M>
 __device__ __forceinline__ void pg_join(const PgAttend& a, const PgCut& c, const PgWork& pw, const PgUnit& un, int first, int step, int count, bool out,
-                                        int f0, int live, LAS float* lds) {
+                                        int f0, int live, PgJoinLds<M>& lds) {
   constexpr int NT = PG_THREADS, T = NT / M >= 64 ? 64 : NT / M < 1 ? 1 : NT / M;   // T threads of a row, neighbours in a wave
   const int tid = threadIdx.x;
-  LAS float *wt = lds, *ls = lds + PG_FAN * M, *rows = ls + PG_FAN * M;
+  LAS float *wt = (LAS float*)lds.weights, *ls = (LAS float*)lds.sums, *rows = (LAS float*)lds.rows;
   // few items (four dims of a row): `groups` threads each, every groups-th part to one of them, its values fetched along
   // with the statistics
   const int items = live * (D / 4), groups = items <= NT / 4 ? 4 : items <= NT / 2 ? 2 : 1, width = NT / groups;
@@ -786,7 +792,7 @@ __device__ __forceinline__ void pg_join(const PgAttend& a, const PgCut& c, const
       }
     }
     if (groups > 1) {   // (items <= width: once)
-      LAS v4f* sums = (LAS v4f*)(rows + 2 * M);
+      LAS v4f* sums = (LAS v4f*)lds.part;
       if (g && i < items) sums[(g - 1) * width + i] = y;
       __syncthreads();
       if (g == 0 && i < items)
@@ -802,7 +808,7 @@ __device__ __forceinline__ void pg_join(const PgAttend& a, const PgCut& c, const
 
 // What follows a part of several: the last workgroup of PG_FAN parts joins them, and the last of those joins theirs.
 template <int TC, int D, int M>
-__device__ __forceinline__ void pg_finish(const PgAttend& a, const PgCut& c, const PgWork& w, const PgUnit& un, int f0, int live, LAS float* lds, int* last) {
+__device__ __forceinline__ void pg_finish(const PgAttend& a, const PgCut& c, const PgWork& w, const PgUnit& un, int f0, int live, PgJoinLds<M>& lds, int* last) {
   const int g = un.split / PG_FAN, groups = pg_up(un.splits, PG_FAN);
   int32_t* joined = w.joined + un.tile_at * (PG_MAXSPLIT / PG_FAN + 1);
   int first = un.part_at + g * PG_FAN, step = 1, count = min(PG_FAN, un.splits - g * PG_FAN);
@@ -842,7 +848,10 @@ struct PgStep {
 template <bool MX>
 struct PgStepLds {
   static constexpr int UNITS = MX ? 544 : 1024;   // of a wave: keys and values of a tile, 8 KB each (MX: values); its state, 16 x (D + 4) floats
-  __attribute__((aligned(16))) uint4 lds[PG_WAVES][UNITS];
+  union {
+    __attribute__((aligned(16))) uint4 lds[PG_WAVES][UNITS];
+    PgJoinLds<16> join;
+  };
   float smx[PG_WAVES][16], sls[PG_WAVES][16];
   int last;
   typename PgFinder<MX>::Lds found;
@@ -1144,7 +1153,7 @@ __device__ __forceinline__ void pg_step(const PgStep& p, int block, int grid, Pg
       pg_put_part<D, 16>(p.w, un.part_at + un.split, r, d, m, l, o);
     }
   }
-  if (un.splits > 1) pg_finish<TC, D, 16>(a, c, p.w, un, f0, live, (LAS float*)lds, &shared.last);
+  if (un.splits > 1) pg_finish<TC, D, 16>(a, c, p.w, un, f0, live, shared.join, &shared.last);
 }
 
 template <int TC>
@@ -1168,10 +1177,20 @@ __device__ __forceinline__ v16f pg_mfma32(uint4 a, uint4 b, v16f c) {   // 32 x 
 // MX: a tile's codes and powers go into LDS as they are and are converted once for all four waves, into the one 16-bit buffer, between two barriers; the
 // next tile's follow into the same place. 9 sequences of up to 700 new rows, 32 / 8 heads of 128: 158 us, with a bf16 cache 146.
 template <int D, bool MX>
+struct PgTiles {
+  __attribute__((aligned(16))) uint4 lds[2][2][8 * D];   // [buffer][keys, values]
+};
+template <int D>
+struct PgTiles<D, true> {
+  __attribute__((aligned(16))) uint4 lds[1][2][8 * D];
+  __attribute__((aligned(16))) uint8_t raw[2 * (64 * D + 1024)];   // keys and values, each codes [64][D], then the powers of 16 keys in 256 bytes
+};
+template <int D, bool MX>
 struct PgPromptLds {
-  static constexpr int BUFFERS = MX ? 1 : 2;
-  __attribute__((aligned(16))) uint4 lds[BUFFERS][2][8 * D];   // [buffer][keys, values]
-  __attribute__((aligned(16))) uint8_t raw[MX ? 2 * (64 * D + 1024) : 16];   // MX: keys and values, each codes [64][D], then the powers of 16 keys in 256 bytes
+  union {
+    PgTiles<D, MX> tiles;
+    PgJoinLds<128> join;
+  };
   int last, tamed, wild;   // tamed: 1 + the last tile whose values were changed; wild: a wave has infinite sums or NaN
   typename PgFinder<MX>::Lds found;
 };
@@ -1179,7 +1198,7 @@ template <int TC, int D, bool FINE, bool MX>   // FINE: weights in parts that ke
 __device__ __forceinline__ void pg_prompt(const PgStep& p, int block, int grid, PgPromptLds<D, MX>& shared) {
   constexpr int N = FINE ? PG_PARTS<TC> : 1;   // parts of a weight
   constexpr int M = 128, KT = 64, UPR = D / 8, KS = D / 16, ND = D / 32, T = KT * UPR, LOADS = MX ? D / 64 + 1 : T / PG_THREADS;   // LOADS: of keys, and of values, per wave and tile
-  auto& lds = shared.lds;
+  auto& lds = shared.tiles.lds;
   int& tamed = shared.tamed;
   const PgAttend& a = p.a;
   PgCut c = p.c;
@@ -1204,7 +1223,9 @@ __device__ __forceinline__ void pg_prompt(const PgStep& p, int block, int grid, 
   static_assert(M == 32 * PG_WAVES && KT == 16 * PG_WAVES, "a wave has 32 rows, and loads 16 keys");
   static_assert(MX || LOADS == 2 || LOADS == 4, "two or four keys x 16 bytes x lanes");
   constexpr int RAW = 64 * D + 1024;   // MX: bytes of a tile's keys, or values
-  const uint32_t mine_lds = MX ? pg_lds_at(shared.raw) : pg_lds_at(&lds[0][0][64 * LOADS * w]);
+  uint32_t mine_lds;
+  if constexpr (MX) mine_lds = pg_lds_at(shared.tiles.raw);
+  else mine_lds = pg_lds_at(&lds[0][0][64 * LOADS * w]);
   // this lane's operands in a tile: of the keys for each 16 dims, of the values for each 32 and for even and odd 16 keys;
   // others are whole multiples of 32 rows further
   int ka[KS], va[ND][2];
@@ -1290,7 +1311,7 @@ __device__ __forceinline__ void pg_prompt(const PgStep& p, int block, int grid, 
     const LAS uint8_t* kl = (const LAS uint8_t*)lds[BUF][0];
     LAS uint8_t* vl = (LAS uint8_t*)lds[BUF][1];
     if constexpr (MX) {   // codes and powers as 16-bit values where the other caches' loads put them
-      const LAS uint8_t* raw = (const LAS uint8_t*)shared.raw;
+      const LAS uint8_t* raw = (const LAS uint8_t*)shared.tiles.raw;
 #pragma unroll
       for (int x = 0; x < 2; x++)
 #pragma unroll
@@ -1489,7 +1510,7 @@ __device__ __forceinline__ void pg_prompt(const PgStep& p, int block, int grid, 
         else pg_put_part<D, M>(p.w, un.part_at + un.split, r, dim, Mx, Ls, o);
       }
   }
-  if (un.splits > 1) pg_finish<TC, D, M>(a, c, p.w, un, f0, live, (LAS float*)lds, &shared.last);
+  if (un.splits > 1) pg_finish<TC, D, M>(a, c, p.w, un, f0, live, shared.join, &shared.last);
 }
 
 template <int TC, int D, bool FINE, bool MX>

@@ -194,9 +194,16 @@ __global__ __launch_bounds__(256) void mx_few_kernel(MxProduct p, int tiles) {  
 // Up to 16 rows. The inner size is cut into L slices of up to CH steps, one to a wave; a wave holds its slice of the rows in registers and
 // goes from tile to tile of 16 columns, whose next codes are on their way while it multiplies. The slices' sums are joined in LDS, in their order, by
 // each of the waves in turn. Bound by memory: 16 x 151936 over 896 16.4 us, 4.7 TB/s, 16 x 32000 over 8192 in mxf4 37 us, 3.8 TB/s.
+// Rows that become bf16 values (FINE) take 256 registers and more, one wave a SIMD: as many workgroups as fit are launched, as each reads the rows anew (with
+// two to a CU 16 x 16384 over 2048 took 15.1 us, with one 10.8; over 4096 19.4 and 16.3).
+template <bool FINE, int L>
+struct MxSlice {
+  static constexpr int WAVES = L < 4 ? 4 : L, EACH = FINE ? 4 / WAVES : 8 / WAVES;   // of a workgroup; workgroups of a CU: as many as its registers hold
+  static_assert(EACH >= 1, "at least one fits");
+};
 template <int F, bool FINE, int L>
-__global__ __launch_bounds__(L < 4 ? 256 : 64 * L) void mx_slice_kernel(MxProduct p, int tiles) {
-  constexpr int CH = 8, WAVES = L < 4 ? 4 : L, G = WAVES / L;   // G: tiles that a workgroup computes at a time
+__global__ __launch_bounds__((64 * MxSlice<FINE, L>::WAVES)) void mx_slice_kernel(MxProduct p, int tiles) {
+  constexpr int CH = 8, WAVES = MxSlice<FINE, L>::WAVES, G = WAVES / L;   // G: tiles that a workgroup computes at a time
   __shared__ __attribute__((aligned(16))) v4f part[2][L > 1 ? WAVES : 1][64];
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int slice = w % L, group = w / L, blocks = p.inner >> 5, steps = (blocks + 3) >> 2, each = (steps + L - 1) / L;

@@ -14,8 +14,6 @@ namespace {
 
 using illp::launch;
 
-constexpr int SLICE_WAVES = 8;   // of a CU: as many as its registers hold
-
 // While this lives the current device is the one that the stream belongs to (a default stream belongs to the current one).
 struct OnStream {
   int rc = ILL_OK;
@@ -60,9 +58,9 @@ hipError_t launch_few(const MxProduct& p, hipStream_t st) {
 }
 template <int F, bool FINE, int L>
 hipError_t launch_slice(const MxProduct& p, hipStream_t st) {
-  constexpr int waves = L < 4 ? 4 : L;
-  const int tiles = (p.cols + 15) / 16, each = std::max(1, SLICE_WAVES / waves);
-  return launch(mx_slice_kernel<F, FINE, L>, std::min(256 * each, (tiles + waves / L - 1) / (waves / L)), 64 * waves, 0, st, p, tiles);
+  using S = MxSlice<FINE, L>;
+  const int tiles = (p.cols + 15) / 16, groups = S::WAVES / L;
+  return launch(mx_slice_kernel<F, FINE, L>, std::min(256 * S::EACH, (tiles + groups - 1) / groups), 64 * S::WAVES, 0, st, p, tiles);
 }
 template <int F, bool FINE, int R>   // (for rows that take up to 64 KB of LDS)
 hipError_t launch_wide(const MxProduct& p, hipStream_t st) {
@@ -106,16 +104,18 @@ template <int F, bool FINE>
 hipError_t launch_product(const MxProduct& p, hipStream_t st) {
   const int steps = (p.inner + 127) / 128;
   // Up to 16 rows: slices from 512 tiles of 16 columns on (us, against the four waves of a workgroup that share a tile, mxf8 unless said otherwise: 16 x 9728 x 896
-  // 5.2 / 6.3, 16 x 16384 x 4096 14.3 / 19.9, mxf4 16 x 32000 x 8192 37 / 61; but 1 x 896 x 4864 7.8 / 4.7). As bf16 values their rows take too many registers:
-  // 1 x 151936 x 896 23.4, with the rows in LDS 18.6. Up to 32 rows in LDS, against tiles of 64 x 64: 32 x 151936 x 896 22.9 / 28.2.
-  if (p.rows <= 16 && p.cols >= 8192 && steps <= 64) {
+  // 5.2 / 6.3, 16 x 16384 x 4096 14.3 / 19.9, mxf4 16 x 32000 x 8192 37 / 61; but 1 x 896 x 4864 7.8 / 4.7). For float32 outputs, as bf16 values, their rows take too many
+  // registers: 1 x 151936 x 896 23.4, with the rows in LDS 18.6. Slices of up to 32 steps: 16 x 16384 x 2048 10.8 / 11.3, 16 x 16384 x 4096 16.3 / 20.0, 16 x 151936 x 1536 40 / 69,
+  // 4 x 32000 x 4096 25.1 / 25.7; fewer rows and columns would do without (1 x 16384 x 2048 9.6 / 7.2, 8 rows 10.0 / 9.3, 16 x 8192 x 1152 5.0 / 4.4). Past 32 steps eight waves leave each
+  // half the registers, and 118 of them spilled: 16 x 32000 x 8192 92.5 / 73.0, 1 x 32000 x 8192 89 / 41. Up to 32 rows in LDS, against tiles of 64 x 64: 32 x 151936 x 896 22.9 / 28.2.
+  if (p.rows <= 16 && p.cols >= 8192 && steps <= (FINE ? 32 : 64)) {
     if constexpr (FINE) {
       if (steps <= 8) return launch_wide<F, FINE, 1>(p, st);
     } else {
       if (steps <= 8) return launch_slice<F, FINE, 1>(p, st);
+      if (steps > 32) return launch_slice<F, FINE, 8>(p, st);
     }
-    if (steps <= 16) return launch_slice<F, FINE, 2>(p, st);
-    return steps <= 32 ? launch_slice<F, FINE, 4>(p, st) : launch_slice<F, FINE, 8>(p, st);
+    return steps <= 16 ? launch_slice<F, FINE, 2>(p, st) : launch_slice<F, FINE, 4>(p, st);
   }
   if (p.rows <= 16) return launch_few<F, FINE>(p, st);
   if (p.rows <= 32 && p.cols >= 16384 && MxWide<F, FINE, 2>::lds(p.inner) <= 64 << 10) return launch_wide<F, FINE, 2>(p, st);

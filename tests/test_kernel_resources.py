@@ -13,19 +13,26 @@ from instantllm_amd import build
 CSRC = Path(__file__).resolve().parents[1] / "instantllm_amd" / "csrc"
 
 
-def _resources(tmp_path, header: str, kernels: list[str]) -> list[dict[str, int]]:
-    """What the compiler says of each kernel, in their order."""
+def _compile(tmp_path, text: str, *flags: str) -> str:
+    """What the compiler says."""
     if not Path(build.HIPCC).exists():
         pytest.skip("no hipcc")
     src = tmp_path / "k.hip"
-    src.write_text(f'#include <hip/hip_runtime.h>\n#include "{CSRC / header}"\n' + "".join(f"template __global__ void {k};\n" for k in kernels))
-    cmd = [build.HIPCC, *build.FLAGS, "-w", "-Rpass-analysis=kernel-resource-usage", "--cuda-device-only", "-c", str(src), "-o", str(tmp_path / "k.o")]
-    said = subprocess.run(cmd, capture_output=True, text=True)
+    src.write_text(text)
+    said = subprocess.run([build.HIPCC, *build.FLAGS, "-w", *flags, str(src)], capture_output=True, text=True)
     assert said.returncode == 0, said.stderr
-    got = [{k.strip(): int(v) for k, v in re.findall(r"remark: [^\n]*?    ([A-Z][\w ]*?)(?: \[[\w/]+\])?: (\d+) \[-Rpass", part)}
-           for part in said.stderr.split("Function Name: ")[1:]]
-    assert len(got) == len(kernels), said.stderr
-    return got
+    return said.stderr
+
+
+def _resources(tmp_path, text: str) -> dict[str, dict[str, int]]:
+    """What the compiler says of each kernel, by its name, in their order."""
+    said = _compile(tmp_path, text, "-Rpass-analysis=kernel-resource-usage", "--cuda-device-only", "-c", "-o", str(tmp_path / "k.o"))
+    names, found = [], []
+    for part in said.split("Function Name: ")[1:]:
+        names.append(part.split(" ")[0])
+        found.append({k.strip(): int(v) for k, v in re.findall(r"remark: [^\n]*?    ([A-Z][\w ]*?)(?: \[[\w/]+\])?: (\d+) \[-Rpass", part)})
+    plain = subprocess.run(["c++filt"], input="\n".join(names), capture_output=True, text=True, check=True).stdout.split("\n")
+    return {re.sub(r"^void ", "", name): f for name, f in zip(plain, found)}
 
 
 # What the 16-bit caches' kernels took before microscaled caches came: (kernel, spilled scalar registers, spilled vector registers,
@@ -37,7 +44,10 @@ PAGED = [("pg_step_kernel<PG_F16, 64, false, false>(PgStep)", 2, 0, 0, 66208), (
 
 def test_attention_over_16_bit_caches(tmp_path):
     """Pays nothing for what only microscaled caches use."""
-    for got, (kernel, sgprs, vgprs, scratch, lds) in zip(_resources(tmp_path, "ill_paged.h", [k[0] for k in PAGED]), PAGED):
+    text = f'#include <hip/hip_runtime.h>\n#include "{CSRC}/ill_paged.h"\n' + "".join(f"template __global__ void {k[0]};\n" for k in PAGED)
+    found = _resources(tmp_path, text)
+    assert len(found) == len(PAGED)
+    for got, (kernel, sgprs, vgprs, scratch, lds) in zip(found.values(), PAGED):
         assert got["SGPRs Spill"] <= sgprs and got["VGPRs Spill"] <= vgprs and got["ScratchSize"] <= scratch, (kernel, got)
         assert got["LDS Size"] <= lds and got["Occupancy"] >= 2, (kernel, got)
 
@@ -68,9 +78,14 @@ static_assert(fits<128, PgPromptLds<128, false>>(128) && fits<128, PgPromptLds<1
 
 def test_joins_have_their_lds(tmp_path):
     """The area of a join holds all that it touches, and ends before what lives on beside it."""
-    if not Path(build.HIPCC).exists():
-        pytest.skip("no hipcc")
-    (tmp_path / "j.hip").write_text(JOINS % CSRC)
-    said = subprocess.run([build.HIPCC, "--offload-arch=gfx950", "-std=c++17", "--cuda-host-only", "-fsyntax-only", "-w", "-Wno-invalid-offsetof", str(tmp_path / "j.hip")],
-                          capture_output=True, text=True)
-    assert said.returncode == 0, said.stderr
+    _compile(tmp_path, JOINS % CSRC, "--cuda-host-only", "-fsyntax-only")
+
+
+def test_products(tmp_path):
+    """No kernel of the microscaled operators spills, and slices are launched with as many workgroups for a CU as it holds."""
+    found = _resources(tmp_path, f'#include "{CSRC}/ill_mx.hip"\n')
+    assert len(found) > 30 and not {k: v for k, v in found.items() if v["VGPRs Spill"] or v["SGPRs Spill"] or v["ScratchSize"]}
+    slices = [(re.fullmatch(r"mx_slice_kernel<(\d), (true|false), (\d)>.*", k), v["Occupancy"]) for k, v in found.items() if k.startswith("mx_slice")]
+    held = "".join(f"static_assert(MxSlice<{m[2]}, {m[3]}>::EACH * MxSlice<{m[2]}, {m[3]}>::WAVES <= {4 * waves}, \"{m[0]}\");\n" for m, waves in slices)
+    assert len(slices) >= 8
+    _compile(tmp_path, f'#include <hip/hip_runtime.h>\n#include "{CSRC}/ill_mx.h"\n{held}', "--cuda-host-only", "-fsyntax-only")

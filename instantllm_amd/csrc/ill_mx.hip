@@ -87,14 +87,17 @@ hipError_t launch_tiles(const MxProduct& p, hipStream_t st) {
   // 2048 x 2048 x 4096 (256) 17.7 / 22; 4096 x 896 x 4864 (224) 19.5 / 25; 3000 x 3000 x 4096 (576) 41 / 37; 3000 x 5000 x 1024 (960) 21 / 19.3.
   // ODD, chosen likewise / 128 x 64 (mxf8) and 128 x 128 (mxf4): mxf8 8192 x 8192 x 8160 620 / 876; 3000 x 5000 x 4064 73 / 109; 4096 x 9728 x 928 61.5 / 73.5; 2048 x 2048 x 4064 30.6 / 39.8;
   // mxf4 8192 x 8192 x 8160 412 / 621; 2048 x 2048 x 4064 25 / 37; 4096 x 9728 x 928 57 / 55.
+  // The limits between them. mxf8 128 x 128 (8) / 128 x 64, by the number of the former: 2176 x 2176 x 4096 (289) 30.9 / 30.5; 2560 x 2304 x 4096 (360) 33.3 / 33.4; 2560 x 2560 x 1024 (400) 13.0 /
+  // 13.9; 2688 x 2688 x 4096 (441) 33.8 / 41.3, over 896 12.6 / 13.9. mxf4 256 x 256 (8) / 128 x 256, 8192 x 8192 over 2048, 2560, 3328 and 3968: 109 / 109, 127 / 130, 153 / 163, 181 / 197.
+  // Float32 outputs of mxf8 rows, 128 x 64 / 64 x 64: 512 x 896 x 4864 (112 of 64 x 64) 29.1 / 19.3; 4096 x 1152 x 896 (1152) 16.3 / 17.1; 5001 x 896 x 4864 57 / 60; 3000 x 5000 x 4096 128 / 147.
   if (tiles(64, 64) <= 512 || p.rows <= 64) return launch_many<F, FINE, 1, 1, 3, ODD>(p, st);
   if constexpr (FINE) {
     return launch_many<F, FINE, 2, 1, 2, ODD>(p, st);
   } else if constexpr (F == MX_F8) {
     if (tiles(256, 128) >= 384) return launch_many<F, FINE, 4, 2, 2, ODD>(p, st);
-    return tiles(128, 128) >= 480 || tiles(128, 128) <= 256 ? launch_many<F, FINE, 2, 1, 3, ODD, 4>(p, st) : launch_many<F, FINE, 2, 1, 2, ODD>(p, st);
+    return tiles(128, 128) >= 384 || tiles(128, 128) <= 256 ? launch_many<F, FINE, 2, 1, 3, ODD, 4>(p, st) : launch_many<F, FINE, 2, 1, 2, ODD>(p, st);
   } else {
-    if (tiles(256, 256) >= 240 && p.inner > 31 * 128) return launch_many<F, FINE, 4, 2, 3, ODD, 4>(p, st);
+    if (tiles(256, 256) >= 240 && p.inner > 16 * 128) return launch_many<F, FINE, 4, 2, 3, ODD, 4>(p, st);
     if (tiles(128, 256) >= 512) return launch_many<F, FINE, 2, 4, 2, ODD>(p, st);
     return tiles(128, 128) <= 256 ? launch_many<F, FINE, 2, 1, 4, ODD, 4>(p, st) : launch_many<F, FINE, 2, 2, 2, ODD>(p, st);
   }

@@ -90,14 +90,17 @@ hipError_t launch_tiles(const MxProduct& p, hipStream_t st) {
   // The limits between them. mxf8 128 x 128 (8) / 128 x 64, by the number of the former: 2176 x 2176 x 4096 (289) 30.9 / 30.5; 2560 x 2304 x 4096 (360) 33.3 / 33.4; 2560 x 2560 x 1024 (400) 13.0 /
   // 13.9; 2688 x 2688 x 4096 (441) 33.8 / 41.3, over 896 12.6 / 13.9. mxf4 256 x 256 (8) / 128 x 256, 8192 x 8192 over 2048, 2560, 3328 and 3968: 109 / 109, 127 / 130, 153 / 163, 181 / 197.
   // Float32 outputs of mxf8 rows, 128 x 64 / 64 x 64: 512 x 896 x 4864 (112 of 64 x 64) 29.1 / 19.3; 4096 x 1152 x 896 (1152) 16.3 / 17.1; 5001 x 896 x 4864 57 / 60; 3000 x 5000 x 4096 128 / 147.
-  if (tiles(64, 64) <= 512 || p.rows <= 64) return launch_many<F, FINE, 1, 1, 3, ODD>(p, st);
+  // No wider than the columns ask for, or products are thrown away: 64 x 64 for up to 64 columns (against the tiles that numbers alone choose: 65536 x 64 x 896 in mxf8 12.8 / 18.9, over
+  // 4096 68 / 74; 100000 x 32 x 4096 97 / 118, in mxf4 60 / 77; 65536 x 64 x 4096 in mxf4 43 / 45, with float32 outputs 70 / 81), 256 columns a tile from 129 on (65536 x 128 x 4096 in
+  // mxf8 71 / 78, over 896 15.2 / 19.9; in mxf4 42 / 48; 65536 x 100 x 4096 74 / 80 and 48 / 52).
+  if (tiles(64, 64) <= 512 || p.rows <= 64 || p.cols <= 64) return launch_many<F, FINE, 1, 1, 3, ODD>(p, st);
   if constexpr (FINE) {
     return launch_many<F, FINE, 2, 1, 2, ODD>(p, st);
   } else if constexpr (F == MX_F8) {
-    if (tiles(256, 128) >= 384) return launch_many<F, FINE, 4, 2, 2, ODD>(p, st);
+    if (tiles(256, 128) >= 384 && p.cols > 128) return launch_many<F, FINE, 4, 2, 2, ODD>(p, st);
     return tiles(128, 128) >= 384 || tiles(128, 128) <= 256 ? launch_many<F, FINE, 2, 1, 3, ODD, 4>(p, st) : launch_many<F, FINE, 2, 1, 2, ODD>(p, st);
   } else {
-    if (tiles(256, 256) >= 240 && p.inner > 16 * 128) return launch_many<F, FINE, 4, 2, 3, ODD, 4>(p, st);
+    if (tiles(256, 256) >= 240 && p.inner > 16 * 128 && p.cols > 128) return launch_many<F, FINE, 4, 2, 3, ODD, 4>(p, st);
     if (tiles(128, 256) >= 512) return launch_many<F, FINE, 2, 4, 2, ODD>(p, st);
     return tiles(128, 128) <= 256 ? launch_many<F, FINE, 2, 1, 4, ODD, 4>(p, st) : launch_many<F, FINE, 2, 2, 2, ODD>(p, st);
   }

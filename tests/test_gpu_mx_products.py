@@ -71,3 +71,43 @@ def test_many_rows_of_few_columns(hip, fmt, rows, cols, inner):
     for dtype in ("f32", "bf16"):
         print("rows", fmt, rows, cols, inner, dtype, flush=True)
         _check(_product(hip, x, w, fmt, dtype, stride=cols + 3), x, w, fmt, dtype)
+
+
+# up to 16 rows from 8192 columns on are slices (one, two and four of them) or, with float32 outputs of mxf8 rows, up to 1024 values in LDS; 17 to 32 rows from
+# 16384 columns on in LDS. Inner sizes whose last step has one block, two or three; numbers of steps that the slices do not divide.
+MANY = [(3, 8200, 96), (16, 8200, 160), (16, 8193, 1120), (3, 8200, 1504), (5, 8197, 4000), (2, 8200, 7968), (32, 16400, 96), (17, 16387, 160), (30, 16400, 1504), (20, 16400, 992)]
+
+
+@pytest.mark.parametrize("fmt", ["mxf8", "mxf4"])
+@pytest.mark.parametrize("rows,cols,inner", MANY)
+def test_powers_far_apart_among_many_columns(hip, fmt, rows, cols, inner):
+    rng = np.random.default_rng([rows, cols, inner])
+    x, w = _any(rng, rows, inner, fmt), _any(rng, cols, inner, "mxf4")
+    for dtype in ("f32", "bf16"):
+        print("powers", fmt, rows, cols, inner, dtype, flush=True)
+        _check(_product(hip, x, w, fmt, dtype), x, w, fmt, dtype)
+
+
+@pytest.mark.parametrize("fmt", ["mxf8", "mxf4"])
+@pytest.mark.parametrize("rows,cols,inner", MANY)
+def test_nan_blocks_among_many_columns(hip, fmt, rows, cols, inner):
+    """Blocks of NaN reach their column's or row's outputs and no other: in a column's last block, where the next bytes are the next column's,
+    in a column's first, in the last block of all, in one of the first step and one of the last; and in a row's first and last."""
+    rng = np.random.default_rng([rows, cols, inner, 1])
+    x, w = _any(rng, rows, inner, fmt, 120, 130), _any(rng, cols, inner, "mxf4", 120, 130)
+    last = inner // 32 - 1
+    at = [(7, last), (19, 0), (33, last), (34, 0), (4097, last // 2), (cols - 20, max(last - 1, 0)), (cols - 3, 0), (cols - 1, last)]
+    for c, b in at:
+        w[1][c, b] = 255
+    for dtype in ("f32", "bf16"):
+        print("nan columns", fmt, rows, cols, inner, dtype, flush=True)
+        val = _product(hip, x, w, fmt, dtype)
+        assert np.isnan(val).sum() == rows * len(at)
+        _check(val, x, w, fmt, dtype)
+    for r, b in ((0, last), (rows - 1, 0)):
+        x[1][r, b] = 255
+    for dtype in ("f32", "bf16"):
+        print("nan rows", fmt, rows, cols, inner, dtype, flush=True)
+        val = _product(hip, x, w, fmt, dtype)
+        assert np.isnan(val).sum() == rows * len(at) + 2 * (cols - len(at))
+        _check(val, x, w, fmt, dtype)

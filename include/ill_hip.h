@@ -406,11 +406,13 @@ ILL_API int ill_mx_dequantize(int format, int dtype, const void* codes, const vo
  * [cols][inner] of format ILL_MXF4, both as ill_mx_quantize writes them. y: row r at r * y_stride elements of type y_dtype, rounded
  * once; aligned to its type (to 16 bytes, with strides of whole 16 bytes, it is stored fastest). inner: a multiple of 32 up to 2^20
  * (from 17 rows on, multiples of 128 are up to 1.5 times as fast); cols up to 2^24, rows up to 2^26, rows x cols up to 2^32.
- * Sums are float32's, in an order that depends on the sizes and types alone. With x of format ILL_MXF8 and a 16-bit y they are the matrix units' own, which
- * drop parts of a product far below the largest of its group: 4e-6 of the result (2-norm) for normal values, 5e-5 for codes of evenly spread
- * exponents. For a float32 y of such x both operands are multiplied as bf16 values: not cut, but values below 2^-126 may count
- * as 0, and ones past bf16's range as infinite. A NaN block makes every output that it belongs to NaN. y overlaps nothing that the
- * call reads. */
+ * Sums are float32's, in an order that depends on the sizes and types alone. With x of format ILL_MXF8 and a 16-bit y they are the
+ * matrix units' own: of eight neighbouring values' products (the first eight, the next, ...) each loses less than 2^-12 of the largest
+ * one's size, and the largest nothing. Before it is rounded an output is so off by 7 x 2^-12 of the sum of its products' sizes at most;
+ * by the 2-norm of all outputs by up to 1e-5 for normal values, and 2e-5 to 7e-5 where every 61st is fifty times as large or codes and
+ * powers have evenly spread exponents. For a float32 y of such x both operands are multiplied as bf16 values: not cut, but values below
+ * 2^-126 may count as 0, and ones past bf16's range as infinite. A NaN block makes every output that it belongs to NaN. y overlaps
+ * nothing that the call reads. */
 ILL_API int ill_mx_product(int x_format, const void* x, const void* x_powers, const void* w, const void* w_powers, int64_t rows, int64_t cols,
                            int64_t inner, const float* bias, int y_dtype, void* y, int64_t y_stride, void* stream);
 

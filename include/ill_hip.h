@@ -370,7 +370,9 @@ ILL_API int ill_paged_append(ill_paged* p, const ill_paged_batch* batch, const i
  * j < sinks. out [rows][heads x head_dim], row r at r * out_stride, of type out_dtype (the
  * handle's, or ILL_F32): the values weighted by the softmax of the scaled scores; zeros for a row
  * that sees nothing (or whose scores are all -inf). Sums are float32, of weights of at most 1 for a
- * bf16 cache (an f16 cache's values cannot overflow them). q [rows][heads x head_dim] is of the
+ * bf16 cache (an f16 cache's values cannot overflow them). For 16-bit outputs the weights are rounded once to
+ * the handle's type before they multiply the values, each by up to 2^-8 (bf16) or 2^-11 (f16) of itself; for
+ * float32 outputs they keep 22 bits and more. q [rows][heads x head_dim] is of the
  * handle's type; out overlaps nothing that the call reads. What a row does not see never reaches it, infinities and NaN included. A value
  * that is infinite or NaN reaches every row that sees it, however small its weight: the output
  * is that infinity, or NaN where the row also sees a NaN or the other one; unless all of the

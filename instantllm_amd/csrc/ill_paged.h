@@ -89,7 +89,7 @@ __global__ __launch_bounds__(256) void pg_append_kernel(PgAppend a, int R) {
   extern __shared__ __attribute__((aligned(16))) uint8_t pg_lds[];
   constexpr int C = D / 16, EB = TX == PG_F32 ? 4 : 2;   // threads of a head; bytes of a value
   const int half = a.rot >> 1;
-  int64_t* place = (int64_t*)pg_lds;             // [R] element offset of the row's slot; -1: no sequence's row; -2: it has no place
+  int64_t* place = (int64_t*)pg_lds;             // [R] element offset of the row's slot (MX: byte offset of its page); -1: no sequence's row; -2: it has no place
   int* angle_of = (int*)(place + R);             // [R] position that turns the row
   float2* cs = (float2*)(angle_of + (R + 1) / 2 * 2);   // [R][half]
   int* slot_of = (int*)(cs + R * half);                 // MX: [R]
@@ -284,7 +284,7 @@ struct PgRead {
 template <int TO, int TC, bool MX, int D>
 __global__ __launch_bounds__(256) void pg_read_kernel(PgRead a, int R) {
   extern __shared__ __attribute__((aligned(16))) uint8_t pg_lds[];
-  int64_t* place = (int64_t*)pg_lds;   // [R] offset of the row's slot (MX: of its page); -1: no sequence's row; -2: it has no place
+  int64_t* place = (int64_t*)pg_lds;   // [R] element offset of the row's slot (MX: byte offset of its page); -1: no sequence's row; -2: it has no place
   int* slot_of = (int*)(place + R);    // [R]
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, first = blockIdx.x * R;
   // The sequences of a wave's rows one after the other, then their places side by side (a lane a row).

@@ -88,7 +88,8 @@ hipError_t launch_tiles(const MxProduct& p, hipStream_t st) {
   // ODD, chosen likewise / 128 x 64 (mxf8) and 128 x 128 (mxf4): mxf8 8192 x 8192 x 8160 620 / 876; 3000 x 5000 x 4064 73 / 109; 4096 x 9728 x 928 61.5 / 73.5; 2048 x 2048 x 4064 30.6 / 39.8;
   // mxf4 8192 x 8192 x 8160 412 / 621; 2048 x 2048 x 4064 25 / 37; 4096 x 9728 x 928 57 / 55.
   // The limits between them. mxf8 128 x 128 (8) / 128 x 64, by the number of the former: 2176 x 2176 x 4096 (289) 30.9 / 30.5; 2560 x 2304 x 4096 (360) 33.3 / 33.4; 2560 x 2560 x 1024 (400) 13.0 /
-  // 13.9; 2688 x 2688 x 4096 (441) 33.8 / 41.3, over 896 12.6 / 13.9. mxf4 256 x 256 (8) / 128 x 256, 8192 x 8192 over 2048, 2560, 3328 and 3968: 109 / 109, 127 / 130, 153 / 163, 181 / 197.
+  // 13.9; 2688 x 2688 x 4096 (441) 33.8 / 41.3, over 896 12.6 / 13.9. mxf4 256 x 256 (8) / 128 x 256, 8192 x 8192 over 2048, 2560, 3328 and 3968: 109 / 109, 127 / 130, 153 / 163, 181 / 197;
+  // 3000 x 5000 over 3584 (240 of the former) 35 / 40, with 128 x 128 45.
   // Float32 outputs of mxf8 rows, 128 x 64 / 64 x 64: 512 x 896 x 4864 (112 of 64 x 64) 29.1 / 19.3; 4096 x 1152 x 896 (1152) 16.3 / 17.1; 5001 x 896 x 4864 57 / 60; 3000 x 5000 x 4096 128 / 147.
   // No wider than the columns ask for, or products are thrown away: 64 x 64 for up to 64 columns (against the tiles that numbers alone choose: 65536 x 64 x 896 in mxf8 12.8 / 18.9, over
   // 4096 68 / 74; 100000 x 32 x 4096 97 / 118, in mxf4 60 / 77; 65536 x 64 x 4096 in mxf4 43 / 45, with float32 outputs 70 / 81), 256 columns a tile from 129 on (65536 x 128 x 4096 in
